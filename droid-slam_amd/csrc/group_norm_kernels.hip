@@ -1,0 +1,687 @@
+// Group normalisation with the activation and residual add around it
+// (modules/extractor.py: GroupNorm of BasicEncoder(norm_fn='group') and its
+// ResidualBlocks), channels last, forward and backward.
+//
+// x is (N, HW, C), C = G cpg channels in G groups; per image and group, over
+// M = HW cpg values:
+//   n   = (x - mean) rstd w_c + b_c,   rstd = 1 / sqrt(var + eps), biased var
+//   mode 0 relu(n)   1 relu(res + relu(n))   2 relu(n + res)   3 n   4 silu(n)
+// backward, with dn = dy times the activation's slope and dres = dy times the
+// outer ReLU's:
+//   dw_c = sum dn xhat,  db_c = sum dn,
+//   dx   = rstd (w dn - (sum_g w dn) / M - xhat (sum_g w dn xhat) / M)
+//
+// Every pass is a stream over maps, bound by HBM (or, for one frame, by the two
+// launches): forward reads x twice and writes y; backward's first pass reads x,
+// dy (and res) and writes dres, its second reads x and dy (dres) and writes dx.
+//
+// Layout of the work.  An image is a flat run of HW C values, cut into pieces
+// of V = 16 B.  Piece f starts at channel (V f) mod C, so with A threads, A a
+// multiple of C / gcd(C, V), a thread that takes pieces t, t + A, t + 2A, ...
+// meets the same V channels every time: its channel constants stay in
+// registers, and any C (odd ones too) streams with 16-B loads; only the last
+// HW C mod V values of an image are read one by one.
+//
+// Statistics: a thread sums its values in fp32 relative to the first one it
+// met (no cancellation where the mean is far from zero) over at most kFlush
+// pieces, then adds them to 64-bit sums; everything after that is 64-bit and
+// added in a fixed order, so results do not depend on the schedule.  mean and
+// rstd are kept in 64 bits for the backward pass: where a ReLU's argument is
+// within rounding of zero its sign is decided in 64 bits, because one wrong
+// sign moves a whole gradient, not its last bit.
+#include "common.hpp"
+
+#include <algorithm>
+
+namespace droid {
+
+namespace {
+
+constexpr int kGnT = 512;      // threads; C / gcd(C, V) <= C <= kGnMaxC fits one thread per piece
+constexpr int kGnMaxC = 512;
+constexpr int kFlush = 32;     // pieces summed in fp32 before they go to 64 bits
+constexpr float kTol = 1e-6f;  // 16 fp32 roundings: a ReLU argument below this share of its terms is re-done in 64 bits
+
+enum { kRelu = 0, kResRelu = 1, kAddRelu = 2, kNone = 3, kSilu = 4 };
+
+template <typename T>
+struct Elem;
+template <>
+struct Elem<_Float16> {
+  static constexpr int V = 8;
+};
+template <>
+struct Elem<__bf16> {
+  static constexpr int V = 8;
+};
+template <>
+struct Elem<float> {
+  static constexpr int V = 4;
+};
+
+template <typename T>
+struct Piece {
+  T v[Elem<T>::V];
+};
+
+// 16 B at any element's alignment (unaligned global accesses are legal)
+template <typename T>
+__device__ __forceinline__ Piece<T> load_piece(const T* p) {
+  Piece<T> r;
+  __builtin_memcpy(&r, p, 16);
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void store_piece(T* p, const Piece<T>& r) {
+  __builtin_memcpy(p, &r, 16);
+}
+// the image's last, short piece: m values
+template <typename T>
+__device__ __forceinline__ Piece<T> load_tail(const T* p, int m) {
+  Piece<T> r;
+#pragma unroll
+  for (int k = 0; k < Elem<T>::V; ++k) r.v[k] = k < m ? p[k] : (T)0.f;
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void store_tail(T* p, const Piece<T>& r, int m) {
+#pragma unroll
+  for (int k = 0; k < Elem<T>::V; ++k)
+    if (k < m) p[k] = r.v[k];
+}
+
+__device__ __forceinline__ float param(const void* p, int dt, int c, float dflt) {
+  if (!p) return dflt;
+  if (dt == 1) return static_cast<const float*>(p)[c];
+  if (dt == 0) return (float)static_cast<const _Float16*>(p)[c];
+  return (float)static_cast<const __bf16*>(p)[c];
+}
+
+// The split of an image's pieces over threads and workgroups.
+struct Split {
+  long pieces;   // full pieces of one image
+  int tail;      // values after them (< V)
+  int active;    // threads that take pieces: a multiple of the channel pattern's period
+  int blocks;    // workgroups an image: block s takes chunks (of `active` pieces) [chunks s / blocks, ...)
+  long chunks;
+};
+
+inline int gcd_i(int a, int b) {
+  while (b) {
+    const int t = a % b;
+    a = b;
+    b = t;
+  }
+  return a;
+}
+
+inline Split gn_split(int N, int HW, int C, int V) {
+  Split s;
+  const long total = (long)HW * C;
+  s.pieces = total / V;
+  s.tail = (int)(total % V);
+  const int period = C / gcd_i(C, V);
+  s.active = kGnT / period * period;
+  s.chunks = std::max<long>(1, (s.pieces + s.active - 1) / s.active);
+  // four workgroups a CU over all images; at least one chunk each
+  s.blocks = (int)std::max<long>(1, std::min<long>(s.chunks, std::max(1, 1024 / N)));
+  return s;
+}
+
+__device__ __forceinline__ double wave_sum(double v, int width) {
+  for (int o = width / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// Lanes that share one of `n` sums: the largest power of two <= min(64, kGnT / n).
+__device__ __forceinline__ int lanes_per(int n) {
+  int l = 1;
+  while (l < 64 && 2 * l * n <= kGnT) l *= 2;
+  return l;
+}
+
+// pass 1 of the forward: part[n][s][g] = (sum, sum of squares) of the block's
+// values, 64-bit.
+template <typename T>
+__global__ void __launch_bounds__(kGnT) gn_stats_kernel(const T* __restrict__ x, int HW, int C, int G, Split sp,
+                                                        double2* __restrict__ part) {
+  constexpr int V = Elem<T>::V;
+  __shared__ double red[kGnT * V];
+  const int n = blockIdx.y, s = blockIdx.x, S = gridDim.x, t = threadIdx.x;
+  const T* xb = x + (long)n * HW * C;
+  const long c0 = sp.chunks * s / S, c1 = sp.chunks * (s + 1) / S;
+  double s1[V], s2[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) s1[k] = s2[k] = 0.0;
+  if (t < sp.active) {
+    const long f1 = min(c1 * sp.active, sp.pieces);
+    for (long f = c0 * sp.active + t; f < f1;) {
+      float a[V], b[V], k0[V];
+      const Piece<T> p0 = load_piece(xb + f * V);
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        k0[k] = (float)p0.v[k];
+        a[k] = b[k] = 0.f;
+      }
+      f += sp.active;
+      int cnt = 1;
+#pragma unroll 4
+      for (; cnt < kFlush && f < f1; ++cnt, f += sp.active) {
+        const Piece<T> p = load_piece(xb + f * V);
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          const float d = (float)p.v[k] - k0[k];
+          a[k] += d;
+          b[k] = fmaf(d, d, b[k]);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < V; ++k) {   // about k0: sum = n k0 + a, squares = b + 2 k0 a + n k0^2
+        const double q = k0[k], da = a[k];
+        s1[k] += cnt * q + da;
+        s2[k] += (double)b[k] + q * (2.0 * da + cnt * q);
+      }
+    }
+    if (sp.tail && c1 == sp.chunks && sp.pieces % sp.active == t) {
+      const Piece<T> p = load_tail(xb + sp.pieces * V, sp.tail);
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const double q = (float)p.v[k];
+        s1[k] += q;
+        s2[k] += q * q;
+      }
+    }
+  }
+  // runs of r = gcd(cpg, V) values lie in one group: add them in registers
+  const int cpg = C / G;
+  int r = V;
+  while (cpg % r) r /= 2;
+  const int runs = V / r;
+  const int per = cpg / r;                       // runs of one group in one period
+  const int copies = sp.active * V / C;          // periods over the active threads
+  const int L = lanes_per(G), g = t / L, l = t % L;
+  double out[2];
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    double (&v)[V] = q ? s2 : s1;
+    if (r >= 2) {
+#pragma unroll
+      for (int k = 0; k < V / 2; ++k) v[k] = v[2 * k] + v[2 * k + 1];
+    }
+    if (r >= 4) {
+#pragma unroll
+      for (int k = 0; k < V / 4; ++k) v[k] = v[2 * k] + v[2 * k + 1];
+    }
+    if (r >= 8) v[0] = v[0] + v[1];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      if (k < runs && t < sp.active) red[t * runs + k] = v[k];
+    __syncthreads();
+    double acc = 0.0;
+    if (g < G)
+      for (int i = l; i < copies * per; i += L) acc += red[(i / per) * (C / r) + g * per + i % per];
+    out[q] = wave_sum(acc, L);
+  }
+  if (g < G && l == 0) part[((long)n * S + s) * G + g] = make_double2(out[0], out[1]);
+}
+
+// mean and rstd of image n's groups from the S partials, in LDS (and to stats)
+__device__ __forceinline__ void gn_finish_stats(const double2* part, int n, int S, int G, long M, float eps,
+                                                double2* st, double2* stats_out) {
+  const int t = threadIdx.x, L = lanes_per(G), g = t / L, l = t % L;
+  double a = 0.0, b = 0.0;
+  if (g < G)
+    for (int s = l; s < S; s += L) {
+      const double2 v = part[((long)n * S + s) * G + g];
+      a += v.x;
+      b += v.y;
+    }
+  a = wave_sum(a, L);
+  b = wave_sum(b, L);
+  if (g < G && l == 0) {
+    const double mean = a / (double)M;
+    double var = b / (double)M - mean * mean;
+    if (var < 0.0) var = 0.0;   // (a NaN stays one)
+    const double2 v = make_double2(mean, 1.0 / sqrt(var + (double)eps));
+    st[g] = v;
+    if (stats_out) stats_out[(long)n * G + g] = v;
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ float relu(float v) { return v < 0.f ? 0.f : v; }   // passes a NaN on, as torch's
+
+template <int MODE>
+__device__ __forceinline__ float gn_act(float n, float r) {
+  if constexpr (MODE == kRelu) return relu(n);
+  if constexpr (MODE == kResRelu) return relu(r + relu(n));
+  if constexpr (MODE == kAddRelu) return relu(n + r);
+  if constexpr (MODE == kSilu) return n * __builtin_amdgcn_rcpf(1.f + __expf(-n));
+  return n;
+}
+
+// A thread's channel constants: n = (x - m) rw + b
+template <int V>
+struct ChanConst {
+  float m[V], rw[V], b[V];
+};
+template <typename T>
+__device__ __forceinline__ void gn_consts(ChanConst<Elem<T>::V>& cc, const double2* st, const void* w, const void* b,
+                                          int wdt, int C, int G) {
+  constexpr int V = Elem<T>::V;
+  const int cpg = C / G;
+  int c = (int)(((long)threadIdx.x * V) % C);
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    const double2 v = st[c / cpg];
+    cc.m[k] = (float)v.x;
+    cc.rw[k] = (float)(v.y * (double)param(w, wdt, c, 1.f));
+    cc.b[k] = param(b, wdt, c, 0.f);
+    c = c + 1 == C ? 0 : c + 1;
+  }
+}
+
+// pass 2 of the forward
+template <typename T, int MODE>
+__global__ void __launch_bounds__(kGnT) gn_apply_kernel(const T* x, const T* res, T* out, const void* __restrict__ w,
+                                                        const void* __restrict__ b, int wdt,
+                                                        const double2* __restrict__ part, int S, int HW, int C, int G,
+                                                        Split sp, float eps, double2* stats_out) {
+  constexpr int V = Elem<T>::V;
+  constexpr bool RES = MODE == kResRelu || MODE == kAddRelu;
+  __shared__ double2 st[kGnMaxC];
+  const int n = blockIdx.y, t = threadIdx.x;
+  gn_finish_stats(part, n, S, G, (long)HW * (C / G), eps, st, blockIdx.x == 0 ? stats_out : nullptr);
+  if (t >= sp.active) return;
+  ChanConst<V> cc;
+  gn_consts<T>(cc, st, w, b, wdt, C, G);
+  const long base = (long)n * HW * C;
+  const long c0 = sp.chunks * blockIdx.x / gridDim.x, c1 = sp.chunks * (blockIdx.x + 1) / gridDim.x;
+  const long f1 = min(c1 * sp.active, sp.pieces);
+  auto piece = [&](const Piece<T>& p, const Piece<T>& rp) {
+    Piece<T> o;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const float nn = fmaf((float)p.v[k] - cc.m[k], cc.rw[k], cc.b[k]);
+      o.v[k] = (T)gn_act<MODE>(nn, RES ? (float)rp.v[k] : 0.f);
+    }
+    return o;
+  };
+#pragma unroll 4
+  for (long f = c0 * sp.active + t; f < f1; f += sp.active) {
+    const Piece<T> p = load_piece(x + base + f * V);
+    Piece<T> rp;
+    if constexpr (RES) rp = load_piece(res + base + f * V);
+    store_piece(out + base + f * V, piece(p, rp));
+  }
+  if (sp.tail && c1 == sp.chunks && sp.pieces % sp.active == t) {
+    const long o = base + sp.pieces * V;
+    const Piece<T> p = load_tail(x + o, sp.tail);
+    Piece<T> rp;
+    if constexpr (RES) rp = load_tail(res + o, sp.tail);
+    store_tail(out + o, piece(p, rp), sp.tail);
+  }
+}
+
+// dn and dres of one value (v: x, r: res, g: dy).  stw: the group's 64-bit
+// (mean, rstd); tolc = kTol (2 |b| + |m rw|), the channel's share of the bound
+// on n's fp32 error.
+template <int MODE>
+__device__ __forceinline__ void gn_slope(float v, float r, float g, float n, float tolc, const double2* stw, float w,
+                                         float b, float& dn, float& dres) {
+  dres = g;
+  if constexpr (MODE == kNone) {
+    dn = g;
+  } else if constexpr (MODE == kSilu) {
+    const float sg = __builtin_amdgcn_rcpf(1.f + __expf(-n));
+    dn = g * sg * (1.f + n * (1.f - sg));
+  } else if constexpr (MODE == kRelu) {
+    bool on = n > 0.f;
+    if (fabsf(n) <= tolc) on = ((double)v - stw->x) * (stw->y * (double)w) + (double)b > 0.0;
+    dn = on ? g : 0.f;
+  } else {
+    const float tol = fmaf(kTol, fabsf(r), tolc);
+    bool on_n = n > 0.f, on_o;
+    float pre;
+    bool near;
+    if constexpr (MODE == kResRelu) {
+      pre = r + fmaxf(n, 0.f);
+      near = fabsf(n) <= tolc || (n > 0.f && fabsf(pre) <= tol);
+    } else {
+      pre = n + r;
+      near = fabsf(pre) <= tol;
+    }
+    on_o = pre > 0.f;
+    if (near) {
+      const double nd = ((double)v - stw->x) * (stw->y * (double)w) + (double)b;
+      on_n = nd > 0.0;
+      on_o = (MODE == kResRelu ? (double)r + fmax(nd, 0.0) : nd + (double)r) > 0.0;
+    }
+    dres = on_o ? g : 0.f;
+    dn = MODE == kResRelu && !on_n ? 0.f : dres;
+  }
+}
+
+// pass 1 of the backward: per block the channel sums of dn and dn xhat
+// (cpart[n][s][c]) and the group sums of w dn and w dn xhat (gpart[n][s][g]);
+// writes dres.
+template <typename T, int MODE>
+__global__ void __launch_bounds__(kGnT) gn_bwd_stats_kernel(const T* __restrict__ x, const T* __restrict__ res,
+                                                            const T* __restrict__ dy, T* __restrict__ dres,
+                                                            const void* __restrict__ w, const void* __restrict__ b,
+                                                            int wdt, const double2* __restrict__ stats, int HW, int C,
+                                                            int G, Split sp, double2* __restrict__ cpart,
+                                                            double2* __restrict__ gpart) {
+  constexpr int V = Elem<T>::V;
+  constexpr bool RES = MODE == kResRelu || MODE == kAddRelu;
+  __shared__ float red[2][kGnT * V];
+  __shared__ double2 sum[kGnT];
+  const int n = blockIdx.y, s = blockIdx.x, S = gridDim.x, t = threadIdx.x;
+  const int cpg = C / G;
+  const double2* st = stats + (long)n * G;
+  ChanConst<V> cc;
+  gn_consts<T>(cc, st, w, b, wdt, C, G);
+  float rs[V], tolc[V], a1[V], a2[V];
+  int cg = (int)(((long)t * V) % C);
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    rs[k] = (float)st[cg / cpg].y;
+    tolc[k] = kTol * (2.f * fabsf(cc.b[k]) + fabsf(cc.m[k] * cc.rw[k]));
+    a1[k] = a2[k] = 0.f;
+    cg = cg + 1 == C ? 0 : cg + 1;
+  }
+  const long base = (long)n * HW * C;
+  const long c0 = sp.chunks * s / S, c1 = sp.chunks * (s + 1) / S;
+  const long f1 = min(c1 * sp.active, sp.pieces);
+  auto piece = [&](const Piece<T>& p, const Piece<T>& rp, const Piece<T>& gp, int m) {
+    Piece<T> o;
+    int c = (int)(((long)t * V) % C);
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const float v = (float)p.v[k], d = v - cc.m[k];
+      const float nn = fmaf(d, cc.rw[k], cc.b[k]);
+      float dn, dr;
+      gn_slope<MODE>(v, RES ? (float)rp.v[k] : 0.f, (float)gp.v[k], nn, tolc[k], st + c / cpg, param(w, wdt, c, 1.f),
+                     cc.b[k], dn, dr);
+      if (k < m) {
+        a1[k] += dn;
+        a2[k] = fmaf(dn, d * rs[k], a2[k]);
+      }
+      o.v[k] = (T)dr;
+      c = c + 1 == C ? 0 : c + 1;
+    }
+    return o;
+  };
+  if (t < sp.active) {
+#pragma unroll 2
+    for (long f = c0 * sp.active + t; f < f1; f += sp.active) {
+      const Piece<T> p = load_piece(x + base + f * V), gp = load_piece(dy + base + f * V);
+      Piece<T> rp;
+      if constexpr (RES) rp = load_piece(res + base + f * V);
+      const Piece<T> o = piece(p, rp, gp, V);
+      if constexpr (RES) store_piece(dres + base + f * V, o);
+    }
+    if (sp.tail && c1 == sp.chunks && sp.pieces % sp.active == t) {
+      const long o0 = base + sp.pieces * V;
+      const Piece<T> p = load_tail(x + o0, sp.tail), gp = load_tail(dy + o0, sp.tail);
+      Piece<T> rp;
+      if constexpr (RES) rp = load_tail(res + o0, sp.tail);
+      const Piece<T> o = piece(p, rp, gp, sp.tail);
+      if constexpr (RES) store_tail(dres + o0, o, sp.tail);
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      red[0][t * V + k] = a1[k];
+      red[1][t * V + k] = a2[k];
+    }
+  }
+  __syncthreads();
+  // channel c: the flat values c, c + C, ... of the active threads, over lanes of
+  // its own (l slow: neighbouring threads read neighbouring channels)
+  const int copies = sp.active * V / C;
+  const int L = max(1, kGnT / C), l = t / C, c = t % C;
+  double u = 0.0, v = 0.0;
+  if (l < L)
+    for (int i = l; i < copies; i += L) {
+      u += (double)red[0][c + i * C];
+      v += (double)red[1][c + i * C];
+    }
+  sum[t] = make_double2(u, v);
+  __syncthreads();
+  if (t < C) {
+    for (int i = 1; i < L; ++i) {
+      u += sum[t + i * C].x;
+      v += sum[t + i * C].y;
+    }
+    cpart[((long)n * S + s) * C + t] = make_double2(u, v);
+    const double wc = (double)param(w, wdt, t, 1.f);
+    sum[t] = make_double2(u * wc, v * wc);
+  }
+  __syncthreads();
+  if (t < G) {
+    u = v = 0.0;
+    for (int i = 0; i < cpg; ++i) {
+      u += sum[t * cpg + i].x;
+      v += sum[t * cpg + i].y;
+    }
+    gpart[((long)n * S + s) * G + t] = make_double2(u, v);
+  }
+}
+
+// pass 2 of the backward: dx; the grid's last row of workgroups (blockIdx.y ==
+// N) adds up the channel sums to dw and db instead.
+template <typename T, int MODE>
+__global__ void __launch_bounds__(kGnT) gn_bwd_apply_kernel(const T* __restrict__ x, const T* __restrict__ dyr,
+                                                            T* __restrict__ dx, const void* __restrict__ w,
+                                                            const void* __restrict__ b, int wdt,
+                                                            const double2* __restrict__ stats, int N, int HW, int C,
+                                                            int G, Split sp, int S, const double2* __restrict__ cpart,
+                                                            const double2* __restrict__ gpart, void* __restrict__ dw,
+                                                            void* __restrict__ db) {
+  constexpr int V = Elem<T>::V;
+  __shared__ double2 sm[kGnT];
+  const int n = blockIdx.y, t = threadIdx.x;
+  if (n == N) {
+    // 16 channels a workgroup, 32 lanes over the N S partials of each
+    const int l = t / 16;
+    for (int c0 = blockIdx.x * 16; c0 < C; c0 += gridDim.x * 16) {
+      const int c = c0 + t % 16;
+      double u = 0.0, v = 0.0;
+      if (c < C)
+        for (int i = l; i < N * S; i += kGnT / 16) {
+          const double2 p = cpart[(long)i * C + c];
+          u += p.x;
+          v += p.y;
+        }
+      __syncthreads();
+      sm[t] = make_double2(u, v);
+      __syncthreads();
+      if (t < 16 && c < C) {
+        u = v = 0.0;
+        for (int i = 0; i < kGnT / 16; ++i) {
+          u += sm[t + 16 * i].x;
+          v += sm[t + 16 * i].y;
+        }
+        if (wdt == 1) {
+          if (dw) static_cast<float*>(dw)[c] = (float)v;
+          if (db) static_cast<float*>(db)[c] = (float)u;
+        } else if (wdt == 0) {
+          if (dw) static_cast<_Float16*>(dw)[c] = (_Float16)(float)v;
+          if (db) static_cast<_Float16*>(db)[c] = (_Float16)(float)u;
+        } else {
+          if (dw) static_cast<__bf16*>(dw)[c] = (__bf16)(float)v;
+          if (db) static_cast<__bf16*>(db)[c] = (__bf16)(float)u;
+        }
+      }
+    }
+    return;
+  }
+  const int cpg = C / G;
+  const double2* st = stats + (long)n * G;
+  {
+    const int L = lanes_per(G), g = t / L, l = t % L;
+    double u = 0.0, v = 0.0;
+    if (g < G)
+      for (int s = l; s < S; s += L) {
+        const double2 p = gpart[((long)n * S + s) * G + g];
+        u += p.x;
+        v += p.y;
+      }
+    u = wave_sum(u, L);
+    v = wave_sum(v, L);
+    const double M = (double)HW * cpg;
+    if (g < G && l == 0) sm[g] = make_double2(u / M, v / M);
+    __syncthreads();
+  }
+  if (t >= sp.active) return;
+  // dx = rstd w dn - rstd (k1 + xhat k2): per channel rw = rstd w, q1 = rstd k1, q2 = rstd^2 k2
+  ChanConst<V> cc;
+  gn_consts<T>(cc, st, w, b, wdt, C, G);
+  float q1[V], q2[V], tolc[V];
+  int cg = (int)(((long)t * V) % C);
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    const double r = st[cg / cpg].y;
+    const double2 kk = sm[cg / cpg];
+    q1[k] = (float)(r * kk.x);
+    q2[k] = (float)(r * r * kk.y);
+    tolc[k] = kTol * (2.f * fabsf(cc.b[k]) + fabsf(cc.m[k] * cc.rw[k]));
+    cg = cg + 1 == C ? 0 : cg + 1;
+  }
+  const long base = (long)n * HW * C;
+  const long c0 = sp.chunks * blockIdx.x / gridDim.x, c1 = sp.chunks * (blockIdx.x + 1) / gridDim.x;
+  const long f1 = min(c1 * sp.active, sp.pieces);
+  // the outer ReLU's slope is in dyr (= dres) already: what is left is mode 0's
+  // ReLU (mode 1's inner one), or SiLU's slope
+  constexpr int LEFT = MODE == kResRelu ? (int)kRelu : MODE == kAddRelu ? (int)kNone : MODE;
+  auto piece = [&](const Piece<T>& p, const Piece<T>& gp) {
+    Piece<T> o;
+    int c = (int)(((long)t * V) % C);
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const float v = (float)p.v[k], d = v - cc.m[k];
+      const float nn = fmaf(d, cc.rw[k], cc.b[k]);
+      float dn, dr;
+      gn_slope<LEFT>(v, 0.f, (float)gp.v[k], nn, tolc[k], st + c / cpg, param(w, wdt, c, 1.f), cc.b[k], dn, dr);
+      o.v[k] = (T)(fmaf(dn, cc.rw[k], -fmaf(d, q2[k], q1[k])));
+      c = c + 1 == C ? 0 : c + 1;
+    }
+    return o;
+  };
+#pragma unroll 2
+  for (long f = c0 * sp.active + t; f < f1; f += sp.active) {
+    const Piece<T> p = load_piece(x + base + f * V), gp = load_piece(dyr + base + f * V);
+    store_piece(dx + base + f * V, piece(p, gp));
+  }
+  if (sp.tail && c1 == sp.chunks && sp.pieces % sp.active == t) {
+    const long o0 = base + sp.pieces * V;
+    const Piece<T> p = load_tail(x + o0, sp.tail), gp = load_tail(dyr + o0, sp.tail);
+    store_tail(dx + o0, piece(p, gp), sp.tail);
+  }
+}
+
+inline int gn_vec(int dtype) { return dtype == 1 ? 4 : 8; }
+
+int gn_check(const char* what, int dtype, int wdtype, int N, int HW, int C, int G, int mode) {
+  if (dtype != 0 && dtype != 1 && dtype != 3)
+    return fail(kInvalidArgument, std::string(what) + ": dtype must be float16, float32 or bfloat16");
+  if (wdtype != 1 && wdtype != dtype)
+    return fail(kInvalidArgument, std::string(what) + ": weight and bias must be float32 or of x's type");
+  if (N < 0 || HW < 0 || C <= 0 || C > kGnMaxC || G <= 0 || C % G || mode < 0 || mode > 4)
+    return fail(kInvalidArgument, std::string(what) + ": bad arguments (0 < C <= 512, C % groups == 0, mode 0..4)");
+  if (N > 65534) return fail(kUnsupported, std::string(what) + ": more than 65534 images");
+  return kOk;
+}
+
+}  // namespace
+
+}  // namespace droid
+
+using namespace droid;
+
+#define GN_MODES(T, KERNEL, ...)                         \
+  switch (mode) {                                        \
+    case kRelu: KERNEL(T, kRelu, __VA_ARGS__); break;       \
+    case kResRelu: KERNEL(T, kResRelu, __VA_ARGS__); break; \
+    case kAddRelu: KERNEL(T, kAddRelu, __VA_ARGS__); break; \
+    case kNone: KERNEL(T, kNone, __VA_ARGS__); break;       \
+    default: KERNEL(T, kSilu, __VA_ARGS__); break;          \
+  }
+#define GN_TYPES(KERNEL, ...)                                  \
+  if (dtype == 0) {                                            \
+    GN_MODES(_Float16, KERNEL, __VA_ARGS__)                    \
+  } else if (dtype == 1) {                                     \
+    GN_MODES(float, KERNEL, __VA_ARGS__)                       \
+  } else {                                                     \
+    GN_MODES(__bf16, KERNEL, __VA_ARGS__)                      \
+  }
+
+extern "C" {
+
+size_t droid_group_norm_workspace(int dtype, int N, int HW, int C, int G, int backward) {
+  if (gn_check("group_norm_workspace", dtype, 1, N, HW, C, G, 0) != kOk || N == 0 || HW == 0) return 0;
+  const Split sp = gn_split(N, HW, C, gn_vec(dtype));
+  return (size_t)N * sp.blocks * (G + (backward ? C : 0)) * sizeof(double2);
+}
+
+int droid_group_norm_act(int dtype, const void* x, const void* res, void* out, const void* weight, const void* bias,
+                         int wdtype, void* stats, int N, int HW, int C, int G, int mode, float eps, void* ws,
+                         size_t ws_bytes, hipStream_t stream) {
+  if (const int st = gn_check("group_norm_act", dtype, wdtype, N, HW, C, G, mode)) return st;
+  if (N == 0 || HW == 0) return kOk;
+  const bool need_res = mode == kResRelu || mode == kAddRelu;
+  if (!x || !out || (need_res && !res)) return fail(kInvalidArgument, "group_norm_act: null map");
+  if (!ws || ws_bytes < droid_group_norm_workspace(dtype, N, HW, C, G, 0))
+    return fail(kInvalidArgument, "group_norm_act: workspace too small");
+  const Split sp = gn_split(N, HW, C, gn_vec(dtype));
+  double2* part = static_cast<double2*>(ws);
+  const dim3 grid(sp.blocks, N);
+#define GN_STATS(T) gn_stats_kernel<T><<<grid, kGnT, 0, stream>>>((const T*)x, HW, C, G, sp, part)
+  if (dtype == 0) GN_STATS(_Float16);
+  else if (dtype == 1) GN_STATS(float);
+  else GN_STATS(__bf16);
+#undef GN_STATS
+  DROID_LAUNCH_CHECK();
+#define GN_APPLY(T, M, ...)                                                                                          \
+  gn_apply_kernel<T, M><<<grid, kGnT, 0, stream>>>((const T*)x, (const T*)res, (T*)out, weight, bias, wdtype, part, \
+                                                   sp.blocks, HW, C, G, sp, eps, (double2*)stats)
+  GN_TYPES(GN_APPLY, 0)
+#undef GN_APPLY
+  DROID_LAUNCH_CHECK();
+  return kOk;
+}
+
+int droid_group_norm_act_backward(int dtype, const void* x, const void* res, const void* dy, const void* weight,
+                                  const void* bias, int wdtype, const void* stats, void* dx, void* dres, void* dweight,
+                                  void* dbias, int N, int HW, int C, int G, int mode, void* ws, size_t ws_bytes,
+                                  hipStream_t stream) {
+  if (const int st = gn_check("group_norm_act_backward", dtype, wdtype, N, HW, C, G, mode)) return st;
+  if (N == 0 || HW == 0) return kOk;
+  const bool need_res = mode == kResRelu || mode == kAddRelu;
+  if (!x || !dy || !dx || !stats || (need_res && (!res || !dres)))
+    return fail(kInvalidArgument, "group_norm_act_backward: null map");
+  if (!ws || ws_bytes < droid_group_norm_workspace(dtype, N, HW, C, G, 1))
+    return fail(kInvalidArgument, "group_norm_act_backward: workspace too small");
+  const Split sp = gn_split(N, HW, C, gn_vec(dtype));
+  double2* gpart = static_cast<double2*>(ws);
+  double2* cpart = gpart + (size_t)N * sp.blocks * G;
+  const double2* st = static_cast<const double2*>(stats);
+#define GN_BSTATS(T, M, ...)                                                                                        \
+  gn_bwd_stats_kernel<T, M><<<dim3(sp.blocks, N), kGnT, 0, stream>>>((const T*)x, (const T*)res, (const T*)dy,      \
+                                                                     (T*)dres, weight, bias, wdtype, st, HW, C, G,  \
+                                                                     sp, cpart, gpart)
+  GN_TYPES(GN_BSTATS, 0)
+#undef GN_BSTATS
+  DROID_LAUNCH_CHECK();
+#define GN_BAPPLY(T, M, ...)                                                                                          \
+  gn_bwd_apply_kernel<T, M><<<dim3(sp.blocks, N + (dweight || dbias ? 1 : 0)), kGnT, 0, stream>>>(                    \
+      (const T*)x, (const T*)(need_res ? dres : dy), (T*)dx, weight, bias, wdtype, st, N, HW, C, G, sp, sp.blocks, \
+      cpart, gpart, dweight, dbias)
+  GN_TYPES(GN_BAPPLY, 0)
+#undef GN_BAPPLY
+  DROID_LAUNCH_CHECK();
+  return kOk;
+}
+
+}  // extern "C"

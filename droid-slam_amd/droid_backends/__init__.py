@@ -821,6 +821,105 @@ def instance_norm_act_f16(x, mode=NORM_RELU, res=None, out=None, eps=1e-5):
     return out
 
 
+NORM_SILU = 4   # group_norm_act only
+_NORM_DTYPES = {torch.float16: 0, torch.float32: 1, torch.bfloat16: 3}
+
+
+def _norm_map(fn, name, t, x=None):
+    """A channels_last (N,C,H,W) map of group_norm_act, of x's shape, type and device where x is given."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s: %s must be a torch.Tensor" % (fn, name))
+    if t.device.type != "cuda":
+        raise RuntimeError("droid_backends: %s: %s must be a HIP device tensor (no CPU path)" % (fn, name))
+    if t.dtype not in _NORM_DTYPES or t.dim() != 4 or not t.is_contiguous(memory_format=torch.channels_last):
+        raise RuntimeError("%s: %s must be a channels_last float16, bfloat16 or float32 (N,C,H,W) tensor" % (fn, name))
+    if x is not None and (t.shape != x.shape or t.dtype != x.dtype or t.device != x.device):
+        raise RuntimeError("%s: %s must match x (shape, type, device)" % (fn, name))
+
+
+def _norm_params(fn, x, num_groups, weight, bias):
+    """The ABI's type code of weight / bias; shapes and types checked."""
+    N, C, H, W = x.shape
+    if C == 0 or C > 512 or num_groups <= 0 or C % num_groups:
+        raise RuntimeError("%s: %d channels in %d groups (0 < C <= 512, C a multiple of the groups)"
+                           % (fn, C, num_groups))
+    wdt = None
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is None:
+            continue
+        if t.device != x.device or t.shape != (C,) or not t.is_contiguous():
+            raise RuntimeError("%s: %s must be a contiguous (C,) tensor on x's device" % (fn, name))
+        if t.dtype not in (torch.float32, x.dtype) or (wdt is not None and t.dtype != wdt):
+            raise RuntimeError("%s: weight and bias must both be float32 or of x's type" % fn)
+        wdt = t.dtype
+    return _NORM_DTYPES[wdt or torch.float32]
+
+
+def group_norm_act(x, num_groups, weight=None, bias=None, mode=NORM_RELU, res=None, out=None, eps=1e-5,
+                   return_stats=False):
+    """nn.GroupNorm + the encoder's activation / residual add
+    (include/droid_backends.h: droid_group_norm_act) on a channels_last
+    (N,C,H,W) tensor, fp16, bf16 or fp32, C <= 512: NORM_RELU relu(n),
+    NORM_RES_RELU relu(res + relu(n)), NORM_ADD_RELU relu(n + res), NORM_ONLY n,
+    NORM_SILU silu(n).  Statistics and arithmetic in >= 32 bits, one rounding at
+    the end.  out may be x or res.  return_stats: also the (N, groups, 2) float64
+    mean and 1/std that group_norm_act_backward takes."""
+    fn = "group_norm_act"
+    _norm_map(fn, "x", x)
+    if mode not in (NORM_RELU, NORM_RES_RELU, NORM_ADD_RELU, NORM_ONLY, NORM_SILU):
+        raise RuntimeError("%s: unknown mode %r" % (fn, mode))
+    if mode in (NORM_RES_RELU, NORM_ADD_RELU):
+        _norm_map(fn, "res", res, x)
+    else:
+        res = None
+    wdt = _norm_params(fn, x, num_groups, weight, bias)
+    if out is None:
+        out = torch.empty_like(x, memory_format=torch.channels_last)
+    else:
+        _norm_map(fn, "out", out, x)
+    N, C, H, W = x.shape
+    dt, hw, dev = _NORM_DTYPES[x.dtype], H * W, x.device
+    stats = torch.empty((N, num_groups, 2), dtype=torch.float64, device=dev) if return_stats else None
+    with torch.cuda.device(dev):
+        ws = torch.empty((lib.droid_group_norm_workspace(dt, N, hw, C, num_groups, 0),), dtype=torch.uint8, device=dev)
+        check(lib.droid_group_norm_act(dt, _ptr(x), _ptr(res), _ptr(out), _ptr(weight), _ptr(bias), wdt, _ptr(stats),
+                                       N, hw, C, num_groups, mode, eps, _ptr(ws), ws.numel(), _stream(x)), fn)
+    return (out, stats) if return_stats else out
+
+
+def group_norm_act_backward(dy, x, stats, num_groups, weight=None, bias=None, mode=NORM_RELU, res=None):
+    """Gradients of group_norm_act: (dx, dres, dweight, dbias); dres is None
+    without a residual, dweight / dbias (summed in 64 bits, in a fixed order)
+    are None where the parameter is.  stats: group_norm_act's."""
+    fn = "group_norm_act_backward"
+    _norm_map(fn, "x", x)
+    _norm_map(fn, "dy", dy, x)
+    if mode not in (NORM_RELU, NORM_RES_RELU, NORM_ADD_RELU, NORM_ONLY, NORM_SILU):
+        raise RuntimeError("%s: unknown mode %r" % (fn, mode))
+    with_res = mode in (NORM_RES_RELU, NORM_ADD_RELU)
+    if with_res:
+        _norm_map(fn, "res", res, x)
+    wdt = _norm_params(fn, x, num_groups, weight, bias)
+    N, C, H, W = x.shape
+    dt, hw, dev = _NORM_DTYPES[x.dtype], H * W, x.device
+    if (stats.dtype != torch.float64 or stats.shape != (N, num_groups, 2) or stats.device != dev
+            or not stats.is_contiguous()):
+        raise RuntimeError("%s: stats must be group_norm_act's contiguous (N, groups, 2) float64 tensor" % fn)
+    dx = torch.empty_like(x, memory_format=torch.channels_last)
+    dres = torch.empty_like(x, memory_format=torch.channels_last) if with_res else None
+    # an empty map launches nothing: its parameters' gradients are sums of nothing
+    new = torch.empty_like if x.numel() else torch.zeros_like
+    dw = new(weight) if weight is not None else None
+    db = new(bias) if bias is not None else None
+    with torch.cuda.device(dev):
+        ws = torch.empty((lib.droid_group_norm_workspace(dt, N, hw, C, num_groups, 1),), dtype=torch.uint8, device=dev)
+        check(lib.droid_group_norm_act_backward(dt, _ptr(x), _ptr(res if with_res else None), _ptr(dy), _ptr(weight),
+                                                _ptr(bias), wdt, _ptr(stats), _ptr(dx), _ptr(dres), _ptr(dw),
+                                                _ptr(db), N, hw, C, num_groups, mode, _ptr(ws), ws.numel(),
+                                                _stream(x)), fn)
+    return dx, dres, dw, db
+
+
 def projmap(poses, disps, intrinsics, ii, jj):
     """droid_kernels.cu:1463-1488 -> [coords (E,H,W,3), valid (E,H,W,1)]."""
     _check_inputs(("poses", "disps", "intrinsics", "ii", "jj"), (poses, disps, intrinsics, ii, jj))

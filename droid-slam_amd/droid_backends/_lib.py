@@ -58,6 +58,10 @@ _SIGS = {
     "droid_frame_distance": ([_p, _p, _p, _p, _p, _i, _i, _i, _f, _p, _p], _i),
     "droid_instance_norm_workspace": ([_i, _i, _i], _sz),
     "droid_instance_norm_act_f16": ([_p, _p, _p, _i, _i, _i, _i, _f, _p, _sz, _p], _i),
+    "droid_group_norm_workspace": ([_i, _i, _i, _i, _i, _i], _sz),
+    "droid_group_norm_act": ([_i, _p, _p, _p, _p, _p, _i, _p, _i, _i, _i, _i, _i, _f, _p, _sz, _p], _i),
+    "droid_group_norm_act_backward": ([_i, _p, _p, _p, _p, _p, _i, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _p, _sz,
+                                       _p], _i),
     "droid_proximity_workspace": ([_i, _i, _i], _sz),
     "droid_proximity_select": ([_p, _i, _i, _i, _i, _i, _f, _p, _p, _i, _i, _i, _p, _p, _p, _p, _sz, _p], _i),
     "droid_projmap": ([_p, _p, _p, _p, _p, _i, _i, _i, _p, _p, _p], _i),

@@ -10,10 +10,42 @@ reference runs it (the parity bridge for the tests).
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 import droid_backends
 
 DIM = 32
+
+
+class GroupNormAct(torch.autograd.Function):
+    """Group norm + activation / residual add (droid_group_norm_act and its
+    backward): statistics in 64 bits, gradients of every input."""
+
+    @staticmethod
+    def forward(ctx, x, num_groups, weight, bias, mode, res, eps):
+        y, stats = droid_backends.group_norm_act(x, num_groups, weight, bias, mode, res, eps=eps, return_stats=True)
+        ctx.save_for_backward(x, weight, bias, res, stats)
+        ctx.num_groups, ctx.mode = num_groups, mode
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, res, stats = ctx.saved_tensors
+        dy = dy.contiguous(memory_format=torch.channels_last)
+        dx, dres, dw, db = droid_backends.group_norm_act_backward(dy, x, stats, ctx.num_groups, weight, bias, ctx.mode,
+                                                                  res)
+        return dx, None, dw, db, None, dres, None
+
+
+def group_norm_act(x, num_groups, weight=None, bias=None, mode=droid_backends.NORM_RELU, res=None, eps=1e-5):
+    """droid_backends.group_norm_act under autograd: x (and res) channels_last
+    (N,C,H,W) fp16 / bf16 / fp32 on the GPU; gradients reach x, weight, bias and res."""
+    if mode not in (droid_backends.NORM_RES_RELU, droid_backends.NORM_ADD_RELU):
+        res = None
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, res)):
+        return GroupNormAct.apply(x, num_groups, weight, bias, mode, res, eps)
+    return droid_backends.group_norm_act(x, num_groups, weight, bias, mode, res, eps=eps)
 
 
 def _norm(kind, planes):

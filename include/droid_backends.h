@@ -30,6 +30,7 @@ extern "C" {
 #define DROID_F16 0
 #define DROID_F32 1
 #define DROID_F64 2
+#define DROID_BF16 3
 
 const char* droid_last_error(void);
 int droid_abi_version(void);
@@ -318,6 +319,28 @@ int droid_proximity_select(const float* d, int t0, int t1, int t, int rad, int n
 size_t droid_instance_norm_workspace(int N, int HW, int C);
 int droid_instance_norm_act_f16(const void* x, const void* res, void* out, int N, int HW, int C, int mode,
                                 float eps, void* ws, size_t ws_bytes, hipStream_t stream);
+
+/* Encoder with group norm (modules/extractor.py: norm_fn 'group'): nn.GroupNorm
+ * of an NHWC map (N, HW, C) of G groups (dtype DROID_F16 / F32 / BF16, C <= 512,
+ * any alignment of an element), fused with the activation / residual add around
+ * it: mode 0..3 as droid_instance_norm_act_f16, 4 silu(n).  weight, bias (C) of
+ * type wdtype (DROID_F32 or dtype), either may be NULL.  Statistics and
+ * arithmetic in >= 32 bits, one rounding at the end.  out may be x or res.
+ * stats: NULL, or (N, G, 2) doubles that receive mean and 1/std for the
+ * backward pass.  ws: droid_group_norm_workspace bytes (backward 0 / 1), used
+ * by this call only until its kernels end. */
+size_t droid_group_norm_workspace(int dtype, int N, int HW, int C, int G, int backward);
+int droid_group_norm_act(int dtype, const void* x, const void* res, void* out, const void* weight, const void* bias,
+                         int wdtype, void* stats, int N, int HW, int C, int G, int mode, float eps, void* ws,
+                         size_t ws_bytes, hipStream_t stream);
+/* its gradients from dy, the forward call's inputs and its stats: dx, dres
+ * (modes 1, 2), dweight and dbias (wdtype, (C), either may be NULL; summed in 64
+ * bits in a fixed order).  Maps must not overlap.  A ReLU argument within fp32
+ * rounding of zero has its sign decided in 64 bits. */
+int droid_group_norm_act_backward(int dtype, const void* x, const void* res, const void* dy, const void* weight,
+                                  const void* bias, int wdtype, const void* stats, void* dx, void* dres, void* dweight,
+                                  void* dbias, int N, int HW, int C, int G, int mode, void* ws, size_t ws_bytes,
+                                  hipStream_t stream);
 
 /* replaces projmap (src/droid.cpp:139-154, droid_kernels.cu:1463-1488)
  * -> coords (E,H,W,3), valid (E,H,W,1) */
