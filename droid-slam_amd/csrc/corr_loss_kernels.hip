@@ -1,0 +1,721 @@
+// Losses over the all-pairs correlation of feature maps, without the volume
+// (the on-demand counterpart of CorrBlock, modules/corr.py:24-38,63-71, for
+// training the features): for the edges e = (i, j) and the query pixels p of
+// frame i
+//   s_pq   = (scale / T) <f1[i][p], f2[j][q]>
+//   loss_p = T^2 (sum_k pi_k log pi_k - sum_k pi_k s_p,idx(k) + log sum_q exp s_pq)
+// with K sparse targets a row: one index, pi = 1, T = 1 (cross entropy), or a
+// teacher's top logits, pi = softmax(t / T) (distillation).  With g = d/d loss:
+//   ds_pq  = g_p T^2 (exp(s_pq - lse_p) - sum_{k: idx(k) = q} pi_k)
+//   df1[i][p] += (scale / T) sum_q ds_pq f2[j][q]
+//   df2[j][q] += (scale / T) sum_p ds_pq f1[i][p]
+// summed over the edges a frame is in.
+//
+// The products run on MFMA 32x32x16 with the streamed frame as the A operand,
+// so that a lane holds 16 streamed rows of ONE stationary row: the running
+// maximum and sum of the softmax need no lane exchange until the very end, and
+// the accumulator's layout is already the B operand's of the second product
+// (its k slots (h, j) carry row 8 (j / 4) + 4 h + j % 4 of 16; the other
+// operand comes by transposed LDS reads in the same order), so the weights ds
+// never pass through LDS.
+#include "lds_dma.hpp"
+
+#include <algorithm>
+#include <cmath>
+
+namespace droid {
+
+namespace {
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bhalf8 __attribute__((ext_vector_type(8)));
+typedef short short4_t __attribute__((vector_size(8)));
+
+constexpr int kLT = 256;       // threads: 4 waves
+constexpr int kRowsB = 128;    // stationary rows of a workgroup, 32 a wave
+constexpr int kRowsY = 64;     // streamed rows a tile
+constexpr int kMaxK = 64;      // sparse targets a row
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kNegBig = -3.0e38f;   // running maximum before the first value (finite: no inf - inf)
+
+template <typename T>
+struct Op;
+template <>
+struct Op<_Float16> {
+  typedef half8 vec8;
+  static __device__ __forceinline__ floatx16 mfma(vec8 a, vec8 b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Op<__bf16> {
+  typedef bhalf8 vec8;
+  static __device__ __forceinline__ floatx16 mfma(vec8 a, vec8 b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+
+// A streamed tile in LDS: kRowsY rows of DP values, the 16-B slot s of row r
+// stored at slot s ^ swz(r).  Rows of 256 B and more meet in the same banks, so
+// r's low two bits move the slot by four and the next two by one: 16
+// consecutive rows read at one slot (the first product) take 16 slots, and 4
+// consecutive rows read at 4 slots (the transposed reads of the second) take
+// 16 slots as well.  128-B rows: two share 256 B already.
+template <int DP>
+__device__ __forceinline__ int swz(int r) {
+  if constexpr (DP == 64) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+  return ((r & 3) << 2) | ((r >> 2) & 3);
+}
+
+// LDS-DMA of rows y0 .. y0 + kRowsY - 1 of a frame (n rows of D values, descriptor
+// rs over them); rows past n, slots past D and the rows that `skip` names land as zeros.
+template <typename T, int DP, typename Skip>
+__device__ __forceinline__ void stage_tile(rsrc_t rs, char* lds, int y0, int n, int D, int wave, int lane, Skip skip) {
+  constexpr int RB = 2 * DP, NI = kRowsY * RB / 1024 / 4;
+#pragma unroll
+  for (int q = 0; q < NI; ++q) {
+    const int o = (wave * NI + q) * 1024;
+    const int row = (o + lane * 16) / RB, sl = (o + lane * 16) % RB / 16;
+    const int s = sl ^ swz<DP>(row);
+    const bool in = y0 + row < n && s * 8 < D && !skip(q);
+    dma16(rs, lds_addr(lds) + o, in ? (unsigned)(((y0 + row) * D + s * 8) * 2) : kOob);
+  }
+}
+
+// The stationary operand: lane (r = lane & 31, h = lane >> 5) holds values
+// 16 k + 8 h .. + 7 of row x0 + r, zeros past the frame.
+template <typename T, int DP>
+__device__ __forceinline__ void load_rows(typename Op<T>::vec8 (&b)[DP / 16], const T* f, int x, int n, int D, int h) {
+#pragma unroll
+  for (int k = 0; k < DP / 16; ++k) {
+    const int d = 16 * k + 8 * h;
+    if (x < n && d < D) b[k] = *reinterpret_cast<const typename Op<T>::vec8*>(f + (long)x * D + d);
+    else b[k] = typename Op<T>::vec8{};
+  }
+}
+
+// s[row of the tile's 32-row block][stationary row] += tile . stationary^T
+template <typename T, int DP>
+__device__ __forceinline__ floatx16 block_product(const char* lds, int blk, const typename Op<T>::vec8 (&b)[DP / 16],
+                                                  int lane) {
+  const int r = 32 * blk + (lane & 31), h = lane >> 5;
+  const char* row = lds + r * 2 * DP;
+  const int x = swz<DP>(r);
+  floatx16 acc;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+#pragma unroll
+  for (int k = 0; k < DP / 16; ++k) {
+    const auto a = *reinterpret_cast<const typename Op<T>::vec8*>(row + (((2 * k + h) ^ x) << 4));
+    acc = Op<T>::mfma(a, b[k], acc);
+  }
+  return acc;
+}
+
+// workgroup -> work item: the 8 XCDs each take a contiguous share, so the
+// workgroups that stream the same frame share an L2.
+__device__ __forceinline__ int xcd_item(int bid, int items) {
+  const int per = (items + 7) / 8;
+  return (bid & 7) * per + (bid >> 3);   // >= items: nothing to do
+}
+
+struct FwdArgs {
+  const void *f1, *f2;
+  const int *e1, *e2;          // (E) frame rows
+  const int* idx;              // (E, P, K)
+  float2* part;                // (E, P, S) running maximum (log2 units) and sum
+  int E, N1, P, N2, Q, D, K, tiles, S, items;
+  float c;                     // scale / T log2(e)
+};
+
+// Per query row the maximum and the sum of 2^(c s - max) over a share of the keys.
+template <typename T, int DP>
+__global__ void __launch_bounds__(kLT) corr_lse_kernel(FwdArgs a) {
+  __shared__ __attribute__((aligned(16))) char tile[2][kRowsY * 2 * DP];
+  const int item = xcd_item(blockIdx.x, a.items);
+  if (item >= a.items) return;
+  const int s = item % a.S, pt = item / a.S % a.tiles, e = item / a.S / a.tiles;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int i = a.e1[e], j = a.e2[e];
+  if (i < 0 || i >= a.N1 || j < 0 || j >= a.N2) return;   // the row kernel answers NaN
+  const int p = pt * kRowsB + wave * 32 + (lane & 31);
+  // rows without a target need no sum; a workgroup of them does nothing
+  bool want = false;
+  if (p < a.P)
+    for (int k = 0; k < a.K; ++k) want |= a.idx[((long)e * a.P + p) * a.K + k] >= 0;
+  if (!__syncthreads_or(want)) return;
+  const T* f1 = static_cast<const T*>(a.f1) + (long)i * a.P * a.D;
+  const T* f2 = static_cast<const T*>(a.f2) + (long)j * a.Q * a.D;
+  const rsrc_t rs = make_rsrc(f2, (unsigned)a.Q * a.D * 2);
+  const int nt = (a.Q + kRowsY - 1) / kRowsY;
+  const int t0 = nt * s / a.S, t1 = nt * (s + 1) / a.S;
+  typename Op<T>::vec8 b[DP / 16];
+  load_rows<T, DP>(b, f1, p, a.P, a.D, lane >> 5);
+  auto none = [](int) { return false; };
+  stage_tile<T, DP>(rs, tile[0], t0 * kRowsY, a.Q, a.D, wave, lane, none);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  float m = kNegBig, l = 0.f;
+  for (int t = t0; t < t1; ++t) {
+    const char* cur = tile[(t - t0) & 1];
+    if (t + 1 < t1) stage_tile<T, DP>(rs, tile[(t + 1 - t0) & 1], (t + 1) * kRowsY, a.Q, a.D, wave, lane, none);
+    floatx16 sc[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) sc[k] = block_product<T, DP>(cur, k, b, lane);
+    if ((t + 1) * kRowsY > a.Q) {   // keys past the end
+      const int y = t * kRowsY + 4 * (lane >> 5);
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int q = 0; q < 16; ++q)
+          if (y + 32 * k + 8 * (q >> 2) + (q & 3) >= a.Q) sc[k][q] = -INFINITY;
+    }
+    float mx = sc[0][0];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int q = 0; q < 16; ++q) mx = fmaxf(mx, sc[k][q]);
+    const float mn = fmaxf(m, mx * a.c);
+    l *= __builtin_amdgcn_exp2f(m - mn);
+    m = mn;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int q = 0; q < 16; ++q) l += __builtin_amdgcn_exp2f(fmaf(sc[k][q], a.c, -m));
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  }
+  const float mo = __shfl_xor(m, 32, 64), lo = __shfl_xor(l, 32, 64);
+  const float mm = fmaxf(m, mo);
+  l = l * __builtin_amdgcn_exp2f(m - mm) + lo * __builtin_amdgcn_exp2f(mo - mm);
+  if (lane < 32 && p < a.P) a.part[((long)e * a.P + p) * a.S + s] = make_float2(mm, l);
+}
+
+struct RowArgs {
+  const void *f1, *f2;
+  const int *e1, *e2, *idx;
+  const float* logits;         // (E, P, K); null: cross entropy
+  const float2* part;
+  float *loss, *lse, *prob;    // (E, P), (E, P) log2 units, (E, P, K)
+  int N1, P, N2, Q, D, K, S;
+  long rows;
+  float scale, invT, T2;
+};
+
+// One query row on 16 lanes: joins the shares of its sum, takes the K target
+// logits as fp32 dot products (a row of D values is 16 lanes x 16 B) and forms
+// the loss.  Rows without a target (all negative, or logits of -inf): loss 0 and lse = +inf, which
+// makes every weight of the backward pass 0.  A target >= Q, an edge outside the
+// frames: NaN.
+template <typename T>
+__global__ void __launch_bounds__(kLT) corr_loss_row_kernel(RowArgs a) {
+  const long row = (long)blockIdx.x * (kLT / 16) + threadIdx.x / 16;
+  const int l = threadIdx.x & 15;
+  if (row >= a.rows) return;   // whole 16-lane groups
+  const int e = (int)(row / a.P);
+  const long p = row % a.P;
+  const int i = a.e1[e], j = a.e2[e];
+  const bool edge = i >= 0 && i < a.N1 && j >= 0 && j < a.N2;
+  const int* idx = a.idx + row * a.K;
+  auto sum16 = [](float v) {
+#pragma unroll
+    for (int o = 8; o; o >>= 1) v += __shfl_xor(v, o, 16);
+    return v;
+  };
+  auto max16 = [](float v) {
+#pragma unroll
+    for (int o = 8; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 16));
+    return v;
+  };
+  // the targets' weights: lane l has entries l, l + 16, ...
+  float pi[kMaxK / 16];
+  float top = -INFINITY;
+  bool used = false, bad = !edge;
+#pragma unroll
+  for (int n = 0; n < kMaxK / 16; ++n) {
+    pi[n] = -INFINITY;
+    const int k = l + 16 * n;
+    if (k < a.K) {
+      const int t = idx[k];
+      if (t >= 0) pi[n] = a.logits ? a.logits[row * a.K + k] * a.invT : 0.f;
+      used |= pi[n] != -INFINITY;          // a logit of -inf: no target either
+      bad |= t >= a.Q || pi[n] != pi[n];
+      top = fmaxf(top, pi[n]);
+    }
+  }
+  const float any = max16(used ? 1.f : 0.f), wrong = max16(bad ? 1.f : 0.f);
+  if (any == 0.f || wrong != 0.f) {
+    const bool ignored = any == 0.f;
+    if (l == 0) {
+      a.loss[row] = ignored ? 0.f : NAN;
+      a.lse[row] = ignored ? INFINITY : NAN;
+    }
+    if (a.prob)
+      for (int k = l; k < a.K; k += 16) a.prob[row * a.K + k] = 0.f;
+    return;
+  }
+  top = max16(top);
+  float tot = 0.f;
+#pragma unroll
+  for (int n = 0; n < kMaxK / 16; ++n) {
+    pi[n] = __expf(pi[n] - top);
+    if (l + 16 * n >= a.K) pi[n] = 0.f;
+    tot += pi[n];
+  }
+  tot = sum16(tot);
+  float ent = 0.f;
+#pragma unroll
+  for (int n = 0; n < kMaxK / 16; ++n) {
+    pi[n] /= tot;
+    if (pi[n] > 0.f) ent += pi[n] * logf(pi[n]);
+    if (a.prob && l + 16 * n < a.K) a.prob[row * a.K + l + 16 * n] = pi[n];
+  }
+  // the row's sum over all keys
+  float m = kNegBig;
+  for (int s = l; s < a.S; s += 16) m = fmaxf(m, a.part[row * a.S + s].x);
+  m = max16(m);
+  float sum = 0.f;
+  for (int s = l; s < a.S; s += 16) {
+    const float2 v = a.part[row * a.S + s];
+    sum += v.y * __builtin_amdgcn_exp2f(v.x - m);
+  }
+  sum = sum16(sum);
+  const float lse2 = m + log2f(sum);
+  // sum_k pi_k s_k, as one dot product with the pi-weighted sum of the target rows
+  const T* f1 = static_cast<const T*>(a.f1) + ((long)i * a.P + p) * a.D;
+  const T* f2 = static_cast<const T*>(a.f2) + (long)j * a.Q * a.D;
+  float dot = 0.f;
+  for (int k = 0; k < a.K; ++k) {
+    const int t = idx[k];
+    float w = 0.f;
+#pragma unroll
+    for (int n = 0; n < kMaxK / 16; ++n)
+      if (k / 16 == n) w = __shfl(pi[n], k & 15, 16);
+    if (t < 0 || w == 0.f) continue;
+    float v = 0.f;
+    for (int d = 8 * l; d < a.D; d += 128) {
+      const auto x = *reinterpret_cast<const typename Op<T>::vec8*>(f1 + d);
+      const auto y = *reinterpret_cast<const typename Op<T>::vec8*>(f2 + (long)t * a.D + d);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v = fmaf((float)x[q], (float)y[q], v);
+    }
+    dot = fmaf(w, v, dot);
+  }
+  dot = sum16(dot);
+  ent = sum16(ent);
+  if (l == 0) {
+    a.loss[row] = a.T2 * (ent + fmaf(lse2, kLn2, -dot * (a.scale * a.invT)));
+    a.lse[row] = lse2;
+  }
+}
+
+// Largest |g| of an edge's rows (fp16: the weights are scaled by a power of two
+// so that their largest is 2^13 .. 2^14 and the small ones stay normal numbers).
+__global__ void __launch_bounds__(kLT) corr_gmax_kernel(const float* __restrict__ g, int P, float* __restrict__ out) {
+  __shared__ float red[kLT / 64];
+  float m = 0.f;
+  for (int p = threadIdx.x; p < P; p += kLT) m = fmaxf(m, fabsf(g[(long)blockIdx.x * P + p]));
+  for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) out[blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+
+struct BwdArgs {
+  const void *f1, *f2;
+  const int *e1, *e2, *idx;
+  const float *prob, *lse, *g; // prob null: 1
+  const float* gmax;           // (E), fp16 only
+  void *d1, *d2;               // (N1, P, D), (N2, Q, D); shared: f1 and f2 are one tensor, d1 has both gradients
+  float* part;                 // (S, rows of d1 and d2, D), S > 1
+  int E, N1, P, N2, Q, D, K, shared, S, tiles1, tiles2, blocks1, items;
+  long rows1, rows;            // rows of d1 (0: not wanted), of d1 and d2
+  float c, out_scale;          // scale / T log2(e); scale T
+};
+
+// Power of two that brings gmax to [2^13, 2^14)
+__device__ __forceinline__ int g_exponent(float gmax) {
+  if (!(gmax > 0.f) || gmax > 3.0e38f) return 0;
+  int ex;
+  frexpf(gmax, &ex);
+  return max(-100, min(100, 14 - ex));
+}
+
+// The gradient of 128 rows x of one frame: over the edges in which the frame is
+// the source (x are queries, the keys stream) and the target (x are keys, the
+// queries stream), tile by tile: weights ds from the recomputed logits, then
+// acc[d][x] += sum_y tile[y][d] ds[y][x].
+template <typename T, int DP>
+__global__ void __launch_bounds__(kLT, DP <= 128 ? 2 : 1) corr_loss_bwd_kernel(BwdArgs a) {
+  typedef typename Op<T>::vec8 vec8;
+  constexpr bool kScaled = sizeof(T) == 2 && !__is_same(T, __bf16);
+  __shared__ __attribute__((aligned(16))) char tile[2][kRowsY * 2 * DP];
+  __shared__ float delta[4][kRowsY][32];   // a wave's sparse terms of the current tile; zero between tiles
+  __shared__ float rowl[2][kRowsY], rowg[2][kRowsY];
+  __shared__ int elist[kLT];
+  __shared__ float redm[4];
+  __shared__ int ecount[4];
+  const int item = xcd_item(blockIdx.x, a.items);
+  if (item >= a.items) return;
+  const bool shared_maps = a.shared;
+  const int split = item % a.S;
+  int w = item / a.S;
+  const bool second = w >= a.blocks1;                // rows of f2
+  if (second) w -= a.blocks1;
+  const int tiles = second ? a.tiles2 : a.tiles1;
+  const int n = w / tiles, x0 = w % tiles * kRowsB;
+  const int R = second ? a.Q : a.P;                  // rows of this frame
+  const T* mine = static_cast<const T*>(second ? a.f2 : a.f1) + (long)n * R * a.D;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const int x = x0 + wave * 32 + (lane & 31);
+  vec8 b[DP / 16];
+  load_rows<T, DP>(b, mine, x, R, a.D, h);
+  floatx16 acc[DP / 32];
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int q = 0; q < 16; ++q) acc[d][q] = 0.f;
+  float (&dl)[kRowsY][32] = delta[wave];
+  for (int q = lane; q < kRowsY * 32; q += 64) (&dl[0][0])[q] = 0.f;
+
+  float mul = 1.f;
+  int ex = 0;
+  if constexpr (kScaled) {
+    float gm = 0.f;
+    for (int e = tid; e < a.E; e += kLT) {
+      const bool src = !second && a.e1[e] == n, dst = (second || shared_maps) && a.e2[e] == n;
+      if (src || dst) gm = fmaxf(gm, a.gmax[e]);
+    }
+    for (int o = 32; o; o >>= 1) gm = fmaxf(gm, __shfl_xor(gm, o, 64));
+    if (lane == 0) redm[wave] = gm;
+    __syncthreads();
+    ex = g_exponent(fmaxf(fmaxf(redm[0], redm[1]), fmaxf(redm[2], redm[3])));
+    mul = ldexpf(1.f, ex);
+  }
+
+  // one streamed frame: `src`: x are this edge's queries, otherwise its keys
+  auto edge = [&](int e, bool src) {
+    const int other = src ? a.e2[e] : a.e1[e];
+    if (other < 0 || other >= (src ? a.N2 : a.N1)) return;
+    const int n_y = src ? a.Q : a.P;
+    const T* fy = static_cast<const T*>(src ? a.f2 : a.f1) + (long)other * n_y * a.D;
+    const rsrc_t rs = make_rsrc(fy, (unsigned)n_y * a.D * 2);
+    const long erow = (long)e * a.P;
+    const int nt = (n_y + kRowsY - 1) / kRowsY;
+    const int t0 = nt * split / a.S, t1 = nt * (split + 1) / a.S;
+    if (t0 == t1) return;
+    float lx = INFINITY, gx = 0.f;
+    if (src) {
+      if (x < R) {
+        lx = a.lse[erow + x];
+        gx = lx == INFINITY ? 0.f : lx == lx ? a.g[erow + x] * mul : NAN;
+      }
+      if (!__syncthreads_or(lx != INFINITY)) return;   // every row ignored: nothing here, whatever the keys hold
+    }
+    constexpr int RB = 2 * DP, NI = kRowsY * RB / 1024 / 4;
+    float fl[NI];    // target role: the staged rows' lse, +inf: an ignored query, whose features must not be read
+    auto flags = [&](int t) {
+#pragma unroll
+      for (int q = 0; q < NI; ++q) {
+        const int y = t * kRowsY + ((wave * NI + q) * 1024 + lane * 16) / RB;
+        fl[q] = !src && y < n_y ? a.lse[erow + y] : src ? 0.f : INFINITY;
+      }
+    };
+    float nl = 0.f, ng = 0.f;   // the next tile's row data, on the first 64 threads
+    auto rowdata = [&](int t) {
+      if (!src && tid < kRowsY) {
+        const int y = t * kRowsY + tid;
+        nl = y < n_y ? a.lse[erow + y] : INFINITY;
+        ng = nl == INFINITY ? 0.f : nl == nl ? a.g[erow + y] * mul : NAN;
+      }
+    };
+    auto skip = [&](int q) { return fl[q] == INFINITY; };
+    flags(t0);
+    rowdata(t0);
+    stage_tile<T, DP>(rs, tile[0], t0 * kRowsY, n_y, a.D, wave, lane, skip);
+    if (t0 + 1 < t1) flags(t0 + 1);
+    if (!src && tid < kRowsY) {
+      rowl[0][tid] = nl;
+      rowg[0][tid] = ng;
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+      const int buf = (t - t0) & 1;
+      const char* cur = tile[buf];
+      if (t + 1 < t1) {
+        stage_tile<T, DP>(rs, tile[buf ^ 1], (t + 1) * kRowsY, n_y, a.D, wave, lane, skip);
+        rowdata(t + 1);
+        if (t + 2 < t1) flags(t + 2);
+      }
+      // the wave's sparse terms of this tile: (row y, pi) of its 32 rows x
+      bool hit = false;
+      const int y0 = t * kRowsY, xw = x0 + wave * 32;
+      auto sparse = [&](bool put) {
+        if (src) {
+          const int rows = min(32, R - xw);
+          for (int q = lane; q < rows * a.K; q += 64) {
+            const int t_ = a.idx[(erow + xw) * a.K + q] - y0;
+            if (t_ >= 0 && t_ < kRowsY) {
+              hit = true;
+              const float pi = a.prob ? a.prob[(erow + xw) * a.K + q] : 1.f;
+              if (put) atomicAdd(&dl[t_][q / a.K], pi);
+              else dl[t_][q / a.K] = 0.f;
+            }
+          }
+        } else {
+          const int rows = min(kRowsY, n_y - y0);
+          for (int q = lane; q < rows * a.K; q += 64) {
+            const int t_ = a.idx[(erow + y0) * a.K + q] - xw;
+            if (t_ >= 0 && t_ < 32) {
+              hit = true;
+              const float pi = a.prob ? a.prob[(erow + y0) * a.K + q] : 1.f;
+              if (put) atomicAdd(&dl[q / a.K][t_], pi);
+              else dl[q / a.K][t_] = 0.f;
+            }
+          }
+        }
+      };
+      sparse(true);
+      const bool any = __ballot(hit) != 0;
+      vec8 ds[4];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const floatx16 sc = block_product<T, DP>(cur, k, b, lane);
+        float wgt[16];
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+          const int y = 32 * k + 8 * (q >> 2) + 4 * h + (q & 3);
+          const float le = src ? lx : rowl[buf][y], gg = src ? gx : rowg[buf][y];
+          // clamped to [0, 1]: a NaN logit of an ignored row counts as 0
+          float pr = __builtin_amdgcn_fmed3f(__builtin_amdgcn_exp2f(fmaf(sc[q], a.c, -le)), 0.f, 1.f);
+          if (any) pr -= dl[y][lane & 31];
+          wgt[q] = gg * pr;
+        }
+#pragma unroll
+        for (int q = 0; q < 16; ++q) ds[2 * k + (q >> 3)][q & 7] = (T)wgt[q];
+      }
+      if (any) sparse(false);
+      // second product: rows d of the transposed tile
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) {
+          short4_t r4[2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            // as the address lane 4 q + p of its 16-lane group: row q, values 4 p .. + 3
+            const int row = 16 * k + 8 * u + 4 * h + ((lane & 15) >> 2);
+            const int col = 32 * d + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+            const char* at = cur + row * RB + (((col >> 3) ^ swz<DP>(row)) << 4) + (col & 7) * 2;
+            r4[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) short4_t*)(uintptr_t)lds_addr(at));
+          }
+          struct { short4_t lo, hi; } both = {r4[0], r4[1]};
+          acc[d] = Op<T>::mfma(__builtin_bit_cast(vec8, both), ds[k], acc[d]);
+        }
+      }
+      if (t + 1 < t1 && !src && tid < kRowsY) {
+        rowl[buf ^ 1][tid] = nl;
+        rowg[buf ^ 1][tid] = ng;
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+    }
+  };
+
+  for (int role = 0; role < 2; ++role) {
+    const bool src = role == 0;
+    if (src ? second : !(second || shared_maps)) continue;
+    const int* mine_e = src ? a.e1 : a.e2;
+    for (int e0 = 0; e0 < a.E; e0 += kLT) {
+      // the chunk's edges at this frame, in order
+      const bool in = e0 + tid < a.E && mine_e[e0 + tid] == n;
+      const unsigned long long bal = __ballot(in);
+      if (lane == 0) ecount[wave] = __popcll(bal);
+      __syncthreads();
+      int at = __popcll(bal & ((1ull << lane) - 1));
+      for (int q = 0; q < wave; ++q) at += ecount[q];
+      if (in) elist[at] = e0 + tid;
+      const int cnt = ecount[0] + ecount[1] + ecount[2] + ecount[3];
+      __syncthreads();
+      for (int q = 0; q < cnt; ++q) edge(__builtin_amdgcn_readfirstlane(elist[q]), src);
+      __syncthreads();
+    }
+  }
+
+  if (x >= R) return;
+  const float out = a.out_scale * (kScaled ? ldexpf(1.f, -ex) : 1.f);
+  const long first = second ? a.rows1 : 0;
+  const long row = (long)n * R + x;
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int c = 32 * d + 8 * q + 4 * h;
+      if (c >= a.D) continue;
+      float v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = acc[d][4 * q + u] * out;
+      if (a.S > 1) {
+        *reinterpret_cast<float4*>(a.part + ((long)split * a.rows + first + row) * a.D + c) =
+            make_float4(v[0], v[1], v[2], v[3]);
+      } else {
+        T* dst = static_cast<T*>(second ? a.d2 : a.d1) + row * a.D + c;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) dst[u] = (T)v[u];
+      }
+    }
+}
+
+// dfmap = the sum of the S shares, in order
+template <typename T>
+__global__ void __launch_bounds__(kLT) corr_loss_join_kernel(const float* __restrict__ part, T* __restrict__ d1,
+                                                             T* __restrict__ d2, long n1, long all, int S) {
+  const long at = ((long)blockIdx.x * kLT + threadIdx.x) * 4;
+  if (at >= all) return;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = 0; s < S; ++s) {
+    const float4 p = *reinterpret_cast<const float4*>(part + s * all + at);
+    v.x += p.x;
+    v.y += p.y;
+    v.z += p.z;
+    v.w += p.w;
+  }
+  T* dst = at < n1 ? d1 + at : d2 + (at - n1);
+  dst[0] = (T)v.x;
+  dst[1] = (T)v.y;
+  dst[2] = (T)v.z;
+  dst[3] = (T)v.w;
+}
+
+// Shares of the streamed axis: enough workgroups for the 256 CUs, no more shares than tiles.
+int fwd_split(int E, int P, int Q) {
+  const long blocks = (long)E * ceil_div(P, kRowsB);
+  return (int)std::max<long>(1, std::min<long>(ceil_div(Q, kRowsY), 1024 / std::max<long>(1, blocks)));
+}
+int bwd_split(long blocks, int P, int Q) {
+  return (int)std::max<long>(1, std::min<long>(ceil_div(std::max(P, Q), kRowsY), 1024 / std::max<long>(1, blocks)));
+}
+
+int corr_loss_check(const std::string& w, int dtype, int E, int N1, int P, int N2, int Q, int D, int K, float scale,
+                    float T) {
+  if (dtype != 0 && dtype != 3) return fail(kInvalidArgument, w + ": features must be float16 or bfloat16");
+  if (E < 0 || N1 < 0 || N2 < 0 || P < 0 || Q <= 0 || D <= 0 || D % 8 || D > 256 || K < 1 || K > kMaxK)
+    return fail(kInvalidArgument, w + ": bad arguments (Q > 0, 0 < D <= 256, D % 8 == 0, 1 <= K <= 64)");
+  if (!(scale > 0.f) || !std::isfinite(scale) || !(T > 0.f) || !std::isfinite(T))
+    return fail(kInvalidArgument, w + ": scale and temperature must be positive and finite");
+  if ((long)std::max(P, Q) * D * 2 > 0x7fffffffL || (long)E * std::max(1, ceil_div(P, kRowsB)) > 0x3fffffL ||
+      (long)(N1 + (long)N2) * ceil_div(std::max(P, Q), kRowsB) > 0x3fffffL)
+    return fail(kUnsupported, w + ": maps too large");
+  return kOk;
+}
+
+size_t gmax_bytes(int E) { return ((size_t)E * sizeof(float) + 15) / 16 * 16; }
+
+bool unaligned(const void* p) { return reinterpret_cast<uintptr_t>(p) & 15; }
+
+}  // namespace
+
+}  // namespace droid
+
+using namespace droid;
+
+#define CORR_DIMS(T, LAUNCH) \
+  if (D <= 64) { LAUNCH(T, 64); } else if (D <= 128) { LAUNCH(T, 128); } else { LAUNCH(T, 256); }
+#define CORR_TYPES(LAUNCH) \
+  if (dtype == 0) { CORR_DIMS(_Float16, LAUNCH) } else { CORR_DIMS(__bf16, LAUNCH) }
+
+extern "C" {
+
+size_t droid_corr_loss_workspace(int E, int N1, int P, int N2, int Q, int D, int backward) {
+  if (E <= 0 || N1 < 0 || P <= 0 || N2 < 0 || Q <= 0 || D <= 0) return 0;
+  if (!backward) return (size_t)E * P * fwd_split(E, P, Q) * sizeof(float2);
+  const long blocks = (long)N1 * ceil_div(P, kRowsB) + (long)N2 * ceil_div(Q, kRowsB);
+  const int S = bwd_split(blocks, P, Q);
+  const size_t rows = (size_t)N1 * P + (size_t)N2 * Q;
+  return gmax_bytes(E) + (S > 1 ? S * rows * D * sizeof(float) : 0);
+}
+
+int droid_corr_loss_forward(int dtype, const void* fmap1, const void* fmap2, const int* f1, const int* f2,
+                            const int* idx, const float* logits, float* loss, float* lse, float* prob, int E, int N1,
+                            int P, int N2, int Q, int D, int K, float scale, float temperature, void* ws,
+                            size_t ws_bytes, hipStream_t stream) {
+  const std::string what = "corr_loss_forward";
+  if (const int st = corr_loss_check(what, dtype, E, N1, P, N2, Q, D, K, scale, temperature)) return st;
+  if (E == 0 || P == 0) return kOk;
+  if (!fmap1 || !fmap2 || !f1 || !f2 || !idx || !loss || !lse || (logits && !prob))
+    return fail(kInvalidArgument, what + ": null tensor");
+  if (!logits && K != 1) return fail(kInvalidArgument, what + ": one target a row without logits");
+  if (unaligned(fmap1) || unaligned(fmap2)) return fail(kInvalidArgument, what + ": features must be 16-B aligned");
+  if (!ws || ws_bytes < droid_corr_loss_workspace(E, N1, P, N2, Q, D, 0))
+    return fail(kInvalidArgument, what + ": workspace too small");
+  FwdArgs a{fmap1, fmap2, f1, f2, idx, static_cast<float2*>(ws), E, N1, P, N2, Q, D, K, ceil_div(P, kRowsB),
+            fwd_split(E, P, Q), 0, scale / temperature * kLog2e};
+  a.items = E * a.tiles * a.S;
+#define LSE(T, DP) corr_lse_kernel<T, DP><<<(a.items + 7) / 8 * 8, kLT, 0, stream>>>(a)
+  CORR_TYPES(LSE)
+#undef LSE
+  DROID_LAUNCH_CHECK();
+  RowArgs r{fmap1, fmap2, f1, f2, idx, logits, a.part, loss, lse, logits ? prob : nullptr, N1, P, N2, Q, D, K, a.S,
+            (long)E * P, scale, 1.f / temperature, temperature * temperature};
+  const int grid = (int)((r.rows + kLT / 16 - 1) / (kLT / 16));
+  if (dtype == 0) corr_loss_row_kernel<_Float16><<<grid, kLT, 0, stream>>>(r);
+  else corr_loss_row_kernel<__bf16><<<grid, kLT, 0, stream>>>(r);
+  DROID_LAUNCH_CHECK();
+  return kOk;
+}
+
+int droid_corr_loss_backward(int dtype, const void* fmap1, const void* fmap2, const int* f1, const int* f2,
+                             const int* idx, const float* prob, const float* lse, const float* gloss, void* dfmap1,
+                             void* dfmap2, int shared, int E, int N1, int P, int N2, int Q, int D, int K, float scale,
+                             float temperature, void* ws, size_t ws_bytes, hipStream_t stream) {
+  const std::string what = "corr_loss_backward";
+  if (const int st = corr_loss_check(what, dtype, E, N1, P, N2, Q, D, K, scale, temperature)) return st;
+  if (E == 0 || P == 0) return fail(kInvalidArgument, what + ": no edges or no queries");
+  if (!fmap1 || !fmap2 || !f1 || !f2 || !idx || !lse || !gloss || (!dfmap1 && !dfmap2))
+    return fail(kInvalidArgument, what + ": null tensor");
+  if (!prob && K != 1) return fail(kInvalidArgument, what + ": one target a row without weights");
+  if (shared && (fmap1 != fmap2 || N1 != N2 || P != Q || dfmap2))
+    return fail(kInvalidArgument, what + ": one shared feature tensor has one gradient");
+  if (unaligned(fmap1) || unaligned(fmap2)) return fail(kInvalidArgument, what + ": features must be 16-B aligned");
+  // the gradients that are wanted; a shared tensor's rows are counted once
+  const int n1 = dfmap1 ? N1 : 0, n2 = dfmap2 ? N2 : 0;
+  if (!ws || ws_bytes < droid_corr_loss_workspace(E, n1, P, n2, Q, D, 1))
+    return fail(kInvalidArgument, what + ": workspace too small");
+  float* gmax = static_cast<float*>(ws);
+  float* part = reinterpret_cast<float*>(static_cast<char*>(ws) + gmax_bytes(E));
+  BwdArgs a{};
+  a.f1 = fmap1, a.f2 = fmap2, a.e1 = f1, a.e2 = f2, a.idx = idx, a.prob = prob, a.lse = lse, a.g = gloss;
+  a.gmax = gmax, a.d1 = dfmap1, a.d2 = dfmap2, a.part = part;
+  a.E = E, a.N1 = N1, a.P = P, a.N2 = N2, a.Q = Q, a.D = D, a.K = K, a.shared = shared != 0;
+  a.tiles1 = ceil_div(P, kRowsB), a.tiles2 = ceil_div(Q, kRowsB);
+  a.blocks1 = n1 * a.tiles1;
+  a.rows1 = (long)n1 * P, a.rows = a.rows1 + (long)n2 * Q;
+  a.c = scale / temperature * kLog2e, a.out_scale = scale * temperature;
+  const long blocks = a.blocks1 + (long)n2 * a.tiles2;
+  a.S = bwd_split(blocks, P, Q);
+  a.items = (int)(blocks * a.S);
+  if (a.items == 0) return kOk;
+  if (dtype == 0) {
+    corr_gmax_kernel<<<E, kLT, 0, stream>>>(gloss, P, gmax);
+    DROID_LAUNCH_CHECK();
+  }
+#define BWD(T, DP) corr_loss_bwd_kernel<T, DP><<<(a.items + 7) / 8 * 8, kLT, 0, stream>>>(a)
+  CORR_TYPES(BWD)
+#undef BWD
+  DROID_LAUNCH_CHECK();
+  if (a.S > 1) {
+    const long v1 = a.rows1 * D, all = a.rows * D;
+    const int grid = (int)((all / 4 + kLT - 1) / kLT);
+    if (dtype == 0)
+      corr_loss_join_kernel<_Float16><<<grid, kLT, 0, stream>>>(part, (_Float16*)dfmap1, (_Float16*)dfmap2, v1, all, a.S);
+    else
+      corr_loss_join_kernel<__bf16><<<grid, kLT, 0, stream>>>(part, (__bf16*)dfmap1, (__bf16*)dfmap2, v1, all, a.S);
+    DROID_LAUNCH_CHECK();
+  }
+  return kOk;
+}
+
+}  // extern "C"

@@ -281,6 +281,103 @@ def corr_alt_ce0(pyramid, f1, f2, coords, w, bias, out=None, order=None):
     return out
 
 
+_LOSS_DTYPES = {torch.float16: 0, torch.bfloat16: 3}
+
+
+def _corr_loss_check(fn, fmap1, fmap2, f1, f2, idx, K):
+    """Shapes and types shared by the two directions -> (keys' tensor, N1, P, N2, Q, D, E)."""
+    shared = fmap2 is None
+    keys = fmap1 if shared else fmap2
+    _check_inputs(("fmap1", "fmap2", "f1", "f2", "idx"), (fmap1, keys, f1, f2, idx))
+    if fmap1.dtype not in _LOSS_DTYPES or keys.dtype != fmap1.dtype:
+        raise RuntimeError("%s: features must be float16 or bfloat16, both the same" % fn)
+    _need(f1, torch.int32, "f1")
+    _need(f2, torch.int32, "f2")
+    _need(idx, torch.int32, "idx")
+    if fmap1.dim() < 3 or keys.dim() < 3 or keys.shape[-1] != fmap1.shape[-1]:
+        raise RuntimeError("%s: features must be (frames, rows..., D), of one D" % fn)
+    D, N1, N2, E = fmap1.shape[-1], fmap1.shape[0], keys.shape[0], f1.numel()
+    if D == 0 or D % 8 or D > 256:
+        raise RuntimeError("%s: D = %d (a multiple of 8 up to 256)" % (fn, D))
+    P, Q = fmap1.shape[1:-1].numel(), keys.shape[1:-1].numel()
+    if f1.dim() != 1 or f2.shape != f1.shape:
+        raise RuntimeError("%s: f1 and f2 must have one entry per edge" % fn)
+    rows = (E,) + tuple(fmap1.shape[1:-1])
+    if tuple(idx.shape) != rows + (() if K is None else (K,)):
+        raise RuntimeError("%s: indices %s do not match the edges' query rows %s" % (fn, tuple(idx.shape), rows))
+    return keys, N1, P, N2, Q, D, E
+
+
+def corr_loss_forward(fmap1, fmap2, f1, f2, idx, logits=None, scale=1.0 / 16, temperature=1.0):
+    """Softmax cross entropy / distillation over the all-pairs correlation,
+    volume-free (include/droid_backends.h: droid_corr_loss_forward).  fmap1
+    (N1, rows..., D) queries, fmap2 (N2, rows..., D) keys (None: fmap1), fp16 or
+    bf16; f1/f2 (E) int32 frame rows of the edges.  idx int32: (E, query rows...)
+    one target key a row, or with float32 logits (E, query rows..., K) K of them;
+    negative = none.  -> loss (E, query rows...) float32, lse, prob: the saved
+    tensors of corr_loss_backward."""
+    fn = "corr_loss_forward"
+    K = None if logits is None else idx.shape[-1]
+    keys, N1, P, N2, Q, D, E = _corr_loss_check(fn, fmap1, fmap2, f1, f2, idx, K)
+    prob = None
+    if logits is not None:
+        _check_inputs(("fmap1", "logits"), (fmap1, logits))
+        _need(logits, torch.float32, "logits")
+        if logits.shape != idx.shape or not 1 <= K <= 64:
+            raise RuntimeError("%s: logits must match idx, 1 <= K <= 64" % fn)
+        prob = torch.empty_like(logits)
+    dev = fmap1.device
+    rows = idx.shape if logits is None else idx.shape[:-1]
+    loss = torch.empty(rows, dtype=torch.float32, device=dev)
+    lse = torch.empty(rows, dtype=torch.float32, device=dev)
+    if loss.numel() == 0:
+        return loss, lse, prob
+    with torch.cuda.device(dev):
+        ws = torch.empty((lib.droid_corr_loss_workspace(E, N1, P, N2, Q, D, 0),), dtype=torch.uint8, device=dev)
+        check(lib.droid_corr_loss_forward(_LOSS_DTYPES[fmap1.dtype], _ptr(fmap1), _ptr(keys), _ptr(f1), _ptr(f2),
+                                          _ptr(idx), _ptr(logits), _ptr(loss), _ptr(lse), _ptr(prob), E, N1, P, N2, Q,
+                                          D, K or 1, scale, temperature, _ptr(ws), ws.numel(), _stream(fmap1)), fn)
+    return loss, lse, prob
+
+
+def corr_loss_backward(gloss, fmap1, fmap2, f1, f2, idx, lse, prob=None, scale=1.0 / 16, temperature=1.0,
+                       need1=True, need2=True):
+    """Gradients of corr_loss_forward -> (dfmap1, dfmap2).  fmap2 None: the
+    features are both queries and keys and dfmap1 has the sum of both roles.
+    need1 / need2: compute only the gradients that are used (None otherwise)."""
+    fn = "corr_loss_backward"
+    K = None if prob is None else idx.shape[-1]
+    keys, N1, P, N2, Q, D, E = _corr_loss_check(fn, fmap1, fmap2, f1, f2, idx, K)
+    shared = fmap2 is None
+    rows = idx.shape if prob is None else idx.shape[:-1]
+    _check_inputs(("fmap1", "gloss", "lse"), (fmap1, gloss, lse))
+    _need(gloss, torch.float32, "gloss")
+    _need(lse, torch.float32, "lse")
+    if gloss.shape != rows or lse.shape != rows:
+        raise RuntimeError("%s: gloss and lse must have one value per query row" % fn)
+    if prob is not None:
+        _check_inputs(("fmap1", "prob"), (fmap1, prob))
+        _need(prob, torch.float32, "prob")
+        if prob.shape != idx.shape:
+            raise RuntimeError("%s: prob must match idx" % fn)
+    need1, need2 = need1 or shared and need2, need2 and not shared
+    if not (need1 or need2):
+        return None, None
+    new = torch.zeros_like if gloss.numel() == 0 else torch.empty_like
+    d1, d2 = new(fmap1) if need1 else None, new(keys) if need2 else None
+    if gloss.numel() == 0:
+        return d1, d2
+    dev = fmap1.device
+    with torch.cuda.device(dev):
+        ws = torch.empty((lib.droid_corr_loss_workspace(E, N1 if need1 else 0, P, N2 if need2 else 0, Q, D, 1),),
+                         dtype=torch.uint8, device=dev)
+        check(lib.droid_corr_loss_backward(_LOSS_DTYPES[fmap1.dtype], _ptr(fmap1), _ptr(keys), _ptr(f1), _ptr(f2),
+                                           _ptr(idx), _ptr(prob), _ptr(lse), _ptr(gloss), _ptr(d1), _ptr(d2),
+                                           int(shared), E, N1, P, N2, Q, D, K or 1, scale, temperature, _ptr(ws),
+                                           ws.numel(), _stream(fmap1)), fn)
+    return d1, d2
+
+
 BA_ORDERS = ("identity", "rcm", "mindeg", "nd")
 
 

@@ -13,7 +13,8 @@ _ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 if _ROOT not in sys.path:
     sys.path.insert(0, _ROOT)
 
-from .corr import AltCorrBlock, CorrBlock  # noqa: E402,F401
+from .corr import (AltCorrBlock, CorrBlock, bilinear_targets, corr_cross_entropy,  # noqa: E402,F401
+                   corr_distillation, nearest_targets)
 from .update import ConvGRU, GraphAgg, UpdateModule  # noqa: E402,F401
 from .depth_video import DepthVideo  # noqa: E402,F401
 from .factor_graph import FactorGraph  # noqa: E402,F401

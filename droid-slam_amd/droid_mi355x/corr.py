@@ -13,6 +13,7 @@ the lookup uses the per-level CorrSampler so the backward kernel runs
 import numpy as np
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 import droid_backends
 
@@ -32,6 +33,84 @@ class CorrSampler(torch.autograd.Function):
         volume, coords = ctx.saved_tensors
         grad_volume, = droid_backends.corr_index_backward(volume, coords, grad_output.contiguous(), ctx.radius)
         return grad_volume, None, None
+
+
+class CorrLoss(torch.autograd.Function):
+    """droid_backends.corr_loss_forward / _backward: gradients of both feature tensors."""
+
+    @staticmethod
+    def forward(ctx, fmap1, fmap2, f1, f2, idx, logits, scale, temperature):
+        loss, lse, prob = droid_backends.corr_loss_forward(fmap1, fmap2, f1, f2, idx, logits, scale, temperature)
+        ctx.save_for_backward(fmap1, fmap2, f1, f2, idx, lse, prob)
+        ctx.scale, ctx.temperature = scale, temperature
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        fmap1, fmap2, f1, f2, idx, lse, prob = ctx.saved_tensors
+        d1, d2 = droid_backends.corr_loss_backward(g.contiguous(), fmap1, fmap2, f1, f2, idx, lse, prob, ctx.scale,
+                                                   ctx.temperature, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        return d1, d2, None, None, None, None, None, None
+
+
+def _corr_loss(fmap1, fmap2, f1, f2, idx, logits, scale, temperature):
+    if torch.is_grad_enabled() and (fmap1.requires_grad or (fmap2 is not None and fmap2.requires_grad)):
+        return CorrLoss.apply(fmap1, fmap2, f1, f2, idx, logits, scale, temperature)
+    return droid_backends.corr_loss_forward(fmap1, fmap2, f1, f2, idx, logits, scale, temperature)[0]
+
+
+def corr_cross_entropy(fmap1, fmap2, f1, f2, target, scale=1.0 / 16):
+    """Cross entropy of the softmax over CorrBlock's all-pairs correlation
+    (corr.py:63-71: <f1, f2> / 16), the volume never formed: for edge e and query
+    row p, -log softmax_q(scale <fmap1[f1[e]][p], fmap2[f2[e]][q]>)[target[e, p]].
+
+    fmap1 (N1, rows..., D) queries, fmap2 (N2, rows..., D) keys or None (the same
+    features, as in a frame graph), fp16 or bf16, D a multiple of 8 up to 256;
+    f1/f2 (E) int32 frame rows; target (E, query rows...) int32 key row, negative:
+    the row is left out (loss 0).  -> loss (E, query rows...) float32, unreduced,
+    differentiable in the features."""
+    return _corr_loss(fmap1, fmap2, f1, f2, target, None, scale, 1.0)
+
+
+def corr_distillation(fmap1, fmap2, f1, f2, idx, logits, scale=1.0 / 16, temperature=1.0):
+    """T^2 KL(pi || softmax_q(scale <fmap1[p], fmap2[q]> / T)) with pi =
+    softmax(logits / T) over a teacher's K <= 64 best keys of each query row: idx
+    (E, query rows..., K) int32 (negative: an empty place), logits the same shape
+    float32 (-inf: weight 0).  Features, edges and result as corr_cross_entropy;
+    no gradient reaches the teacher's logits.  With logits = log(weight) the rows
+    of bilinear_targets give sub-pixel correspondences."""
+    return _corr_loss(fmap1, fmap2, f1, f2, idx, logits, scale, temperature)
+
+
+def nearest_targets(coords, ht, wd, valid=None):
+    """The key row of each reprojected coordinate (DepthVideo.reproject: (..., 2)
+    as (x, y)) in an (ht, wd) map: int32 (...), -1 outside the map or where valid
+    is zero - corr_cross_entropy's target."""
+    x, y = coords[..., 0].round(), coords[..., 1].round()
+    ok = (x >= 0) & (x < wd) & (y >= 0) & (y < ht)
+    if valid is not None:
+        ok = ok & (valid > 0)
+    return torch.where(ok, y * wd + x, torch.full_like(x, -1)).to(torch.int32)
+
+
+def bilinear_targets(coords, ht, wd, valid=None):
+    """The four pixels around each reprojected coordinate and the logarithms of
+    their bilinear weights, (..., 4) int32 and float32 - corr_distillation's idx
+    and logits (temperature 1).  Neighbours outside the map: -1."""
+    x0, y0 = coords[..., 0].floor(), coords[..., 1].floor()
+    fx, fy = coords[..., 0] - x0, coords[..., 1] - y0
+    ok = torch.isfinite(coords).all(-1)
+    if valid is not None:
+        ok = ok & (valid > 0)
+    idx, w = [], []
+    for dy, wy in ((0, 1 - fy), (1, fy)):
+        for dx, wx in ((0, 1 - fx), (1, fx)):
+            x, y = x0 + dx, y0 + dy
+            inside = ok & (x >= 0) & (x < wd) & (y >= 0) & (y < ht)
+            idx.append(torch.where(inside, y * wd + x, torch.full_like(x, -1)).to(torch.int32))
+            w.append(torch.where(inside, wx * wy, torch.zeros_like(wx)))
+    return torch.stack(idx, -1), torch.stack(w, -1).float().log()
 
 
 def _avg_pool2(x, max_elems=1 << 30):

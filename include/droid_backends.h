@@ -137,6 +137,34 @@ int droid_corr_alt_ce0_ordered(const void* const* pyr, const int* Hl, const int*
                                const int* order, const float* coords, const void* w, const float* bias, void* out,
                                int E, int H, int W, hipStream_t stream);
 
+/* Losses over the all-pairs correlation of features, volume-free (the training
+ * counterpart of CorrBlock, modules/corr.py:24-38,63-71).  fmap1 (N1,P,D) queries,
+ * fmap2 (N2,Q,D) keys, DROID_F16 or DROID_BF16, 16-B aligned, D % 8 == 0, D <= 256;
+ * edges f1/f2 (E) int32 frame rows; idx (E,P,K) int32 target keys, negative = none
+ * (K <= 64).  With s_pq = scale / T <fmap1[f1[e]][p], fmap2[f2[e]][q]>:
+ *   logits NULL, K = 1: softmax cross entropy, loss[e][p] = T^2 (log sum_q e^s_pq - s_p,idx);
+ *   logits (E,P,K) f32: pi = softmax(logits / T) over the row's targets,
+ *   loss[e][p] = T^2 KL(pi || softmax_q(s_pq))          (f32).
+ * A row without a target: loss 0, no gradient, its query features unread by the
+ * sums.  A target >= Q, an edge outside the frames: loss NaN.
+ * Outputs for the backward pass: lse (E,P) f32 (log2 units; +inf: no target), prob
+ * (E,P,K) f32 (with logits only).
+ * ws: droid_corr_loss_workspace bytes (backward: with N1 / N2 = 0 for a gradient
+ * that is not wanted, N2 = 0 for shared features), used until the kernels end. */
+size_t droid_corr_loss_workspace(int E, int N1, int P, int N2, int Q, int D, int backward);
+int droid_corr_loss_forward(int dtype, const void* fmap1, const void* fmap2, const int* f1, const int* f2,
+                            const int* idx, const float* logits, float* loss, float* lse, float* prob, int E, int N1,
+                            int P, int N2, int Q, int D, int K, float scale, float temperature, void* ws,
+                            size_t ws_bytes, hipStream_t stream);
+/* gloss (E,P) f32 -> dfmap1 (N1,P,D), dfmap2 (N2,Q,D) of the features' type, each
+ * element written once (either may be NULL); shared != 0: fmap1 == fmap2 and dfmap1
+ * receives the sum of both roles (dfmap2 NULL).  No atomics on global memory: the
+ * result does not depend on the schedule. */
+int droid_corr_loss_backward(int dtype, const void* fmap1, const void* fmap2, const int* f1, const int* f2,
+                             const int* idx, const float* prob, const float* lse, const float* gloss, void* dfmap1,
+                             void* dfmap2, int shared, int E, int N1, int P, int N2, int Q, int D, int K, float scale,
+                             float temperature, void* ws, size_t ws_bytes, hipStream_t stream);
+
 /* ---- update operator ----------------------------------------------------
  * Implicit-GEMM convolution on MFMA (UpdateModule / ConvGRU convs,
  * droid_net.py:78-143, modules/gru.py:19-32), NHWC fp16 in, fp32 accumulate.
