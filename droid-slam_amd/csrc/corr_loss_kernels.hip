@@ -22,6 +22,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstddef>
 
 namespace droid {
 
@@ -78,7 +79,7 @@ __device__ __forceinline__ void stage_tile(rsrc_t rs, char* lds, int y0, int n, 
     const int o = (wave * NI + q) * 1024;
     const int row = (o + lane * 16) / RB, sl = (o + lane * 16) % RB / 16;
     const int s = sl ^ swz<DP>(row);
-    const bool in = y0 + row < n && s * 8 < D && !skip(q);
+    const bool in = y0 + row < n && s * 8 < D && !skip(row);
     dma16(rs, lds_addr(lds) + o, in ? (unsigned)(((y0 + row) * D + s * 8) * 2) : kOob);
   }
 }
@@ -95,22 +96,33 @@ __device__ __forceinline__ void load_rows(typename Op<T>::vec8 (&b)[DP / 16], co
   }
 }
 
-// s[row of the tile's 32-row block][stationary row] += tile . stationary^T
+// LDS byte address of lane (r = lane & 31, h)'s first 16 B of tile row r; its
+// k-th pair of slots is at the address XOR (k << 5) (rows are aligned to their
+// size), 32 rows further at + 32 rows.
+template <int DP>
+__device__ __forceinline__ unsigned row_addr(unsigned tile, int lane) {
+  const int r = lane & 31, h = lane >> 5;
+  return tile + r * 2 * DP + ((h ^ swz<DP>(r)) << 4);
+}
+
+// s[row of the tile's 32-row block][stationary row] = tile . stationary^T
 template <typename T, int DP>
-__device__ __forceinline__ floatx16 block_product(const char* lds, int blk, const typename Op<T>::vec8 (&b)[DP / 16],
-                                                  int lane) {
-  const int r = 32 * blk + (lane & 31), h = lane >> 5;
-  const char* row = lds + r * 2 * DP;
-  const int x = swz<DP>(r);
+__device__ __forceinline__ floatx16 block_product(unsigned row0, int blk, const typename Op<T>::vec8 (&b)[DP / 16]) {
+  typedef const __attribute__((address_space(3))) typename Op<T>::vec8* ptr;
   floatx16 acc;
 #pragma unroll
   for (int i = 0; i < 16; ++i) acc[i] = 0.f;
 #pragma unroll
-  for (int k = 0; k < DP / 16; ++k) {
-    const auto a = *reinterpret_cast<const typename Op<T>::vec8*>(row + (((2 * k + h) ^ x) << 4));
-    acc = Op<T>::mfma(a, b[k], acc);
-  }
+  for (int k = 0; k < DP / 16; ++k)
+    acc = Op<T>::mfma(*(ptr)(uintptr_t)((row0 ^ (k << 5)) + blk * 64 * DP), b[k], acc);
   return acc;
+}
+
+// v, as a value that the compiler knows nothing of: what is computed from it is
+// computed here and not kept in registers over the loops around.
+__device__ __forceinline__ int fresh(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
 }
 
 // workgroup -> work item: the 8 XCDs each take a contiguous share, so the
@@ -132,7 +144,7 @@ struct FwdArgs {
 // Per query row the maximum and the sum of 2^(c s - max) over a share of the keys.
 template <typename T, int DP>
 __global__ void __launch_bounds__(kLT) corr_lse_kernel(FwdArgs a) {
-  __shared__ __attribute__((aligned(16))) char tile[2][kRowsY * 2 * DP];
+  __shared__ __attribute__((aligned(1024))) char tile[2][kRowsY * 2 * DP];
   const int item = xcd_item(blockIdx.x, a.items);
   if (item >= a.items) return;
   const int s = item % a.S, pt = item / a.S % a.tiles, e = item / a.S / a.tiles;
@@ -158,11 +170,11 @@ __global__ void __launch_bounds__(kLT) corr_lse_kernel(FwdArgs a) {
   __syncthreads();
   float m = kNegBig, l = 0.f;
   for (int t = t0; t < t1; ++t) {
-    const char* cur = tile[(t - t0) & 1];
+    const unsigned row0 = row_addr<DP>(lds_addr(tile[(t - t0) & 1]), lane);
     if (t + 1 < t1) stage_tile<T, DP>(rs, tile[(t + 1 - t0) & 1], (t + 1) * kRowsY, a.Q, a.D, wave, lane, none);
     floatx16 sc[2];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) sc[k] = block_product<T, DP>(cur, k, b, lane);
+    for (int k = 0; k < 2; ++k) sc[k] = block_product<T, DP>(row0, k, b);
     if ((t + 1) * kRowsY > a.Q) {   // keys past the end
       const int y = t * kRowsY + 4 * (lane >> 5);
 #pragma unroll
@@ -342,23 +354,247 @@ __device__ __forceinline__ int g_exponent(float gmax) {
   return max(-100, min(100, 14 - ex));
 }
 
-// The gradient of 128 rows x of one frame: over the edges in which the frame is
-// the source (x are queries, the keys stream) and the target (x are keys, the
-// queries stream), tile by tile: weights ds from the recomputed logits, then
+// What a workgroup of the gradient kernel keeps in LDS (dynamic: the sparse
+// entries' part depends on K).
+template <int DP>
+struct BwdShared {
+  char tile[2][kRowsY * 2 * DP];           // rows aligned to their size
+  float delta[4][kRowsY][32];              // a wave's sparse terms of the current tile; zero between tiles
+  float rowl[3][kRowsY], rowg[3][kRowsY];  // the streamed queries' lse and g, two tiles ahead
+  int elist[kLT];
+  int ecount[4];
+  float redm[4];
+  __attribute__((aligned(16))) int ent[1]; // 128 K sparse entries: a wave's rows each (SRC), two tiles (else)
+};
+template <int DP>
+size_t bwd_lds(int K) {
+  return offsetof(BwdShared<DP>, ent) + (size_t)kRowsB * K * sizeof(int);
+}
+
+// One edge e of the stationary frame: SRC: the rows x are its queries and the
+// keys stream; otherwise x are its keys and the queries stream.  Tile by tile
+// the logits are recomputed, turned into weights ds, and
 // acc[d][x] += sum_y tile[y][d] ds[y][x].
+//
+// The sparse targets of a tile (pi at (y, x)) go through a dense, wave-private
+// LDS image of the tile that is read only where one was put: the subtraction
+// happens in fp32, before the rounding (p - pi of a well-trained row is a small
+// difference).  To find them a wave compares its 32 rows' K entries (SRC, in LDS
+// for the whole edge) or the tile's 64 K (staged with the tile) with the range
+// it holds.
+template <typename T, int DP, bool SRC>
+__device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, int e, int split, int R, int x0,
+                                         float mul, const typename Op<T>::vec8 (&b)[DP / 16],
+                                         floatx16 (&acc)[DP / 32]) {
+  typedef typename Op<T>::vec8 vec8;
+  typedef int int4_t __attribute__((ext_vector_type(4)));
+  typedef int int4_u __attribute__((ext_vector_type(4), aligned(4)));
+  constexpr int RB = 2 * DP, NI = kRowsY * RB / 1024 / 4;
+  const int tid = fresh(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const int xw = x0 + wave * 32, x = xw + (lane & 31);
+  const int other = SRC ? a.e2[e] : a.e1[e];
+  if (other < 0 || other >= (SRC ? a.N2 : a.N1)) return;
+  const int n_y = SRC ? a.Q : a.P;
+  const rsrc_t rs = make_rsrc(static_cast<const T*>(SRC ? a.f2 : a.f1) + (long)other * n_y * a.D,
+                              (unsigned)n_y * a.D * 2);
+  const int nt = (n_y + kRowsY - 1) / kRowsY;
+  const int t0 = nt * split / a.S, t1 = nt * (split + 1) / a.S;
+  if (t0 == t1) return;
+  const float* lse = a.lse + (long)e * a.P;
+  const float* g = a.g + (long)e * a.P;
+  const int* idx = a.idx + (long)e * a.P * a.K;
+  const float* prob = a.prob ? a.prob + (long)e * a.P * a.K : nullptr;
+  const int K = a.K;
+  float lx = INFINITY, gx = 0.f;
+  if constexpr (SRC) {
+    if (x < R) {
+      lx = lse[x];
+      gx = lx == INFINITY ? 0.f : lx == lx ? g[x] * mul : NAN;
+    }
+    if (!__syncthreads_or(lx != INFINITY)) return;   // every row left out: nothing here, whatever the keys hold
+    for (int q = tid; q < kRowsB * K; q += kLT) sh.ent[q] = x0 + q / K < R ? idx[(long)x0 * K + q] : -1;
+  }
+  // Streamed queries: entries come one tile ahead, lse and g two: lse = +inf
+  // marks a left-out row, whose features must not be read, before it is staged.
+  float nl = 0.f, ng = 0.f;
+  int4_t ne = {-1, -1, -1, -1};
+  auto rows = [&](int t) {
+    if (!SRC && tid < kRowsY) {
+      const unsigned y = t * kRowsY + tid;
+      nl = y < (unsigned)n_y ? lse[y] : INFINITY;
+      ng = nl == INFINITY ? 0.f : nl == nl ? g[y] * mul : NAN;
+    }
+  };
+  auto put_rows = [&](int slot) {
+    if (!SRC && tid < kRowsY) {
+      sh.rowl[slot][tid] = nl;
+      sh.rowg[slot][tid] = ng;
+    }
+  };
+  auto piece = [&](int t, int q) -> int4_t {   // entries 4 q .. + 3 of tile t
+    const unsigned at = t * kRowsY * K + 4 * q;
+    const int left = n_y * K - (int)at;
+    int4_t v = {-1, -1, -1, -1};
+    if (left >= 4) v = *reinterpret_cast<const int4_u*>(idx + at);
+    else if (left > 0) {
+      v.x = idx[at];
+      if (left > 1) v.y = idx[at + 1];
+      if (left > 2) v.z = idx[at + 2];
+    }
+    return v;
+  };
+  auto entries = [&](int t) {
+    if (!SRC && tid < 16 * K) ne = piece(t, tid);   // K <= 16: all of them
+  };
+  auto put_entries = [&](int t, int buf) {
+    if constexpr (!SRC) {
+      int4_t* to = reinterpret_cast<int4_t*>(sh.ent + buf * kRowsY * K);
+      if (tid < 16 * K) to[tid] = ne;
+      for (int q = tid + kLT; q < 16 * K; q += kLT) to[q] = piece(t, q);
+    }
+  };
+  int slot = 0;   // of tile t's row data
+  auto stage = [&](int t, int buf, int sl) {
+    stage_tile<T, DP>(rs, sh.tile[buf], t * kRowsY, n_y, a.D, wave, lane,
+                      [&](int row) { return !SRC && sh.rowl[sl][row] == INFINITY; });
+  };
+  entries(t0);
+  put_entries(t0, 0);
+  rows(t0);
+  put_rows(0);
+  if (t0 + 1 < t1) rows(t0 + 1);
+  put_rows(1);
+  if constexpr (!SRC) __syncthreads();
+  stage(t0, 0, 0);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  for (int t = t0; t < t1; ++t) {
+    const int buf = (t - t0) & 1, next = slot == 2 ? 0 : slot + 1, after = next == 2 ? 0 : next + 1;
+    const unsigned cur = lds_addr(sh.tile[buf]), row0 = row_addr<DP>(cur, fresh(lane));
+    if (t + 1 < t1) {
+      stage(t + 1, buf ^ 1, next);
+      entries(t + 1);
+      if (t + 2 < t1) rows(t + 2);
+    }
+    // this tile's sparse terms
+    const int base = SRC ? t * kRowsY : xw, n4 = SRC ? 8 * K : 16 * K;
+    constexpr unsigned span = SRC ? kRowsY : 32;
+    const int4_t* ent = reinterpret_cast<const int4_t*>(sh.ent + (SRC ? wave * 32 * K : buf * kRowsY * K));
+    bool hit = false;
+    for (int q = lane; q < n4; q += 64) {
+      const int4_t v = ent[q] - base;
+      hit |= (unsigned)v.x < span || (unsigned)v.y < span || (unsigned)v.z < span || (unsigned)v.w < span;
+    }
+    const bool any = __ballot(hit) != 0;
+    float (&dl)[kRowsY][32] = sh.delta[wave];
+    auto sparse = [&](bool put) {
+      for (int q = lane; q < 4 * n4; q += 64) {
+        const int v = reinterpret_cast<const int*>(ent)[q] - base;
+        if ((unsigned)v < span) {
+          const int row = q / K;
+          float& c = SRC ? dl[v][row] : dl[row][v];
+          if (put) atomicAdd(&c, prob ? prob[(long)(SRC ? xw : t * kRowsY) * K + q] : 1.f);
+          else c = 0.f;
+        }
+      }
+    };
+    if (any) sparse(true);
+    vec8 ds[4];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const floatx16 sc = block_product<T, DP>(row0, k, b);
+      float pr[16], gr[16];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float4 l4, g4;
+        if constexpr (!SRC) {
+          l4 = *reinterpret_cast<const float4*>(&sh.rowl[slot][32 * k + 8 * q + 4 * h]);
+          g4 = *reinterpret_cast<const float4*>(&sh.rowg[slot][32 * k + 8 * q + 4 * h]);
+        } else {
+          l4 = make_float4(lx, lx, lx, lx);
+          g4 = make_float4(gx, gx, gx, gx);
+        }
+        const float lq[4] = {l4.x, l4.y, l4.z, l4.w}, gq[4] = {g4.x, g4.y, g4.z, g4.w};
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          // clamped to [0, 1]: a NaN logit of a left-out row counts as 0
+          pr[4 * q + u] =
+              __builtin_amdgcn_fmed3f(__builtin_amdgcn_exp2f(fmaf(sc[4 * q + u], a.c, -lq[u])), 0.f, 1.f);
+          gr[4 * q + u] = gq[u];
+        }
+      }
+      if (any) {
+        const int v = fresh(lane);
+        const float* col = &dl[4 * (v >> 5)][v & 31];
+#pragma unroll
+        for (int q = 0; q < 16; ++q) pr[q] -= col[(32 * k + 8 * (q >> 2) + (q & 3)) * 32];
+      }
+#pragma unroll
+      for (int q = 0; q < 16; ++q) ds[2 * k + (q >> 3)][q & 7] = (T)(gr[q] * pr[q]);
+    }
+    if (any) sparse(false);
+    // second product: rows d of the transposed tile.  As the address lane 4 q + p
+    // of its 16-lane group a lane points at row 16 k + 8 u + 4 h + q, values
+    // 32 d + 16 ((lane >> 4) & 1) + 4 p .. + 3; d and u move the swizzled address by
+    // an XOR, k and u by whole rows.
+    {
+      const int v = fresh(lane), q4 = ((v & 15) >> 2) + 4 * (v >> 5), s0 = 2 * ((v >> 4) & 1) + ((v >> 1) & 1);
+      const unsigned tr0 = cur + q4 * RB + ((s0 ^ swz<DP>(q4)) << 4) + (v & 1) * 8;
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          short4_t r4[2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            r4[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)(uintptr_t)(
+                (tr0 ^ (d << 6 | u << 5)) + (16 * k + 8 * u) * RB));
+          struct { short4_t lo, hi; } both = {r4[0], r4[1]};
+          acc[d] = Op<T>::mfma(__builtin_bit_cast(vec8, both), ds[k], acc[d]);
+        }
+      }
+    }
+    if (t + 1 < t1) put_entries(t + 1, buf ^ 1);
+    if (t + 2 < t1) put_rows(after);
+    slot = next;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  }
+}
+
+// The edges at frame n in one role, 256 at a time, in order.
+template <typename T, int DP, bool SRC>
+__device__ __forceinline__ void bwd_role(const BwdArgs& a, BwdShared<DP>& sh, int n, int split, int R, int x0,
+                                         float mul, const typename Op<T>::vec8 (&b)[DP / 16],
+                                         floatx16 (&acc)[DP / 32]) {
+  const int tid = fresh(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int* at_n = SRC ? a.e1 : a.e2;
+  for (int e0 = 0; e0 < a.E; e0 += kLT) {
+    const bool in = e0 + tid < a.E && at_n[e0 + tid] == n;
+    const unsigned long long bal = __ballot(in);
+    if (lane == 0) sh.ecount[wave] = __popcll(bal);
+    __syncthreads();
+    int at = __popcll(bal & ((1ull << lane) - 1));
+    for (int q = 0; q < wave; ++q) at += sh.ecount[q];
+    if (in) sh.elist[at] = e0 + tid;
+    const int cnt = __builtin_amdgcn_readfirstlane(sh.ecount[0] + sh.ecount[1] + sh.ecount[2] + sh.ecount[3]);
+    __syncthreads();
+    for (int q = 0; q < cnt; ++q)
+      bwd_edge<T, DP, SRC>(a, sh, __builtin_amdgcn_readfirstlane(sh.elist[q]), split, R, x0, mul, b, acc);
+    __syncthreads();
+  }
+}
+
+// The gradient of 128 rows x of one frame, over the edges in which the frame is
+// the source (its rows are queries) and the target (its rows are keys), summed
+// in registers and written once.
 template <typename T, int DP>
 __global__ void __launch_bounds__(kLT, DP <= 128 ? 2 : 1) corr_loss_bwd_kernel(BwdArgs a) {
-  typedef typename Op<T>::vec8 vec8;
-  constexpr bool kScaled = sizeof(T) == 2 && !__is_same(T, __bf16);
-  __shared__ __attribute__((aligned(16))) char tile[2][kRowsY * 2 * DP];
-  __shared__ float delta[4][kRowsY][32];   // a wave's sparse terms of the current tile; zero between tiles
-  __shared__ float rowl[2][kRowsY], rowg[2][kRowsY];
-  __shared__ int elist[kLT];
-  __shared__ float redm[4];
-  __shared__ int ecount[4];
+  constexpr bool kScaled = !__is_same(T, __bf16);
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  BwdShared<DP>& sh = *reinterpret_cast<BwdShared<DP>*>(lds);
   const int item = xcd_item(blockIdx.x, a.items);
   if (item >= a.items) return;
-  const bool shared_maps = a.shared;
   const int split = item % a.S;
   int w = item / a.S;
   const bool second = w >= a.blocks1;                // rows of f2
@@ -369,186 +605,37 @@ __global__ void __launch_bounds__(kLT, DP <= 128 ? 2 : 1) corr_loss_bwd_kernel(B
   const T* mine = static_cast<const T*>(second ? a.f2 : a.f1) + (long)n * R * a.D;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int x = x0 + wave * 32 + (lane & 31);
-  vec8 b[DP / 16];
+  typename Op<T>::vec8 b[DP / 16];
   load_rows<T, DP>(b, mine, x, R, a.D, h);
   floatx16 acc[DP / 32];
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
     for (int q = 0; q < 16; ++q) acc[d][q] = 0.f;
-  float (&dl)[kRowsY][32] = delta[wave];
-  for (int q = lane; q < kRowsY * 32; q += 64) (&dl[0][0])[q] = 0.f;
+  for (int q = lane; q < kRowsY * 32; q += 64) (&sh.delta[wave][0][0])[q] = 0.f;
 
+  const bool is_src = !second, is_dst = second || a.shared;
   float mul = 1.f;
   int ex = 0;
   if constexpr (kScaled) {
     float gm = 0.f;
-    for (int e = tid; e < a.E; e += kLT) {
-      const bool src = !second && a.e1[e] == n, dst = (second || shared_maps) && a.e2[e] == n;
-      if (src || dst) gm = fmaxf(gm, a.gmax[e]);
-    }
+    for (int e = tid; e < a.E; e += kLT)
+      if ((is_src && a.e1[e] == n) || (is_dst && a.e2[e] == n)) gm = fmaxf(gm, a.gmax[e]);
     for (int o = 32; o; o >>= 1) gm = fmaxf(gm, __shfl_xor(gm, o, 64));
-    if (lane == 0) redm[wave] = gm;
+    if (lane == 0) sh.redm[wave] = gm;
     __syncthreads();
-    ex = g_exponent(fmaxf(fmaxf(redm[0], redm[1]), fmaxf(redm[2], redm[3])));
+    ex = g_exponent(fmaxf(fmaxf(sh.redm[0], sh.redm[1]), fmaxf(sh.redm[2], sh.redm[3])));
     mul = ldexpf(1.f, ex);
   }
 
-  // one streamed frame: `src`: x are this edge's queries, otherwise its keys
-  auto edge = [&](int e, bool src) {
-    const int other = src ? a.e2[e] : a.e1[e];
-    if (other < 0 || other >= (src ? a.N2 : a.N1)) return;
-    const int n_y = src ? a.Q : a.P;
-    const T* fy = static_cast<const T*>(src ? a.f2 : a.f1) + (long)other * n_y * a.D;
-    const rsrc_t rs = make_rsrc(fy, (unsigned)n_y * a.D * 2);
-    const long erow = (long)e * a.P;
-    const int nt = (n_y + kRowsY - 1) / kRowsY;
-    const int t0 = nt * split / a.S, t1 = nt * (split + 1) / a.S;
-    if (t0 == t1) return;
-    float lx = INFINITY, gx = 0.f;
-    if (src) {
-      if (x < R) {
-        lx = a.lse[erow + x];
-        gx = lx == INFINITY ? 0.f : lx == lx ? a.g[erow + x] * mul : NAN;
-      }
-      if (!__syncthreads_or(lx != INFINITY)) return;   // every row ignored: nothing here, whatever the keys hold
-    }
-    constexpr int RB = 2 * DP, NI = kRowsY * RB / 1024 / 4;
-    float fl[NI];    // target role: the staged rows' lse, +inf: an ignored query, whose features must not be read
-    auto flags = [&](int t) {
-#pragma unroll
-      for (int q = 0; q < NI; ++q) {
-        const int y = t * kRowsY + ((wave * NI + q) * 1024 + lane * 16) / RB;
-        fl[q] = !src && y < n_y ? a.lse[erow + y] : src ? 0.f : INFINITY;
-      }
-    };
-    float nl = 0.f, ng = 0.f;   // the next tile's row data, on the first 64 threads
-    auto rowdata = [&](int t) {
-      if (!src && tid < kRowsY) {
-        const int y = t * kRowsY + tid;
-        nl = y < n_y ? a.lse[erow + y] : INFINITY;
-        ng = nl == INFINITY ? 0.f : nl == nl ? a.g[erow + y] * mul : NAN;
-      }
-    };
-    auto skip = [&](int q) { return fl[q] == INFINITY; };
-    flags(t0);
-    rowdata(t0);
-    stage_tile<T, DP>(rs, tile[0], t0 * kRowsY, n_y, a.D, wave, lane, skip);
-    if (t0 + 1 < t1) flags(t0 + 1);
-    if (!src && tid < kRowsY) {
-      rowl[0][tid] = nl;
-      rowg[0][tid] = ng;
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    for (int t = t0; t < t1; ++t) {
-      const int buf = (t - t0) & 1;
-      const char* cur = tile[buf];
-      if (t + 1 < t1) {
-        stage_tile<T, DP>(rs, tile[buf ^ 1], (t + 1) * kRowsY, n_y, a.D, wave, lane, skip);
-        rowdata(t + 1);
-        if (t + 2 < t1) flags(t + 2);
-      }
-      // the wave's sparse terms of this tile: (row y, pi) of its 32 rows x
-      bool hit = false;
-      const int y0 = t * kRowsY, xw = x0 + wave * 32;
-      auto sparse = [&](bool put) {
-        if (src) {
-          const int rows = min(32, R - xw);
-          for (int q = lane; q < rows * a.K; q += 64) {
-            const int t_ = a.idx[(erow + xw) * a.K + q] - y0;
-            if (t_ >= 0 && t_ < kRowsY) {
-              hit = true;
-              const float pi = a.prob ? a.prob[(erow + xw) * a.K + q] : 1.f;
-              if (put) atomicAdd(&dl[t_][q / a.K], pi);
-              else dl[t_][q / a.K] = 0.f;
-            }
-          }
-        } else {
-          const int rows = min(kRowsY, n_y - y0);
-          for (int q = lane; q < rows * a.K; q += 64) {
-            const int t_ = a.idx[(erow + y0) * a.K + q] - xw;
-            if (t_ >= 0 && t_ < 32) {
-              hit = true;
-              const float pi = a.prob ? a.prob[(erow + y0) * a.K + q] : 1.f;
-              if (put) atomicAdd(&dl[q / a.K][t_], pi);
-              else dl[q / a.K][t_] = 0.f;
-            }
-          }
-        }
-      };
-      sparse(true);
-      const bool any = __ballot(hit) != 0;
-      vec8 ds[4];
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const floatx16 sc = block_product<T, DP>(cur, k, b, lane);
-        float wgt[16];
-#pragma unroll
-        for (int q = 0; q < 16; ++q) {
-          const int y = 32 * k + 8 * (q >> 2) + 4 * h + (q & 3);
-          const float le = src ? lx : rowl[buf][y], gg = src ? gx : rowg[buf][y];
-          // clamped to [0, 1]: a NaN logit of an ignored row counts as 0
-          float pr = __builtin_amdgcn_fmed3f(__builtin_amdgcn_exp2f(fmaf(sc[q], a.c, -le)), 0.f, 1.f);
-          if (any) pr -= dl[y][lane & 31];
-          wgt[q] = gg * pr;
-        }
-#pragma unroll
-        for (int q = 0; q < 16; ++q) ds[2 * k + (q >> 3)][q & 7] = (T)wgt[q];
-      }
-      if (any) sparse(false);
-      // second product: rows d of the transposed tile
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d) {
-          short4_t r4[2];
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            // as the address lane 4 q + p of its 16-lane group: row q, values 4 p .. + 3
-            const int row = 16 * k + 8 * u + 4 * h + ((lane & 15) >> 2);
-            const int col = 32 * d + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-            const char* at = cur + row * RB + (((col >> 3) ^ swz<DP>(row)) << 4) + (col & 7) * 2;
-            r4[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) short4_t*)(uintptr_t)lds_addr(at));
-          }
-          struct { short4_t lo, hi; } both = {r4[0], r4[1]};
-          acc[d] = Op<T>::mfma(__builtin_bit_cast(vec8, both), ds[k], acc[d]);
-        }
-      }
-      if (t + 1 < t1 && !src && tid < kRowsY) {
-        rowl[buf ^ 1][tid] = nl;
-        rowg[buf ^ 1][tid] = ng;
-      }
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
-    }
-  };
-
-  for (int role = 0; role < 2; ++role) {
-    const bool src = role == 0;
-    if (src ? second : !(second || shared_maps)) continue;
-    const int* mine_e = src ? a.e1 : a.e2;
-    for (int e0 = 0; e0 < a.E; e0 += kLT) {
-      // the chunk's edges at this frame, in order
-      const bool in = e0 + tid < a.E && mine_e[e0 + tid] == n;
-      const unsigned long long bal = __ballot(in);
-      if (lane == 0) ecount[wave] = __popcll(bal);
-      __syncthreads();
-      int at = __popcll(bal & ((1ull << lane) - 1));
-      for (int q = 0; q < wave; ++q) at += ecount[q];
-      if (in) elist[at] = e0 + tid;
-      const int cnt = ecount[0] + ecount[1] + ecount[2] + ecount[3];
-      __syncthreads();
-      for (int q = 0; q < cnt; ++q) edge(__builtin_amdgcn_readfirstlane(elist[q]), src);
-      __syncthreads();
-    }
-  }
+  // the two roles one after the other: in one loop the compiler keeps both roles'
+  // values in registers and spills
+  if (is_src) bwd_role<T, DP, true>(a, sh, n, split, R, x0, mul, b, acc);
+  if (is_dst) bwd_role<T, DP, false>(a, sh, n, split, R, x0, mul, b, acc);
 
   if (x >= R) return;
   const float out = a.out_scale * (kScaled ? ldexpf(1.f, -ex) : 1.f);
-  const long first = second ? a.rows1 : 0;
-  const long row = (long)n * R + x;
+  const long row = (second ? a.rows1 : 0) + (long)n * R + x;
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
@@ -559,12 +646,12 @@ __global__ void __launch_bounds__(kLT, DP <= 128 ? 2 : 1) corr_loss_bwd_kernel(B
 #pragma unroll
       for (int u = 0; u < 4; ++u) v[u] = acc[d][4 * q + u] * out;
       if (a.S > 1) {
-        *reinterpret_cast<float4*>(a.part + ((long)split * a.rows + first + row) * a.D + c) =
+        *reinterpret_cast<float4*>(a.part + ((long)split * a.rows + row) * a.D + c) =
             make_float4(v[0], v[1], v[2], v[3]);
       } else {
-        T* dst = static_cast<T*>(second ? a.d2 : a.d1) + row * a.D + c;
-#pragma unroll
-        for (int u = 0; u < 4; ++u) dst[u] = (T)v[u];
+        typedef T t4 __attribute__((ext_vector_type(4)));
+        *reinterpret_cast<t4*>(static_cast<T*>(second ? a.d2 : a.d1) + (row - (second ? a.rows1 : 0)) * a.D + c) =
+            t4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
       }
     }
 }
@@ -606,7 +693,7 @@ int corr_loss_check(const std::string& w, int dtype, int E, int N1, int P, int N
     return fail(kInvalidArgument, w + ": bad arguments (Q > 0, 0 < D <= 256, D % 8 == 0, 1 <= K <= 64)");
   if (!(scale > 0.f) || !std::isfinite(scale) || !(T > 0.f) || !std::isfinite(T))
     return fail(kInvalidArgument, w + ": scale and temperature must be positive and finite");
-  if ((long)std::max(P, Q) * D * 2 > 0x7fffffffL || (long)E * std::max(1, ceil_div(P, kRowsB)) > 0x3fffffL ||
+  if ((long)std::max(P, Q) * D * 2 > 0x7fffffffL || (long)P * K > 0x1fffffffL || (long)E * std::max(1, ceil_div(P, kRowsB)) > 0x3fffffL ||
       (long)(N1 + (long)N2) * ceil_div(std::max(P, Q), kRowsB) > 0x3fffffL)
     return fail(kUnsupported, w + ": maps too large");
   return kOk;
@@ -702,7 +789,8 @@ int droid_corr_loss_backward(int dtype, const void* fmap1, const void* fmap2, co
     corr_gmax_kernel<<<E, kLT, 0, stream>>>(gloss, P, gmax);
     DROID_LAUNCH_CHECK();
   }
-#define BWD(T, DP) corr_loss_bwd_kernel<T, DP><<<(a.items + 7) / 8 * 8, kLT, 0, stream>>>(a)
+  const int grid = (a.items + 7) / 8 * 8;
+#define BWD(T, DP) corr_loss_bwd_kernel<T, DP><<<grid, kLT, bwd_lds<DP>(K), stream>>>(a)
   CORR_TYPES(BWD)
 #undef BWD
   DROID_LAUNCH_CHECK();
