@@ -340,9 +340,10 @@ struct BwdArgs {
   const float *prob, *lse, *g; // prob null: 1
   const float* gmax;           // (E), fp16 only
   void *d1, *d2;               // (N1, P, D), (N2, Q, D); shared: f1 and f2 are one tensor, d1 has both gradients
-  float* part;                 // (S, rows of d1 and d2, D), S > 1
-  int E, N1, P, N2, Q, D, K, shared, S, tiles1, tiles2, blocks1, items;
-  long rows1, rows;            // rows of d1 (0: not wanted), of d1 and d2
+  float *part1, *part2;        // (S1, N1 P, D), (S2, N2 Q, D) where a gradient is made of several shares
+  int E, N1, P, N2, Q, D, K, shared;
+  int S1, S2, tiles1, tiles2;  // shares of the streamed rows; 128-row tiles a frame
+  int items1, items;           // workgroups of d1 (0: not wanted), of d1 and d2
   float c, out_scale;          // scale / T log2(e); scale T
 };
 
@@ -383,7 +384,7 @@ size_t bwd_lds(int K) {
 // for the whole edge) or the tile's 64 K (staged with the tile) with the range
 // it holds.
 template <typename T, int DP, bool SRC>
-__device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, int e, int split, int R, int x0,
+__device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, int e, int split, int S, int R, int x0,
                                          float mul, const typename Op<T>::vec8 (&b)[DP / 16],
                                          floatx16 (&acc)[DP / 32]) {
   typedef typename Op<T>::vec8 vec8;
@@ -398,7 +399,7 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
   const rsrc_t rs = make_rsrc(static_cast<const T*>(SRC ? a.f2 : a.f1) + (long)other * n_y * a.D,
                               (unsigned)n_y * a.D * 2);
   const int nt = (n_y + kRowsY - 1) / kRowsY;
-  const int t0 = nt * split / a.S, t1 = nt * (split + 1) / a.S;
+  const int t0 = nt * split / S, t1 = nt * (split + 1) / S;
   if (t0 == t1) return;
   const float* lse = a.lse + (long)e * a.P;
   const float* g = a.g + (long)e * a.P;
@@ -564,7 +565,7 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
 
 // The edges at frame n in one role, 256 at a time, in order.
 template <typename T, int DP, bool SRC>
-__device__ __forceinline__ void bwd_role(const BwdArgs& a, BwdShared<DP>& sh, int n, int split, int R, int x0,
+__device__ __forceinline__ void bwd_role(const BwdArgs& a, BwdShared<DP>& sh, int n, int split, int S, int R, int x0,
                                          float mul, const typename Op<T>::vec8 (&b)[DP / 16],
                                          floatx16 (&acc)[DP / 32]) {
   const int tid = fresh(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -580,7 +581,7 @@ __device__ __forceinline__ void bwd_role(const BwdArgs& a, BwdShared<DP>& sh, in
     const int cnt = __builtin_amdgcn_readfirstlane(sh.ecount[0] + sh.ecount[1] + sh.ecount[2] + sh.ecount[3]);
     __syncthreads();
     for (int q = 0; q < cnt; ++q)
-      bwd_edge<T, DP, SRC>(a, sh, __builtin_amdgcn_readfirstlane(sh.elist[q]), split, R, x0, mul, b, acc);
+      bwd_edge<T, DP, SRC>(a, sh, __builtin_amdgcn_readfirstlane(sh.elist[q]), split, S, R, x0, mul, b, acc);
     __syncthreads();
   }
 }
@@ -595,11 +596,9 @@ __global__ void __launch_bounds__(kLT, DP <= 128 ? 2 : 1) corr_loss_bwd_kernel(B
   BwdShared<DP>& sh = *reinterpret_cast<BwdShared<DP>*>(lds);
   const int item = xcd_item(blockIdx.x, a.items);
   if (item >= a.items) return;
-  const int split = item % a.S;
-  int w = item / a.S;
-  const bool second = w >= a.blocks1;                // rows of f2
-  if (second) w -= a.blocks1;
-  const int tiles = second ? a.tiles2 : a.tiles1;
+  const bool second = item >= a.items1;              // rows of f2
+  const int S = second ? a.S2 : a.S1, split = (second ? item - a.items1 : item) % S;
+  const int w = (second ? item - a.items1 : item) / S, tiles = second ? a.tiles2 : a.tiles1;
   const int n = w / tiles, x0 = w % tiles * kRowsB;
   const int R = second ? a.Q : a.P;                  // rows of this frame
   const T* mine = static_cast<const T*>(second ? a.f2 : a.f1) + (long)n * R * a.D;
@@ -630,12 +629,12 @@ __global__ void __launch_bounds__(kLT, DP <= 128 ? 2 : 1) corr_loss_bwd_kernel(B
 
   // the two roles one after the other: in one loop the compiler keeps both roles'
   // values in registers and spills
-  if (is_src) bwd_role<T, DP, true>(a, sh, n, split, R, x0, mul, b, acc);
-  if (is_dst) bwd_role<T, DP, false>(a, sh, n, split, R, x0, mul, b, acc);
+  if (is_src) bwd_role<T, DP, true>(a, sh, n, split, S, R, x0, mul, b, acc);
+  if (is_dst) bwd_role<T, DP, false>(a, sh, n, split, S, R, x0, mul, b, acc);
 
   if (x >= R) return;
   const float out = a.out_scale * (kScaled ? ldexpf(1.f, -ex) : 1.f);
-  const long row = (second ? a.rows1 : 0) + (long)n * R + x;
+  const long row = (long)n * R + x;
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
@@ -645,12 +644,12 @@ __global__ void __launch_bounds__(kLT, DP <= 128 ? 2 : 1) corr_loss_bwd_kernel(B
       float v[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) v[u] = acc[d][4 * q + u] * out;
-      if (a.S > 1) {
-        *reinterpret_cast<float4*>(a.part + ((long)split * a.rows + row) * a.D + c) =
-            make_float4(v[0], v[1], v[2], v[3]);
+      if (S > 1) {
+        float* part = (second ? a.part2 : a.part1) + (long)split * (second ? a.N2 : a.N1) * R * a.D;
+        *reinterpret_cast<float4*>(part + row * a.D + c) = make_float4(v[0], v[1], v[2], v[3]);
       } else {
         typedef T t4 __attribute__((ext_vector_type(4)));
-        *reinterpret_cast<t4*>(static_cast<T*>(second ? a.d2 : a.d1) + (row - (second ? a.rows1 : 0)) * a.D + c) =
+        *reinterpret_cast<t4*>(static_cast<T*>(second ? a.d2 : a.d1) + row * a.D + c) =
             t4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
       }
     }
@@ -658,23 +657,20 @@ __global__ void __launch_bounds__(kLT, DP <= 128 ? 2 : 1) corr_loss_bwd_kernel(B
 
 // dfmap = the sum of the S shares, in order
 template <typename T>
-__global__ void __launch_bounds__(kLT) corr_loss_join_kernel(const float* __restrict__ part, T* __restrict__ d1,
-                                                             T* __restrict__ d2, long n1, long all, int S) {
+__global__ void __launch_bounds__(kLT) corr_loss_join_kernel(const float* __restrict__ part, T* __restrict__ d,
+                                                             long n, int S) {
   const long at = ((long)blockIdx.x * kLT + threadIdx.x) * 4;
-  if (at >= all) return;
+  if (at >= n) return;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int s = 0; s < S; ++s) {
-    const float4 p = *reinterpret_cast<const float4*>(part + s * all + at);
+    const float4 p = *reinterpret_cast<const float4*>(part + s * n + at);
     v.x += p.x;
     v.y += p.y;
     v.z += p.z;
     v.w += p.w;
   }
-  T* dst = at < n1 ? d1 + at : d2 + (at - n1);
-  dst[0] = (T)v.x;
-  dst[1] = (T)v.y;
-  dst[2] = (T)v.z;
-  dst[3] = (T)v.w;
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  *reinterpret_cast<t4*>(d + at) = t4{(T)v.x, (T)v.y, (T)v.z, (T)v.w};
 }
 
 // Shares of the streamed axis: enough workgroups for the 256 CUs, no more shares than tiles.
@@ -682,8 +678,41 @@ int fwd_split(int E, int P, int Q) {
   const long blocks = (long)E * ceil_div(P, kRowsB);
   return (int)std::max<long>(1, std::min<long>(ceil_div(Q, kRowsY), 1024 / std::max<long>(1, blocks)));
 }
-int bwd_split(long blocks, int P, int Q) {
-  return (int)std::max<long>(1, std::min<long>(ceil_div(std::max(P, Q), kRowsY), 1024 / std::max<long>(1, blocks)));
+
+// The gradient's work split.  A workgroup's time is the tiles it streams (about
+// E / N1 frames of Q / 64 tiles for a tile of f1's rows), and `slots` of them run
+// at once; more shares even out the last round but write fp32 partial sums and
+// read them back.  Takes the cheapest of the candidates in units of one tile's
+// time (measured 2 us; 10 MB of partial sums at the copy rate).
+struct BwdPlan {
+  int tiles1, tiles2, S1, S2;
+  long items1, items;
+  size_t part1, part2;   // floats
+};
+BwdPlan bwd_plan(int E, int N1, int P, int N2, int Q, int D, bool shared) {
+  BwdPlan b{};
+  b.tiles1 = ceil_div(P, kRowsB), b.tiles2 = ceil_div(Q, kRowsB);
+  const int yt1 = ceil_div(Q, kRowsY), yt2 = ceil_div(P, kRowsY);
+  const double w1 = N1 ? (double)E / N1 * yt1 * (shared ? 2 : 1) : 0, w2 = N2 ? (double)E / N2 * yt2 : 0;
+  const long n1 = (long)N1 * b.tiles1, n2 = (long)N2 * b.tiles2;
+  const int slots = D <= 128 ? 512 : 256;
+  const double per = (n1 * w1 + n2 * w2) / slots;   // tiles a slot
+  double best = INFINITY;
+  for (int r = 1; r <= 12; ++r) {
+    const double grain = std::max(4.0, per / r);
+    const int S1 = (int)std::min<double>(yt1, std::max(1.0, std::ceil(w1 / grain - 0.25)));
+    const int S2 = (int)std::min<double>(yt2, std::max(1.0, std::ceil(w2 / grain - 0.25)));
+    const long items = n1 * S1 + n2 * S2;
+    const size_t p1 = S1 > 1 ? (size_t)S1 * N1 * P * D : 0, p2 = S2 > 1 ? (size_t)S2 * N2 * Q * D : 0;
+    const double each = std::max(w1 / S1, w2 / S2) + 2.0;   // and two tiles' time to begin and end
+    const double time = (items + slots - 1) / slots * each + (p1 + p2) * 8e-7;
+    if (time < best) {
+      best = time;
+      b.S1 = S1, b.S2 = S2, b.part1 = p1, b.part2 = p2;
+      b.items1 = n1 * S1, b.items = items;
+    }
+  }
+  return b;
 }
 
 int corr_loss_check(const std::string& w, int dtype, int E, int N1, int P, int N2, int Q, int D, int K, float scale,
@@ -716,13 +745,11 @@ using namespace droid;
 
 extern "C" {
 
-size_t droid_corr_loss_workspace(int E, int N1, int P, int N2, int Q, int D, int backward) {
+size_t droid_corr_loss_workspace(int E, int N1, int P, int N2, int Q, int D, int shared, int backward) {
   if (E <= 0 || N1 < 0 || P <= 0 || N2 < 0 || Q <= 0 || D <= 0) return 0;
   if (!backward) return (size_t)E * P * fwd_split(E, P, Q) * sizeof(float2);
-  const long blocks = (long)N1 * ceil_div(P, kRowsB) + (long)N2 * ceil_div(Q, kRowsB);
-  const int S = bwd_split(blocks, P, Q);
-  const size_t rows = (size_t)N1 * P + (size_t)N2 * Q;
-  return gmax_bytes(E) + (S > 1 ? S * rows * D * sizeof(float) : 0);
+  const BwdPlan b = bwd_plan(E, N1, P, N2, Q, D, shared);
+  return gmax_bytes(E) + (b.part1 + b.part2) * sizeof(float);
 }
 
 int droid_corr_loss_forward(int dtype, const void* fmap1, const void* fmap2, const int* f1, const int* f2,
@@ -736,7 +763,7 @@ int droid_corr_loss_forward(int dtype, const void* fmap1, const void* fmap2, con
     return fail(kInvalidArgument, what + ": null tensor");
   if (!logits && K != 1) return fail(kInvalidArgument, what + ": one target a row without logits");
   if (unaligned(fmap1) || unaligned(fmap2)) return fail(kInvalidArgument, what + ": features must be 16-B aligned");
-  if (!ws || ws_bytes < droid_corr_loss_workspace(E, N1, P, N2, Q, D, 0))
+  if (!ws || ws_bytes < droid_corr_loss_workspace(E, N1, P, N2, Q, D, 0, 0))
     return fail(kInvalidArgument, what + ": workspace too small");
   FwdArgs a{fmap1, fmap2, f1, f2, idx, static_cast<float2*>(ws), E, N1, P, N2, Q, D, K, ceil_div(P, kRowsB),
             fwd_split(E, P, Q), 0, scale / temperature * kLog2e};
@@ -769,22 +796,20 @@ int droid_corr_loss_backward(int dtype, const void* fmap1, const void* fmap2, co
   if (unaligned(fmap1) || unaligned(fmap2)) return fail(kInvalidArgument, what + ": features must be 16-B aligned");
   // the gradients that are wanted; a shared tensor's rows are counted once
   const int n1 = dfmap1 ? N1 : 0, n2 = dfmap2 ? N2 : 0;
-  if (!ws || ws_bytes < droid_corr_loss_workspace(E, n1, P, n2, Q, D, 1))
+  if (!ws || ws_bytes < droid_corr_loss_workspace(E, n1, P, n2, Q, D, shared, 1))
     return fail(kInvalidArgument, what + ": workspace too small");
+  const BwdPlan b = bwd_plan(E, n1, P, n2, Q, D, shared != 0);
+  if (b.items == 0) return kOk;
+  if (b.items > 0x3fffffffL) return fail(kUnsupported, what + ": maps too large");
   float* gmax = static_cast<float*>(ws);
-  float* part = reinterpret_cast<float*>(static_cast<char*>(ws) + gmax_bytes(E));
   BwdArgs a{};
   a.f1 = fmap1, a.f2 = fmap2, a.e1 = f1, a.e2 = f2, a.idx = idx, a.prob = prob, a.lse = lse, a.g = gloss;
-  a.gmax = gmax, a.d1 = dfmap1, a.d2 = dfmap2, a.part = part;
+  a.gmax = gmax, a.d1 = dfmap1, a.d2 = dfmap2;
+  a.part1 = reinterpret_cast<float*>(static_cast<char*>(ws) + gmax_bytes(E)), a.part2 = a.part1 + b.part1;
   a.E = E, a.N1 = N1, a.P = P, a.N2 = N2, a.Q = Q, a.D = D, a.K = K, a.shared = shared != 0;
-  a.tiles1 = ceil_div(P, kRowsB), a.tiles2 = ceil_div(Q, kRowsB);
-  a.blocks1 = n1 * a.tiles1;
-  a.rows1 = (long)n1 * P, a.rows = a.rows1 + (long)n2 * Q;
+  a.S1 = b.S1, a.S2 = b.S2, a.tiles1 = b.tiles1, a.tiles2 = b.tiles2;
+  a.items1 = (int)b.items1, a.items = (int)b.items;
   a.c = scale / temperature * kLog2e, a.out_scale = scale * temperature;
-  const long blocks = a.blocks1 + (long)n2 * a.tiles2;
-  a.S = bwd_split(blocks, P, Q);
-  a.items = (int)(blocks * a.S);
-  if (a.items == 0) return kOk;
   if (dtype == 0) {
     corr_gmax_kernel<<<E, kLT, 0, stream>>>(gloss, P, gmax);
     DROID_LAUNCH_CHECK();
@@ -794,13 +819,13 @@ int droid_corr_loss_backward(int dtype, const void* fmap1, const void* fmap2, co
   CORR_TYPES(BWD)
 #undef BWD
   DROID_LAUNCH_CHECK();
-  if (a.S > 1) {
-    const long v1 = a.rows1 * D, all = a.rows * D;
-    const int grid = (int)((all / 4 + kLT - 1) / kLT);
-    if (dtype == 0)
-      corr_loss_join_kernel<_Float16><<<grid, kLT, 0, stream>>>(part, (_Float16*)dfmap1, (_Float16*)dfmap2, v1, all, a.S);
-    else
-      corr_loss_join_kernel<__bf16><<<grid, kLT, 0, stream>>>(part, (__bf16*)dfmap1, (__bf16*)dfmap2, v1, all, a.S);
+  for (int q = 0; q < 2; ++q) {
+    if (!(q ? b.part2 : b.part1)) continue;
+    const long n = q ? (long)N2 * Q * D : (long)N1 * P * D;
+    const float* part = q ? a.part2 : a.part1;
+    const int jg = (int)((n / 4 + kLT - 1) / kLT), S = q ? a.S2 : a.S1;
+    if (dtype == 0) corr_loss_join_kernel<_Float16><<<jg, kLT, 0, stream>>>(part, (_Float16*)(q ? dfmap2 : dfmap1), n, S);
+    else corr_loss_join_kernel<__bf16><<<jg, kLT, 0, stream>>>(part, (__bf16*)(q ? dfmap2 : dfmap1), n, S);
     DROID_LAUNCH_CHECK();
   }
   return kOk;
