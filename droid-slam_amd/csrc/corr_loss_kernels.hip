@@ -322,32 +322,45 @@ __global__ void __launch_bounds__(kLT) corr_loss_row_kernel(RowArgs a) {
   }
 }
 
-// Largest |g| of an edge's rows (fp16: the weights are scaled by a power of two
-// so that their largest is 2^13 .. 2^14 and the small ones stay normal numbers).
-__global__ void __launch_bounds__(kLT) corr_gmax_kernel(const float* __restrict__ g, int P, float* __restrict__ out) {
-  __shared__ float red[kLT / 64];
-  float m = 0.f;
-  for (int p = threadIdx.x; p < P; p += kLT) m = fmaxf(m, fabsf(g[(long)blockIdx.x * P + p]));
-  for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
-  __syncthreads();
-  if (threadIdx.x == 0) out[blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-}
+// ---- the gradient -----------------------------------------------------------
+//
+// A work item is 128 rows x of one frame, held in registers; its steps are the
+// 64-row tiles y of the frames that share an edge with it, streamed through LDS:
+// the logits s[y][x] are recomputed, turned into weights
+//   ds = g1[x] (p1 - pi1) + g2[y] (p2 - pi2)
+// (1: an edge in which x are the queries and y keys, 2: one in which y are the
+// queries), and acc[d][x] += sum_y tile[y][d] ds[y][x].  An edge (i, j) of one
+// feature tensor is done together with its reverse (j, i), where the graph has
+// it: both need the same logits and the same second product.
+//
+// The steps of all items, end to end, are cut into equal shares, one for each
+// workgroup that the chip holds at once; an item that a cut goes through is
+// summed from fp32 parts, in order, by the join kernel.  (Items of their own
+// workgroup each left half the chip idle in the last round: 560 items on 512
+// places took 1137 us, shares of the streamed axis by a cost model 867 us, with
+// uneven graphs up to twice their even share.)
+
+constexpr int kUnitBoth = 3, kUnitOne = 2;   // cost of a step with both directions / one (measured about 3 : 2)
+constexpr int kMinUnits = 16;                // smallest share worth a workgroup
 
 struct BwdArgs {
   const void *f1, *f2;
   const int *e1, *e2, *idx;
   const float *prob, *lse, *g; // prob null: 1
-  const float* gmax;           // (E), fp16 only
-  void *d1, *d2;               // (N1, P, D), (N2, Q, D); shared: f1 and f2 are one tensor, d1 has both gradients
-  float *part1, *part2;        // (S1, N1 P, D), (S2, N2 Q, D) where a gradient is made of several shares
+  void *d1, *d2;               // (N1, P, D), (N2, Q, D)
+  float* gmax;                 // (E) largest |g|
+  int* partner;                // (E) the reverse edge that is done together with this one, -1: none
+  long long* first;            // (V + 1) units before frame slot v; the slots: f1's frames (d1 wanted), then f2's
+  int* expo;                   // (V) fp16: exponent that scales the slot's weights
+  float* part;                 // (G, 2, 128, D)
   int E, N1, P, N2, Q, D, K, shared;
-  int S1, S2, tiles1, tiles2;  // shares of the streamed rows; 128-row tiles a frame
-  int items1, items;           // workgroups of d1 (0: not wanted), of d1 and d2
+  int tiles1, tiles2;          // 128-row tiles of a frame
+  int n1, V, G;                // slots of f1, all slots, workgroups
   float c, out_scale;          // scale / T log2(e); scale T
 };
 
-// Power of two that brings gmax to [2^13, 2^14)
+// Power of two that brings gmax to [2^13, 2^14): an fp16 weight's largest value
+// stays far from 65504 and the small ones stay normal numbers.
 __device__ __forceinline__ int g_exponent(float gmax) {
   if (!(gmax > 0.f) || gmax > 3.0e38f) return 0;
   int ex;
@@ -355,79 +368,189 @@ __device__ __forceinline__ int g_exponent(float gmax) {
   return max(-100, min(100, 14 - ex));
 }
 
+// One workgroup an edge: the largest |g| of its rows, and the reverse edge it
+// is paired with (the k-th copy of (i, j) with the k-th of (j, i)).
+__global__ void __launch_bounds__(kLT) corr_edge_kernel(BwdArgs a) {
+  __shared__ float red[kLT / 64];
+  __shared__ int cnt[kLT / 64];
+  const int e = blockIdx.x, tid = threadIdx.x, wave = tid >> 6;
+  float m = 0.f;
+  for (int p = tid; p < a.P; p += kLT) m = fmaxf(m, fabsf(a.g[(long)e * a.P + p]));
+  for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  if ((tid & 63) == 0) red[wave] = m;
+  __syncthreads();
+  if (tid == 0) {
+    a.gmax[e] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    a.partner[e] = -1;
+  }
+  if (!a.shared) return;
+  const int i = a.e1[e], j = a.e2[e];
+  int rank = 0;
+  for (int q = tid; q < e; q += kLT) rank += a.e1[q] == i && a.e2[q] == j;
+  for (int o = 32; o; o >>= 1) rank += __shfl_xor(rank, o, 64);
+  if ((tid & 63) == 0) cnt[wave] = rank;
+  __syncthreads();
+  rank = cnt[0] + cnt[1] + cnt[2] + cnt[3];
+  for (int q0 = 0; q0 < a.E; q0 += kLT) {
+    const int q = q0 + tid;
+    const bool rev = q < a.E && a.e1[q] == j && a.e2[q] == i;
+    const unsigned long long bal = __ballot(rev);
+    __syncthreads();
+    if ((tid & 63) == 0) cnt[wave] = __popcll(bal);
+    __syncthreads();
+    int at = __popcll(bal & ((1ull << (tid & 63)) - 1));
+    for (int u = 0; u < wave; ++u) at += cnt[u];
+    if (rev && at == rank) a.partner[e] = q;
+    rank -= cnt[0] + cnt[1] + cnt[2] + cnt[3];
+    if (rank < 0) break;
+  }
+}
+
+// Whether both ends of edge e are frames (otherwise it takes no part).
+__device__ __forceinline__ bool edge_in(const BwdArgs& a, int e) {
+  return (unsigned)a.e1[e] < (unsigned)a.N1 && (unsigned)a.e2[e] < (unsigned)a.N2;
+}
+__device__ __forceinline__ int y_tiles(int rows) { return (rows + kRowsY - 1) / kRowsY; }
+
+// One workgroup: the units of every frame slot's items and their running sum.
+__global__ void __launch_bounds__(1024) corr_plan_kernel(BwdArgs a) {
+  constexpr int kChunk = 1024;
+  __shared__ int both[kChunk], src[kChunk], dst[kChunk];
+  __shared__ float gm[kChunk];
+  __shared__ long long wsum[16];
+  const int tid = threadIdx.x;
+  long long base = 0;
+  for (int v0 = 0; v0 < a.V; v0 += kChunk) {
+    both[tid] = src[tid] = dst[tid] = 0;
+    gm[tid] = 0.f;
+    __syncthreads();
+    for (int e = tid; e < a.E; e += kChunk) {
+      if (!edge_in(a, e)) continue;
+      // the edge's slot as source, and as target (one tensor: both in f1's slots)
+      const int vs = a.n1 ? a.e1[e] - v0 : -1;
+      const int vd = a.shared ? a.e2[e] - v0 : a.V > a.n1 ? a.n1 + a.e2[e] - v0 : -1;
+      const bool paired = a.partner[e] >= 0;
+      if ((unsigned)vs < (unsigned)kChunk) {
+        atomicAdd(paired ? &both[vs] : &src[vs], 1);
+        atomicMax(reinterpret_cast<int*>(&gm[vs]), __float_as_int(a.gmax[e]));   // >= 0: ordered as integers
+      }
+      if ((unsigned)vd < (unsigned)kChunk) {
+        if (!paired) atomicAdd(&dst[vd], 1);   // paired: its reverse counts it
+        atomicMax(reinterpret_cast<int*>(&gm[vd]), __float_as_int(a.gmax[e]));
+      }
+    }
+    __syncthreads();
+    const int v = v0 + tid;
+    long long u = 0;
+    if (v < a.V) {
+      const bool first = v < a.n1;
+      const int tiles = first ? a.tiles1 : a.tiles2;
+      u = (long long)tiles * ((both[tid] * (long long)kUnitBoth + src[tid] * (long long)kUnitOne) * y_tiles(a.Q) +
+                              dst[tid] * (long long)kUnitOne * y_tiles(a.P));
+      a.expo[v] = g_exponent(gm[tid]);
+    }
+    // inclusive scan over the chunk
+    long long s = u;
+    for (int o = 1; o < 64; o <<= 1) {
+      const long long w = __shfl_up(s, o, 64);
+      if ((tid & 63) >= o) s += w;
+    }
+    if ((tid & 63) == 63) wsum[tid >> 6] = s;
+    __syncthreads();
+    for (int w = 0; w < (tid >> 6); ++w) s += wsum[w];
+    if (v < a.V) a.first[v + 1] = base + s;
+    if (v == 0) a.first[0] = 0;
+    long long all = 0;
+    for (int w = 0; w < 16; ++w) all += wsum[w];
+    base += all;
+    __syncthreads();
+  }
+}
+
+// Units of one workgroup's share.
+__device__ __forceinline__ long long share_units(const BwdArgs& a) {
+  return max((a.first[a.V] + a.G - 1) / a.G, (long long)kMinUnits);
+}
+// The frame slot that holds unit u (first[v] <= u < first[v + 1]).
+__device__ __forceinline__ int slot_of(const BwdArgs& a, long long u) {
+  int lo = 0, hi = a.V - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (a.first[mid + 1] > u) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo;
+}
+
 // What a workgroup of the gradient kernel keeps in LDS (dynamic: the sparse
 // entries' part depends on K).
 template <int DP>
 struct BwdShared {
   char tile[2][kRowsY * 2 * DP];           // rows aligned to their size
-  float delta[4][kRowsY][32];              // a wave's sparse terms of the current tile; zero between tiles
+  float delta[4][32][32];                  // a wave's sparse terms of half a tile; zero between uses
   float rowl[3][kRowsY], rowg[3][kRowsY];  // the streamed queries' lse and g, two tiles ahead
+  float xg[kRowsB];                        // the stationary queries' g
   int elist[kLT];
   int ecount[4];
-  float redm[4];
-  __attribute__((aligned(16))) int ent[1]; // 128 K sparse entries: a wave's rows each (SRC), two tiles (else)
+  __attribute__((aligned(16))) int ent[1]; // sparse entries: of the 128 rows x, and of two tiles (128 K each)
 };
 template <int DP>
 size_t bwd_lds(int K) {
-  return offsetof(BwdShared<DP>, ent) + (size_t)kRowsB * K * sizeof(int);
+  return offsetof(BwdShared<DP>, ent) + (size_t)2 * kRowsB * K * sizeof(int);
 }
 
-// One edge e of the stationary frame: SRC: the rows x are its queries and the
-// keys stream; otherwise x are its keys and the queries stream.  Tile by tile
-// the logits are recomputed, turned into weights ds, and
-// acc[d][x] += sum_y tile[y][d] ds[y][x].
+// The steps [t0, t1) of one edge (es: x are its queries) and / or its reverse
+// (ed: the streamed rows y are its queries).
 //
-// The sparse targets of a tile (pi at (y, x)) go through a dense, wave-private
-// LDS image of the tile that is read only where one was put: the subtraction
-// happens in fp32, before the rounding (p - pi of a well-trained row is a small
-// difference).  To find them a wave compares its 32 rows' K entries (SRC, in LDS
-// for the whole edge) or the tile's 64 K (staged with the tile) with the range
-// it holds.
-template <typename T, int DP, bool SRC>
-__device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, int e, int split, int S, int R, int x0,
-                                         float mul, const typename Op<T>::vec8 (&b)[DP / 16],
+// The sparse targets (g pi at (y, x)) go through a dense, wave-private LDS image
+// of half a tile that is read only where one was put: the subtraction happens in
+// fp32, before the rounding (p - pi of a well-trained row is a small
+// difference).  To find them a wave compares its 32 rows' K entries (in LDS for
+// the whole edge) and the tile's 64 K (staged with the tile) with the range it
+// holds.
+template <typename T, int DP, bool SRC, bool DST>
+__device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, int es, int ed, int t0, int t1, int R,
+                                         int x0, float mul, const typename Op<T>::vec8 (&b)[DP / 16],
                                          floatx16 (&acc)[DP / 32]) {
   typedef typename Op<T>::vec8 vec8;
   typedef int int4_t __attribute__((ext_vector_type(4)));
   typedef int int4_u __attribute__((ext_vector_type(4), aligned(4)));
-  constexpr int RB = 2 * DP, NI = kRowsY * RB / 1024 / 4;
+  constexpr int RB = 2 * DP;
   const int tid = fresh(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int xw = x0 + wave * 32, x = xw + (lane & 31);
-  const int other = SRC ? a.e2[e] : a.e1[e];
-  if (other < 0 || other >= (SRC ? a.N2 : a.N1)) return;
-  const int n_y = SRC ? a.Q : a.P;
-  const rsrc_t rs = make_rsrc(static_cast<const T*>(SRC ? a.f2 : a.f1) + (long)other * n_y * a.D,
+  const int n_y = SRC ? a.Q : a.P, K = a.K;
+  const rsrc_t rs = make_rsrc(static_cast<const T*>(SRC ? a.f2 : a.f1) + (long)(SRC ? a.e2[es] : a.e1[ed]) * n_y * a.D,
                               (unsigned)n_y * a.D * 2);
-  const int nt = (n_y + kRowsY - 1) / kRowsY;
-  const int t0 = nt * split / S, t1 = nt * (split + 1) / S;
-  if (t0 == t1) return;
-  const float* lse = a.lse + (long)e * a.P;
-  const float* g = a.g + (long)e * a.P;
-  const int* idx = a.idx + (long)e * a.P * a.K;
-  const float* prob = a.prob ? a.prob + (long)e * a.P * a.K : nullptr;
-  const int K = a.K;
+  const float* lse = a.lse + (long)ed * a.P;      // of the streamed queries
+  const float* g = a.g + (long)ed * a.P;
+  const int* idx = a.idx + (long)ed * a.P * K;
   float lx = INFINITY, gx = 0.f;
+  bool live = false;   // a stationary row has a target
   if constexpr (SRC) {
     if (x < R) {
-      lx = lse[x];
-      gx = lx == INFINITY ? 0.f : lx == lx ? g[x] * mul : NAN;
+      lx = a.lse[(long)es * a.P + x];
+      gx = lx == INFINITY ? 0.f : lx == lx ? a.g[(long)es * a.P + x] * mul : NAN;
     }
-    if (!__syncthreads_or(lx != INFINITY)) return;   // every row left out: nothing here, whatever the keys hold
-    for (int q = tid; q < kRowsB * K; q += kLT) sh.ent[q] = x0 + q / K < R ? idx[(long)x0 * K + q] : -1;
+    live = __syncthreads_or(lx != INFINITY);
+    if (!DST && !live) return;   // every row left out: nothing here, whatever the keys hold
+    if (lane < 32) sh.xg[wave * 32 + lane] = gx;
+    const int* xi = a.idx + ((long)es * a.P + x0) * K;
+    for (int q = tid; q < kRowsB * K; q += kLT) sh.ent[q] = x0 + q / K < R ? xi[q] : -1;
   }
   // Streamed queries: entries come one tile ahead, lse and g two: lse = +inf
-  // marks a left-out row, whose features must not be read, before it is staged.
+  // marks a left-out row, whose features must not be read (unless as live keys)
+  // before it is staged.
   float nl = 0.f, ng = 0.f;
   int4_t ne = {-1, -1, -1, -1};
   auto rows = [&](int t) {
-    if (!SRC && tid < kRowsY) {
+    if (DST && tid < kRowsY) {
       const unsigned y = t * kRowsY + tid;
       nl = y < (unsigned)n_y ? lse[y] : INFINITY;
       ng = nl == INFINITY ? 0.f : nl == nl ? g[y] * mul : NAN;
     }
   };
   auto put_rows = [&](int slot) {
-    if (!SRC && tid < kRowsY) {
+    if (DST && tid < kRowsY) {
       sh.rowl[slot][tid] = nl;
       sh.rowg[slot][tid] = ng;
     }
@@ -445,27 +568,28 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
     return v;
   };
   auto entries = [&](int t) {
-    if (!SRC && tid < 16 * K) ne = piece(t, tid);   // K <= 16: all of them
+    if (DST && tid < 16 * K) ne = piece(t, tid);   // K <= 16: all of them
   };
+  int* const yent = sh.ent + kRowsB * K;
   auto put_entries = [&](int t, int buf) {
-    if constexpr (!SRC) {
-      int4_t* to = reinterpret_cast<int4_t*>(sh.ent + buf * kRowsY * K);
+    if constexpr (DST) {
+      int4_t* to = reinterpret_cast<int4_t*>(yent + buf * kRowsY * K);
       if (tid < 16 * K) to[tid] = ne;
       for (int q = tid + kLT; q < 16 * K; q += kLT) to[q] = piece(t, q);
     }
   };
-  int slot = 0;   // of tile t's row data
   auto stage = [&](int t, int buf, int sl) {
     stage_tile<T, DP>(rs, sh.tile[buf], t * kRowsY, n_y, a.D, wave, lane,
-                      [&](int row) { return !SRC && sh.rowl[sl][row] == INFINITY; });
+                      [&](int row) { return DST && sh.rowl[sl][row] == INFINITY && !(SRC && live); });
   };
+  int slot = 0;   // of tile t's row data
   entries(t0);
   put_entries(t0, 0);
   rows(t0);
   put_rows(0);
   if (t0 + 1 < t1) rows(t0 + 1);
   put_rows(1);
-  if constexpr (!SRC) __syncthreads();
+  if constexpr (DST) __syncthreads();
   stage(t0, 0, 0);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
@@ -477,63 +601,91 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
       entries(t + 1);
       if (t + 2 < t1) rows(t + 2);
     }
-    // this tile's sparse terms
-    const int base = SRC ? t * kRowsY : xw, n4 = SRC ? 8 * K : 16 * K;
-    constexpr unsigned span = SRC ? kRowsY : 32;
-    const int4_t* ent = reinterpret_cast<const int4_t*>(sh.ent + (SRC ? wave * 32 * K : buf * kRowsY * K));
-    bool hit = false;
-    for (int q = lane; q < n4; q += 64) {
-      const int4_t v = ent[q] - base;
-      hit |= (unsigned)v.x < span || (unsigned)v.y < span || (unsigned)v.z < span || (unsigned)v.w < span;
-    }
-    const bool any = __ballot(hit) != 0;
-    float (&dl)[kRowsY][32] = sh.delta[wave];
-    auto sparse = [&](bool put) {
-      for (int q = lane; q < 4 * n4; q += 64) {
-        const int v = reinterpret_cast<const int*>(ent)[q] - base;
-        if ((unsigned)v < span) {
-          const int row = q / K;
-          float& c = SRC ? dl[v][row] : dl[row][v];
-          if (put) atomicAdd(&c, prob ? prob[(long)(SRC ? xw : t * kRowsY) * K + q] : 1.f);
-          else c = 0.f;
+    // which halves of the tile hold a sparse term of the wave's rows
+    bool hit[2] = {false, false};
+    const int4_t* xent = reinterpret_cast<const int4_t*>(sh.ent + wave * 32 * K);
+    const int4_t* tent = reinterpret_cast<const int4_t*>(yent + buf * kRowsY * K);
+    if constexpr (SRC)
+      for (int q = lane; q < 8 * K; q += 64) {
+        const int4_t v = xent[q] - t * kRowsY;
+        hit[0] |= (unsigned)v.x < 32u || (unsigned)v.y < 32u || (unsigned)v.z < 32u || (unsigned)v.w < 32u;
+        hit[1] |= (unsigned)v.x - 32u < 32u || (unsigned)v.y - 32u < 32u || (unsigned)v.z - 32u < 32u ||
+                  (unsigned)v.w - 32u < 32u;
+      }
+    if constexpr (DST)
+      for (int q = lane; q < 16 * K; q += 64) {
+        const int4_t v = tent[q] - xw;
+        // (a row's entries may lie in both halves of 64 K: decided by the row below)
+        const bool in = (unsigned)v.x < 32u || (unsigned)v.y < 32u || (unsigned)v.z < 32u || (unsigned)v.w < 32u;
+        hit[0] |= in && q < 8 * K;
+        hit[1] |= in && q >= 8 * K;
+      }
+    float (&dl)[32][32] = sh.delta[wave];
+    auto sparse = [&](int k, bool put) {
+      if constexpr (SRC) {
+        const int* ent = reinterpret_cast<const int*>(xent);
+        for (int q = lane; q < 32 * K; q += 64) {
+          const int v = ent[q] - t * kRowsY - 32 * k;
+          if ((unsigned)v < 32u) {
+            const int row = q / K;
+            if (put) atomicAdd(&dl[v][row], sh.xg[wave * 32 + row] *
+                                                (a.prob ? a.prob[((long)es * a.P + xw) * K + q] : 1.f));
+            else dl[v][row] = 0.f;
+          }
+        }
+      }
+      if constexpr (DST) {
+        const int* ent = reinterpret_cast<const int*>(tent) + 32 * K * k;
+        for (int q = lane; q < 32 * K; q += 64) {
+          const int v = ent[q] - xw;
+          if ((unsigned)v < 32u) {
+            const int row = q / K;
+            if (put)
+              atomicAdd(&dl[row][v], sh.rowg[slot][32 * k + row] *
+                                         (a.prob ? a.prob[((long)ed * a.P + t * kRowsY + 32 * k) * K + q] : 1.f));
+            else dl[row][v] = 0.f;
+          }
         }
       }
     };
-    if (any) sparse(true);
     vec8 ds[4];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
+      const bool any = __ballot(hit[k]) != 0;
+      if (any) sparse(k, true);
       const floatx16 sc = block_product<T, DP>(row0, k, b);
-      float pr[16], gr[16];
+      float wg[16];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        float4 l4, g4;
-        if constexpr (!SRC) {
-          l4 = *reinterpret_cast<const float4*>(&sh.rowl[slot][32 * k + 8 * q + 4 * h]);
-          g4 = *reinterpret_cast<const float4*>(&sh.rowg[slot][32 * k + 8 * q + 4 * h]);
-        } else {
-          l4 = make_float4(lx, lx, lx, lx);
-          g4 = make_float4(gx, gx, gx, gx);
+        float lq[4], gq[4];
+        if constexpr (DST) {
+          const float4 l4 = *reinterpret_cast<const float4*>(&sh.rowl[slot][32 * k + 8 * q + 4 * h]);
+          const float4 g4 = *reinterpret_cast<const float4*>(&sh.rowg[slot][32 * k + 8 * q + 4 * h]);
+          lq[0] = l4.x, lq[1] = l4.y, lq[2] = l4.z, lq[3] = l4.w;
+          gq[0] = g4.x, gq[1] = g4.y, gq[2] = g4.z, gq[3] = g4.w;
         }
-        const float lq[4] = {l4.x, l4.y, l4.z, l4.w}, gq[4] = {g4.x, g4.y, g4.z, g4.w};
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          // clamped to [0, 1]: a NaN logit of a left-out row counts as 0
-          pr[4 * q + u] =
-              __builtin_amdgcn_fmed3f(__builtin_amdgcn_exp2f(fmaf(sc[4 * q + u], a.c, -lq[u])), 0.f, 1.f);
-          gr[4 * q + u] = gq[u];
+          // p clamped to [0, 1]: a NaN logit of a left-out row counts as 0
+          const float s = sc[4 * q + u];
+          float w = 0.f;
+          if constexpr (SRC)
+            w = gx * __builtin_amdgcn_fmed3f(__builtin_amdgcn_exp2f(fmaf(s, a.c, -lx)), 0.f, 1.f);
+          if constexpr (DST)
+            w = fmaf(gq[u], __builtin_amdgcn_fmed3f(__builtin_amdgcn_exp2f(fmaf(s, a.c, -lq[u])), 0.f, 1.f), w);
+          wg[4 * q + u] = w;
         }
       }
       if (any) {
         const int v = fresh(lane);
         const float* col = &dl[4 * (v >> 5)][v & 31];
 #pragma unroll
-        for (int q = 0; q < 16; ++q) pr[q] -= col[(32 * k + 8 * (q >> 2) + (q & 3)) * 32];
+        for (int q = 0; q < 16; ++q) wg[q] -= col[(8 * (q >> 2) + (q & 3)) * 32];
+        sparse(k, false);
       }
 #pragma unroll
-      for (int q = 0; q < 16; ++q) ds[2 * k + (q >> 3)][q & 7] = (T)(gr[q] * pr[q]);
+      for (int q = 0; q < 16; ++q) ds[2 * k + (q >> 3)][q & 7] = (T)wg[q];
     }
-    if (any) sparse(false);
     // second product: rows d of the transposed tile.  As the address lane 4 q + p
     // of its 16-lane group a lane points at row 16 k + 8 u + 4 h + q, values
     // 32 d + 16 ((lane >> 4) & 1) + 4 p .. + 3; d and u move the swizzled address by
@@ -563,114 +715,132 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
   }
 }
 
-// The edges at frame n in one role, 256 at a time, in order.
-template <typename T, int DP, bool SRC>
-__device__ __forceinline__ void bwd_role(const BwdArgs& a, BwdShared<DP>& sh, int n, int split, int S, int R, int x0,
-                                         float mul, const typename Op<T>::vec8 (&b)[DP / 16],
-                                         floatx16 (&acc)[DP / 32]) {
+// The edges of one kind at frame n, 256 at a time, in order; `at`: units of the
+// item before this kind's first edge (moved past its last), [u0, u1) the units
+// that are done here.
+template <typename T, int DP, bool SRC, bool DST>
+__device__ __forceinline__ void bwd_kind(const BwdArgs& a, BwdShared<DP>& sh, int n, long long& at, long long u0,
+                                         long long u1, int R, int x0, float mul,
+                                         const typename Op<T>::vec8 (&b)[DP / 16], floatx16 (&acc)[DP / 32]) {
   const int tid = fresh(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int* at_n = SRC ? a.e1 : a.e2;
-  for (int e0 = 0; e0 < a.E; e0 += kLT) {
-    const bool in = e0 + tid < a.E && at_n[e0 + tid] == n;
+  constexpr int unit = SRC && DST ? kUnitBoth : kUnitOne;
+  const int nt = y_tiles(SRC ? a.Q : a.P);
+  for (int e0 = 0; e0 < a.E && at < u1; e0 += kLT) {
+    const int e = e0 + tid;
+    bool in = e < a.E && (SRC ? a.e1 : a.e2)[e] == n;
+    if (in) in = edge_in(a, e) && (SRC && DST) == (a.partner[e] >= 0);
     const unsigned long long bal = __ballot(in);
     if (lane == 0) sh.ecount[wave] = __popcll(bal);
     __syncthreads();
-    int at = __popcll(bal & ((1ull << lane) - 1));
-    for (int q = 0; q < wave; ++q) at += sh.ecount[q];
-    if (in) sh.elist[at] = e0 + tid;
+    int pos = __popcll(bal & ((1ull << lane) - 1));
+    for (int q = 0; q < wave; ++q) pos += sh.ecount[q];
+    if (in) sh.elist[pos] = e;
     const int cnt = __builtin_amdgcn_readfirstlane(sh.ecount[0] + sh.ecount[1] + sh.ecount[2] + sh.ecount[3]);
     __syncthreads();
-    for (int q = 0; q < cnt; ++q)
-      bwd_edge<T, DP, SRC>(a, sh, __builtin_amdgcn_readfirstlane(sh.elist[q]), split, S, R, x0, mul, b, acc);
+    for (int q = 0; q < cnt && at < u1; ++q, at += (long long)nt * unit) {
+      // a step is done by the share that its first unit lies in
+      const int t0 = (int)max(0ll, (u0 - at + unit - 1) / unit), t1 = (int)min((long long)nt, (u1 - at + unit - 1) / unit);
+      if (t0 >= t1) continue;
+      const int eq = __builtin_amdgcn_readfirstlane(sh.elist[q]);
+      const int er = SRC && DST ? __builtin_amdgcn_readfirstlane(a.partner[eq]) : eq;
+      bwd_edge<T, DP, SRC, DST>(a, sh, eq, er, t0, t1, R, x0, mul, b, acc);
+    }
     __syncthreads();
   }
 }
 
-// The gradient of 128 rows x of one frame, over the edges in which the frame is
-// the source (its rows are queries) and the target (its rows are keys), summed
-// in registers and written once.
+// One workgroup: its share of the units, item by item.
 template <typename T, int DP>
 __global__ void __launch_bounds__(kLT, DP <= 128 ? 2 : 1) corr_loss_bwd_kernel(BwdArgs a) {
   constexpr bool kScaled = !__is_same(T, __bf16);
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   BwdShared<DP>& sh = *reinterpret_cast<BwdShared<DP>*>(lds);
-  const int item = xcd_item(blockIdx.x, a.items);
-  if (item >= a.items) return;
-  const bool second = item >= a.items1;              // rows of f2
-  const int S = second ? a.S2 : a.S1, split = (second ? item - a.items1 : item) % S;
-  const int w = (second ? item - a.items1 : item) / S, tiles = second ? a.tiles2 : a.tiles1;
-  const int n = w / tiles, x0 = w % tiles * kRowsB;
-  const int R = second ? a.Q : a.P;                  // rows of this frame
-  const T* mine = static_cast<const T*>(second ? a.f2 : a.f1) + (long)n * R * a.D;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-  const int x = x0 + wave * 32 + (lane & 31);
-  typename Op<T>::vec8 b[DP / 16];
-  load_rows<T, DP>(b, mine, x, R, a.D, h);
-  floatx16 acc[DP / 32];
+  const int block = xcd_item(blockIdx.x, a.G);
+  if (block >= a.G) return;
+  const long long share = share_units(a), all = a.first[a.V];
+  long long u = block * share;
+  const long long end = min(u + share, all);
+  for (int q = lane; q < 32 * 32; q += 64) (&sh.delta[wave][0][0])[q] = 0.f;
+  while (u < end) {
+    const int v = slot_of(a, u);
+    const bool second = v >= a.n1;
+    const int n = second ? v - a.n1 : v, tiles = second ? a.tiles2 : a.tiles1, R = second ? a.Q : a.P;
+    const long long per = (a.first[v + 1] - a.first[v]) / tiles;   // units of each of the frame's items
+    const int w = (int)((u - a.first[v]) / per), x0 = w * kRowsB;
+    const long long item = a.first[v] + w * per;
+    const long long u0 = u - item, u1 = min(per, end - item);
+    const int x = x0 + wave * 32 + (lane & 31);
+    typename Op<T>::vec8 b[DP / 16];
+    load_rows<T, DP>(b, static_cast<const T*>(second ? a.f2 : a.f1) + (long)n * R * a.D, x, R, a.D, h);
+    floatx16 acc[DP / 32];
 #pragma unroll
-  for (int d = 0; d < DP / 32; ++d)
+    for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-    for (int q = 0; q < 16; ++q) acc[d][q] = 0.f;
-  for (int q = lane; q < kRowsY * 32; q += 64) (&sh.delta[wave][0][0])[q] = 0.f;
+      for (int q = 0; q < 16; ++q) acc[d][q] = 0.f;
+    const int ex = kScaled ? a.expo[v] : 0;
+    const float mul = kScaled ? ldexpf(1.f, ex) : 1.f;
+    // the kinds one after the other: in one loop the compiler keeps the values of
+    // all of them in registers and spills
+    long long at = 0;
+    if (a.shared) bwd_kind<T, DP, true, true>(a, sh, n, at, u0, u1, R, x0, mul, b, acc);
+    if (!second) bwd_kind<T, DP, true, false>(a, sh, n, at, u0, u1, R, x0, mul, b, acc);
+    if (second || a.shared) bwd_kind<T, DP, false, true>(a, sh, n, at, u0, u1, R, x0, mul, b, acc);
 
-  const bool is_src = !second, is_dst = second || a.shared;
-  float mul = 1.f;
-  int ex = 0;
-  if constexpr (kScaled) {
-    float gm = 0.f;
-    for (int e = tid; e < a.E; e += kLT)
-      if ((is_src && a.e1[e] == n) || (is_dst && a.e2[e] == n)) gm = fmaxf(gm, a.gmax[e]);
-    for (int o = 32; o; o >>= 1) gm = fmaxf(gm, __shfl_xor(gm, o, 64));
-    if (lane == 0) sh.redm[wave] = gm;
-    __syncthreads();
-    ex = g_exponent(fmaxf(fmaxf(sh.redm[0], sh.redm[1]), fmaxf(sh.redm[2], sh.redm[3])));
-    mul = ldexpf(1.f, ex);
-  }
-
-  // the two roles one after the other: in one loop the compiler keeps both roles'
-  // values in registers and spills
-  if (is_src) bwd_role<T, DP, true>(a, sh, n, split, S, R, x0, mul, b, acc);
-  if (is_dst) bwd_role<T, DP, false>(a, sh, n, split, S, R, x0, mul, b, acc);
-
-  if (x >= R) return;
-  const float out = a.out_scale * (kScaled ? ldexpf(1.f, -ex) : 1.f);
-  const long row = (long)n * R + x;
+    const float out = a.out_scale * (kScaled ? ldexpf(1.f, -ex) : 1.f);
+    const bool whole = u0 == 0 && u1 == per;
+    const int xi = fresh(x);
+    if (xi < R) {
 #pragma unroll
-  for (int d = 0; d < DP / 32; ++d)
+      for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int c = 32 * d + 8 * q + 4 * h;
-      if (c >= a.D) continue;
-      float v[4];
+        for (int q = 0; q < 4; ++q) {
+          const int c = 32 * d + 8 * q + 4 * h;
+          if (c >= a.D) continue;
+          float o[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) v[u] = acc[d][4 * q + u] * out;
-      if (S > 1) {
-        float* part = (second ? a.part2 : a.part1) + (long)split * (second ? a.N2 : a.N1) * R * a.D;
-        *reinterpret_cast<float4*>(part + row * a.D + c) = make_float4(v[0], v[1], v[2], v[3]);
-      } else {
-        typedef T t4 __attribute__((ext_vector_type(4)));
-        *reinterpret_cast<t4*>(static_cast<T*>(second ? a.d2 : a.d1) + row * a.D + c) =
-            t4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
-      }
+          for (int k = 0; k < 4; ++k) o[k] = acc[d][4 * q + k] * out;
+          if (whole) {
+            typedef T t4 __attribute__((ext_vector_type(4)));
+            *reinterpret_cast<t4*>(static_cast<T*>(second ? a.d2 : a.d1) + ((long)n * R + xi) * a.D + c) =
+                t4{(T)o[0], (T)o[1], (T)o[2], (T)o[3]};
+          } else {
+            float* p = a.part + ((long)(2 * block + (u0 == 0)) * kRowsB + (xi - x0)) * a.D + c;
+            *reinterpret_cast<float4*>(p) = make_float4(o[0], o[1], o[2], o[3]);
+          }
+        }
     }
+    u = item + u1;
+  }
 }
 
-// dfmap = the sum of the S shares, in order
+// One workgroup an item: adds up, in order, the parts of one that several
+// shares have worked on; zeros where no edge reaches the frame.
 template <typename T>
-__global__ void __launch_bounds__(kLT) corr_loss_join_kernel(const float* __restrict__ part, T* __restrict__ d,
-                                                             long n, int S) {
-  const long at = ((long)blockIdx.x * kLT + threadIdx.x) * 4;
-  if (at >= n) return;
-  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s = 0; s < S; ++s) {
-    const float4 p = *reinterpret_cast<const float4*>(part + s * n + at);
-    v.x += p.x;
-    v.y += p.y;
-    v.z += p.z;
-    v.w += p.w;
+__global__ void __launch_bounds__(kLT) corr_loss_join_kernel(BwdArgs a) {
+  const int items1 = a.n1 * a.tiles1;
+  const bool second = (int)blockIdx.x >= items1;
+  const int w = second ? blockIdx.x - items1 : blockIdx.x, tiles = second ? a.tiles2 : a.tiles1;
+  const int n = w / tiles, x0 = w % tiles * kRowsB, R = second ? a.Q : a.P, v = second ? a.n1 + n : n;
+  const long long per = (a.first[v + 1] - a.first[v]) / tiles, item = a.first[v] + w % tiles * per;
+  const long long share = share_units(a);
+  const int b0 = (int)(item / share), b1 = per ? (int)((item + per - 1) / share) : b0;
+  if (per && b0 == b1) return;
+  T* d = static_cast<T*>(second ? a.d2 : a.d1) + ((long)n * R + x0) * a.D;
+  const int total = min(kRowsB, R - x0) * a.D;
+  for (int q = threadIdx.x * 4; q < total; q += kLT * 4) {
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (per)
+      for (int b = b0; b <= b1; ++b) {
+        const float4 p = *reinterpret_cast<const float4*>(a.part + (long)(2 * b + (b == b0)) * kRowsB * a.D + q);
+        s.x += p.x;
+        s.y += p.y;
+        s.z += p.z;
+        s.w += p.w;
+      }
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<t4*>(d + q) = t4{(T)s.x, (T)s.y, (T)s.z, (T)s.w};
   }
-  typedef T t4 __attribute__((ext_vector_type(4)));
-  *reinterpret_cast<t4*>(d + at) = t4{(T)v.x, (T)v.y, (T)v.z, (T)v.w};
 }
 
 // Shares of the streamed axis: enough workgroups for the 256 CUs, no more shares than tiles.
@@ -679,40 +849,23 @@ int fwd_split(int E, int P, int Q) {
   return (int)std::max<long>(1, std::min<long>(ceil_div(Q, kRowsY), 1024 / std::max<long>(1, blocks)));
 }
 
-// The gradient's work split.  A workgroup's time is the tiles it streams (about
-// E / N1 frames of Q / 64 tiles for a tile of f1's rows), and `slots` of them run
-// at once; more shares even out the last round but write fp32 partial sums and
-// read them back.  Takes the cheapest of the candidates in units of one tile's
-// time (measured 2 us; 10 MB of partial sums at the copy rate).
-struct BwdPlan {
-  int tiles1, tiles2, S1, S2;
-  long items1, items;
-  size_t part1, part2;   // floats
+// Workgroups of the gradient kernel: as many as run at once - two a CU while
+// both fit its LDS (K <= 16 at D <= 128).
+int bwd_groups(int D, int K) { return device_cu_count() * (D <= 128 && K <= 16 ? 2 : 1); }
+
+// The gradient's workspace, in bytes from its start.
+struct BwdSpace {
+  size_t gmax, partner, first, expo, part, bytes;
 };
-BwdPlan bwd_plan(int E, int N1, int P, int N2, int Q, int D, bool shared) {
-  BwdPlan b{};
-  b.tiles1 = ceil_div(P, kRowsB), b.tiles2 = ceil_div(Q, kRowsB);
-  const int yt1 = ceil_div(Q, kRowsY), yt2 = ceil_div(P, kRowsY);
-  const double w1 = N1 ? (double)E / N1 * yt1 * (shared ? 2 : 1) : 0, w2 = N2 ? (double)E / N2 * yt2 : 0;
-  const long n1 = (long)N1 * b.tiles1, n2 = (long)N2 * b.tiles2;
-  const int slots = D <= 128 ? 512 : 256;
-  const double per = (n1 * w1 + n2 * w2) / slots;   // tiles a slot
-  double best = INFINITY;
-  for (int r = 1; r <= 12; ++r) {
-    const double grain = std::max(4.0, per / r);
-    const int S1 = (int)std::min<double>(yt1, std::max(1.0, std::ceil(w1 / grain - 0.25)));
-    const int S2 = (int)std::min<double>(yt2, std::max(1.0, std::ceil(w2 / grain - 0.25)));
-    const long items = n1 * S1 + n2 * S2;
-    const size_t p1 = S1 > 1 ? (size_t)S1 * N1 * P * D : 0, p2 = S2 > 1 ? (size_t)S2 * N2 * Q * D : 0;
-    const double each = std::max(w1 / S1, w2 / S2) + 2.0;   // and two tiles' time to begin and end
-    const double time = (items + slots - 1) / slots * each + (p1 + p2) * 8e-7;
-    if (time < best) {
-      best = time;
-      b.S1 = S1, b.S2 = S2, b.part1 = p1, b.part2 = p2;
-      b.items1 = n1 * S1, b.items = items;
-    }
-  }
-  return b;
+BwdSpace bwd_space(int E, int V, int D) {
+  auto up = [](size_t n) { return (n + 15) / 16 * 16; };
+  BwdSpace s{};
+  s.partner = s.gmax + up((size_t)E * 4);
+  s.first = s.partner + up((size_t)E * 4);
+  s.expo = s.first + up(((size_t)V + 1) * 8);
+  s.part = s.expo + up((size_t)V * 4);
+  s.bytes = s.part + (size_t)2 * bwd_groups(D, 1) * kRowsB * D * 4;
+  return s;
 }
 
 int corr_loss_check(const std::string& w, int dtype, int E, int N1, int P, int N2, int Q, int D, int K, float scale,
@@ -727,8 +880,6 @@ int corr_loss_check(const std::string& w, int dtype, int E, int N1, int P, int N
     return fail(kUnsupported, w + ": maps too large");
   return kOk;
 }
-
-size_t gmax_bytes(int E) { return ((size_t)E * sizeof(float) + 15) / 16 * 16; }
 
 bool unaligned(const void* p) { return reinterpret_cast<uintptr_t>(p) & 15; }
 
@@ -745,11 +896,10 @@ using namespace droid;
 
 extern "C" {
 
-size_t droid_corr_loss_workspace(int E, int N1, int P, int N2, int Q, int D, int shared, int backward) {
+size_t droid_corr_loss_workspace(int E, int N1, int P, int N2, int Q, int D, int backward) {
   if (E <= 0 || N1 < 0 || P <= 0 || N2 < 0 || Q <= 0 || D <= 0) return 0;
   if (!backward) return (size_t)E * P * fwd_split(E, P, Q) * sizeof(float2);
-  const BwdPlan b = bwd_plan(E, N1, P, N2, Q, D, shared);
-  return gmax_bytes(E) + (b.part1 + b.part2) * sizeof(float);
+  return bwd_space(E, N1 + N2, D).bytes;
 }
 
 int droid_corr_loss_forward(int dtype, const void* fmap1, const void* fmap2, const int* f1, const int* f2,
@@ -763,7 +913,7 @@ int droid_corr_loss_forward(int dtype, const void* fmap1, const void* fmap2, con
     return fail(kInvalidArgument, what + ": null tensor");
   if (!logits && K != 1) return fail(kInvalidArgument, what + ": one target a row without logits");
   if (unaligned(fmap1) || unaligned(fmap2)) return fail(kInvalidArgument, what + ": features must be 16-B aligned");
-  if (!ws || ws_bytes < droid_corr_loss_workspace(E, N1, P, N2, Q, D, 0, 0))
+  if (!ws || ws_bytes < droid_corr_loss_workspace(E, N1, P, N2, Q, D, 0))
     return fail(kInvalidArgument, what + ": workspace too small");
   FwdArgs a{fmap1, fmap2, f1, f2, idx, static_cast<float2*>(ws), E, N1, P, N2, Q, D, K, ceil_div(P, kRowsB),
             fwd_split(E, P, Q), 0, scale / temperature * kLog2e};
@@ -796,38 +946,34 @@ int droid_corr_loss_backward(int dtype, const void* fmap1, const void* fmap2, co
   if (unaligned(fmap1) || unaligned(fmap2)) return fail(kInvalidArgument, what + ": features must be 16-B aligned");
   // the gradients that are wanted; a shared tensor's rows are counted once
   const int n1 = dfmap1 ? N1 : 0, n2 = dfmap2 ? N2 : 0;
-  if (!ws || ws_bytes < droid_corr_loss_workspace(E, n1, P, n2, Q, D, shared, 1))
+  if (!ws || ws_bytes < droid_corr_loss_workspace(E, n1, P, n2, Q, D, 1))
     return fail(kInvalidArgument, what + ": workspace too small");
-  const BwdPlan b = bwd_plan(E, n1, P, n2, Q, D, shared != 0);
-  if (b.items == 0) return kOk;
-  if (b.items > 0x3fffffffL) return fail(kUnsupported, what + ": maps too large");
-  float* gmax = static_cast<float*>(ws);
+  if (n1 + n2 == 0) return kOk;
+  char* const w = static_cast<char*>(ws);
+  const BwdSpace sp = bwd_space(E, n1 + n2, D);
   BwdArgs a{};
   a.f1 = fmap1, a.f2 = fmap2, a.e1 = f1, a.e2 = f2, a.idx = idx, a.prob = prob, a.lse = lse, a.g = gloss;
-  a.gmax = gmax, a.d1 = dfmap1, a.d2 = dfmap2;
-  a.part1 = reinterpret_cast<float*>(static_cast<char*>(ws) + gmax_bytes(E)), a.part2 = a.part1 + b.part1;
+  a.d1 = dfmap1, a.d2 = dfmap2;
+  a.gmax = reinterpret_cast<float*>(w + sp.gmax), a.partner = reinterpret_cast<int*>(w + sp.partner);
+  a.first = reinterpret_cast<long long*>(w + sp.first), a.expo = reinterpret_cast<int*>(w + sp.expo);
+  a.part = reinterpret_cast<float*>(w + sp.part);
   a.E = E, a.N1 = N1, a.P = P, a.N2 = N2, a.Q = Q, a.D = D, a.K = K, a.shared = shared != 0;
-  a.S1 = b.S1, a.S2 = b.S2, a.tiles1 = b.tiles1, a.tiles2 = b.tiles2;
-  a.items1 = (int)b.items1, a.items = (int)b.items;
+  a.tiles1 = ceil_div(P, kRowsB), a.tiles2 = ceil_div(Q, kRowsB);
+  a.n1 = n1, a.V = n1 + n2, a.G = bwd_groups(D, K);
   a.c = scale / temperature * kLog2e, a.out_scale = scale * temperature;
-  if (dtype == 0) {
-    corr_gmax_kernel<<<E, kLT, 0, stream>>>(gloss, P, gmax);
-    DROID_LAUNCH_CHECK();
-  }
-  const int grid = (a.items + 7) / 8 * 8;
+  corr_edge_kernel<<<E, kLT, 0, stream>>>(a);
+  DROID_LAUNCH_CHECK();
+  corr_plan_kernel<<<1, 1024, 0, stream>>>(a);
+  DROID_LAUNCH_CHECK();
+  const int grid = (a.G + 7) / 8 * 8;
 #define BWD(T, DP) corr_loss_bwd_kernel<T, DP><<<grid, kLT, bwd_lds<DP>(K), stream>>>(a)
   CORR_TYPES(BWD)
 #undef BWD
   DROID_LAUNCH_CHECK();
-  for (int q = 0; q < 2; ++q) {
-    if (!(q ? b.part2 : b.part1)) continue;
-    const long n = q ? (long)N2 * Q * D : (long)N1 * P * D;
-    const float* part = q ? a.part2 : a.part1;
-    const int jg = (int)((n / 4 + kLT - 1) / kLT), S = q ? a.S2 : a.S1;
-    if (dtype == 0) corr_loss_join_kernel<_Float16><<<jg, kLT, 0, stream>>>(part, (_Float16*)(q ? dfmap2 : dfmap1), n, S);
-    else corr_loss_join_kernel<__bf16><<<jg, kLT, 0, stream>>>(part, (__bf16*)(q ? dfmap2 : dfmap1), n, S);
-    DROID_LAUNCH_CHECK();
-  }
+  const int items = n1 * a.tiles1 + n2 * a.tiles2;
+  if (dtype == 0) corr_loss_join_kernel<_Float16><<<items, kLT, 0, stream>>>(a);
+  else corr_loss_join_kernel<__bf16><<<items, kLT, 0, stream>>>(a);
+  DROID_LAUNCH_CHECK();
   return kOk;
 }
 
