@@ -22,7 +22,6 @@
 
 #include <algorithm>
 #include <cmath>
-#include <cstddef>
 
 namespace droid {
 
@@ -341,6 +340,7 @@ __global__ void __launch_bounds__(kLT) corr_loss_row_kernel(RowArgs a) {
 // uneven graphs up to twice their even share.)
 
 constexpr int kUnitBoth = 3, kUnitOne = 2;   // cost of a step with both directions / one (measured about 3 : 2)
+constexpr int kJoin = 8;                     // workgroups that join one item
 constexpr int kMinUnits = 16;                // smallest share worth a workgroup
 
 struct BwdArgs {
@@ -482,40 +482,34 @@ __device__ __forceinline__ int slot_of(const BwdArgs& a, long long u) {
   return lo;
 }
 
-// What a workgroup of the gradient kernel keeps in LDS (dynamic: the sparse
-// entries' part depends on K).
+constexpr int kHitTiles = 1024;   // tiles with a hit mask at a time (65536 streamed rows; beyond: all are looked at)
+
+// What a workgroup of the gradient kernel keeps in LDS.
 template <int DP>
 struct BwdShared {
   char tile[2][kRowsY * 2 * DP];           // rows aligned to their size
   float delta[4][32][32];                  // a wave's sparse terms of half a tile; zero between uses
   float rowl[3][kRowsY], rowg[3][kRowsY];  // the streamed queries' lse and g, two tiles ahead
-  float xg[kRowsB];                        // the stationary queries' g
   int elist[kLT];
   int ecount[4];
-  __attribute__((aligned(16))) int ent[1]; // sparse entries: of the 128 rows x, and of two tiles (128 K each)
+  unsigned hits[kHitTiles];                // per tile: byte k, bit w: half k has a sparse term of wave w's rows
 };
-template <int DP>
-size_t bwd_lds(int K) {
-  return offsetof(BwdShared<DP>, ent) + (size_t)2 * kRowsB * K * sizeof(int);
-}
 
 // The steps [t0, t1) of one edge (es: x are its queries) and / or its reverse
 // (ed: the streamed rows y are its queries).
 //
 // The sparse targets (g pi at (y, x)) go through a dense, wave-private LDS image
-// of half a tile that is read only where one was put: the subtraction happens in
-// fp32, before the rounding (p - pi of a well-trained row is a small
-// difference).  To find them a wave compares its 32 rows' K entries (in LDS for
-// the whole edge) and the tile's 64 K (staged with the tile) with the range it
-// holds.
+// of half a tile, used only where there is one: the subtraction happens in fp32,
+// before the rounding (p - pi of a well-trained row is a small difference).
+// Which half tiles those are is found once an edge, for all waves, from the
+// 128 K entries of the rows x and the streamed rows' K entries.
 template <typename T, int DP, bool SRC, bool DST>
 __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, int es, int ed, int t0, int t1, int R,
                                          int x0, float mul, const typename Op<T>::vec8 (&b)[DP / 16],
                                          floatx16 (&acc)[DP / 32]) {
   typedef typename Op<T>::vec8 vec8;
-  typedef int int4_t __attribute__((ext_vector_type(4)));
-  typedef int int4_u __attribute__((ext_vector_type(4), aligned(4)));
-  constexpr int RB = 2 * DP;
+  typedef const __attribute__((address_space(3))) vec8* ptr;
+  constexpr int RB = 2 * DP, KD = DP / 16;
   const int tid = fresh(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int xw = x0 + wave * 32, x = xw + (lane & 31);
   const int n_y = SRC ? a.Q : a.P, K = a.K;
@@ -523,7 +517,8 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
                               (unsigned)n_y * a.D * 2);
   const float* lse = a.lse + (long)ed * a.P;      // of the streamed queries
   const float* g = a.g + (long)ed * a.P;
-  const int* idx = a.idx + (long)ed * a.P * K;
+  const int* xidx = a.idx + ((long)es * a.P + x0) * K;   // of the rows x, as queries of es
+  const int* yidx = a.idx + (long)ed * a.P * K;          // of the streamed queries
   float lx = INFINITY, gx = 0.f;
   bool live = false;   // a stationary row has a target
   if constexpr (SRC) {
@@ -533,15 +528,34 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
     }
     live = __syncthreads_or(lx != INFINITY);
     if (!DST && !live) return;   // every row left out: nothing here, whatever the keys hold
-    if (lane < 32) sh.xg[wave * 32 + lane] = gx;
-    const int* xi = a.idx + ((long)es * a.P + x0) * K;
-    for (int q = tid; q < kRowsB * K; q += kLT) sh.ent[q] = x0 + q / K < R ? xi[q] : -1;
   }
-  // Streamed queries: entries come one tile ahead, lse and g two: lse = +inf
-  // marks a left-out row, whose features must not be read (unless as live keys)
-  // before it is staged.
+  const bool masked = t1 - t0 <= kHitTiles;
+  if (masked) {
+    for (int q = tid; q < t1 - t0; q += kLT) sh.hits[q] = 0;
+    __syncthreads();
+    const unsigned span = (unsigned)(t1 - t0) * kRowsY;
+    if constexpr (SRC) {
+      const int n = min(kRowsB, R - x0) * K;
+      for (int q = tid; q < n; q += kLT) {
+        const unsigned y = xidx[q] - t0 * kRowsY;
+        if (y < span) atomicOr(&sh.hits[y / kRowsY], 1u << ((y & 32) / 4 + q / K / 32));
+      }
+    }
+    if constexpr (DST) {
+      const unsigned first = t0 * kRowsY * K, n = min(n_y, t1 * kRowsY) * K - first;
+#pragma unroll 4
+      for (unsigned q = tid; q < n; q += kLT) {
+        const unsigned v = yidx[first + q] - x0;
+        if (v < kRowsB) {
+          const unsigned y = q / K;
+          atomicOr(&sh.hits[y / kRowsY], 1u << ((y & 32) / 4 + v / 32));
+        }
+      }
+    }
+  }
+  // Streamed queries' lse and g, two tiles ahead: lse = +inf marks a left-out row,
+  // whose features must not be read (unless as live keys) before it is staged.
   float nl = 0.f, ng = 0.f;
-  int4_t ne = {-1, -1, -1, -1};
   auto rows = [&](int t) {
     if (DST && tid < kRowsY) {
       const unsigned y = t * kRowsY + tid;
@@ -555,36 +569,11 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
       sh.rowg[slot][tid] = ng;
     }
   };
-  auto piece = [&](int t, int q) -> int4_t {   // entries 4 q .. + 3 of tile t
-    const unsigned at = t * kRowsY * K + 4 * q;
-    const int left = n_y * K - (int)at;
-    int4_t v = {-1, -1, -1, -1};
-    if (left >= 4) v = *reinterpret_cast<const int4_u*>(idx + at);
-    else if (left > 0) {
-      v.x = idx[at];
-      if (left > 1) v.y = idx[at + 1];
-      if (left > 2) v.z = idx[at + 2];
-    }
-    return v;
-  };
-  auto entries = [&](int t) {
-    if (DST && tid < 16 * K) ne = piece(t, tid);   // K <= 16: all of them
-  };
-  int* const yent = sh.ent + kRowsB * K;
-  auto put_entries = [&](int t, int buf) {
-    if constexpr (DST) {
-      int4_t* to = reinterpret_cast<int4_t*>(yent + buf * kRowsY * K);
-      if (tid < 16 * K) to[tid] = ne;
-      for (int q = tid + kLT; q < 16 * K; q += kLT) to[q] = piece(t, q);
-    }
-  };
   auto stage = [&](int t, int buf, int sl) {
     stage_tile<T, DP>(rs, sh.tile[buf], t * kRowsY, n_y, a.D, wave, lane,
                       [&](int row) { return DST && sh.rowl[sl][row] == INFINITY && !(SRC && live); });
   };
   int slot = 0;   // of tile t's row data
-  entries(t0);
-  put_entries(t0, 0);
   rows(t0);
   put_rows(0);
   if (t0 + 1 < t1) rows(t0 + 1);
@@ -596,64 +585,61 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1, next = slot == 2 ? 0 : slot + 1, after = next == 2 ? 0 : next + 1;
     const unsigned cur = lds_addr(sh.tile[buf]), row0 = row_addr<DP>(cur, fresh(lane));
+    // both halves' operands of the first product before anything else
+    vec8 fa[2][KD];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int d = 0; d < KD; ++d) fa[k][d] = *(ptr)(uintptr_t)((row0 ^ (d << 5)) + k * 64 * DP);
+    const unsigned hm = masked ? __builtin_amdgcn_readfirstlane(sh.hits[t - t0]) >> wave : 0x101u;
     if (t + 1 < t1) {
       stage(t + 1, buf ^ 1, next);
-      entries(t + 1);
       if (t + 2 < t1) rows(t + 2);
     }
-    // which halves of the tile hold a sparse term of the wave's rows
-    bool hit[2] = {false, false};
-    const int4_t* xent = reinterpret_cast<const int4_t*>(sh.ent + wave * 32 * K);
-    const int4_t* tent = reinterpret_cast<const int4_t*>(yent + buf * kRowsY * K);
-    if constexpr (SRC)
-      for (int q = lane; q < 8 * K; q += 64) {
-        const int4_t v = xent[q] - t * kRowsY;
-        hit[0] |= (unsigned)v.x < 32u || (unsigned)v.y < 32u || (unsigned)v.z < 32u || (unsigned)v.w < 32u;
-        hit[1] |= (unsigned)v.x - 32u < 32u || (unsigned)v.y - 32u < 32u || (unsigned)v.z - 32u < 32u ||
-                  (unsigned)v.w - 32u < 32u;
-      }
-    if constexpr (DST)
-      for (int q = lane; q < 16 * K; q += 64) {
-        const int4_t v = tent[q] - xw;
-        // (a row's entries may lie in both halves of 64 K: decided by the row below)
-        const bool in = (unsigned)v.x < 32u || (unsigned)v.y < 32u || (unsigned)v.z < 32u || (unsigned)v.w < 32u;
-        hit[0] |= in && q < 8 * K;
-        hit[1] |= in && q >= 8 * K;
-      }
     float (&dl)[32][32] = sh.delta[wave];
     auto sparse = [&](int k, bool put) {
+      const int y0 = t * kRowsY + 32 * k;
       if constexpr (SRC) {
-        const int* ent = reinterpret_cast<const int*>(xent);
-        for (int q = lane; q < 32 * K; q += 64) {
-          const int v = ent[q] - t * kRowsY - 32 * k;
+        const int n = min(32, R - xw) * K;
+        for (int q = lane; q < n; q += 64) {
+          const int v = xidx[wave * 32 * K + q] - y0;
           if ((unsigned)v < 32u) {
             const int row = q / K;
-            if (put) atomicAdd(&dl[v][row], sh.xg[wave * 32 + row] *
-                                                (a.prob ? a.prob[((long)es * a.P + xw) * K + q] : 1.f));
-            else dl[v][row] = 0.f;
+            if (put) {
+              const long at = (long)es * a.P + xw + row;
+              const float le = a.lse[at], gg = le == INFINITY ? 0.f : a.g[at] * mul;
+              atomicAdd(&dl[v][row], gg * (a.prob ? a.prob[((long)es * a.P + xw) * K + q] : 1.f));
+            } else {
+              dl[v][row] = 0.f;
+            }
           }
         }
       }
       if constexpr (DST) {
-        const int* ent = reinterpret_cast<const int*>(tent) + 32 * K * k;
-        for (int q = lane; q < 32 * K; q += 64) {
-          const int v = ent[q] - xw;
+        const int n = min(32, n_y - y0) * K;
+        for (int q = lane; q < n; q += 64) {
+          const int v = yidx[(unsigned)y0 * K + q] - xw;
           if ((unsigned)v < 32u) {
             const int row = q / K;
             if (put)
               atomicAdd(&dl[row][v], sh.rowg[slot][32 * k + row] *
-                                         (a.prob ? a.prob[((long)ed * a.P + t * kRowsY + 32 * k) * K + q] : 1.f));
+                                         (a.prob ? a.prob[((long)ed * a.P + y0) * K + q] : 1.f));
             else dl[row][v] = 0.f;
           }
         }
       }
     };
+    floatx16 sc[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sc[k][i] = 0.f;
+#pragma unroll
+      for (int d = 0; d < KD; ++d) sc[k] = Op<T>::mfma(fa[k][d], b[d], sc[k]);
+    }
     vec8 ds[4];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const bool any = __ballot(hit[k]) != 0;
-      if (any) sparse(k, true);
-      const floatx16 sc = block_product<T, DP>(row0, k, b);
       float wg[16];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -667,7 +653,7 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           // p clamped to [0, 1]: a NaN logit of a left-out row counts as 0
-          const float s = sc[4 * q + u];
+          const float s = sc[k][4 * q + u];
           float w = 0.f;
           if constexpr (SRC)
             w = gx * __builtin_amdgcn_fmed3f(__builtin_amdgcn_exp2f(fmaf(s, a.c, -lx)), 0.f, 1.f);
@@ -676,7 +662,8 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
           wg[4 * q + u] = w;
         }
       }
-      if (any) {
+      if (hm >> (8 * k) & 1) {
+        sparse(k, true);
         const int v = fresh(lane);
         const float* col = &dl[4 * (v >> 5)][v & 31];
 #pragma unroll
@@ -707,7 +694,6 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
         }
       }
     }
-    if (t + 1 < t1) put_entries(t + 1, buf ^ 1);
     if (t + 2 < t1) put_rows(after);
     slot = next;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -753,8 +739,7 @@ __device__ __forceinline__ void bwd_kind(const BwdArgs& a, BwdShared<DP>& sh, in
 template <typename T, int DP>
 __global__ void __launch_bounds__(kLT, DP <= 128 ? 2 : 1) corr_loss_bwd_kernel(BwdArgs a) {
   constexpr bool kScaled = !__is_same(T, __bf16);
-  extern __shared__ __attribute__((aligned(1024))) char lds[];
-  BwdShared<DP>& sh = *reinterpret_cast<BwdShared<DP>*>(lds);
+  __shared__ __attribute__((aligned(1024))) BwdShared<DP> sh;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int block = xcd_item(blockIdx.x, a.G);
   if (block >= a.G) return;
@@ -814,7 +799,7 @@ __global__ void __launch_bounds__(kLT, DP <= 128 ? 2 : 1) corr_loss_bwd_kernel(B
   }
 }
 
-// One workgroup an item: adds up, in order, the parts of one that several
+// kJoin workgroups an item: add up, in order, the parts of one that several
 // shares have worked on; zeros where no edge reaches the frame.
 template <typename T>
 __global__ void __launch_bounds__(kLT) corr_loss_join_kernel(BwdArgs a) {
@@ -828,9 +813,10 @@ __global__ void __launch_bounds__(kLT) corr_loss_join_kernel(BwdArgs a) {
   if (per && b0 == b1) return;
   T* d = static_cast<T*>(second ? a.d2 : a.d1) + ((long)n * R + x0) * a.D;
   const int total = min(kRowsB, R - x0) * a.D;
-  for (int q = threadIdx.x * 4; q < total; q += kLT * 4) {
+  for (int q = (blockIdx.y * kLT + threadIdx.x) * 4; q < total; q += kLT * 4 * kJoin) {
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
     if (per)
+#pragma unroll 4
       for (int b = b0; b <= b1; ++b) {
         const float4 p = *reinterpret_cast<const float4*>(a.part + (long)(2 * b + (b == b0)) * kRowsB * a.D + q);
         s.x += p.x;
@@ -849,9 +835,8 @@ int fwd_split(int E, int P, int Q) {
   return (int)std::max<long>(1, std::min<long>(ceil_div(Q, kRowsY), 1024 / std::max<long>(1, blocks)));
 }
 
-// Workgroups of the gradient kernel: as many as run at once - two a CU while
-// both fit its LDS (K <= 16 at D <= 128).
-int bwd_groups(int D, int K) { return device_cu_count() * (D <= 128 && K <= 16 ? 2 : 1); }
+// Workgroups of the gradient kernel: as many as run at once (by its registers).
+int bwd_groups(int D) { return device_cu_count() * (D <= 128 ? 2 : 1); }
 
 // The gradient's workspace, in bytes from its start.
 struct BwdSpace {
@@ -864,7 +849,7 @@ BwdSpace bwd_space(int E, int V, int D) {
   s.first = s.partner + up((size_t)E * 4);
   s.expo = s.first + up(((size_t)V + 1) * 8);
   s.part = s.expo + up((size_t)V * 4);
-  s.bytes = s.part + (size_t)2 * bwd_groups(D, 1) * kRowsB * D * 4;
+  s.bytes = s.part + (size_t)2 * bwd_groups(D) * kRowsB * D * 4;
   return s;
 }
 
@@ -959,20 +944,20 @@ int droid_corr_loss_backward(int dtype, const void* fmap1, const void* fmap2, co
   a.part = reinterpret_cast<float*>(w + sp.part);
   a.E = E, a.N1 = N1, a.P = P, a.N2 = N2, a.Q = Q, a.D = D, a.K = K, a.shared = shared != 0;
   a.tiles1 = ceil_div(P, kRowsB), a.tiles2 = ceil_div(Q, kRowsB);
-  a.n1 = n1, a.V = n1 + n2, a.G = bwd_groups(D, K);
+  a.n1 = n1, a.V = n1 + n2, a.G = bwd_groups(D);
   a.c = scale / temperature * kLog2e, a.out_scale = scale * temperature;
   corr_edge_kernel<<<E, kLT, 0, stream>>>(a);
   DROID_LAUNCH_CHECK();
   corr_plan_kernel<<<1, 1024, 0, stream>>>(a);
   DROID_LAUNCH_CHECK();
   const int grid = (a.G + 7) / 8 * 8;
-#define BWD(T, DP) corr_loss_bwd_kernel<T, DP><<<grid, kLT, bwd_lds<DP>(K), stream>>>(a)
+#define BWD(T, DP) corr_loss_bwd_kernel<T, DP><<<grid, kLT, 0, stream>>>(a)
   CORR_TYPES(BWD)
 #undef BWD
   DROID_LAUNCH_CHECK();
   const int items = n1 * a.tiles1 + n2 * a.tiles2;
-  if (dtype == 0) corr_loss_join_kernel<_Float16><<<items, kLT, 0, stream>>>(a);
-  else corr_loss_join_kernel<__bf16><<<items, kLT, 0, stream>>>(a);
+  if (dtype == 0) corr_loss_join_kernel<_Float16><<<dim3(items, kJoin), kLT, 0, stream>>>(a);
+  else corr_loss_join_kernel<__bf16><<<dim3(items, kJoin), kLT, 0, stream>>>(a);
   DROID_LAUNCH_CHECK();
   return kOk;
 }
