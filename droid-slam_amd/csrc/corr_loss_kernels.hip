@@ -117,6 +117,15 @@ __device__ __forceinline__ floatx16 block_product(unsigned row0, int blk, const 
   return acc;
 }
 
+// All of the wave's loads have landed, LDS-DMA included.  The builtin, not inline
+// asm: the compiler does not count the DMAs, and where it cannot see that its own
+// loads have landed it waits for "them" - in fact the DMAs in flight - again in
+// every turn of the loop that follows.
+__device__ __forceinline__ void loads_done() {
+  __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
+  asm volatile("" ::: "memory");
+}
+
 // v, as a value that the compiler knows nothing of: what is computed from it is
 // computed here and not kept in registers over the loops around.
 __device__ __forceinline__ int fresh(int v) {
@@ -165,7 +174,7 @@ __global__ void __launch_bounds__(kLT) corr_lse_kernel(FwdArgs a) {
   load_rows<T, DP>(b, f1, p, a.P, a.D, lane >> 5);
   auto none = [](int) { return false; };
   stage_tile<T, DP>(rs, tile[0], t0 * kRowsY, a.Q, a.D, wave, lane, none);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  loads_done();
   __syncthreads();
   float m = kNegBig, l = 0.f;
   for (int t = t0; t < t1; ++t) {
@@ -194,7 +203,7 @@ __global__ void __launch_bounds__(kLT) corr_lse_kernel(FwdArgs a) {
     for (int k = 0; k < 2; ++k)
 #pragma unroll
       for (int q = 0; q < 16; ++q) l += __builtin_amdgcn_exp2f(fmaf(sc[k][q], a.c, -m));
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    loads_done();
     __syncthreads();
   }
   const float mo = __shfl_xor(m, 32, 64), lo = __shfl_xor(l, 32, 64);
@@ -482,7 +491,8 @@ __device__ __forceinline__ int slot_of(const BwdArgs& a, long long u) {
   return lo;
 }
 
-constexpr int kHitTiles = 1024;   // tiles with a hit mask at a time (65536 streamed rows; beyond: all are looked at)
+constexpr int kChunk = 32;       // tiles whose sparse records are in LDS at a time
+constexpr int kRecords = 3072;   // of them; where a chunk has more, its entries are read again half tile by half tile
 
 // What a workgroup of the gradient kernel keeps in LDS.
 template <int DP>
@@ -492,7 +502,11 @@ struct BwdShared {
   float rowl[3][kRowsY], rowg[3][kRowsY];  // the streamed queries' lse and g, two tiles ahead
   int elist[kLT];
   int ecount[4];
-  unsigned hits[kHitTiles];                // per tile: byte k, bit w: half k has a sparse term of wave w's rows
+  unsigned long long skip[3];              // left-out rows of the streamed tile
+  int bucket[kChunk * 8 + 1];              // ends of the sparse records of (half tile, wave)
+  int wsum[4];
+  unsigned char pos[kRecords][2];          // y, x in the wave's half tile
+  float val[kRecords];                     // g pi
 };
 
 // The steps [t0, t1) of one edge (es: x are its queries) and / or its reverse
@@ -500,15 +514,17 @@ struct BwdShared {
 //
 // The sparse targets (g pi at (y, x)) go through a dense, wave-private LDS image
 // of half a tile, used only where there is one: the subtraction happens in fp32,
-// before the rounding (p - pi of a well-trained row is a small difference).
-// Which half tiles those are is found once an edge, for all waves, from the
-// 128 K entries of the rows x and the streamed rows' K entries.
+// before the rounding (p - pi of a well-trained row is a small difference).  For
+// every kChunk tiles the entries of the rows x and of the streamed rows are
+// sorted by half tile and wave into LDS (two passes over them: count, place), so
+// that the loop meets them without a load from memory.
 template <typename T, int DP, bool SRC, bool DST>
 __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, int es, int ed, int t0, int t1, int R,
                                          int x0, float mul, const typename Op<T>::vec8 (&b)[DP / 16],
                                          floatx16 (&acc)[DP / 32]) {
   typedef typename Op<T>::vec8 vec8;
   typedef const __attribute__((address_space(3))) vec8* ptr;
+  typedef int int4_u __attribute__((ext_vector_type(4), aligned(4)));
   constexpr int RB = 2 * DP, KD = DP / 16;
   const int tid = fresh(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int xw = x0 + wave * 32, x = xw + (lane & 31);
@@ -517,8 +533,6 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
                               (unsigned)n_y * a.D * 2);
   const float* lse = a.lse + (long)ed * a.P;      // of the streamed queries
   const float* g = a.g + (long)ed * a.P;
-  const int* xidx = a.idx + ((long)es * a.P + x0) * K;   // of the rows x, as queries of es
-  const int* yidx = a.idx + (long)ed * a.P * K;          // of the streamed queries
   float lx = INFINITY, gx = 0.f;
   bool live = false;   // a stationary row has a target
   if constexpr (SRC) {
@@ -529,106 +543,141 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
     live = __syncthreads_or(lx != INFINITY);
     if (!DST && !live) return;   // every row left out: nothing here, whatever the keys hold
   }
-  const bool masked = t1 - t0 <= kHitTiles;
-  if (masked) {
-    for (int q = tid; q < t1 - t0; q += kLT) sh.hits[q] = 0;
-    __syncthreads();
-    const unsigned span = (unsigned)(t1 - t0) * kRowsY;
+  // f(y, x, value) for every sparse term of the streamed rows [y0, y1) and the rows
+  // x0 + [xa, xb), over `n` threads
+  auto each_term = [&](int y0, int y1, int xa, int xb, int from, int n, auto f) {
     if constexpr (SRC) {
-      const int n = min(kRowsB, R - x0) * K;
-      for (int q = tid; q < n; q += kLT) {
-        const unsigned y = xidx[q] - t0 * kRowsY;
-        if (y < span) atomicOr(&sh.hits[y / kRowsY], 1u << ((y & 32) / 4 + q / K / 32));
-      }
-    }
-    if constexpr (DST) {
-      const unsigned first = t0 * kRowsY * K, n = min(n_y, t1 * kRowsY) * K - first;
-#pragma unroll 4
-      for (unsigned q = tid; q < n; q += kLT) {
-        const unsigned v = yidx[first + q] - x0;
-        if (v < kRowsB) {
-          const unsigned y = q / K;
-          atomicOr(&sh.hits[y / kRowsY], 1u << ((y & 32) / 4 + v / 32));
+      const long row0 = (long)es * a.P + x0;
+      const int* p = a.idx + row0 * K;
+      const int last = min(xb, R - x0) * K;
+      for (int q = xa * K + from; q < last; q += n) {
+        const int y = p[q];
+        if (y >= y0 && y < y1) {
+          const int r = q / K;
+          f(y, r, [&] {
+            return (a.lse[row0 + r] == INFINITY ? 0.f : a.g[row0 + r] * mul) * (a.prob ? a.prob[row0 * K + q] : 1.f);
+          });
         }
       }
     }
-  }
+    if constexpr (DST) {
+      const long row0 = (long)ed * a.P + y0;
+      const int* p = a.idx + row0 * K;
+      const int total = (y1 - y0) * K;
+      auto one = [&](int q, int v) {
+        v -= x0;
+        if (v >= xa && v < xb) {
+          const int r = q / K;
+          f(y0 + r, v, [&] {
+            return (a.lse[row0 + r] == INFINITY ? 0.f : a.g[row0 + r] * mul) * (a.prob ? a.prob[row0 * K + q] : 1.f);
+          });
+        }
+      };
+      int q = 4 * from;
+#pragma unroll 4
+      for (; q + 3 < total; q += 4 * n) {
+        const int4_u v = *reinterpret_cast<const int4_u*>(p + q);
+        one(q, v.x);
+        one(q + 1, v.y);
+        one(q + 2, v.z);
+        one(q + 3, v.w);
+      }
+      for (; q < total; ++q) one(q, p[q]);   // the last piece, on one thread
+    }
+  };
+  int c0 = 0;            // the chunk's first tile
+  bool stored = false;   // its records are in LDS
+  auto chunk = [&](int t) {   // between barriers: called where all waves are past the last chunk
+    c0 = t;
+    const int ya = t * kRowsY, yb = min(min(t + kChunk, t1) * kRowsY, n_y);
+    const int y_first = ya;
+    for (int q = tid; q <= kChunk * 8; q += kLT) sh.bucket[q] = 0;
+    __syncthreads();
+    auto bucket = [&](int y, int v) { return (y - y_first) / 32 * 4 + v / 32; };
+    each_term(ya, yb, 0, kRowsB, tid, kLT, [&](int y, int v, auto) { atomicAdd(&sh.bucket[bucket(y, v)], 1); });
+    __syncthreads();
+    // exclusive sums of the kChunk * 8 = kLT counts
+    const int n = sh.bucket[tid];
+    int s = n;
+    for (int o = 1; o < 64; o <<= 1) {
+      const int u = __shfl_up(s, o, 64);
+      if (lane >= o) s += u;
+    }
+    if (lane == 63) sh.wsum[wave] = s;
+    __syncthreads();
+    for (int q = 0; q < wave; ++q) s += sh.wsum[q];
+    stored = sh.wsum[0] + sh.wsum[1] + sh.wsum[2] + sh.wsum[3] <= kRecords;
+    sh.bucket[tid] = stored ? s - n : n;   // not stored: the counts, for whether to look at all
+    __syncthreads();
+    if (stored)
+      each_term(ya, yb, 0, kRowsB, tid, kLT, [&](int y, int v, auto value) {
+        const int at = atomicAdd(&sh.bucket[bucket(y, v)], 1);   // ends as the bucket's end
+        sh.pos[at][0] = (unsigned char)(y & 31);
+        sh.pos[at][1] = (unsigned char)(v & 31);
+        sh.val[at] = value();
+      });
+    __syncthreads();
+  };
   // Streamed queries' lse and g, two tiles ahead: lse = +inf marks a left-out row,
   // whose features must not be read (unless as live keys) before it is staged.
-  float nl = 0.f, ng = 0.f;
+  float nl = INFINITY, ng = 0.f;
   auto rows = [&](int t) {
     if (DST && tid < kRowsY) {
       const unsigned y = t * kRowsY + tid;
-      nl = y < (unsigned)n_y ? lse[y] : INFINITY;
-      ng = nl == INFINITY ? 0.f : nl == nl ? g[y] * mul : NAN;
+      nl = INFINITY;
+      if (y < (unsigned)n_y) nl = lse[y], ng = g[y];
     }
   };
   auto put_rows = [&](int slot) {
-    if (DST && tid < kRowsY) {
+    if (DST && tid < kRowsY) {   // the first wave
+      const unsigned long long out = __ballot(nl == INFINITY);
       sh.rowl[slot][tid] = nl;
-      sh.rowg[slot][tid] = ng;
+      sh.rowg[slot][tid] = nl == INFINITY ? 0.f : nl == nl ? ng * mul : NAN;
+      if (tid == 0) sh.skip[slot] = SRC && live ? 0 : out;
     }
   };
-  auto stage = [&](int t, int buf, int sl) {
-    stage_tile<T, DP>(rs, sh.tile[buf], t * kRowsY, n_y, a.D, wave, lane,
-                      [&](int row) { return DST && sh.rowl[sl][row] == INFINITY && !(SRC && live); });
+  auto stage = [&](int t, int buf, unsigned long long out) {
+    if (out == 0)
+      stage_tile<T, DP>(rs, sh.tile[buf], t * kRowsY, n_y, a.D, wave, lane, [](int) { return false; });
+    else
+      stage_tile<T, DP>(rs, sh.tile[buf], t * kRowsY, n_y, a.D, wave, lane, [&](int row) { return out >> row & 1; });
+  };
+  auto skipped = [&](int sl) -> unsigned long long {
+    if (!DST) return 0;
+    const unsigned long long m = sh.skip[sl];
+    return (unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)(m >> 32)) << 32 |
+           (unsigned)__builtin_amdgcn_readfirstlane((int)m);
   };
   int slot = 0;   // of tile t's row data
   rows(t0);
   put_rows(0);
   if (t0 + 1 < t1) rows(t0 + 1);
   put_rows(1);
-  if constexpr (DST) __syncthreads();
-  stage(t0, 0, 0);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  chunk(t0);
+  stage(t0, 0, skipped(0));
+  loads_done();
   __syncthreads();
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1, next = slot == 2 ? 0 : slot + 1, after = next == 2 ? 0 : next + 1;
+    if (t == c0 + kChunk) chunk(t);
     const unsigned cur = lds_addr(sh.tile[buf]), row0 = row_addr<DP>(cur, fresh(lane));
+    const unsigned long long out = t + 1 < t1 ? skipped(next) : 0;
+    const int bk = ((t - c0) * 2) * 4 + wave;   // the wave's records: half 0, half 1
+    const int lo0 = __builtin_amdgcn_readfirstlane(sh.bucket[bk > 0 ? bk - 1 : kChunk * 8]),
+              hi0 = __builtin_amdgcn_readfirstlane(sh.bucket[bk]),
+              lo1 = __builtin_amdgcn_readfirstlane(sh.bucket[bk + 3]),
+              hi1 = __builtin_amdgcn_readfirstlane(sh.bucket[bk + 4]);
     // both halves' operands of the first product before anything else
     vec8 fa[2][KD];
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
       for (int d = 0; d < KD; ++d) fa[k][d] = *(ptr)(uintptr_t)((row0 ^ (d << 5)) + k * 64 * DP);
-    const unsigned hm = masked ? __builtin_amdgcn_readfirstlane(sh.hits[t - t0]) >> wave : 0x101u;
     if (t + 1 < t1) {
-      stage(t + 1, buf ^ 1, next);
+      stage(t + 1, buf ^ 1, out);
       if (t + 2 < t1) rows(t + 2);
     }
     float (&dl)[32][32] = sh.delta[wave];
-    auto sparse = [&](int k, bool put) {
-      const int y0 = t * kRowsY + 32 * k;
-      if constexpr (SRC) {
-        const int n = min(32, R - xw) * K;
-        for (int q = lane; q < n; q += 64) {
-          const int v = xidx[wave * 32 * K + q] - y0;
-          if ((unsigned)v < 32u) {
-            const int row = q / K;
-            if (put) {
-              const long at = (long)es * a.P + xw + row;
-              const float le = a.lse[at], gg = le == INFINITY ? 0.f : a.g[at] * mul;
-              atomicAdd(&dl[v][row], gg * (a.prob ? a.prob[((long)es * a.P + xw) * K + q] : 1.f));
-            } else {
-              dl[v][row] = 0.f;
-            }
-          }
-        }
-      }
-      if constexpr (DST) {
-        const int n = min(32, n_y - y0) * K;
-        for (int q = lane; q < n; q += 64) {
-          const int v = yidx[(unsigned)y0 * K + q] - xw;
-          if ((unsigned)v < 32u) {
-            const int row = q / K;
-            if (put)
-              atomicAdd(&dl[row][v], sh.rowg[slot][32 * k + row] *
-                                         (a.prob ? a.prob[((long)ed * a.P + y0) * K + q] : 1.f));
-            else dl[row][v] = 0.f;
-          }
-        }
-      }
-    };
     floatx16 sc[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -662,13 +711,18 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
           wg[4 * q + u] = w;
         }
       }
-      if (hm >> (8 * k) & 1) {
-        sparse(k, true);
-        const int v = fresh(lane);
+      const int lo = k ? lo1 : lo0, hi = k ? hi1 : hi0;
+      if (stored ? lo < hi : hi > 0) {
+        const int v = fresh(lane), y0 = t * kRowsY + 32 * k;
+        if (stored)
+          for (int q = lo + v; q < hi; q += 64) atomicAdd(&dl[sh.pos[q][0]][sh.pos[q][1]], sh.val[q]);
+        else
+          each_term(y0, min(y0 + 32, n_y), wave * 32, wave * 32 + 32, v, 64,
+                    [&](int y, int xx, auto value) { atomicAdd(&dl[y - y0][xx & 31], value()); });
         const float* col = &dl[4 * (v >> 5)][v & 31];
 #pragma unroll
         for (int q = 0; q < 16; ++q) wg[q] -= col[(8 * (q >> 2) + (q & 3)) * 32];
-        sparse(k, false);
+        for (int q = v; q < 32 * 32 / 4; q += 64) reinterpret_cast<float4*>(&dl[0][0])[q] = make_float4(0.f, 0.f, 0.f, 0.f);
       }
 #pragma unroll
       for (int q = 0; q < 16; ++q) ds[2 * k + (q >> 3)][q & 7] = (T)wg[q];
@@ -696,7 +750,7 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
     }
     if (t + 2 < t1) put_rows(after);
     slot = next;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    loads_done();
     __syncthreads();
   }
 }
