@@ -357,7 +357,9 @@ struct BwdArgs {
   const int *e1, *e2, *idx;
   const float *prob, *lse, *g; // prob null: 1
   void *d1, *d2;               // (N1, P, D), (N2, Q, D)
-  float* gmax;                 // (E) largest |g|
+  float* gmax;                 // (E) largest |g|; -1: no row has a target
+  int* flags;                  // (E) 1: a row is left out, 2: a g is negative
+  bhalf8* aux;                 // (E, tiles of P, 64) the queries' exponents (corr_edge_kernel)
   int* partner;                // (E) the reverse edge that is done together with this one, -1: none
   long long* first;            // (V + 1) units before frame slot v; the slots: f1's frames (d1 wanted), then f2's
   int* expo;                   // (V) fp16: exponent that scales the slot's weights
@@ -368,6 +370,8 @@ struct BwdArgs {
   float c, out_scale;          // scale / T log2(e); scale T
 };
 
+__host__ __device__ __forceinline__ int y_tiles(int rows) { return (rows + kRowsY - 1) / kRowsY; }
+
 // Power of two that brings gmax to [2^13, 2^14): an fp16 weight's largest value
 // stays far from 65504 and the small ones stay normal numbers.
 __device__ __forceinline__ int g_exponent(float gmax) {
@@ -377,19 +381,42 @@ __device__ __forceinline__ int g_exponent(float gmax) {
   return max(-100, min(100, 14 - ex));
 }
 
-// One workgroup an edge: the largest |g| of its rows, and the reverse edge it
-// is paired with (the k-th copy of (i, j) with the k-th of (j, i)).
+// One workgroup an edge: what the gradient kernel wants of its rows, and the
+// reverse edge it may be paired with (the k-th copy of (i, j) with the k-th of
+// (j, i)).  A row's exponent v = (log2 |g| - lse) / c, in units of the dot
+// product, is kept as the sum of three bf16 (24 bits), then g's sign.
 __global__ void __launch_bounds__(kLT) corr_edge_kernel(BwdArgs a) {
   __shared__ float red[kLT / 64];
-  __shared__ int cnt[kLT / 64];
+  __shared__ int cnt[kLT / 64], fl[kLT / 64];
   const int e = blockIdx.x, tid = threadIdx.x, wave = tid >> 6;
-  float m = 0.f;
-  for (int p = tid; p < a.P; p += kLT) m = fmaxf(m, fabsf(a.g[(long)e * a.P + p]));
-  for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-  if ((tid & 63) == 0) red[wave] = m;
+  const int padded = y_tiles(a.P) * kRowsY;
+  float m = -1.f;
+  int f = 0;
+  for (int p = tid; p < padded; p += kLT) {
+    const float l = p < a.P ? a.lse[(long)e * a.P + p] : INFINITY;
+    float v = -INFINITY, g = 0.f;
+    if (l != INFINITY) {
+      g = a.g[(long)e * a.P + p];
+      m = fmaxf(fmaxf(m, 0.f), fabsf(g));
+      v = (log2f(fabsf(g)) - l) / a.c;
+      if (g < 0.f) f |= 2;
+    } else if (p < a.P) {
+      f |= 1;
+    }
+    const __bf16 hi = (__bf16)v, z = (__bf16)0.f;
+    const float r1 = fabsf((float)hi) < INFINITY ? v - (float)hi : 0.f;
+    const __bf16 mid = (__bf16)r1, lo = (__bf16)(r1 - (float)mid);
+    a.aux[(long)e * padded + p] = bhalf8{hi, mid, lo, (__bf16)(g < 0.f ? -1.f : 1.f), z, z, z, z};
+  }
+  for (int o = 32; o; o >>= 1) {
+    m = fmaxf(m, __shfl_xor(m, o, 64));
+    f |= __shfl_xor(f, o, 64);
+  }
+  if ((tid & 63) == 0) red[wave] = m, fl[wave] = f;
   __syncthreads();
   if (tid == 0) {
     a.gmax[e] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    a.flags[e] = fl[0] | fl[1] | fl[2] | fl[3];
     a.partner[e] = -1;
   }
   if (!a.shared) return;
@@ -415,11 +442,15 @@ __global__ void __launch_bounds__(kLT) corr_edge_kernel(BwdArgs a) {
   }
 }
 
-// Whether both ends of edge e are frames (otherwise it takes no part).
+// Whether edge e takes part: both ends are frames and a row has a target.
 __device__ __forceinline__ bool edge_in(const BwdArgs& a, int e) {
-  return (unsigned)a.e1[e] < (unsigned)a.N1 && (unsigned)a.e2[e] < (unsigned)a.N2;
+  return (unsigned)a.e1[e] < (unsigned)a.N1 && (unsigned)a.e2[e] < (unsigned)a.N2 && a.gmax[e] >= 0.f;
 }
-__device__ __forceinline__ int y_tiles(int rows) { return (rows + kRowsY - 1) / kRowsY; }
+// Whether it is done together with its reverse.
+__device__ __forceinline__ bool edge_paired(const BwdArgs& a, int e) {
+  const int r = a.partner[e];
+  return r >= 0 && a.gmax[r] >= 0.f;
+}
 
 // One workgroup: the units of every frame slot's items and their running sum.
 __global__ void __launch_bounds__(1024) corr_plan_kernel(BwdArgs a) {
@@ -438,7 +469,7 @@ __global__ void __launch_bounds__(1024) corr_plan_kernel(BwdArgs a) {
       // the edge's slot as source, and as target (one tensor: both in f1's slots)
       const int vs = a.n1 ? a.e1[e] - v0 : -1;
       const int vd = a.shared ? a.e2[e] - v0 : a.V > a.n1 ? a.n1 + a.e2[e] - v0 : -1;
-      const bool paired = a.partner[e] >= 0;
+      const bool paired = edge_paired(a, e);
       if ((unsigned)vs < (unsigned)kChunk) {
         atomicAdd(paired ? &both[vs] : &src[vs], 1);
         atomicMax(reinterpret_cast<int*>(&gm[vs]), __float_as_int(a.gmax[e]));   // >= 0: ordered as integers
@@ -499,10 +530,9 @@ template <int DP>
 struct BwdShared {
   char tile[2][kRowsY * 2 * DP];           // rows aligned to their size
   float delta[4][32][32];                  // a wave's sparse terms of half a tile; zero between uses
-  float rowl[3][kRowsY], rowg[3][kRowsY];  // the streamed queries' lse and g, two tiles ahead
+  bhalf8 aux[3][kRowsY];                   // the streamed queries' exponents, two tiles ahead
   int elist[kLT];
   int ecount[4];
-  unsigned long long skip[3];              // left-out rows of the streamed tile
   int bucket[kChunk * 8 + 1];              // ends of the sparse records of (half tile, wave)
   int wsum[4];
   unsigned char pos[kRecords][2];          // y, x in the wave's half tile
@@ -520,7 +550,7 @@ struct BwdShared {
 // that the loop meets them without a load from memory.
 template <typename T, int DP, bool SRC, bool DST>
 __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, int es, int ed, int t0, int t1, int R,
-                                         int x0, float mul, const typename Op<T>::vec8 (&b)[DP / 16],
+                                         int x0, int ex, const typename Op<T>::vec8 (&b)[DP / 16],
                                          floatx16 (&acc)[DP / 32]) {
   typedef typename Op<T>::vec8 vec8;
   typedef const __attribute__((address_space(3))) vec8* ptr;
@@ -531,8 +561,7 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
   const int n_y = SRC ? a.Q : a.P, K = a.K;
   const rsrc_t rs = make_rsrc(static_cast<const T*>(SRC ? a.f2 : a.f1) + (long)(SRC ? a.e2[es] : a.e1[ed]) * n_y * a.D,
                               (unsigned)n_y * a.D * 2);
-  const float* lse = a.lse + (long)ed * a.P;      // of the streamed queries
-  const float* g = a.g + (long)ed * a.P;
+  const float mul = ldexpf(1.f, ex), fex = (float)ex;
   float lx = INFINITY, gx = 0.f;
   bool live = false;   // a stationary row has a target
   if constexpr (SRC) {
@@ -577,11 +606,14 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
 #pragma unroll 4
       for (; q + 3 < total; q += 4 * n) {
         const int4_u v = *reinterpret_cast<const int4_u*>(p + q);
-        one(q, v.x);
-        one(q + 1, v.y);
-        one(q + 2, v.z);
-        one(q + 3, v.w);
+        const int lo = x0 + xa;
+        const unsigned span = xb - xa;
+        if ((unsigned)(v.x - lo) < span || (unsigned)(v.y - lo) < span || (unsigned)(v.z - lo) < span ||
+            (unsigned)(v.w - lo) < span)
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) one(q + c, c & 2 ? (c & 1 ? v.w : v.z) : c & 1 ? v.y : v.x);
       }
+#pragma unroll 1
       for (; q < total; ++q) one(q, p[q]);   // the last piece, on one thread
     }
   };
@@ -618,65 +650,50 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
       });
     __syncthreads();
   };
-  // Streamed queries' lse and g, two tiles ahead: lse = +inf marks a left-out row,
-  // whose features must not be read (unless as live keys) before it is staged.
-  float nl = INFINITY, ng = 0.f;
-  auto rows = [&](int t) {
-    if (DST && tid < kRowsY) {
-      const unsigned y = t * kRowsY + tid;
-      nl = INFINITY;
-      if (y < (unsigned)n_y) nl = lse[y], ng = g[y];
-    }
+  // Streamed queries: |g| mul p2 = 2^(c (s + v) + ex) with their exponents v, which
+  // one more MFMA step adds (three bf16 times ones).  They are staged two tiles
+  // ahead: v = -inf marks a row without a gradient, whose features must not be
+  // read (unless as live keys) when its tile is staged.
+  const rsrc_t raux = make_rsrc(a.aux + (long)ed * y_tiles(a.P) * kRowsY, (unsigned)y_tiles(a.P) * kRowsY * 16);
+  auto stage_aux = [&](int t, int slot) {
+    if (DST && wave == 0) dma16(raux, lds_addr(sh.aux[slot]), (unsigned)(t * kRowsY + lane) * 16);
   };
-  auto put_rows = [&](int slot) {
-    if (DST && tid < kRowsY) {   // the first wave
-      const unsigned long long out = __ballot(nl == INFINITY);
-      sh.rowl[slot][tid] = nl;
-      sh.rowg[slot][tid] = nl == INFINITY ? 0.f : nl == nl ? ng * mul : NAN;
-      if (tid == 0) sh.skip[slot] = SRC && live ? 0 : out;
-    }
-  };
-  auto stage = [&](int t, int buf, unsigned long long out) {
-    if (out == 0)
+  const int ef = DST ? a.flags[ed] : 0;
+  const bool holes = (ef & 1) && !(SRC && live), neg = ef & 2;
+  const __bf16 one = (__bf16)(h ? 0.f : 1.f), z16 = (__bf16)0.f;
+  const bhalf8 ones = {one, one, one, z16, z16, z16, z16, z16};
+  auto stage = [&](int t, int buf, int slot) {
+    if (!holes)
       stage_tile<T, DP>(rs, sh.tile[buf], t * kRowsY, n_y, a.D, wave, lane, [](int) { return false; });
     else
-      stage_tile<T, DP>(rs, sh.tile[buf], t * kRowsY, n_y, a.D, wave, lane, [&](int row) { return out >> row & 1; });
+      stage_tile<T, DP>(rs, sh.tile[buf], t * kRowsY, n_y, a.D, wave, lane,
+                        [&](int row) { return (float)sh.aux[slot][row][0] == -INFINITY; });
   };
-  auto skipped = [&](int sl) -> unsigned long long {
-    if (!DST) return 0;
-    const unsigned long long m = sh.skip[sl];
-    return (unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)(m >> 32)) << 32 |
-           (unsigned)__builtin_amdgcn_readfirstlane((int)m);
-  };
-  int slot = 0;   // of tile t's row data
-  rows(t0);
-  put_rows(0);
-  if (t0 + 1 < t1) rows(t0 + 1);
-  put_rows(1);
+  int slot = 0;   // of tile t's exponents
+  stage_aux(t0, 0);
+  if (t0 + 1 < t1) stage_aux(t0 + 1, 1);
   chunk(t0);
-  stage(t0, 0, skipped(0));
+  loads_done();
+  __syncthreads();
+  stage(t0, 0, 0);
   loads_done();
   __syncthreads();
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1, next = slot == 2 ? 0 : slot + 1, after = next == 2 ? 0 : next + 1;
     if (t == c0 + kChunk) chunk(t);
     const unsigned cur = lds_addr(sh.tile[buf]), row0 = row_addr<DP>(cur, fresh(lane));
-    const unsigned long long out = t + 1 < t1 ? skipped(next) : 0;
-    const int bk = ((t - c0) * 2) * 4 + wave;   // the wave's records: half 0, half 1
-    const int lo0 = __builtin_amdgcn_readfirstlane(sh.bucket[bk > 0 ? bk - 1 : kChunk * 8]),
-              hi0 = __builtin_amdgcn_readfirstlane(sh.bucket[bk]),
-              lo1 = __builtin_amdgcn_readfirstlane(sh.bucket[bk + 3]),
-              hi1 = __builtin_amdgcn_readfirstlane(sh.bucket[bk + 4]);
+    if (t + 1 < t1) {
+      stage(t + 1, buf ^ 1, next);
+      if (t + 2 < t1) stage_aux(t + 2, after);
+    }
     // both halves' operands of the first product before anything else
     vec8 fa[2][KD];
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
       for (int d = 0; d < KD; ++d) fa[k][d] = *(ptr)(uintptr_t)((row0 ^ (d << 5)) + k * 64 * DP);
-    if (t + 1 < t1) {
-      stage(t + 1, buf ^ 1, out);
-      if (t + 2 < t1) rows(t + 2);
-    }
+    const int bk = ((t - c0) * 2) * 4 + wave;   // the wave's records: half 0, half 1
+    const int4 br = make_int4(sh.bucket[bk > 0 ? bk - 1 : kChunk * 8], sh.bucket[bk], sh.bucket[bk + 3], sh.bucket[bk + 4]);
     float (&dl)[32][32] = sh.delta[wave];
     floatx16 sc[2];
 #pragma unroll
@@ -691,27 +708,25 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
     for (int k = 0; k < 2; ++k) {
       float wg[16];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        float lq[4], gq[4];
-        if constexpr (DST) {
-          const float4 l4 = *reinterpret_cast<const float4*>(&sh.rowl[slot][32 * k + 8 * q + 4 * h]);
-          const float4 g4 = *reinterpret_cast<const float4*>(&sh.rowg[slot][32 * k + 8 * q + 4 * h]);
-          lq[0] = l4.x, lq[1] = l4.y, lq[2] = l4.z, lq[3] = l4.w;
-          gq[0] = g4.x, gq[1] = g4.y, gq[2] = g4.z, gq[3] = g4.w;
-        }
+      for (int q = 0; q < 16; ++q) wg[q] = 0.f;
+      if constexpr (DST) {
+        bhalf8 v = sh.aux[slot][32 * k + (lane & 31)];
+        if (h) v = bhalf8{z16, z16, z16, z16, z16, z16, z16, z16};   // (0 times an infinity is not 0)
+        const floatx16 s2 = Op<__bf16>::mfma(v, ones, sc[k]);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          // p clamped to [0, 1]: a NaN logit of a left-out row counts as 0
-          const float s = sc[k][4 * q + u];
-          float w = 0.f;
-          if constexpr (SRC)
-            w = gx * __builtin_amdgcn_fmed3f(__builtin_amdgcn_exp2f(fmaf(s, a.c, -lx)), 0.f, 1.f);
-          if constexpr (DST)
-            w = fmaf(gq[u], __builtin_amdgcn_fmed3f(__builtin_amdgcn_exp2f(fmaf(s, a.c, -lq[u])), 0.f, 1.f), w);
-          wg[4 * q + u] = w;
+        for (int q = 0; q < 16; ++q) wg[q] = __builtin_amdgcn_exp2f(fmaf(s2[q], a.c, fex));
+        if (neg) {
+#pragma unroll
+          for (int q = 0; q < 16; ++q) wg[q] *= (float)sh.aux[slot][32 * k + 8 * (q >> 2) + 4 * h + (q & 3)][3];
         }
       }
-      const int lo = k ? lo1 : lo0, hi = k ? hi1 : hi0;
+      if constexpr (SRC) {
+        // p1 clamped to [0, 1]: a NaN logit of a left-out row counts as 0
+#pragma unroll
+        for (int q = 0; q < 16; ++q)
+          wg[q] = fmaf(gx, __builtin_amdgcn_fmed3f(__builtin_amdgcn_exp2f(fmaf(sc[k][q], a.c, -lx)), 0.f, 1.f), wg[q]);
+      }
+      const int lo = __builtin_amdgcn_readfirstlane(k ? br.z : br.x), hi = __builtin_amdgcn_readfirstlane(k ? br.w : br.y);
       if (stored ? lo < hi : hi > 0) {
         const int v = fresh(lane), y0 = t * kRowsY + 32 * k;
         if (stored)
@@ -748,7 +763,6 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
         }
       }
     }
-    if (t + 2 < t1) put_rows(after);
     slot = next;
     loads_done();
     __syncthreads();
@@ -760,7 +774,7 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
 // that are done here.
 template <typename T, int DP, bool SRC, bool DST>
 __device__ __forceinline__ void bwd_kind(const BwdArgs& a, BwdShared<DP>& sh, int n, long long& at, long long u0,
-                                         long long u1, int R, int x0, float mul,
+                                         long long u1, int R, int x0, int ex,
                                          const typename Op<T>::vec8 (&b)[DP / 16], floatx16 (&acc)[DP / 32]) {
   const int tid = fresh(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   constexpr int unit = SRC && DST ? kUnitBoth : kUnitOne;
@@ -768,7 +782,7 @@ __device__ __forceinline__ void bwd_kind(const BwdArgs& a, BwdShared<DP>& sh, in
   for (int e0 = 0; e0 < a.E && at < u1; e0 += kLT) {
     const int e = e0 + tid;
     bool in = e < a.E && (SRC ? a.e1 : a.e2)[e] == n;
-    if (in) in = edge_in(a, e) && (SRC && DST) == (a.partner[e] >= 0);
+    if (in) in = edge_in(a, e) && (SRC && DST) == edge_paired(a, e);
     const unsigned long long bal = __ballot(in);
     if (lane == 0) sh.ecount[wave] = __popcll(bal);
     __syncthreads();
@@ -783,7 +797,7 @@ __device__ __forceinline__ void bwd_kind(const BwdArgs& a, BwdShared<DP>& sh, in
       if (t0 >= t1) continue;
       const int eq = __builtin_amdgcn_readfirstlane(sh.elist[q]);
       const int er = SRC && DST ? __builtin_amdgcn_readfirstlane(a.partner[eq]) : eq;
-      bwd_edge<T, DP, SRC, DST>(a, sh, eq, er, t0, t1, R, x0, mul, b, acc);
+      bwd_edge<T, DP, SRC, DST>(a, sh, eq, er, t0, t1, R, x0, ex, b, acc);
     }
     __syncthreads();
   }
@@ -818,13 +832,12 @@ __global__ void __launch_bounds__(kLT, DP <= 128 ? 2 : 1) corr_loss_bwd_kernel(B
 #pragma unroll
       for (int q = 0; q < 16; ++q) acc[d][q] = 0.f;
     const int ex = kScaled ? a.expo[v] : 0;
-    const float mul = kScaled ? ldexpf(1.f, ex) : 1.f;
     // the kinds one after the other: in one loop the compiler keeps the values of
     // all of them in registers and spills
     long long at = 0;
-    if (a.shared) bwd_kind<T, DP, true, true>(a, sh, n, at, u0, u1, R, x0, mul, b, acc);
-    if (!second) bwd_kind<T, DP, true, false>(a, sh, n, at, u0, u1, R, x0, mul, b, acc);
-    if (second || a.shared) bwd_kind<T, DP, false, true>(a, sh, n, at, u0, u1, R, x0, mul, b, acc);
+    if (a.shared) bwd_kind<T, DP, true, true>(a, sh, n, at, u0, u1, R, x0, ex, b, acc);
+    if (!second) bwd_kind<T, DP, true, false>(a, sh, n, at, u0, u1, R, x0, ex, b, acc);
+    if (second || a.shared) bwd_kind<T, DP, false, true>(a, sh, n, at, u0, u1, R, x0, ex, b, acc);
 
     const float out = a.out_scale * (kScaled ? ldexpf(1.f, -ex) : 1.f);
     const bool whole = u0 == 0 && u1 == per;
@@ -894,15 +907,17 @@ int bwd_groups(int D) { return device_cu_count() * (D <= 128 ? 2 : 1); }
 
 // The gradient's workspace, in bytes from its start.
 struct BwdSpace {
-  size_t gmax, partner, first, expo, part, bytes;
+  size_t gmax, partner, flags, first, expo, aux, part, bytes;
 };
-BwdSpace bwd_space(int E, int V, int D) {
+BwdSpace bwd_space(int E, int P, int V, int D) {
   auto up = [](size_t n) { return (n + 15) / 16 * 16; };
   BwdSpace s{};
   s.partner = s.gmax + up((size_t)E * 4);
-  s.first = s.partner + up((size_t)E * 4);
+  s.flags = s.partner + up((size_t)E * 4);
+  s.first = s.flags + up((size_t)E * 4);
   s.expo = s.first + up(((size_t)V + 1) * 8);
-  s.part = s.expo + up((size_t)V * 4);
+  s.aux = s.expo + up((size_t)V * 4);
+  s.part = s.aux + (size_t)E * y_tiles(P) * kRowsY * 16;
   s.bytes = s.part + (size_t)2 * bwd_groups(D) * kRowsB * D * 4;
   return s;
 }
@@ -938,7 +953,7 @@ extern "C" {
 size_t droid_corr_loss_workspace(int E, int N1, int P, int N2, int Q, int D, int backward) {
   if (E <= 0 || N1 < 0 || P <= 0 || N2 < 0 || Q <= 0 || D <= 0) return 0;
   if (!backward) return (size_t)E * P * fwd_split(E, P, Q) * sizeof(float2);
-  return bwd_space(E, N1 + N2, D).bytes;
+  return bwd_space(E, P, N1 + N2, D).bytes;
 }
 
 int droid_corr_loss_forward(int dtype, const void* fmap1, const void* fmap2, const int* f1, const int* f2,
@@ -989,13 +1004,14 @@ int droid_corr_loss_backward(int dtype, const void* fmap1, const void* fmap2, co
     return fail(kInvalidArgument, what + ": workspace too small");
   if (n1 + n2 == 0) return kOk;
   char* const w = static_cast<char*>(ws);
-  const BwdSpace sp = bwd_space(E, n1 + n2, D);
+  const BwdSpace sp = bwd_space(E, P, n1 + n2, D);
   BwdArgs a{};
   a.f1 = fmap1, a.f2 = fmap2, a.e1 = f1, a.e2 = f2, a.idx = idx, a.prob = prob, a.lse = lse, a.g = gloss;
   a.d1 = dfmap1, a.d2 = dfmap2;
   a.gmax = reinterpret_cast<float*>(w + sp.gmax), a.partner = reinterpret_cast<int*>(w + sp.partner);
   a.first = reinterpret_cast<long long*>(w + sp.first), a.expo = reinterpret_cast<int*>(w + sp.expo);
-  a.part = reinterpret_cast<float*>(w + sp.part);
+  a.part = reinterpret_cast<float*>(w + sp.part), a.flags = reinterpret_cast<int*>(w + sp.flags);
+  a.aux = reinterpret_cast<bhalf8*>(w + sp.aux);
   a.E = E, a.N1 = N1, a.P = P, a.N2 = N2, a.Q = Q, a.D = D, a.K = K, a.shared = shared != 0;
   a.tiles1 = ceil_div(P, kRowsB), a.tiles2 = ceil_div(Q, kRowsB);
   a.n1 = n1, a.V = n1 + n2, a.G = bwd_groups(D);
