@@ -225,8 +225,9 @@ struct RowArgs {
 
 // One query row on 16 lanes: joins the shares of its sum, takes the K target
 // logits as fp32 dot products (a row of D values is 16 lanes x 16 B) and forms
-// the loss.  Rows without a target (all negative, or logits of -inf): loss 0 and lse = +inf, which
-// makes every weight of the backward pass 0.  A target >= Q, an edge outside the
+// the loss.  Rows without a target (all negative, or logits of -inf): loss 0 and lse = +inf, or -inf
+// where the row's features are not all finite (the backward pass must not touch
+// those).  A target >= Q, an edge outside the
 // frames: NaN.
 template <typename T>
 __global__ void __launch_bounds__(kLT) corr_loss_row_kernel(RowArgs a) {
@@ -265,11 +266,20 @@ __global__ void __launch_bounds__(kLT) corr_loss_row_kernel(RowArgs a) {
     }
   }
   const float any = max16(used ? 1.f : 0.f), wrong = max16(bad ? 1.f : 0.f);
+  const T* f1 = static_cast<const T*>(a.f1) + ((long)i * a.P + p) * a.D;
   if (any == 0.f || wrong != 0.f) {
     const bool ignored = any == 0.f;
+    float finite = 0.f;   // 0 while every feature is
+    if (ignored && edge)
+      for (int d = 8 * l; d < a.D; d += 128) {
+        const auto x = *reinterpret_cast<const typename Op<T>::vec8*>(f1 + d);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) finite = fmaf((float)x[q], 0.f, finite);
+      }
+    finite = sum16(finite);
     if (l == 0) {
       a.loss[row] = ignored ? 0.f : NAN;
-      a.lse[row] = ignored ? INFINITY : NAN;
+      a.lse[row] = !ignored ? NAN : finite == 0.f ? INFINITY : -INFINITY;
     }
     if (a.prob)
       for (int k = l; k < a.K; k += 16) a.prob[row * a.K + k] = 0.f;
@@ -301,9 +311,8 @@ __global__ void __launch_bounds__(kLT) corr_loss_row_kernel(RowArgs a) {
     sum += v.y * __builtin_amdgcn_exp2f(v.x - m);
   }
   sum = sum16(sum);
-  const float lse2 = m + log2f(sum);
+  const float lse2 = sum > 0.f ? m + log2f(sum) : NAN;
   // sum_k pi_k s_k, as one dot product with the pi-weighted sum of the target rows
-  const T* f1 = static_cast<const T*>(a.f1) + ((long)i * a.P + p) * a.D;
   const T* f2 = static_cast<const T*>(a.f2) + (long)j * a.Q * a.D;
   float dot = 0.f;
   for (int k = 0; k < a.K; ++k) {
@@ -348,9 +357,9 @@ __global__ void __launch_bounds__(kLT) corr_loss_row_kernel(RowArgs a) {
 // places took 1137 us, shares of the streamed axis by a cost model 867 us, with
 // uneven graphs up to twice their even share.)
 
-constexpr int kUnitBoth = 3, kUnitOne = 2;   // cost of a step with both directions / one (measured about 3 : 2)
+constexpr int kUnitBoth = 6, kUnitSrc = 4, kUnitDst = 5;   // relative cost of a step (measured 6300 : 4100 : 5400 clk)
 constexpr int kJoin = 8;                     // workgroups that join one item
-constexpr int kMinUnits = 16;                // smallest share worth a workgroup
+constexpr int kMinUnits = 32;                // smallest share worth a workgroup
 
 struct BwdArgs {
   const void *f1, *f2;
@@ -358,7 +367,7 @@ struct BwdArgs {
   const float *prob, *lse, *g; // prob null: 1
   void *d1, *d2;               // (N1, P, D), (N2, Q, D)
   float* gmax;                 // (E) largest |g|; -1: no row has a target
-  int* flags;                  // (E) 1: a row is left out, 2: a g is negative
+  int* flags;                  // (E) 1: a left-out row is not finite, 2: a g is negative
   bhalf8* aux;                 // (E, tiles of P, 64) the queries' exponents (corr_edge_kernel)
   int* partner;                // (E) the reverse edge that is done together with this one, -1: none
   long long* first;            // (V + 1) units before frame slot v; the slots: f1's frames (d1 wanted), then f2's
@@ -395,12 +404,12 @@ __global__ void __launch_bounds__(kLT) corr_edge_kernel(BwdArgs a) {
   for (int p = tid; p < padded; p += kLT) {
     const float l = p < a.P ? a.lse[(long)e * a.P + p] : INFINITY;
     float v = -INFINITY, g = 0.f;
-    if (l != INFINITY) {
+    if (fabsf(l) != INFINITY) {
       g = a.g[(long)e * a.P + p];
       m = fmaxf(fmaxf(m, 0.f), fabsf(g));
       v = (log2f(fabsf(g)) - l) / a.c;
       if (g < 0.f) f |= 2;
-    } else if (p < a.P) {
+    } else if (l < 0.f) {
       f |= 1;
     }
     const __bf16 hi = (__bf16)v, z = (__bf16)0.f;
@@ -485,8 +494,8 @@ __global__ void __launch_bounds__(1024) corr_plan_kernel(BwdArgs a) {
     if (v < a.V) {
       const bool first = v < a.n1;
       const int tiles = first ? a.tiles1 : a.tiles2;
-      u = (long long)tiles * ((both[tid] * (long long)kUnitBoth + src[tid] * (long long)kUnitOne) * y_tiles(a.Q) +
-                              dst[tid] * (long long)kUnitOne * y_tiles(a.P));
+      u = (long long)tiles * ((both[tid] * (long long)kUnitBoth + src[tid] * (long long)kUnitSrc) * y_tiles(a.Q) +
+                              dst[tid] * (long long)kUnitDst * y_tiles(a.P));
       a.expo[v] = g_exponent(gm[tid]);
     }
     // inclusive scan over the chunk
@@ -522,7 +531,7 @@ __device__ __forceinline__ int slot_of(const BwdArgs& a, long long u) {
   return lo;
 }
 
-constexpr int kChunk = 32;       // tiles whose sparse records are in LDS at a time
+constexpr int kChunk = 32;       // at most as many tiles' sparse records are in LDS at a time
 constexpr int kRecords = 3072;   // of them; where a chunk has more, its entries are read again half tile by half tile
 
 // What a workgroup of the gradient kernel keeps in LDS.
@@ -566,7 +575,7 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
   bool live = false;   // a stationary row has a target
   if constexpr (SRC) {
     if (x < R) {
-      lx = a.lse[(long)es * a.P + x];
+      lx = fabsf(a.lse[(long)es * a.P + x]) == INFINITY ? INFINITY : a.lse[(long)es * a.P + x];
       gx = lx == INFINITY ? 0.f : lx == lx ? a.g[(long)es * a.P + x] * mul : NAN;
     }
     live = __syncthreads_or(lx != INFINITY);
@@ -584,7 +593,7 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
         if (y >= y0 && y < y1) {
           const int r = q / K;
           f(y, r, [&] {
-            return (a.lse[row0 + r] == INFINITY ? 0.f : a.g[row0 + r] * mul) * (a.prob ? a.prob[row0 * K + q] : 1.f);
+            return (fabsf(a.lse[row0 + r]) == INFINITY ? 0.f : a.g[row0 + r] * mul) * (a.prob ? a.prob[row0 * K + q] : 1.f);
           });
         }
       }
@@ -598,7 +607,7 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
         if (v >= xa && v < xb) {
           const int r = q / K;
           f(y0 + r, v, [&] {
-            return (a.lse[row0 + r] == INFINITY ? 0.f : a.g[row0 + r] * mul) * (a.prob ? a.prob[row0 * K + q] : 1.f);
+            return (fabsf(a.lse[row0 + r]) == INFINITY ? 0.f : a.g[row0 + r] * mul) * (a.prob ? a.prob[row0 * K + q] : 1.f);
           });
         }
       };
@@ -617,18 +626,21 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
       for (; q < total; ++q) one(q, p[q]);   // the last piece, on one thread
     }
   };
+  // 256 K terms an edge where the targets are spread evenly: chunks of about a
+  // third of what fits
+  const int ct = max(2, min(kChunk, kRecords / 768 * y_tiles(n_y) / K));
   int c0 = 0;            // the chunk's first tile
   bool stored = false;   // its records are in LDS
   auto chunk = [&](int t) {   // between barriers: called where all waves are past the last chunk
     c0 = t;
-    const int ya = t * kRowsY, yb = min(min(t + kChunk, t1) * kRowsY, n_y);
+    const int ya = t * kRowsY, yb = min(min(t + ct, t1) * kRowsY, n_y);
     const int y_first = ya;
     for (int q = tid; q <= kChunk * 8; q += kLT) sh.bucket[q] = 0;
     __syncthreads();
     auto bucket = [&](int y, int v) { return (y - y_first) / 32 * 4 + v / 32; };
     each_term(ya, yb, 0, kRowsB, tid, kLT, [&](int y, int v, auto) { atomicAdd(&sh.bucket[bucket(y, v)], 1); });
     __syncthreads();
-    // exclusive sums of the kChunk * 8 = kLT counts
+    // exclusive sums of the kChunk * 8 = kLT counts (those past ct tiles are 0)
     const int n = sh.bucket[tid];
     int s = n;
     for (int o = 1; o < 64; o <<= 1) {
@@ -652,8 +664,8 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
   };
   // Streamed queries: |g| mul p2 = 2^(c (s + v) + ex) with their exponents v, which
   // one more MFMA step adds (three bf16 times ones).  They are staged two tiles
-  // ahead: v = -inf marks a row without a gradient, whose features must not be
-  // read (unless as live keys) when its tile is staged.
+  // ahead: v = -inf marks a row without a gradient; where such rows are not finite
+  // they are staged as zeros (unless they are live keys: then the NaN is theirs).
   const rsrc_t raux = make_rsrc(a.aux + (long)ed * y_tiles(a.P) * kRowsY, (unsigned)y_tiles(a.P) * kRowsY * 16);
   auto stage_aux = [&](int t, int slot) {
     if (DST && wave == 0) dma16(raux, lds_addr(sh.aux[slot]), (unsigned)(t * kRowsY + lane) * 16);
@@ -680,7 +692,7 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
   __syncthreads();
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1, next = slot == 2 ? 0 : slot + 1, after = next == 2 ? 0 : next + 1;
-    if (t == c0 + kChunk) chunk(t);
+    if (t == c0 + ct) chunk(t);
     const unsigned cur = lds_addr(sh.tile[buf]), row0 = row_addr<DP>(cur, fresh(lane));
     if (t + 1 < t1) {
       stage(t + 1, buf ^ 1, next);
@@ -703,6 +715,26 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
 #pragma unroll
       for (int d = 0; d < KD; ++d) sc[k] = Op<T>::mfma(fa[k][d], b[d], sc[k]);
     }
+    // The second product's operand: rows d of the transposed tile.  As the address
+    // lane 4 q + p of its 16-lane group a lane points at row 16 k + 8 u + 4 h + q,
+    // values 32 d + 16 ((lane >> 4) & 1) + 4 p .. + 3; d and u move the swizzled
+    // address by an XOR, k and u by whole rows.
+    const int tv = fresh(lane), q4 = ((tv & 15) >> 2) + 4 * (tv >> 5), s0 = 2 * ((tv >> 4) & 1) + ((tv >> 1) & 1);
+    const unsigned tr0 = cur + q4 * RB + ((s0 ^ swz<DP>(q4)) << 4) + (tv & 1) * 8;
+    auto transposed = [&](int d, int k) {
+      struct { short4_t lo, hi; } both = {
+          __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) short4_t*)(uintptr_t)((tr0 ^ (d << 6)) + 16 * k * RB)),
+          __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) short4_t*)(uintptr_t)((tr0 ^ (d << 6 | 32)) + (16 * k + 8) * RB))};
+      return __builtin_bit_cast(vec8, both);
+    };
+    constexpr int kAhead = DP / 64;   // half of them are read before the weights are formed
+    vec8 ft[kAhead][4];
+#pragma unroll
+    for (int d = 0; d < kAhead; ++d)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) ft[d][k] = transposed(d, k);
     vec8 ds[4];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -742,27 +774,10 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
 #pragma unroll
       for (int q = 0; q < 16; ++q) ds[2 * k + (q >> 3)][q & 7] = (T)wg[q];
     }
-    // second product: rows d of the transposed tile.  As the address lane 4 q + p
-    // of its 16-lane group a lane points at row 16 k + 8 u + 4 h + q, values
-    // 32 d + 16 ((lane >> 4) & 1) + 4 p .. + 3; d and u move the swizzled address by
-    // an XOR, k and u by whole rows.
-    {
-      const int v = fresh(lane), q4 = ((v & 15) >> 2) + 4 * (v >> 5), s0 = 2 * ((v >> 4) & 1) + ((v >> 1) & 1);
-      const unsigned tr0 = cur + q4 * RB + ((s0 ^ swz<DP>(q4)) << 4) + (v & 1) * 8;
 #pragma unroll
-      for (int d = 0; d < DP / 32; ++d) {
+    for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          short4_t r4[2];
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-            r4[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)(uintptr_t)(
-                (tr0 ^ (d << 6 | u << 5)) + (16 * k + 8 * u) * RB));
-          struct { short4_t lo, hi; } both = {r4[0], r4[1]};
-          acc[d] = Op<T>::mfma(__builtin_bit_cast(vec8, both), ds[k], acc[d]);
-        }
-      }
-    }
+      for (int k = 0; k < 4; ++k) acc[d] = Op<T>::mfma(d < kAhead ? ft[d < kAhead ? d : 0][k] : transposed(d, k), ds[k], acc[d]);
     slot = next;
     loads_done();
     __syncthreads();
@@ -777,7 +792,7 @@ __device__ __forceinline__ void bwd_kind(const BwdArgs& a, BwdShared<DP>& sh, in
                                          long long u1, int R, int x0, int ex,
                                          const typename Op<T>::vec8 (&b)[DP / 16], floatx16 (&acc)[DP / 32]) {
   const int tid = fresh(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  constexpr int unit = SRC && DST ? kUnitBoth : kUnitOne;
+  constexpr int unit = SRC && DST ? kUnitBoth : SRC ? kUnitSrc : kUnitDst;
   const int nt = y_tiles(SRC ? a.Q : a.P);
   for (int e0 = 0; e0 < a.E && at < u1; e0 += kLT) {
     const int e = e0 + tid;
