@@ -133,6 +133,18 @@ __device__ __forceinline__ int fresh(int v) {
   return v;
 }
 
+// Asks the scheduler for N groups of one matrix, V vector and X transcendental
+// instructions.
+template <int N, int V, int X>
+__device__ __forceinline__ void interleave() {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x002, V, 0);
+    __builtin_amdgcn_sched_group_barrier(0x400, X, 0);
+  }
+}
+
 // workgroup -> work item: the 8 XCDs each take a contiguous share, so the
 // workgroups that stream the same frame share an L2.
 __device__ __forceinline__ int xcd_item(int bid, int items) {
@@ -458,7 +470,7 @@ __device__ __forceinline__ bool edge_in(const BwdArgs& a, int e) {
 // Whether it is done together with its reverse.
 __device__ __forceinline__ bool edge_paired(const BwdArgs& a, int e) {
   const int r = a.partner[e];
-  return r >= 0 && a.gmax[r] >= 0.f;
+  return r >= 0 && a.gmax[r] >= 0.f && !((a.flags[e] | a.flags[r]) & 2);
 }
 
 // One workgroup: the units of every frame slot's items and their running sum.
@@ -549,7 +561,8 @@ struct BwdShared {
 };
 
 // The steps [t0, t1) of one edge (es: x are its queries) and / or its reverse
-// (ed: the streamed rows y are its queries).
+// (ed: the streamed rows y are its queries; NEG: some g of it are negative, which
+// the exponents do not hold).
 //
 // The sparse targets (g pi at (y, x)) go through a dense, wave-private LDS image
 // of half a tile, used only where there is one: the subtraction happens in fp32,
@@ -557,7 +570,7 @@ struct BwdShared {
 // every kChunk tiles the entries of the rows x and of the streamed rows are
 // sorted by half tile and wave into LDS (two passes over them: count, place), so
 // that the loop meets them without a load from memory.
-template <typename T, int DP, bool SRC, bool DST>
+template <typename T, int DP, bool SRC, bool DST, bool NEG>
 __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, int es, int ed, int t0, int t1, int R,
                                          int x0, int ex, const typename Op<T>::vec8 (&b)[DP / 16],
                                          floatx16 (&acc)[DP / 32]) {
@@ -671,7 +684,7 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
     if (DST && wave == 0) dma16(raux, lds_addr(sh.aux[slot]), (unsigned)(t * kRowsY + lane) * 16);
   };
   const int ef = DST ? a.flags[ed] : 0;
-  const bool holes = (ef & 1) && !(SRC && live), neg = ef & 2;
+  const bool holes = (ef & 1) && !(SRC && live);
   const __bf16 one = (__bf16)(h ? 0.f : 1.f), z16 = (__bf16)0.f;
   const bhalf8 ones = {one, one, one, z16, z16, z16, z16, z16};
   auto stage = [&](int t, int buf, int slot) {
@@ -704,17 +717,16 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
     for (int k = 0; k < 2; ++k)
 #pragma unroll
       for (int d = 0; d < KD; ++d) fa[k][d] = *(ptr)(uintptr_t)((row0 ^ (d << 5)) + k * 64 * DP);
+    bhalf8 av[2];
+    if constexpr (DST)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        av[k] = sh.aux[slot][32 * k + (lane & 31)];
+        if (h) av[k] = bhalf8{z16, z16, z16, z16, z16, z16, z16, z16};   // (0 times an infinity is not 0)
+      }
     const int bk = ((t - c0) * 2) * 4 + wave;   // the wave's records: half 0, half 1
     const int4 br = make_int4(sh.bucket[bk > 0 ? bk - 1 : kChunk * 8], sh.bucket[bk], sh.bucket[bk + 3], sh.bucket[bk + 4]);
     float (&dl)[32][32] = sh.delta[wave];
-    floatx16 sc[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) sc[k][i] = 0.f;
-#pragma unroll
-      for (int d = 0; d < KD; ++d) sc[k] = Op<T>::mfma(fa[k][d], b[d], sc[k]);
-    }
     // The second product's operand: rows d of the transposed tile.  As the address
     // lane 4 q + p of its 16-lane group a lane points at row 16 k + 8 u + 4 h + q,
     // values 32 d + 16 ((lane >> 4) & 1) + 4 p .. + 3; d and u move the swizzled
@@ -729,37 +741,41 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
               (__attribute__((address_space(3))) short4_t*)(uintptr_t)((tr0 ^ (d << 6 | 32)) + (16 * k + 8) * RB))};
       return __builtin_bit_cast(vec8, both);
     };
-    constexpr int kAhead = DP / 64;   // half of them are read before the weights are formed
-    vec8 ft[kAhead][4];
+    auto product = [&](int k) {
+      floatx16 sc;
 #pragma unroll
-    for (int d = 0; d < kAhead; ++d)
+      for (int i = 0; i < 16; ++i) sc[i] = 0.f;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) ft[d][k] = transposed(d, k);
-    vec8 ds[4];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      float wg[16];
+      for (int d = 0; d < KD; ++d) sc = Op<T>::mfma(fa[k][d], b[d], sc);
+      return sc;
+    };
+    float wg[16];
+    auto weights = [&](int k, const floatx16& sc) {
 #pragma unroll
       for (int q = 0; q < 16; ++q) wg[q] = 0.f;
       if constexpr (DST) {
-        bhalf8 v = sh.aux[slot][32 * k + (lane & 31)];
-        if (h) v = bhalf8{z16, z16, z16, z16, z16, z16, z16, z16};   // (0 times an infinity is not 0)
-        const floatx16 s2 = Op<__bf16>::mfma(v, ones, sc[k]);
+        const floatx16 s2 = Op<__bf16>::mfma(av[k], ones, sc);
 #pragma unroll
-        for (int q = 0; q < 16; ++q) wg[q] = __builtin_amdgcn_exp2f(fmaf(s2[q], a.c, fex));
-        if (neg) {
-#pragma unroll
-          for (int q = 0; q < 16; ++q) wg[q] *= (float)sh.aux[slot][32 * k + 8 * (q >> 2) + 4 * h + (q & 3)][3];
+        for (int q = 0; q < 16; ++q) {
+          wg[q] = __builtin_amdgcn_exp2f(fmaf(s2[q], a.c, fex));
+          if constexpr (NEG) wg[q] *= (float)sh.aux[slot][32 * k + 8 * (q >> 2) + 4 * h + (q & 3)][3];
         }
       }
       if constexpr (SRC) {
         // p1 clamped to [0, 1]: a NaN logit of a left-out row counts as 0
 #pragma unroll
-        for (int q = 0; q < 16; ++q)
-          wg[q] = fmaf(gx, __builtin_amdgcn_fmed3f(__builtin_amdgcn_exp2f(fmaf(sc[k][q], a.c, -lx)), 0.f, 1.f), wg[q]);
+        for (int q = 0; q < 16; ++q) {
+          const float p1 = __builtin_amdgcn_fmed3f(__builtin_amdgcn_exp2f(fmaf(sc[q], a.c, -lx)), 0.f, 1.f);
+          wg[q] = DST ? fmaf(gx, p1, wg[q]) : gx * p1;
+        }
       }
-      const int lo = __builtin_amdgcn_readfirstlane(k ? br.z : br.x), hi = __builtin_amdgcn_readfirstlane(k ? br.w : br.y);
-      if (stored ? lo < hi : hi > 0) {
+    };
+    vec8 ds[2];
+    auto sparse_and_round = [&](int k) {
+      // (no branch on `stored` here: the weights' instructions would sink below it)
+      const int lo = __builtin_amdgcn_readfirstlane(k ? br.z : br.x) & -(int)stored;
+      const int hi = __builtin_amdgcn_readfirstlane(k ? br.w : br.y);
+      if (lo < hi) {
         const int v = fresh(lane), y0 = t * kRowsY + 32 * k;
         if (stored)
           for (int q = lo + v; q < hi; q += 64) atomicAdd(&dl[sh.pos[q][0]][sh.pos[q][1]], sh.val[q]);
@@ -772,12 +788,45 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
         for (int q = v; q < 32 * 32 / 4; q += 64) reinterpret_cast<float4*>(&dl[0][0])[q] = make_float4(0.f, 0.f, 0.f, 0.f);
       }
 #pragma unroll
-      for (int q = 0; q < 16; ++q) ds[2 * k + (q >> 3)][q & 7] = (T)wg[q];
+      for (int q = 0; q < 16; ++q) ds[q >> 3][q & 7] = (T)wg[q];
+    };
+    // The order of a step, per half: logits, weights, second product - with one
+    // half's matrix instructions between the other's vector ones (the wave issues
+    // in order; two waves a SIMD do not fill its gaps by themselves).
+    const floatx16 sc0 = product(0);
+    __builtin_amdgcn_sched_barrier(0);
+    const floatx16 sc1 = product(1);
+    weights(0, sc0);
+    interleave<KD, SRC && DST ? 7 : 4, SRC && DST ? 4 : 2>();
+    __builtin_amdgcn_sched_barrier(0);
+    vec8 ft[2][DP / 32];
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) ft[k][d] = transposed(d, k);
+    sparse_and_round(0);
+    {
+      const vec8 d0 = ds[0], d1 = ds[1];
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d) {
+        acc[d] = Op<T>::mfma(ft[0][d], d0, acc[d]);
+        acc[d] = Op<T>::mfma(ft[1][d], d1, acc[d]);
+      }
+      weights(1, sc1);
+      interleave<DP / 16, SRC && DST ? 7 : 4, SRC && DST ? 4 : 2>();
+      __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) acc[d] = Op<T>::mfma(d < kAhead ? ft[d < kAhead ? d : 0][k] : transposed(d, k), ds[k], acc[d]);
+      for (int k = 0; k < 2; ++k) ft[k][d] = transposed(d, 2 + k);
+    sparse_and_round(1);
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) {
+      acc[d] = Op<T>::mfma(ft[0][d], ds[0], acc[d]);
+      acc[d] = Op<T>::mfma(ft[1][d], ds[1], acc[d]);
+    }
     slot = next;
     loads_done();
     __syncthreads();
@@ -787,7 +836,7 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
 // The edges of one kind at frame n, 256 at a time, in order; `at`: units of the
 // item before this kind's first edge (moved past its last), [u0, u1) the units
 // that are done here.
-template <typename T, int DP, bool SRC, bool DST>
+template <typename T, int DP, bool SRC, bool DST, bool NEG = false>
 __device__ __forceinline__ void bwd_kind(const BwdArgs& a, BwdShared<DP>& sh, int n, long long& at, long long u0,
                                          long long u1, int R, int x0, int ex,
                                          const typename Op<T>::vec8 (&b)[DP / 16], floatx16 (&acc)[DP / 32]) {
@@ -797,7 +846,7 @@ __device__ __forceinline__ void bwd_kind(const BwdArgs& a, BwdShared<DP>& sh, in
   for (int e0 = 0; e0 < a.E && at < u1; e0 += kLT) {
     const int e = e0 + tid;
     bool in = e < a.E && (SRC ? a.e1 : a.e2)[e] == n;
-    if (in) in = edge_in(a, e) && (SRC && DST) == edge_paired(a, e);
+    if (in) in = edge_in(a, e) && (SRC && DST) == edge_paired(a, e) && (SRC || ((a.flags[e] & 2) != 0) == NEG);
     const unsigned long long bal = __ballot(in);
     if (lane == 0) sh.ecount[wave] = __popcll(bal);
     __syncthreads();
@@ -812,7 +861,7 @@ __device__ __forceinline__ void bwd_kind(const BwdArgs& a, BwdShared<DP>& sh, in
       if (t0 >= t1) continue;
       const int eq = __builtin_amdgcn_readfirstlane(sh.elist[q]);
       const int er = SRC && DST ? __builtin_amdgcn_readfirstlane(a.partner[eq]) : eq;
-      bwd_edge<T, DP, SRC, DST>(a, sh, eq, er, t0, t1, R, x0, ex, b, acc);
+      bwd_edge<T, DP, SRC, DST, NEG>(a, sh, eq, er, t0, t1, R, x0, ex, b, acc);
     }
     __syncthreads();
   }
@@ -852,7 +901,10 @@ __global__ void __launch_bounds__(kLT, DP <= 128 ? 2 : 1) corr_loss_bwd_kernel(B
     long long at = 0;
     if (a.shared) bwd_kind<T, DP, true, true>(a, sh, n, at, u0, u1, R, x0, ex, b, acc);
     if (!second) bwd_kind<T, DP, true, false>(a, sh, n, at, u0, u1, R, x0, ex, b, acc);
-    if (second || a.shared) bwd_kind<T, DP, false, true>(a, sh, n, at, u0, u1, R, x0, ex, b, acc);
+    if (second || a.shared) {
+      bwd_kind<T, DP, false, true>(a, sh, n, at, u0, u1, R, x0, ex, b, acc);
+      bwd_kind<T, DP, false, true, true>(a, sh, n, at, u0, u1, R, x0, ex, b, acc);
+    }
 
     const float out = a.out_scale * (kScaled ? ldexpf(1.f, -ex) : 1.f);
     const bool whole = u0 == 0 && u1 == per;
