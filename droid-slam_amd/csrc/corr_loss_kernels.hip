@@ -22,6 +22,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace droid {
 
@@ -55,6 +56,19 @@ struct Op<__bf16> {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
 };
+
+// lds_dma.hpp's dma16 with 4 B a lane.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void dma4(rsrc_t rs, unsigned lds, unsigned voff) {
+  const rsrc_t r = {__builtin_amdgcn_readfirstlane(rs.x), __builtin_amdgcn_readfirstlane(rs.y),
+                    __builtin_amdgcn_readfirstlane(rs.z), __builtin_amdgcn_readfirstlane(rs.w)};
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(r)
+               : "memory", "m0");
+}
+#pragma clang diagnostic pop
 
 // A streamed tile in LDS: kRowsY rows of DP values, the 16-B slot s of row r
 // stored at slot s ^ swz(r).  Rows of 256 B and more meet in the same banks, so
@@ -126,23 +140,20 @@ __device__ __forceinline__ void loads_done() {
   asm volatile("" ::: "memory");
 }
 
+// The same, but for the wave's last N LDS-DMAs (and one of the first wave's, where
+// AUX).
+template <int N, bool AUX>
+__device__ __forceinline__ void loads_left(int wave) {
+  if (AUX && wave == 0) __builtin_amdgcn_s_waitcnt(0x0f70 | (N + 1));
+  else __builtin_amdgcn_s_waitcnt(0x0f70 | N);
+  asm volatile("" ::: "memory");
+}
+
 // v, as a value that the compiler knows nothing of: what is computed from it is
 // computed here and not kept in registers over the loops around.
 __device__ __forceinline__ int fresh(int v) {
   asm volatile("" : "+v"(v));
   return v;
-}
-
-// Asks the scheduler for N groups of one matrix, V vector and X transcendental
-// instructions.
-template <int N, int V, int X>
-__device__ __forceinline__ void interleave() {
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-    __builtin_amdgcn_sched_group_barrier(0x002, V, 0);
-    __builtin_amdgcn_sched_group_barrier(0x400, X, 0);
-  }
 }
 
 // workgroup -> work item: the 8 XCDs each take a contiguous share, so the
@@ -353,7 +364,7 @@ __global__ void __launch_bounds__(kLT) corr_loss_row_kernel(RowArgs a) {
 
 // ---- the gradient -----------------------------------------------------------
 //
-// A work item is 128 rows x of one frame, held in registers; its steps are the
+// A work item is 256 rows x of one frame (128 where D > 128), held in registers; its steps are the
 // 64-row tiles y of the frames that share an edge with it, streamed through LDS:
 // the logits s[y][x] are recomputed, turned into weights
 //   ds = g1[x] (p1 - pi1) + g2[y] (p2 - pi2)
@@ -370,6 +381,13 @@ __global__ void __launch_bounds__(kLT) corr_loss_row_kernel(RowArgs a) {
 // uneven graphs up to twice their even share.)
 
 constexpr int kUnitBoth = 6, kUnitSrc = 4, kUnitDst = 5;   // relative cost of a step (measured 6300 : 4100 : 5400 clk)
+// Rows x of a wave, in 32s.  Two where their accumulators fit the registers of one
+// wave a SIMD: a tile read from LDS then serves twice the products.  With one (two
+// waves a SIMD) the LDS pipe bound the kernel: four clips 508 us, the same without
+// exponentials 511 us, without the second product 347 us.
+template <int DP>
+constexpr int kXH = DP <= 128 ? 2 : 1;
+constexpr int bwd_rows(int D) { return 128 * (D <= 128 ? 2 : 1); }
 constexpr int kJoin = 8;                     // workgroups that join one item
 constexpr int kMinUnits = 32;                // smallest share worth a workgroup
 
@@ -380,13 +398,13 @@ struct BwdArgs {
   void *d1, *d2;               // (N1, P, D), (N2, Q, D)
   float* gmax;                 // (E) largest |g|; -1: no row has a target
   int* flags;                  // (E) 1: a left-out row is not finite, 2: a g is negative
-  bhalf8* aux;                 // (E, tiles of P, 64) the queries' exponents (corr_edge_kernel)
+  float* expn;                 // (E, tiles of P, 64) the queries' exponents: log2 |g| - lse, -inf: no gradient
   int* partner;                // (E) the reverse edge that is done together with this one, -1: none
   long long* first;            // (V + 1) units before frame slot v; the slots: f1's frames (d1 wanted), then f2's
   int* expo;                   // (V) fp16: exponent that scales the slot's weights
   float* part;                 // (G, 2, 128, D)
   int E, N1, P, N2, Q, D, K, shared;
-  int tiles1, tiles2;          // 128-row tiles of a frame
+  int tiles1, tiles2;          // items of a frame (bwd_rows rows each)
   int n1, V, G;                // slots of f1, all slots, workgroups
   float c, out_scale;          // scale / T log2(e); scale T
 };
@@ -404,8 +422,7 @@ __device__ __forceinline__ int g_exponent(float gmax) {
 
 // One workgroup an edge: what the gradient kernel wants of its rows, and the
 // reverse edge it may be paired with (the k-th copy of (i, j) with the k-th of
-// (j, i)).  A row's exponent v = (log2 |g| - lse) / c, in units of the dot
-// product, is kept as the sum of three bf16 (24 bits), then g's sign.
+// (j, i)).
 __global__ void __launch_bounds__(kLT) corr_edge_kernel(BwdArgs a) {
   __shared__ float red[kLT / 64];
   __shared__ int cnt[kLT / 64], fl[kLT / 64];
@@ -415,19 +432,16 @@ __global__ void __launch_bounds__(kLT) corr_edge_kernel(BwdArgs a) {
   int f = 0;
   for (int p = tid; p < padded; p += kLT) {
     const float l = p < a.P ? a.lse[(long)e * a.P + p] : INFINITY;
-    float v = -INFINITY, g = 0.f;
+    float v = -INFINITY;
     if (fabsf(l) != INFINITY) {
-      g = a.g[(long)e * a.P + p];
+      const float g = a.g[(long)e * a.P + p];
       m = fmaxf(fmaxf(m, 0.f), fabsf(g));
-      v = (log2f(fabsf(g)) - l) / a.c;
+      v = log2f(fabsf(g)) - l;
       if (g < 0.f) f |= 2;
     } else if (l < 0.f) {
       f |= 1;
     }
-    const __bf16 hi = (__bf16)v, z = (__bf16)0.f;
-    const float r1 = fabsf((float)hi) < INFINITY ? v - (float)hi : 0.f;
-    const __bf16 mid = (__bf16)r1, lo = (__bf16)(r1 - (float)mid);
-    a.aux[(long)e * padded + p] = bhalf8{hi, mid, lo, (__bf16)(g < 0.f ? -1.f : 1.f), z, z, z, z};
+    a.expn[(long)e * padded + p] = v;
   }
   for (int o = 32; o; o >>= 1) {
     m = fmaxf(m, __shfl_xor(m, o, 64));
@@ -506,8 +520,8 @@ __global__ void __launch_bounds__(1024) corr_plan_kernel(BwdArgs a) {
     if (v < a.V) {
       const bool first = v < a.n1;
       const int tiles = first ? a.tiles1 : a.tiles2;
-      u = (long long)tiles * ((both[tid] * (long long)kUnitBoth + src[tid] * (long long)kUnitSrc) * y_tiles(a.Q) +
-                              dst[tid] * (long long)kUnitDst * y_tiles(a.P));
+      u = (long long)tiles * ((both[tid] * (long long)kUnitBoth + src[tid] * (long long)kUnitSrc) * (y_tiles(a.Q) + 1) +
+                              dst[tid] * (long long)kUnitDst * (y_tiles(a.P) + 1));
       a.expo[v] = g_exponent(gm[tid]);
     }
     // inclusive scan over the chunk
@@ -544,14 +558,14 @@ __device__ __forceinline__ int slot_of(const BwdArgs& a, long long u) {
 }
 
 constexpr int kChunk = 32;       // at most as many tiles' sparse records are in LDS at a time
-constexpr int kRecords = 3072;   // of them; where a chunk has more, its entries are read again half tile by half tile
+constexpr int kRecords = 6144;   // of them; where a chunk has more, its entries are read again half tile by half tile
 
 // What a workgroup of the gradient kernel keeps in LDS.
 template <int DP>
 struct BwdShared {
-  char tile[2][kRowsY * 2 * DP];           // rows aligned to their size
-  float delta[4][32][32];                  // a wave's sparse terms of half a tile; zero between uses
-  bhalf8 aux[3][kRowsY];                   // the streamed queries' exponents, two tiles ahead
+  char tile[3][kRowsY * 2 * DP];           // rows aligned to their size; two tiles ahead
+  float delta[4][32][32 * kXH<DP>];        // a wave's sparse terms of half a tile; zero between uses
+  float expn[4][kRowsY];                   // the streamed queries' exponents, three tiles ahead
   int elist[kLT];
   int ecount[4];
   int bucket[kChunk * 8 + 1];              // ends of the sparse records of (half tile, wave)
@@ -572,26 +586,31 @@ struct BwdShared {
 // that the loop meets them without a load from memory.
 template <typename T, int DP, bool SRC, bool DST, bool NEG>
 __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, int es, int ed, int t0, int t1, int R,
-                                         int x0, int ex, const typename Op<T>::vec8 (&b)[DP / 16],
-                                         floatx16 (&acc)[DP / 32]) {
+                                         int x0, int ex, const typename Op<T>::vec8 (&b)[kXH<DP>][DP / 16],
+                                         floatx16 (&acc)[kXH<DP>][DP / 32]) {
   typedef typename Op<T>::vec8 vec8;
   typedef const __attribute__((address_space(3))) vec8* ptr;
   typedef int int4_u __attribute__((ext_vector_type(4), aligned(4)));
-  constexpr int RB = 2 * DP, KD = DP / 16;
+  constexpr int RB = 2 * DP, KD = DP / 16, XH = kXH<DP>, XW = 32 * XH;   // XW rows a wave
+  constexpr int NI = kRowsY * RB / 4096;                                 // LDS-DMAs of a tile a wave
   const int tid = fresh(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-  const int xw = x0 + wave * 32, x = xw + (lane & 31);
   const int n_y = SRC ? a.Q : a.P, K = a.K;
   const rsrc_t rs = make_rsrc(static_cast<const T*>(SRC ? a.f2 : a.f1) + (long)(SRC ? a.e2[es] : a.e1[ed]) * n_y * a.D,
                               (unsigned)n_y * a.D * 2);
   const float mul = ldexpf(1.f, ex), fex = (float)ex;
-  float lx = INFINITY, gx = 0.f;
+  float lx[XH], gx[XH];
   bool live = false;   // a stationary row has a target
   if constexpr (SRC) {
-    if (x < R) {
-      lx = fabsf(a.lse[(long)es * a.P + x]) == INFINITY ? INFINITY : a.lse[(long)es * a.P + x];
-      gx = lx == INFINITY ? 0.f : lx == lx ? a.g[(long)es * a.P + x] * mul : NAN;
+    bool any = false;
+#pragma unroll
+    for (int j = 0; j < XH; ++j) {
+      const int x = x0 + wave * XW + 32 * j + (lane & 31);
+      lx[j] = x < R ? a.lse[(long)es * a.P + x] : INFINITY;
+      if (fabsf(lx[j]) == INFINITY) lx[j] = INFINITY;
+      gx[j] = lx[j] == INFINITY ? 0.f : lx[j] == lx[j] ? a.g[(long)es * a.P + x] * mul : NAN;
+      any |= lx[j] != INFINITY;
     }
-    live = __syncthreads_or(lx != INFINITY);
+    live = __syncthreads_or(any);
     if (!DST && !live) return;   // every row left out: nothing here, whatever the keys hold
   }
   // f(y, x, value) for every sparse term of the streamed rows [y0, y1) and the rows
@@ -639,9 +658,9 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
       for (; q < total; ++q) one(q, p[q]);   // the last piece, on one thread
     }
   };
-  // 256 K terms an edge where the targets are spread evenly: chunks of about a
-  // third of what fits
-  const int ct = max(2, min(kChunk, kRecords / 768 * y_tiles(n_y) / K));
+  // 512 K terms an edge where the targets are spread evenly (256 rows x): chunks of
+  // about a third of what fits
+  const int ct = max(2, min(kChunk, kRecords / (3 * 2 * 4 * XW) * y_tiles(n_y) / K));
   int c0 = 0;            // the chunk's first tile
   bool stored = false;   // its records are in LDS
   auto chunk = [&](int t) {   // between barriers: called where all waves are past the last chunk
@@ -650,8 +669,8 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
     const int y_first = ya;
     for (int q = tid; q <= kChunk * 8; q += kLT) sh.bucket[q] = 0;
     __syncthreads();
-    auto bucket = [&](int y, int v) { return (y - y_first) / 32 * 4 + v / 32; };
-    each_term(ya, yb, 0, kRowsB, tid, kLT, [&](int y, int v, auto) { atomicAdd(&sh.bucket[bucket(y, v)], 1); });
+    auto bucket = [&](int y, int v) { return (y - y_first) / 32 * 4 + v / XW; };
+    each_term(ya, yb, 0, 4 * XW, tid, kLT, [&](int y, int v, auto) { atomicAdd(&sh.bucket[bucket(y, v)], 1); });
     __syncthreads();
     // exclusive sums of the kChunk * 8 = kLT counts (those past ct tiles are 0)
     const int n = sh.bucket[tid];
@@ -667,66 +686,58 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
     sh.bucket[tid] = stored ? s - n : n;   // not stored: the counts, for whether to look at all
     __syncthreads();
     if (stored)
-      each_term(ya, yb, 0, kRowsB, tid, kLT, [&](int y, int v, auto value) {
+      each_term(ya, yb, 0, 4 * XW, tid, kLT, [&](int y, int v, auto value) {
         const int at = atomicAdd(&sh.bucket[bucket(y, v)], 1);   // ends as the bucket's end
         sh.pos[at][0] = (unsigned char)(y & 31);
-        sh.pos[at][1] = (unsigned char)(v & 31);
+        sh.pos[at][1] = (unsigned char)(v & (XW - 1));
         sh.val[at] = value();
       });
     __syncthreads();
   };
-  // Streamed queries: |g| mul p2 = 2^(c (s + v) + ex) with their exponents v, which
-  // one more MFMA step adds (three bf16 times ones).  They are staged two tiles
-  // ahead: v = -inf marks a row without a gradient; where such rows are not finite
-  // they are staged as zeros (unless they are live keys: then the NaN is theirs).
-  const rsrc_t raux = make_rsrc(a.aux + (long)ed * y_tiles(a.P) * kRowsY, (unsigned)y_tiles(a.P) * kRowsY * 16);
-  auto stage_aux = [&](int t, int slot) {
-    if (DST && wave == 0) dma16(raux, lds_addr(sh.aux[slot]), (unsigned)(t * kRowsY + lane) * 16);
+  // Streamed queries: |g| mul p2 = 2^(c s + v + ex) with their exponents v.  They
+  // are staged a tile further ahead: v = -inf marks a row without a gradient; where
+  // such rows are not finite they are staged as zeros (unless they are live keys:
+  // then the NaN is theirs).
+  const rsrc_t rex = make_rsrc(a.expn + (long)ed * y_tiles(a.P) * kRowsY, (unsigned)y_tiles(a.P) * kRowsY * 4);
+  auto stage_expn = [&](int t) {
+    if (DST && wave == 0) dma4(rex, lds_addr(sh.expn[(t - t0) & 3]), (unsigned)(t * kRowsY + lane) * 4);
   };
   const int ef = DST ? a.flags[ed] : 0;
   const bool holes = (ef & 1) && !(SRC && live);
-  const __bf16 one = (__bf16)(h ? 0.f : 1.f), z16 = (__bf16)0.f;
-  const bhalf8 ones = {one, one, one, z16, z16, z16, z16, z16};
-  auto stage = [&](int t, int buf, int slot) {
+  auto stage = [&](int t, int buf) {
     if (!holes)
       stage_tile<T, DP>(rs, sh.tile[buf], t * kRowsY, n_y, a.D, wave, lane, [](int) { return false; });
     else
       stage_tile<T, DP>(rs, sh.tile[buf], t * kRowsY, n_y, a.D, wave, lane,
-                        [&](int row) { return (float)sh.aux[slot][row][0] == -INFINITY; });
+                        [&](int row) { return sh.expn[(t - t0) & 3][row] == -INFINITY; });
   };
-  int slot = 0;   // of tile t's exponents
-  stage_aux(t0, 0);
-  if (t0 + 1 < t1) stage_aux(t0 + 1, 1);
+  // Before the loop: the exponents of three tiles, the features of two.
+  stage_expn(t0);
+  if (t0 + 1 < t1) stage_expn(t0 + 1);
+  if (t0 + 2 < t1) stage_expn(t0 + 2);
   chunk(t0);
   loads_done();
   __syncthreads();
-  stage(t0, 0, 0);
+  stage(t0, 0);
+  if (t0 + 1 < t1) stage(t0 + 1, 1);
   loads_done();
   __syncthreads();
+  int buf = 0;   // of tile t
   for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1, next = slot == 2 ? 0 : slot + 1, after = next == 2 ? 0 : next + 1;
     if (t == c0 + ct) chunk(t);
     const unsigned cur = lds_addr(sh.tile[buf]), row0 = row_addr<DP>(cur, fresh(lane));
-    if (t + 1 < t1) {
-      stage(t + 1, buf ^ 1, next);
-      if (t + 2 < t1) stage_aux(t + 2, after);
+    if (t + 2 < t1) {
+      stage(t + 2, buf == 0 ? 2 : buf - 1);
+      if (t + 3 < t1) stage_expn(t + 3);
     }
-    // both halves' operands of the first product before anything else
     vec8 fa[2][KD];
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
       for (int d = 0; d < KD; ++d) fa[k][d] = *(ptr)(uintptr_t)((row0 ^ (d << 5)) + k * 64 * DP);
-    bhalf8 av[2];
-    if constexpr (DST)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        av[k] = sh.aux[slot][32 * k + (lane & 31)];
-        if (h) av[k] = bhalf8{z16, z16, z16, z16, z16, z16, z16, z16};   // (0 times an infinity is not 0)
-      }
     const int bk = ((t - c0) * 2) * 4 + wave;   // the wave's records: half 0, half 1
     const int4 br = make_int4(sh.bucket[bk > 0 ? bk - 1 : kChunk * 8], sh.bucket[bk], sh.bucket[bk + 3], sh.bucket[bk + 4]);
-    float (&dl)[32][32] = sh.delta[wave];
+    float (&dl)[32][XW] = sh.delta[wave];
     // The second product's operand: rows d of the transposed tile.  As the address
     // lane 4 q + p of its 16-lane group a lane points at row 16 k + 8 u + 4 h + q,
     // values 32 d + 16 ((lane >> 4) & 1) + 4 p .. + 3; d and u move the swizzled
@@ -741,36 +752,65 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
               (__attribute__((address_space(3))) short4_t*)(uintptr_t)((tr0 ^ (d << 6 | 32)) + (16 * k + 8) * RB))};
       return __builtin_bit_cast(vec8, both);
     };
-    auto product = [&](int k) {
-      floatx16 sc;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) sc[i] = 0.f;
-#pragma unroll
-      for (int d = 0; d < KD; ++d) sc = Op<T>::mfma(fa[k][d], b[d], sc);
-      return sc;
+    floatx16 sc[2][XH];
+    float wg[XH][16];
+    // the n-th matrix instruction of a half's logits, and of the second product
+    constexpr int kS = KD * XH, kP = 2 * (DP / 32) * XH;
+    auto logit = [&](int k, int n) {
+      sc[k][n % XH] = Op<T>::mfma(fa[k][n / XH], b[n % XH][n / XH], sc[k][n % XH]);
     };
-    float wg[16];
-    auto weights = [&](int k, const floatx16& sc) {
+    auto zero = [&](int k) {
 #pragma unroll
-      for (int q = 0; q < 16; ++q) wg[q] = 0.f;
-      if constexpr (DST) {
-        const floatx16 s2 = Op<__bf16>::mfma(av[k], ones, sc);
+      for (int j = 0; j < XH; ++j)
 #pragma unroll
-        for (int q = 0; q < 16; ++q) {
-          wg[q] = __builtin_amdgcn_exp2f(fmaf(s2[q], a.c, fex));
-          if constexpr (NEG) wg[q] *= (float)sh.aux[slot][32 * k + 8 * (q >> 2) + 4 * h + (q & 3)][3];
-        }
-      }
-      if constexpr (SRC) {
-        // p1 clamped to [0, 1]: a NaN logit of a left-out row counts as 0
-#pragma unroll
-        for (int q = 0; q < 16; ++q) {
-          const float p1 = __builtin_amdgcn_fmed3f(__builtin_amdgcn_exp2f(fmaf(sc[q], a.c, -lx)), 0.f, 1.f);
-          wg[q] = DST ? fmaf(gx, p1, wg[q]) : gx * p1;
-        }
-      }
+        for (int i = 0; i < 16; ++i) sc[k][j][i] = 0.f;
     };
-    vec8 ds[2];
+    float ve[16];   // the exponents of the half's rows in this lane's places
+    auto exponents = [&](int k) {
+      if constexpr (DST)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float4 v = *reinterpret_cast<const float4*>(&sh.expn[(t - t0) & 3][32 * k + 8 * q + 4 * h]);
+          ve[4 * q] = v.x + fex, ve[4 * q + 1] = v.y + fex, ve[4 * q + 2] = v.z + fex, ve[4 * q + 3] = v.w + fex;
+        }
+    };
+    // The weights of half k with N matrix instructions between them, in exactly this
+    // order (left to itself the scheduler puts them one after the other): per matrix
+    // instruction the exponentials of some elements and the sums of the ones before.
+    auto weights = [&](int k, auto matrix, auto n_tag) {
+      constexpr int N = decltype(n_tag)::value, E = 16 * XH / N;   // elements per matrix instruction
+      static_assert(16 * XH % N == 0, "elements per matrix instruction");
+      float p1[2][E];
+      auto finish = [&](int n) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const int j = (n * E + e) / 16, q = (n * E + e) % 16;
+          if constexpr (SRC) wg[j][q] = DST ? fmaf(gx[j], p1[n & 1][e], wg[j][q]) : gx[j] * p1[n & 1][e];
+        }
+      };
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        matrix(n);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const int j = (n * E + e) / 16, q = (n * E + e) % 16;
+          if constexpr (DST) {
+            wg[j][q] = __builtin_amdgcn_exp2f(fmaf(sc[k][j][q], a.c, ve[q]));
+            if constexpr (NEG) {
+              const int y = t * kRowsY + 32 * k + 8 * (q >> 2) + 4 * h + (q & 3);
+              if (y < n_y && a.g[(long)ed * a.P + y] < 0.f) wg[j][q] = -wg[j][q];
+            }
+          }
+          // p1 clamped to [0, 1]: a NaN logit of a left-out row counts as 0
+          if constexpr (SRC)
+            p1[n & 1][e] = __builtin_amdgcn_fmed3f(__builtin_amdgcn_exp2f(fmaf(sc[k][j][q], a.c, -lx[j])), 0.f, 1.f);
+        }
+        if (n) finish(n - 1);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      finish(N - 1);
+    };
+    vec8 ds[XH][2];
     auto sparse_and_round = [&](int k) {
       // (no branch on `stored` here: the weights' instructions would sink below it)
       const int lo = __builtin_amdgcn_readfirstlane(k ? br.z : br.x) & -(int)stored;
@@ -780,55 +820,53 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
         if (stored)
           for (int q = lo + v; q < hi; q += 64) atomicAdd(&dl[sh.pos[q][0]][sh.pos[q][1]], sh.val[q]);
         else
-          each_term(y0, min(y0 + 32, n_y), wave * 32, wave * 32 + 32, v, 64,
-                    [&](int y, int xx, auto value) { atomicAdd(&dl[y - y0][xx & 31], value()); });
+          each_term(y0, min(y0 + 32, n_y), wave * XW, wave * XW + XW, v, 64,
+                    [&](int y, int xx, auto value) { atomicAdd(&dl[y - y0][xx & (XW - 1)], value()); });
         const float* col = &dl[4 * (v >> 5)][v & 31];
 #pragma unroll
-        for (int q = 0; q < 16; ++q) wg[q] -= col[(8 * (q >> 2) + (q & 3)) * 32];
-        for (int q = v; q < 32 * 32 / 4; q += 64) reinterpret_cast<float4*>(&dl[0][0])[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int j = 0; j < XH; ++j)
+#pragma unroll
+          for (int q = 0; q < 16; ++q) wg[j][q] -= col[(8 * (q >> 2) + (q & 3)) * XW + 32 * j];
+        for (int q = v; q < 32 * XW / 4; q += 64) reinterpret_cast<float4*>(&dl[0][0])[q] = make_float4(0.f, 0.f, 0.f, 0.f);
       }
 #pragma unroll
-      for (int q = 0; q < 16; ++q) ds[q >> 3][q & 7] = (T)wg[q];
+      for (int j = 0; j < XH; ++j)
+#pragma unroll
+        for (int q = 0; q < 16; ++q) ds[j][q >> 3][q & 7] = (T)wg[j][q];
     };
-    // The order of a step, per half: logits, weights, second product - with one
-    // half's matrix instructions between the other's vector ones (the wave issues
-    // in order; two waves a SIMD do not fill its gaps by themselves).
-    const floatx16 sc0 = product(0);
-    __builtin_amdgcn_sched_barrier(0);
-    const floatx16 sc1 = product(1);
-    weights(0, sc0);
-    interleave<KD, SRC && DST ? 7 : 4, SRC && DST ? 4 : 2>();
-    __builtin_amdgcn_sched_barrier(0);
     vec8 ft[2][DP / 32];
+    auto read_transposed = [&](int half) {
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
+      for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-      for (int k = 0; k < 2; ++k) ft[k][d] = transposed(d, k);
+        for (int k = 0; k < 2; ++k) ft[k][d] = transposed(d, 2 * half + k);
+    };
+    auto product = [&](int n) {
+      const int k = n / (kP / 2), d = n % (kP / 2) / XH, j = n % XH;
+      acc[j][d] = Op<T>::mfma(ft[k][d], ds[j][k], acc[j][d]);
+    };
+    // A step: half 0's logits; half 1's between half 0's weights; half 0's second
+    // product between half 1's weights; half 1's second product.
+    zero(0);
+    zero(1);
+    exponents(0);
+#pragma unroll
+    for (int n = 0; n < kS; ++n) logit(0, n);
+    __builtin_amdgcn_sched_barrier(0);
+    weights(0, [&](int n) { logit(1, n); }, std::integral_constant<int, kS>());
+    exponents(1);
+    read_transposed(0);
     sparse_and_round(0);
-    {
-      const vec8 d0 = ds[0], d1 = ds[1];
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int d = 0; d < DP / 32; ++d) {
-        acc[d] = Op<T>::mfma(ft[0][d], d0, acc[d]);
-        acc[d] = Op<T>::mfma(ft[1][d], d1, acc[d]);
-      }
-      weights(1, sc1);
-      interleave<DP / 16, SRC && DST ? 7 : 4, SRC && DST ? 4 : 2>();
-      __builtin_amdgcn_sched_barrier(0);
-    }
-#pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) ft[k][d] = transposed(d, 2 + k);
+    __builtin_amdgcn_sched_barrier(0);
+    weights(1, product, std::integral_constant<int, kP>());
+    read_transposed(1);
     sparse_and_round(1);
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d) {
-      acc[d] = Op<T>::mfma(ft[0][d], ds[0], acc[d]);
-      acc[d] = Op<T>::mfma(ft[1][d], ds[1], acc[d]);
-    }
-    slot = next;
-    loads_done();
+    for (int n = 0; n < kP; ++n) product(n);
+    buf = buf == 2 ? 0 : buf + 1;
+    // tile t + 1 has landed; the loads of t + 2 (and t + 3's exponents) stay in flight
+    if (t + 3 < t1) loads_left<NI, DST>(wave);
+    else loads_done();
     __syncthreads();
   }
 }
@@ -839,7 +877,8 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
 template <typename T, int DP, bool SRC, bool DST, bool NEG = false>
 __device__ __forceinline__ void bwd_kind(const BwdArgs& a, BwdShared<DP>& sh, int n, long long& at, long long u0,
                                          long long u1, int R, int x0, int ex,
-                                         const typename Op<T>::vec8 (&b)[DP / 16], floatx16 (&acc)[DP / 32]) {
+                                         const typename Op<T>::vec8 (&b)[kXH<DP>][DP / 16],
+                                         floatx16 (&acc)[kXH<DP>][DP / 32]) {
   const int tid = fresh(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   constexpr int unit = SRC && DST ? kUnitBoth : SRC ? kUnitSrc : kUnitDst;
   const int nt = y_tiles(SRC ? a.Q : a.P);
@@ -855,7 +894,7 @@ __device__ __forceinline__ void bwd_kind(const BwdArgs& a, BwdShared<DP>& sh, in
     if (in) sh.elist[pos] = e;
     const int cnt = __builtin_amdgcn_readfirstlane(sh.ecount[0] + sh.ecount[1] + sh.ecount[2] + sh.ecount[3]);
     __syncthreads();
-    for (int q = 0; q < cnt && at < u1; ++q, at += (long long)nt * unit) {
+    for (int q = 0; q < cnt && at < u1; ++q, at += (long long)(nt + 1) * unit) {   // one step's time to begin an edge
       // a step is done by the share that its first unit lies in
       const int t0 = (int)max(0ll, (u0 - at + unit - 1) / unit), t1 = (int)min((long long)nt, (u1 - at + unit - 1) / unit);
       if (t0 >= t1) continue;
@@ -869,8 +908,9 @@ __device__ __forceinline__ void bwd_kind(const BwdArgs& a, BwdShared<DP>& sh, in
 
 // One workgroup: its share of the units, item by item.
 template <typename T, int DP>
-__global__ void __launch_bounds__(kLT, DP <= 128 ? 2 : 1) corr_loss_bwd_kernel(BwdArgs a) {
+__global__ void __launch_bounds__(kLT, 1) corr_loss_bwd_kernel(BwdArgs a) {
   constexpr bool kScaled = !__is_same(T, __bf16);
+  constexpr int XH = kXH<DP>, rows = bwd_rows(DP);
   __shared__ __attribute__((aligned(1024))) BwdShared<DP> sh;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int block = xcd_item(blockIdx.x, a.G);
@@ -878,23 +918,26 @@ __global__ void __launch_bounds__(kLT, DP <= 128 ? 2 : 1) corr_loss_bwd_kernel(B
   const long long share = share_units(a), all = a.first[a.V];
   long long u = block * share;
   const long long end = min(u + share, all);
-  for (int q = lane; q < 32 * 32; q += 64) (&sh.delta[wave][0][0])[q] = 0.f;
+  for (int q = lane; q < 32 * 32 * XH; q += 64) (&sh.delta[wave][0][0])[q] = 0.f;
   while (u < end) {
     const int v = slot_of(a, u);
     const bool second = v >= a.n1;
     const int n = second ? v - a.n1 : v, tiles = second ? a.tiles2 : a.tiles1, R = second ? a.Q : a.P;
     const long long per = (a.first[v + 1] - a.first[v]) / tiles;   // units of each of the frame's items
-    const int w = (int)((u - a.first[v]) / per), x0 = w * kRowsB;
+    const int w = (int)((u - a.first[v]) / per), x0 = w * rows;
     const long long item = a.first[v] + w * per;
     const long long u0 = u - item, u1 = min(per, end - item);
-    const int x = x0 + wave * 32 + (lane & 31);
-    typename Op<T>::vec8 b[DP / 16];
-    load_rows<T, DP>(b, static_cast<const T*>(second ? a.f2 : a.f1) + (long)n * R * a.D, x, R, a.D, h);
-    floatx16 acc[DP / 32];
+    typename Op<T>::vec8 b[XH][DP / 16];
+    floatx16 acc[XH][DP / 32];
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
+    for (int j = 0; j < XH; ++j) {
+      load_rows<T, DP>(b[j], static_cast<const T*>(second ? a.f2 : a.f1) + (long)n * R * a.D,
+                       x0 + (wave * XH + j) * 32 + (lane & 31), R, a.D, h);
 #pragma unroll
-      for (int q = 0; q < 16; ++q) acc[d][q] = 0.f;
+      for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int q = 0; q < 16; ++q) acc[j][d][q] = 0.f;
+    }
     const int ex = kScaled ? a.expo[v] : 0;
     // the kinds one after the other: in one loop the compiler keeps the values of
     // all of them in registers and spills
@@ -908,8 +951,10 @@ __global__ void __launch_bounds__(kLT, DP <= 128 ? 2 : 1) corr_loss_bwd_kernel(B
 
     const float out = a.out_scale * (kScaled ? ldexpf(1.f, -ex) : 1.f);
     const bool whole = u0 == 0 && u1 == per;
-    const int xi = fresh(x);
-    if (xi < R) {
+#pragma unroll
+    for (int j = 0; j < XH; ++j) {
+      const int x = x0 + (wave * XH + j) * 32 + (fresh(lane) & 31);
+      if (x >= R) continue;
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
@@ -918,13 +963,13 @@ __global__ void __launch_bounds__(kLT, DP <= 128 ? 2 : 1) corr_loss_bwd_kernel(B
           if (c >= a.D) continue;
           float o[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) o[k] = acc[d][4 * q + k] * out;
+          for (int k = 0; k < 4; ++k) o[k] = acc[j][d][4 * q + k] * out;
           if (whole) {
             typedef T t4 __attribute__((ext_vector_type(4)));
-            *reinterpret_cast<t4*>(static_cast<T*>(second ? a.d2 : a.d1) + ((long)n * R + xi) * a.D + c) =
+            *reinterpret_cast<t4*>(static_cast<T*>(second ? a.d2 : a.d1) + ((long)n * R + x) * a.D + c) =
                 t4{(T)o[0], (T)o[1], (T)o[2], (T)o[3]};
           } else {
-            float* p = a.part + ((long)(2 * block + (u0 == 0)) * kRowsB + (xi - x0)) * a.D + c;
+            float* p = a.part + ((long)(2 * block + (u0 == 0)) * rows + (x - x0)) * a.D + c;
             *reinterpret_cast<float4*>(p) = make_float4(o[0], o[1], o[2], o[3]);
           }
         }
@@ -940,19 +985,19 @@ __global__ void __launch_bounds__(kLT) corr_loss_join_kernel(BwdArgs a) {
   const int items1 = a.n1 * a.tiles1;
   const bool second = (int)blockIdx.x >= items1;
   const int w = second ? blockIdx.x - items1 : blockIdx.x, tiles = second ? a.tiles2 : a.tiles1;
-  const int n = w / tiles, x0 = w % tiles * kRowsB, R = second ? a.Q : a.P, v = second ? a.n1 + n : n;
+  const int n = w / tiles, rows = bwd_rows(a.D), x0 = w % tiles * rows, R = second ? a.Q : a.P, v = second ? a.n1 + n : n;
   const long long per = (a.first[v + 1] - a.first[v]) / tiles, item = a.first[v] + w % tiles * per;
   const long long share = share_units(a);
   const int b0 = (int)(item / share), b1 = per ? (int)((item + per - 1) / share) : b0;
   if (per && b0 == b1) return;
   T* d = static_cast<T*>(second ? a.d2 : a.d1) + ((long)n * R + x0) * a.D;
-  const int total = min(kRowsB, R - x0) * a.D;
+  const int total = min(rows, R - x0) * a.D;
   for (int q = (blockIdx.y * kLT + threadIdx.x) * 4; q < total; q += kLT * 4 * kJoin) {
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
     if (per)
 #pragma unroll 4
       for (int b = b0; b <= b1; ++b) {
-        const float4 p = *reinterpret_cast<const float4*>(a.part + (long)(2 * b + (b == b0)) * kRowsB * a.D + q);
+        const float4 p = *reinterpret_cast<const float4*>(a.part + (long)(2 * b + (b == b0)) * rows * a.D + q);
         s.x += p.x;
         s.y += p.y;
         s.z += p.z;
@@ -969,12 +1014,12 @@ int fwd_split(int E, int P, int Q) {
   return (int)std::max<long>(1, std::min<long>(ceil_div(Q, kRowsY), 1024 / std::max<long>(1, blocks)));
 }
 
-// Workgroups of the gradient kernel: as many as run at once (by its registers).
-int bwd_groups(int D) { return device_cu_count() * (D <= 128 ? 2 : 1); }
+// Workgroups of the gradient kernel: as many as run at once, one a CU by its registers.
+int bwd_groups() { return device_cu_count(); }
 
 // The gradient's workspace, in bytes from its start.
 struct BwdSpace {
-  size_t gmax, partner, flags, first, expo, aux, part, bytes;
+  size_t gmax, partner, flags, first, expo, expn, part, bytes;
 };
 BwdSpace bwd_space(int E, int P, int V, int D) {
   auto up = [](size_t n) { return (n + 15) / 16 * 16; };
@@ -983,9 +1028,9 @@ BwdSpace bwd_space(int E, int P, int V, int D) {
   s.flags = s.partner + up((size_t)E * 4);
   s.first = s.flags + up((size_t)E * 4);
   s.expo = s.first + up(((size_t)V + 1) * 8);
-  s.aux = s.expo + up((size_t)V * 4);
-  s.part = s.aux + (size_t)E * y_tiles(P) * kRowsY * 16;
-  s.bytes = s.part + (size_t)2 * bwd_groups(D) * kRowsB * D * 4;
+  s.expn = s.expo + up((size_t)V * 4);
+  s.part = s.expn + (size_t)E * y_tiles(P) * kRowsY * 4;
+  s.bytes = s.part + (size_t)2 * bwd_groups() * bwd_rows(D) * D * 4;
   return s;
 }
 
@@ -1078,10 +1123,10 @@ int droid_corr_loss_backward(int dtype, const void* fmap1, const void* fmap2, co
   a.gmax = reinterpret_cast<float*>(w + sp.gmax), a.partner = reinterpret_cast<int*>(w + sp.partner);
   a.first = reinterpret_cast<long long*>(w + sp.first), a.expo = reinterpret_cast<int*>(w + sp.expo);
   a.part = reinterpret_cast<float*>(w + sp.part), a.flags = reinterpret_cast<int*>(w + sp.flags);
-  a.aux = reinterpret_cast<bhalf8*>(w + sp.aux);
+  a.expn = reinterpret_cast<float*>(w + sp.expn);
   a.E = E, a.N1 = N1, a.P = P, a.N2 = N2, a.Q = Q, a.D = D, a.K = K, a.shared = shared != 0;
-  a.tiles1 = ceil_div(P, kRowsB), a.tiles2 = ceil_div(Q, kRowsB);
-  a.n1 = n1, a.V = n1 + n2, a.G = bwd_groups(D);
+  a.tiles1 = ceil_div(P, bwd_rows(D)), a.tiles2 = ceil_div(Q, bwd_rows(D));
+  a.n1 = n1, a.V = n1 + n2, a.G = bwd_groups();
   a.c = scale / temperature * kLog2e, a.out_scale = scale * temperature;
   corr_edge_kernel<<<E, kLT, 0, stream>>>(a);
   DROID_LAUNCH_CHECK();
