@@ -82,18 +82,29 @@ __device__ __forceinline__ int swz(int r) {
   return ((r & 3) << 2) | ((r >> 2) & 3);
 }
 
-// LDS-DMA of rows y0 .. y0 + kRowsY - 1 of a frame (n rows of D values, descriptor
-// rs over them); rows past n, slots past D and the rows that `skip` names land as zeros.
-template <typename T, int DP, typename Skip>
-__device__ __forceinline__ void stage_tile(rsrc_t rs, char* lds, int y0, int n, int D, int wave, int lane, Skip skip) {
-  constexpr int RB = 2 * DP, NI = kRowsY * RB / 1024 / 4;
+// LDS-DMA of rows y0 .. y0 + kRowsY - 1 of a frame (n rows of D values): a lane's
+// source within the tile does not depend on the tile (`off`: kOob past D), the
+// descriptor starts at the tile's first row and ends with the frame, so that rows
+// past it land as zeros; no vector instruction a load.
+template <int DP>
+constexpr int kDmas = kRowsY * 2 * DP / 4096;   // a wave
+template <int DP>
+__device__ __forceinline__ void lane_offsets(unsigned (&off)[kDmas<DP>], int D, int wave, int lane) {
+  constexpr int RB = 2 * DP;
 #pragma unroll
-  for (int q = 0; q < NI; ++q) {
-    const int o = (wave * NI + q) * 1024;
-    const int row = (o + lane * 16) / RB, sl = (o + lane * 16) % RB / 16;
-    const int s = sl ^ swz<DP>(row);
-    const bool in = y0 + row < n && s * 8 < D && !skip(row);
-    dma16(rs, lds_addr(lds) + o, in ? (unsigned)(((y0 + row) * D + s * 8) * 2) : kOob);
+  for (int q = 0; q < kDmas<DP>; ++q) {
+    const int o = (wave * kDmas<DP> + q) * 1024 + lane * 16, row = o / RB, s = (o % RB / 16) ^ swz<DP>(row);
+    off[q] = s * 8 < D ? (unsigned)(row * D + s * 8) * 2 : kOob;
+  }
+}
+template <typename T, int DP, typename Skip>
+__device__ __forceinline__ void stage_tile(const T* frame, char* lds, int y0, int n, int D,
+                                           const unsigned (&off)[kDmas<DP>], int wave, int lane, Skip skip) {
+  const rsrc_t rs = make_rsrc(frame + (long)y0 * D, (unsigned)(n - y0) * D * 2);
+#pragma unroll
+  for (int q = 0; q < kDmas<DP>; ++q) {
+    const int o = (wave * kDmas<DP> + q) * 1024;
+    dma16(rs, lds_addr(lds) + o, skip((o + lane * 16) / (2 * DP)) ? kOob : off[q]);
   }
 }
 
@@ -140,11 +151,11 @@ __device__ __forceinline__ void loads_done() {
   asm volatile("" ::: "memory");
 }
 
-// The same, but for the wave's last N LDS-DMAs (and one of the first wave's, where
-// AUX).
+// The same, but for the wave's last N LDS-DMAs (and one more of the first two
+// waves, where AUX).
 template <int N, bool AUX>
 __device__ __forceinline__ void loads_left(int wave) {
-  if (AUX && wave == 0) __builtin_amdgcn_s_waitcnt(0x0f70 | (N + 1));
+  if (AUX && wave < 2) __builtin_amdgcn_s_waitcnt(0x0f70 | (N + 1));
   else __builtin_amdgcn_s_waitcnt(0x0f70 | N);
   asm volatile("" ::: "memory");
 }
@@ -190,19 +201,20 @@ __global__ void __launch_bounds__(kLT) corr_lse_kernel(FwdArgs a) {
   if (!__syncthreads_or(want)) return;
   const T* f1 = static_cast<const T*>(a.f1) + (long)i * a.P * a.D;
   const T* f2 = static_cast<const T*>(a.f2) + (long)j * a.Q * a.D;
-  const rsrc_t rs = make_rsrc(f2, (unsigned)a.Q * a.D * 2);
+  unsigned off[kDmas<DP>];
+  lane_offsets<DP>(off, a.D, wave, lane);
   const int nt = (a.Q + kRowsY - 1) / kRowsY;
   const int t0 = nt * s / a.S, t1 = nt * (s + 1) / a.S;
   typename Op<T>::vec8 b[DP / 16];
   load_rows<T, DP>(b, f1, p, a.P, a.D, lane >> 5);
   auto none = [](int) { return false; };
-  stage_tile<T, DP>(rs, tile[0], t0 * kRowsY, a.Q, a.D, wave, lane, none);
+  stage_tile<T, DP>(f2, tile[0], t0 * kRowsY, a.Q, a.D, off, wave, lane, none);
   loads_done();
   __syncthreads();
   float m = kNegBig, l = 0.f;
   for (int t = t0; t < t1; ++t) {
     const unsigned row0 = row_addr<DP>(lds_addr(tile[(t - t0) & 1]), lane);
-    if (t + 1 < t1) stage_tile<T, DP>(rs, tile[(t + 1 - t0) & 1], (t + 1) * kRowsY, a.Q, a.D, wave, lane, none);
+    if (t + 1 < t1) stage_tile<T, DP>(f2, tile[(t + 1 - t0) & 1], (t + 1) * kRowsY, a.Q, a.D, off, wave, lane, none);
     floatx16 sc[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) sc[k] = block_product<T, DP>(row0, k, b);
@@ -389,6 +401,8 @@ template <int DP>
 constexpr int kXH = DP <= 128 ? 2 : 1;
 constexpr int bwd_rows(int D) { return 128 * (D <= 128 ? 2 : 1); }
 constexpr int kJoin = 8;                     // workgroups that join one item
+constexpr int kET = 1024;                    // threads of the edge kernel
+constexpr int kMaxGroups = 8192;             // of 64 keys: frames of up to 524288 rows
 constexpr int kMinUnits = 32;                // smallest share worth a workgroup
 
 struct BwdArgs {
@@ -398,6 +412,8 @@ struct BwdArgs {
   void *d1, *d2;               // (N1, P, D), (N2, Q, D)
   float* gmax;                 // (E) largest |g|; -1: no row has a target
   int* flags;                  // (E) 1: a left-out row is not finite, 2: a g is negative
+  int* first_rec;              // (E, groups + 1) the records of each 64 keys
+  uint2* rec;                  // (E, P K) query row << 6 | key & 63, and g pi
   float* expn;                 // (E, tiles of P, 64) the queries' exponents: log2 |g| - lse, -inf: no gradient
   int* partner;                // (E) the reverse edge that is done together with this one, -1: none
   long long* first;            // (V + 1) units before frame slot v; the slots: f1's frames (d1 wanted), then f2's
@@ -406,6 +422,7 @@ struct BwdArgs {
   int E, N1, P, N2, Q, D, K, shared;
   int tiles1, tiles2;          // items of a frame (bwd_rows rows each)
   int n1, V, G;                // slots of f1, all slots, workgroups
+  int groups;                  // of 64 keys a frame
   float c, out_scale;          // scale / T log2(e); scale T
 };
 
@@ -420,12 +437,14 @@ __device__ __forceinline__ int g_exponent(float gmax) {
   return max(-100, min(100, 14 - ex));
 }
 
-// One workgroup an edge: what the gradient kernel wants of its rows, and the
-// reverse edge it may be paired with (the k-th copy of (i, j) with the k-th of
-// (j, i)).
-__global__ void __launch_bounds__(kLT) corr_edge_kernel(BwdArgs a) {
+// One workgroup an edge: what the gradient kernel wants of its rows, its sparse
+// terms by 64 keys (a counting sort), and the reverse edge it may be paired with
+// (the k-th copy of (i, j) with the k-th of (j, i)).
+__global__ void __launch_bounds__(kET) corr_edge_kernel(BwdArgs a) {
+  constexpr int kLT = kET;
   __shared__ float red[kLT / 64];
   __shared__ int cnt[kLT / 64], fl[kLT / 64];
+  __shared__ int bucket[kMaxGroups];
   const int e = blockIdx.x, tid = threadIdx.x, wave = tid >> 6;
   const int padded = y_tiles(a.P) * kRowsY;
   float m = -1.f;
@@ -450,18 +469,66 @@ __global__ void __launch_bounds__(kLT) corr_edge_kernel(BwdArgs a) {
   if ((tid & 63) == 0) red[wave] = m, fl[wave] = f;
   __syncthreads();
   if (tid == 0) {
-    a.gmax[e] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    a.flags[e] = fl[0] | fl[1] | fl[2] | fl[3];
+    for (int w = 1; w < kLT / 64; ++w) m = fmaxf(m, red[w]), f |= fl[w];
+    a.gmax[e] = fmaxf(m, red[0]);
+    a.flags[e] = f | fl[0];
     a.partner[e] = -1;
+  }
+  // The records.  Their order within a bucket is that of the atomics; terms of one
+  // place (y, x) are added in LDS in any order anyway.  More keys than buckets: a
+  // bucket holds several groups, told apart by the reader (rec holds the key's low
+  // bits only), so such sizes are refused on the host.
+  const long ent = (long)e * a.P * a.K;
+  const int total = a.P * a.K;
+  for (int q = tid; q < a.groups; q += kLT) bucket[q] = 0;
+  __syncthreads();
+  for (int q = tid; q < total; q += kLT) {
+    const unsigned v = a.idx[ent + q];
+    if (v < (unsigned)a.Q) atomicAdd(&bucket[v / 64], 1);
+  }
+  __syncthreads();
+  int carry = 0;
+  for (int q0 = 0; q0 < a.groups; q0 += kLT) {
+    const int q = q0 + tid, n = q < a.groups ? bucket[q] : 0;
+    int s = n;
+    for (int o = 1; o < 64; o <<= 1) {
+      const int u = __shfl_up(s, o, 64);
+      if ((tid & 63) >= o) s += u;
+    }
+    __syncthreads();
+    if ((tid & 63) == 63) cnt[wave] = s;
+    __syncthreads();
+    int all = 0;
+    for (int w = 0; w < kLT / 64; ++w) {
+      if (w < wave) s += cnt[w];
+      all += cnt[w];
+    }
+    if (q < a.groups) {
+      bucket[q] = carry + s - n;
+      a.first_rec[(long)e * (a.groups + 1) + q] = carry + s - n;
+    }
+    carry += all;
+  }
+  if (tid == 0) a.first_rec[(long)e * (a.groups + 1) + a.groups] = carry;
+  __syncthreads();
+  for (int q = tid; q < total; q += kLT) {
+    const unsigned v = a.idx[ent + q];
+    if (v >= (unsigned)a.Q) continue;
+    const int p = q / a.K, at = atomicAdd(&bucket[v / 64], 1);
+    const float pi = a.prob ? a.prob[ent + q] : 1.f;
+    const bool out = fabsf(a.lse[(long)e * a.P + p]) == INFINITY;
+    a.rec[ent + at] = make_uint2((unsigned)p << 6 | (v & 63), __float_as_uint(out || pi == 0.f ? 0.f : a.g[(long)e * a.P + p] * pi));
   }
   if (!a.shared) return;
   const int i = a.e1[e], j = a.e2[e];
   int rank = 0;
   for (int q = tid; q < e; q += kLT) rank += a.e1[q] == i && a.e2[q] == j;
   for (int o = 32; o; o >>= 1) rank += __shfl_xor(rank, o, 64);
+  __syncthreads();
   if ((tid & 63) == 0) cnt[wave] = rank;
   __syncthreads();
-  rank = cnt[0] + cnt[1] + cnt[2] + cnt[3];
+  rank = 0;
+  for (int w = 0; w < kLT / 64; ++w) rank += cnt[w];
   for (int q0 = 0; q0 < a.E; q0 += kLT) {
     const int q = q0 + tid;
     const bool rev = q < a.E && a.e1[q] == j && a.e2[q] == i;
@@ -472,7 +539,7 @@ __global__ void __launch_bounds__(kLT) corr_edge_kernel(BwdArgs a) {
     int at = __popcll(bal & ((1ull << (tid & 63)) - 1));
     for (int u = 0; u < wave; ++u) at += cnt[u];
     if (rev && at == rank) a.partner[e] = q;
-    rank -= cnt[0] + cnt[1] + cnt[2] + cnt[3];
+    for (int w = 0; w < kLT / 64; ++w) rank -= cnt[w];
     if (rank < 0) break;
   }
 }
@@ -557,21 +624,21 @@ __device__ __forceinline__ int slot_of(const BwdArgs& a, long long u) {
   return lo;
 }
 
-constexpr int kChunk = 32;       // at most as many tiles' sparse records are in LDS at a time
-constexpr int kRecords = 6144;   // of them; where a chunk has more, its entries are read again half tile by half tile
+constexpr int kHalves = 256;   // half tiles of one pass over an edge (longer frames: several passes)
 
 // What a workgroup of the gradient kernel keeps in LDS.
 template <int DP>
 struct BwdShared {
+  static constexpr int records = DP <= 128 ? 2048 : 512;   // sparse terms of a wave and a pass
   char tile[3][kRowsY * 2 * DP];           // rows aligned to their size; two tiles ahead
   float delta[4][32][32 * kXH<DP>];        // a wave's sparse terms of half a tile; zero between uses
-  float expn[4][kRowsY];                   // the streamed queries' exponents, three tiles ahead
+  float expn[4][kRowsY], yg[4][kRowsY];    // the streamed queries' exponents and g, three tiles ahead
+  float xg[bwd_rows(DP)];                  // the stationary queries' g
   int elist[kLT];
   int ecount[4];
-  int bucket[kChunk * 8 + 1];              // ends of the sparse records of (half tile, wave)
-  int wsum[4];
-  unsigned char pos[kRecords][2];          // y, x in the wave's half tile
-  float val[kRecords];                     // g pi
+  int ends[4][kHalves + 1];                // a wave's records: where those of each half tile end
+  float val[4][records];                   // g pi
+  unsigned short pos[4][records];          // y << 6 | x in the half tile
 };
 
 // The steps [t0, t1) of one edge (es: x are its queries) and / or its reverse
@@ -580,23 +647,21 @@ struct BwdShared {
 //
 // The sparse targets (g pi at (y, x)) go through a dense, wave-private LDS image
 // of half a tile, used only where there is one: the subtraction happens in fp32,
-// before the rounding (p - pi of a well-trained row is a small difference).  For
-// every kChunk tiles the entries of the rows x and of the streamed rows are
-// sorted by half tile and wave into LDS (two passes over them: count, place), so
-// that the loop meets them without a load from memory.
+// before the rounding (p - pi of a well-trained row is a small difference).
+// Before the steps a wave sorts the terms of its rows (its own targets, and the
+// edge kernel's records of its keys) by half tile into LDS; where they do not fit,
+// it reads them again at each half tile that has some.
 template <typename T, int DP, bool SRC, bool DST, bool NEG>
 __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, int es, int ed, int t0, int t1, int R,
                                          int x0, int ex, const typename Op<T>::vec8 (&b)[kXH<DP>][DP / 16],
                                          floatx16 (&acc)[kXH<DP>][DP / 32]) {
   typedef typename Op<T>::vec8 vec8;
   typedef const __attribute__((address_space(3))) vec8* ptr;
-  typedef int int4_u __attribute__((ext_vector_type(4), aligned(4)));
   constexpr int RB = 2 * DP, KD = DP / 16, XH = kXH<DP>, XW = 32 * XH;   // XW rows a wave
-  constexpr int NI = kRowsY * RB / 4096;                                 // LDS-DMAs of a tile a wave
+  constexpr bool kScaled = !__is_same(T, __bf16);
   const int tid = fresh(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int n_y = SRC ? a.Q : a.P, K = a.K;
-  const rsrc_t rs = make_rsrc(static_cast<const T*>(SRC ? a.f2 : a.f1) + (long)(SRC ? a.e2[es] : a.e1[ed]) * n_y * a.D,
-                              (unsigned)n_y * a.D * 2);
+  const T* const frame = static_cast<const T*>(SRC ? a.f2 : a.f1) + (long)(SRC ? a.e2[es] : a.e1[ed]) * n_y * a.D;
   const float mul = ldexpf(1.f, ex), fex = (float)ex;
   float lx[XH], gx[XH];
   bool live = false;   // a stationary row has a target
@@ -609,135 +674,115 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
       if (fabsf(lx[j]) == INFINITY) lx[j] = INFINITY;
       gx[j] = lx[j] == INFINITY ? 0.f : lx[j] == lx[j] ? a.g[(long)es * a.P + x] * mul : NAN;
       any |= lx[j] != INFINITY;
+      if (h == 0) sh.xg[wave * XW + 32 * j + lane] = gx[j];
     }
     live = __syncthreads_or(any);
     if (!DST && !live) return;   // every row left out: nothing here, whatever the keys hold
   }
-  // f(y, x, value) for every sparse term of the streamed rows [y0, y1) and the rows
-  // x0 + [xa, xb), over `n` threads
-  auto each_term = [&](int y0, int y1, int xa, int xb, int from, int n, auto f) {
+  // f(y, x, value) for the sparse terms of the streamed rows [ya, yb) and the wave's
+  // rows x (from 0), over its lanes
+  auto each_term = [&](int ya, int yb, auto f) {
+    const int v = fresh(lane);
     if constexpr (SRC) {
-      const long row0 = (long)es * a.P + x0;
-      const int* p = a.idx + row0 * K;
-      const int last = min(xb, R - x0) * K;
-      for (int q = xa * K + from; q < last; q += n) {
-        const int y = p[q];
-        if (y >= y0 && y < y1) {
+      const long first = (long)es * a.P + x0 + wave * XW;
+      const int n = min(XW, R - x0 - wave * XW) * K;
+#pragma unroll 4
+      for (int q = v; q < n; q += 64) {
+        const int y = a.idx[first * K + q];
+        if (y >= ya && y < yb) {
           const int r = q / K;
-          f(y, r, [&] {
-            return (fabsf(a.lse[row0 + r]) == INFINITY ? 0.f : a.g[row0 + r] * mul) * (a.prob ? a.prob[row0 * K + q] : 1.f);
-          });
+          const float pi = a.prob ? a.prob[first * K + q] : 1.f;
+          if (pi != 0.f) f(y, r, sh.xg[wave * XW + r] * pi);
         }
       }
     }
     if constexpr (DST) {
-      const long row0 = (long)ed * a.P + y0;
-      const int* p = a.idx + row0 * K;
-      const int total = (y1 - y0) * K;
-      auto one = [&](int q, int v) {
-        v -= x0;
-        if (v >= xa && v < xb) {
-          const int r = q / K;
-          f(y0 + r, v, [&] {
-            return (fabsf(a.lse[row0 + r]) == INFINITY ? 0.f : a.g[row0 + r] * mul) * (a.prob ? a.prob[row0 * K + q] : 1.f);
-          });
-        }
-      };
-      int q = 4 * from;
+      // the wave's rows are one group of 64 keys, or half of one
+      const int x = x0 + wave * XW, group = x / 64;
+      if (x < R) {
+        const int* p = a.first_rec + (long)ed * (a.groups + 1) + group;
+        const int lo = p[0], hi = p[1];
+        const uint2* rec = a.rec + (long)ed * a.P * K;
 #pragma unroll 4
-      for (; q + 3 < total; q += 4 * n) {
-        const int4_u v = *reinterpret_cast<const int4_u*>(p + q);
-        const int lo = x0 + xa;
-        const unsigned span = xb - xa;
-        if ((unsigned)(v.x - lo) < span || (unsigned)(v.y - lo) < span || (unsigned)(v.z - lo) < span ||
-            (unsigned)(v.w - lo) < span)
-#pragma unroll 1
-          for (int c = 0; c < 4; ++c) one(q + c, c & 2 ? (c & 1 ? v.w : v.z) : c & 1 ? v.y : v.x);
+        for (int q = lo + v; q < hi; q += 64) {
+          const uint2 r = rec[q];
+          const int y = r.x >> 6, k = (int)(r.x & 63) - (x & 63);
+          if (y >= ya && y < yb && (XW == 64 || (k >= 0 && k < XW))) f(y, k, __uint_as_float(r.y) * mul);
+        }
       }
+    }
+  };
+  bool stored;
+  {
+    // count by half tile, running sum, place: all of it the wave's own
+    int (&ends)[kHalves + 1] = sh.ends[wave];
+    const int ya = t0 * kRowsY, yb = t1 * kRowsY;
+    for (int q = lane; q <= kHalves; q += 64) ends[q] = 0;
+    each_term(ya, yb, [&](int y, int, float) { atomicAdd(&ends[(y - ya) / 32], 1); });
+    int carry = 0;
 #pragma unroll 1
-      for (; q < total; ++q) one(q, p[q]);   // the last piece, on one thread
+    for (int q = lane; q < kHalves; q += 64) {
+      const int n = ends[q];
+      int s = n;
+      for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(s, o, 64);
+        if (lane >= o) s += u;
+      }
+      ends[q] = carry + s - n;
+      carry += __shfl(s, 63, 64);
     }
-  };
-  // 512 K terms an edge where the targets are spread evenly (256 rows x): chunks of
-  // about a third of what fits
-  const int ct = max(2, min(kChunk, kRecords / (3 * 2 * 4 * XW) * y_tiles(n_y) / K));
-  int c0 = 0;            // the chunk's first tile
-  bool stored = false;   // its records are in LDS
-  auto chunk = [&](int t) {   // between barriers: called where all waves are past the last chunk
-    c0 = t;
-    const int ya = t * kRowsY, yb = min(min(t + ct, t1) * kRowsY, n_y);
-    const int y_first = ya;
-    for (int q = tid; q <= kChunk * 8; q += kLT) sh.bucket[q] = 0;
-    __syncthreads();
-    auto bucket = [&](int y, int v) { return (y - y_first) / 32 * 4 + v / XW; };
-    each_term(ya, yb, 0, 4 * XW, tid, kLT, [&](int y, int v, auto) { atomicAdd(&sh.bucket[bucket(y, v)], 1); });
-    __syncthreads();
-    // exclusive sums of the kChunk * 8 = kLT counts (those past ct tiles are 0)
-    const int n = sh.bucket[tid];
-    int s = n;
-    for (int o = 1; o < 64; o <<= 1) {
-      const int u = __shfl_up(s, o, 64);
-      if (lane >= o) s += u;
-    }
-    if (lane == 63) sh.wsum[wave] = s;
-    __syncthreads();
-    for (int q = 0; q < wave; ++q) s += sh.wsum[q];
-    stored = sh.wsum[0] + sh.wsum[1] + sh.wsum[2] + sh.wsum[3] <= kRecords;
-    sh.bucket[tid] = stored ? s - n : n;   // not stored: the counts, for whether to look at all
-    __syncthreads();
+    stored = carry <= BwdShared<DP>::records;
     if (stored)
-      each_term(ya, yb, 0, 4 * XW, tid, kLT, [&](int y, int v, auto value) {
-        const int at = atomicAdd(&sh.bucket[bucket(y, v)], 1);   // ends as the bucket's end
-        sh.pos[at][0] = (unsigned char)(y & 31);
-        sh.pos[at][1] = (unsigned char)(v & (XW - 1));
-        sh.val[at] = value();
+      each_term(ya, yb, [&](int y, int x, float value) {
+        const int at = atomicAdd(&ends[(y - ya) / 32], 1);   // ends as the half tile's end
+        sh.pos[wave][at] = (unsigned short)((y & 31) << 6 | x);
+        sh.val[wave][at] = value;
       });
-    __syncthreads();
-  };
+    else   // the starts become ends
+      for (int q = lane; q < kHalves; q += 64) ends[q] = q + 1 < kHalves ? ends[q + 1] : carry;
+  }
   // Streamed queries: |g| mul p2 = 2^(c s + v + ex) with their exponents v.  They
   // are staged a tile further ahead: v = -inf marks a row without a gradient; where
   // such rows are not finite they are staged as zeros (unless they are live keys:
   // then the NaN is theirs).
   const rsrc_t rex = make_rsrc(a.expn + (long)ed * y_tiles(a.P) * kRowsY, (unsigned)y_tiles(a.P) * kRowsY * 4);
-  auto stage_expn = [&](int t) {
+  const rsrc_t rg = make_rsrc(a.g + (long)ed * a.P, (unsigned)a.P * 4);
+  auto stage_rows = [&](int t) {
     if (DST && wave == 0) dma4(rex, lds_addr(sh.expn[(t - t0) & 3]), (unsigned)(t * kRowsY + lane) * 4);
+    if (DST && wave == 1) dma4(rg, lds_addr(sh.yg[(t - t0) & 3]), (unsigned)(t * kRowsY + lane) * 4);
   };
   const int ef = DST ? a.flags[ed] : 0;
   const bool holes = (ef & 1) && !(SRC && live);
+  unsigned off[kDmas<DP>];
+  lane_offsets<DP>(off, a.D, wave, lane);
   auto stage = [&](int t, int buf) {
     if (!holes)
-      stage_tile<T, DP>(rs, sh.tile[buf], t * kRowsY, n_y, a.D, wave, lane, [](int) { return false; });
+      stage_tile<T, DP>(frame, sh.tile[buf], t * kRowsY, n_y, a.D, off, wave, lane, [](int) { return false; });
     else
-      stage_tile<T, DP>(rs, sh.tile[buf], t * kRowsY, n_y, a.D, wave, lane,
+      stage_tile<T, DP>(frame, sh.tile[buf], t * kRowsY, n_y, a.D, off, wave, lane,
                         [&](int row) { return sh.expn[(t - t0) & 3][row] == -INFINITY; });
   };
-  // Before the loop: the exponents of three tiles, the features of two.
-  stage_expn(t0);
-  if (t0 + 1 < t1) stage_expn(t0 + 1);
-  if (t0 + 2 < t1) stage_expn(t0 + 2);
-  chunk(t0);
-  loads_done();
-  __syncthreads();
+  // Before the loop: the row data of three tiles, the features of two.
+  stage_rows(t0);
+  if (t0 + 1 < t1) stage_rows(t0 + 1);
+  if (t0 + 2 < t1) stage_rows(t0 + 2);
+  if (holes) {
+    loads_done();
+    __syncthreads();
+  }
   stage(t0, 0);
   if (t0 + 1 < t1) stage(t0 + 1, 1);
   loads_done();
   __syncthreads();
   int buf = 0;   // of tile t
   for (int t = t0; t < t1; ++t) {
-    if (t == c0 + ct) chunk(t);
+    const int ahead = buf == 0 ? 2 : buf - 1;
     const unsigned cur = lds_addr(sh.tile[buf]), row0 = row_addr<DP>(cur, fresh(lane));
-    if (t + 2 < t1) {
-      stage(t + 2, buf == 0 ? 2 : buf - 1);
-      if (t + 3 < t1) stage_expn(t + 3);
-    }
     vec8 fa[2][KD];
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
       for (int d = 0; d < KD; ++d) fa[k][d] = *(ptr)(uintptr_t)((row0 ^ (d << 5)) + k * 64 * DP);
-    const int bk = ((t - c0) * 2) * 4 + wave;   // the wave's records: half 0, half 1
-    const int4 br = make_int4(sh.bucket[bk > 0 ? bk - 1 : kChunk * 8], sh.bucket[bk], sh.bucket[bk + 3], sh.bucket[bk + 4]);
-    float (&dl)[32][XW] = sh.delta[wave];
     // The second product's operand: rows d of the transposed tile.  As the address
     // lane 4 q + p of its 16-lane group a lane points at row 16 k + 8 u + 4 h + q,
     // values 32 d + 16 ((lane >> 4) & 1) + 4 p .. + 3; d and u move the swizzled
@@ -770,8 +815,9 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
       if constexpr (DST)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const float4 v = *reinterpret_cast<const float4*>(&sh.expn[(t - t0) & 3][32 * k + 8 * q + 4 * h]);
-          ve[4 * q] = v.x + fex, ve[4 * q + 1] = v.y + fex, ve[4 * q + 2] = v.z + fex, ve[4 * q + 3] = v.w + fex;
+          float4 v = *reinterpret_cast<const float4*>(&sh.expn[(t - t0) & 3][32 * k + 8 * q + 4 * h]);
+          if constexpr (kScaled) v.x += fex, v.y += fex, v.z += fex, v.w += fex;
+          ve[4 * q] = v.x, ve[4 * q + 1] = v.y, ve[4 * q + 2] = v.z, ve[4 * q + 3] = v.w;
         }
     };
     // The weights of half k with N matrix instructions between them, in exactly this
@@ -796,10 +842,8 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
           const int j = (n * E + e) / 16, q = (n * E + e) % 16;
           if constexpr (DST) {
             wg[j][q] = __builtin_amdgcn_exp2f(fmaf(sc[k][j][q], a.c, ve[q]));
-            if constexpr (NEG) {
-              const int y = t * kRowsY + 32 * k + 8 * (q >> 2) + 4 * h + (q & 3);
-              if (y < n_y && a.g[(long)ed * a.P + y] < 0.f) wg[j][q] = -wg[j][q];
-            }
+            if constexpr (NEG)
+              if (sh.yg[(t - t0) & 3][32 * k + 8 * (q >> 2) + 4 * h + (q & 3)] < 0.f) wg[j][q] = -wg[j][q];
           }
           // p1 clamped to [0, 1]: a NaN logit of a left-out row counts as 0
           if constexpr (SRC)
@@ -810,62 +854,70 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
       }
       finish(N - 1);
     };
+    // the wave's records of this tile: [lo, mid) in half 0, [mid, hi) in half 1
+    const int half = 2 * (t - t0), br[3] = {half ? sh.ends[wave][half - 1] : 0, sh.ends[wave][half], sh.ends[wave][half + 1]};
     vec8 ds[XH][2];
     auto sparse_and_round = [&](int k) {
-      // (no branch on `stored` here: the weights' instructions would sink below it)
-      const int lo = __builtin_amdgcn_readfirstlane(k ? br.z : br.x) & -(int)stored;
-      const int hi = __builtin_amdgcn_readfirstlane(k ? br.w : br.y);
+      const int lo = __builtin_amdgcn_readfirstlane(br[k]), hi = __builtin_amdgcn_readfirstlane(br[k + 1]);
       if (lo < hi) {
-        const int v = fresh(lane), y0 = t * kRowsY + 32 * k;
+        float (&dl)[32][XW] = sh.delta[wave];
+        const int v = fresh(lane), ya = t * kRowsY + 32 * k;
         if (stored)
-          for (int q = lo + v; q < hi; q += 64) atomicAdd(&dl[sh.pos[q][0]][sh.pos[q][1]], sh.val[q]);
+          for (int q = lo + v; q < hi; q += 64) atomicAdd(&dl[0][0] + (XW == 64 ? sh.pos[wave][q] : (sh.pos[wave][q] >> 6) * XW + (sh.pos[wave][q] & 63)), sh.val[wave][q]);
         else
-          each_term(y0, min(y0 + 32, n_y), wave * XW, wave * XW + XW, v, 64,
-                    [&](int y, int xx, auto value) { atomicAdd(&dl[y - y0][xx & (XW - 1)], value()); });
+          each_term(ya, ya + 32, [&](int y, int x, float value) { atomicAdd(&dl[y - ya][x], value); });
         const float* col = &dl[4 * (v >> 5)][v & 31];
 #pragma unroll
         for (int j = 0; j < XH; ++j)
 #pragma unroll
           for (int q = 0; q < 16; ++q) wg[j][q] -= col[(8 * (q >> 2) + (q & 3)) * XW + 32 * j];
-        for (int q = v; q < 32 * XW / 4; q += 64) reinterpret_cast<float4*>(&dl[0][0])[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (stored)
+          for (int q = lo + v; q < hi; q += 64) (&dl[0][0])[XW == 64 ? sh.pos[wave][q] : (sh.pos[wave][q] >> 6) * XW + (sh.pos[wave][q] & 63)] = 0.f;
+        else
+          for (int q = v; q < 32 * XW / 4; q += 64) reinterpret_cast<float4*>(&dl[0][0])[q] = make_float4(0.f, 0.f, 0.f, 0.f);
       }
 #pragma unroll
       for (int j = 0; j < XH; ++j)
 #pragma unroll
         for (int q = 0; q < 16; ++q) ds[j][q >> 3][q & 7] = (T)wg[j][q];
     };
-    vec8 ft[2][DP / 32];
+    vec8 ft[2][2][DP / 32];
     auto read_transposed = [&](int half) {
 #pragma unroll
-      for (int d = 0; d < DP / 32; ++d)
+      for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int k = 0; k < 2; ++k) ft[k][d] = transposed(d, 2 * half + k);
+        for (int d = 0; d < DP / 32; ++d) ft[half][k][d] = transposed(d, 2 * half + k);
     };
-    auto product = [&](int n) {
+    auto product = [&](int half, int n) {
       const int k = n / (kP / 2), d = n % (kP / 2) / XH, j = n % XH;
-      acc[j][d] = Op<T>::mfma(ft[k][d], ds[j][k], acc[j][d]);
+      acc[j][d] = Op<T>::mfma(ft[half][k][d], ds[j][k], acc[j][d]);
     };
-    // A step: half 0's logits; half 1's between half 0's weights; half 0's second
-    // product between half 1's weights; half 1's second product.
+    // A step: half 0's logits, with the next loads issued between them; half 1's
+    // between half 0's weights; half 0's second product between half 1's weights;
+    // half 1's second product.
     zero(0);
     zero(1);
     exponents(0);
 #pragma unroll
     for (int n = 0; n < kS; ++n) logit(0, n);
+    if (t + 2 < t1) {
+      stage(t + 2, ahead);
+      if (t + 3 < t1) stage_rows(t + 3);
+    }
+    read_transposed(0);
     __builtin_amdgcn_sched_barrier(0);
     weights(0, [&](int n) { logit(1, n); }, std::integral_constant<int, kS>());
     exponents(1);
-    read_transposed(0);
     sparse_and_round(0);
-    __builtin_amdgcn_sched_barrier(0);
-    weights(1, product, std::integral_constant<int, kP>());
     read_transposed(1);
+    __builtin_amdgcn_sched_barrier(0);
+    weights(1, [&](int n) { product(0, n); }, std::integral_constant<int, kP>());
     sparse_and_round(1);
 #pragma unroll
-    for (int n = 0; n < kP; ++n) product(n);
+    for (int n = 0; n < kP; ++n) product(1, n);
     buf = buf == 2 ? 0 : buf + 1;
-    // tile t + 1 has landed; the loads of t + 2 (and t + 3's exponents) stay in flight
-    if (t + 3 < t1) loads_left<NI, DST>(wave);
+    // tile t + 1 has landed; the loads of t + 2 (and t + 3's row data) stay in flight
+    if (t + 3 < t1) loads_left<kDmas<DP>, DST>(wave);
     else loads_done();
     __syncthreads();
   }
@@ -900,7 +952,8 @@ __device__ __forceinline__ void bwd_kind(const BwdArgs& a, BwdShared<DP>& sh, in
       if (t0 >= t1) continue;
       const int eq = __builtin_amdgcn_readfirstlane(sh.elist[q]);
       const int er = SRC && DST ? __builtin_amdgcn_readfirstlane(a.partner[eq]) : eq;
-      bwd_edge<T, DP, SRC, DST, NEG>(a, sh, eq, er, t0, t1, R, x0, ex, b, acc);
+      for (int t = t0; t < t1; t += kHalves / 2)
+        bwd_edge<T, DP, SRC, DST, NEG>(a, sh, eq, er, t, min(t1, t + kHalves / 2), R, x0, ex, b, acc);
     }
     __syncthreads();
   }
@@ -1019,16 +1072,18 @@ int bwd_groups() { return device_cu_count(); }
 
 // The gradient's workspace, in bytes from its start.
 struct BwdSpace {
-  size_t gmax, partner, flags, first, expo, expn, part, bytes;
+  size_t gmax, partner, flags, first, expo, first_rec, rec, expn, part, bytes;
 };
-BwdSpace bwd_space(int E, int P, int V, int D) {
+BwdSpace bwd_space(int E, int P, int Q, int V, int D, int K) {
   auto up = [](size_t n) { return (n + 15) / 16 * 16; };
   BwdSpace s{};
   s.partner = s.gmax + up((size_t)E * 4);
   s.flags = s.partner + up((size_t)E * 4);
   s.first = s.flags + up((size_t)E * 4);
   s.expo = s.first + up(((size_t)V + 1) * 8);
-  s.expn = s.expo + up((size_t)V * 4);
+  s.first_rec = s.expo + up((size_t)V * 4);
+  s.rec = s.first_rec + up((size_t)E * (ceil_div(Q, 64) + 1) * 4);
+  s.expn = s.rec + up((size_t)E * P * K * 8);
   s.part = s.expn + (size_t)E * y_tiles(P) * kRowsY * 4;
   s.bytes = s.part + (size_t)2 * bwd_groups() * bwd_rows(D) * D * 4;
   return s;
@@ -1041,7 +1096,7 @@ int corr_loss_check(const std::string& w, int dtype, int E, int N1, int P, int N
     return fail(kInvalidArgument, w + ": bad arguments (Q > 0, 0 < D <= 256, D % 8 == 0, 1 <= K <= 64)");
   if (!(scale > 0.f) || !std::isfinite(scale) || !(T > 0.f) || !std::isfinite(T))
     return fail(kInvalidArgument, w + ": scale and temperature must be positive and finite");
-  if ((long)std::max(P, Q) * D * 2 > 0x7fffffffL || (long)P * K > 0x1fffffffL || (long)E * std::max(1, ceil_div(P, kRowsB)) > 0x3fffffL ||
+  if (std::max(P, Q) > 64 * kMaxGroups || (long)std::max(P, Q) * D * 2 > 0x7fffffffL || (long)P * K > 0x1fffffffL || (long)E * std::max(1, ceil_div(P, kRowsB)) > 0x3fffffL ||
       (long)(N1 + (long)N2) * ceil_div(std::max(P, Q), kRowsB) > 0x3fffffL)
     return fail(kUnsupported, w + ": maps too large");
   return kOk;
@@ -1062,10 +1117,10 @@ using namespace droid;
 
 extern "C" {
 
-size_t droid_corr_loss_workspace(int E, int N1, int P, int N2, int Q, int D, int backward) {
-  if (E <= 0 || N1 < 0 || P <= 0 || N2 < 0 || Q <= 0 || D <= 0) return 0;
+size_t droid_corr_loss_workspace(int E, int N1, int P, int N2, int Q, int D, int K, int backward) {
+  if (E <= 0 || N1 < 0 || P <= 0 || N2 < 0 || Q <= 0 || D <= 0 || K <= 0) return 0;
   if (!backward) return (size_t)E * P * fwd_split(E, P, Q) * sizeof(float2);
-  return bwd_space(E, P, N1 + N2, D).bytes;
+  return bwd_space(E, P, Q, N1 + N2, D, K).bytes;
 }
 
 int droid_corr_loss_forward(int dtype, const void* fmap1, const void* fmap2, const int* f1, const int* f2,
@@ -1079,7 +1134,7 @@ int droid_corr_loss_forward(int dtype, const void* fmap1, const void* fmap2, con
     return fail(kInvalidArgument, what + ": null tensor");
   if (!logits && K != 1) return fail(kInvalidArgument, what + ": one target a row without logits");
   if (unaligned(fmap1) || unaligned(fmap2)) return fail(kInvalidArgument, what + ": features must be 16-B aligned");
-  if (!ws || ws_bytes < droid_corr_loss_workspace(E, N1, P, N2, Q, D, 0))
+  if (!ws || ws_bytes < droid_corr_loss_workspace(E, N1, P, N2, Q, D, K, 0))
     return fail(kInvalidArgument, what + ": workspace too small");
   FwdArgs a{fmap1, fmap2, f1, f2, idx, static_cast<float2*>(ws), E, N1, P, N2, Q, D, K, ceil_div(P, kRowsB),
             fwd_split(E, P, Q), 0, scale / temperature * kLog2e};
@@ -1112,23 +1167,24 @@ int droid_corr_loss_backward(int dtype, const void* fmap1, const void* fmap2, co
   if (unaligned(fmap1) || unaligned(fmap2)) return fail(kInvalidArgument, what + ": features must be 16-B aligned");
   // the gradients that are wanted; a shared tensor's rows are counted once
   const int n1 = dfmap1 ? N1 : 0, n2 = dfmap2 ? N2 : 0;
-  if (!ws || ws_bytes < droid_corr_loss_workspace(E, n1, P, n2, Q, D, 1))
+  if (!ws || ws_bytes < droid_corr_loss_workspace(E, n1, P, n2, Q, D, K, 1))
     return fail(kInvalidArgument, what + ": workspace too small");
   if (n1 + n2 == 0) return kOk;
   char* const w = static_cast<char*>(ws);
-  const BwdSpace sp = bwd_space(E, P, n1 + n2, D);
+  const BwdSpace sp = bwd_space(E, P, Q, n1 + n2, D, K);
   BwdArgs a{};
   a.f1 = fmap1, a.f2 = fmap2, a.e1 = f1, a.e2 = f2, a.idx = idx, a.prob = prob, a.lse = lse, a.g = gloss;
   a.d1 = dfmap1, a.d2 = dfmap2;
   a.gmax = reinterpret_cast<float*>(w + sp.gmax), a.partner = reinterpret_cast<int*>(w + sp.partner);
   a.first = reinterpret_cast<long long*>(w + sp.first), a.expo = reinterpret_cast<int*>(w + sp.expo);
   a.part = reinterpret_cast<float*>(w + sp.part), a.flags = reinterpret_cast<int*>(w + sp.flags);
-  a.expn = reinterpret_cast<float*>(w + sp.expn);
+  a.expn = reinterpret_cast<float*>(w + sp.expn), a.first_rec = reinterpret_cast<int*>(w + sp.first_rec);
+  a.rec = reinterpret_cast<uint2*>(w + sp.rec), a.groups = ceil_div(Q, 64);
   a.E = E, a.N1 = N1, a.P = P, a.N2 = N2, a.Q = Q, a.D = D, a.K = K, a.shared = shared != 0;
   a.tiles1 = ceil_div(P, bwd_rows(D)), a.tiles2 = ceil_div(Q, bwd_rows(D));
   a.n1 = n1, a.V = n1 + n2, a.G = bwd_groups();
   a.c = scale / temperature * kLog2e, a.out_scale = scale * temperature;
-  corr_edge_kernel<<<E, kLT, 0, stream>>>(a);
+  corr_edge_kernel<<<E, kET, 0, stream>>>(a);
   DROID_LAUNCH_CHECK();
   corr_plan_kernel<<<1, 1024, 0, stream>>>(a);
   DROID_LAUNCH_CHECK();

@@ -333,7 +333,7 @@ def corr_loss_forward(fmap1, fmap2, f1, f2, idx, logits=None, scale=1.0 / 16, te
     if loss.numel() == 0:
         return loss, lse, prob
     with torch.cuda.device(dev):
-        ws = torch.empty((lib.droid_corr_loss_workspace(E, N1, P, N2, Q, D, 0),), dtype=torch.uint8, device=dev)
+        ws = torch.empty((lib.droid_corr_loss_workspace(E, N1, P, N2, Q, D, K or 1, 0),), dtype=torch.uint8, device=dev)
         check(lib.droid_corr_loss_forward(_LOSS_DTYPES[fmap1.dtype], _ptr(fmap1), _ptr(keys), _ptr(f1), _ptr(f2),
                                           _ptr(idx), _ptr(logits), _ptr(loss), _ptr(lse), _ptr(prob), E, N1, P, N2, Q,
                                           D, K or 1, scale, temperature, _ptr(ws), ws.numel(), _stream(fmap1)), fn)
@@ -369,8 +369,8 @@ def corr_loss_backward(gloss, fmap1, fmap2, f1, f2, idx, lse, prob=None, scale=1
         return d1, d2
     dev = fmap1.device
     with torch.cuda.device(dev):
-        ws = torch.empty((lib.droid_corr_loss_workspace(E, N1 if need1 else 0, P, N2 if need2 else 0, Q, D, 1),),
-                         dtype=torch.uint8, device=dev)
+        ws = torch.empty((lib.droid_corr_loss_workspace(E, N1 if need1 else 0, P, N2 if need2 else 0, Q, D, K or 1,
+                                                        1),), dtype=torch.uint8, device=dev)
         check(lib.droid_corr_loss_backward(_LOSS_DTYPES[fmap1.dtype], _ptr(fmap1), _ptr(keys), _ptr(f1), _ptr(f2),
                                            _ptr(idx), _ptr(prob), _ptr(lse), _ptr(gloss), _ptr(d1), _ptr(d2),
                                            int(shared), E, N1, P, N2, Q, D, K or 1, scale, temperature, _ptr(ws),

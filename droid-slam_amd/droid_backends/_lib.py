@@ -62,7 +62,7 @@ _SIGS = {
     "droid_group_norm_act": ([_i, _p, _p, _p, _p, _p, _i, _p, _i, _i, _i, _i, _i, _f, _p, _sz, _p], _i),
     "droid_group_norm_act_backward": ([_i, _p, _p, _p, _p, _p, _i, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _p, _sz,
                                        _p], _i),
-    "droid_corr_loss_workspace": ([_i] * 7, _sz),
+    "droid_corr_loss_workspace": ([_i] * 8, _sz),
     "droid_corr_loss_forward": ([_i] + [_p] * 9 + [_i] * 7 + [_f, _f, _p, _sz, _p], _i),
     "droid_corr_loss_backward": ([_i] + [_p] * 10 + [_i] * 8 + [_f, _f, _p, _sz, _p], _i),
     "droid_proximity_workspace": ([_i, _i, _i], _sz),

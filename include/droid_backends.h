@@ -151,7 +151,7 @@ int droid_corr_alt_ce0_ordered(const void* const* pyr, const int* Hl, const int*
  * (E,P,K) f32 (with logits only).
  * ws: droid_corr_loss_workspace bytes (backward: N1 / N2 = 0 for a gradient that is not
  * wanted, N2 = 0 with shared), used until the kernels end. */
-size_t droid_corr_loss_workspace(int E, int N1, int P, int N2, int Q, int D, int backward);
+size_t droid_corr_loss_workspace(int E, int N1, int P, int N2, int Q, int D, int K, int backward);
 int droid_corr_loss_forward(int dtype, const void* fmap1, const void* fmap2, const int* f1, const int* f2,
                             const int* idx, const float* logits, float* loss, float* lse, float* prob, int E, int N1,
                             int P, int N2, int Q, int D, int K, float scale, float temperature, void* ws,
