@@ -402,6 +402,7 @@ constexpr int kXH = DP <= 128 ? 2 : 1;
 constexpr int bwd_rows(int D) { return 128 * (D <= 128 ? 2 : 1); }
 constexpr int kJoin = 8;                     // workgroups that join one item
 constexpr int kET = 1024;                    // threads of the edge kernel
+constexpr float kRange = 40.f;                // see edge_paired
 constexpr int kMaxGroups = 8192;             // of 64 keys: frames of up to 524288 rows
 constexpr int kMinUnits = 32;                // smallest share worth a workgroup
 
@@ -412,6 +413,7 @@ struct BwdArgs {
   void *d1, *d2;               // (N1, P, D), (N2, Q, D)
   float* gmax;                 // (E) largest |g|; -1: no row has a target
   int* flags;                  // (E) 1: a left-out row is not finite, 2: a g is negative
+  float2* range;               // (E) smallest and largest lse of the rows with a target
   int* first_rec;              // (E, groups + 1) the records of each 64 keys
   uint2* rec;                  // (E, P K) query row << 6 | key & 63, and g pi
   float* expn;                 // (E, tiles of P, 64) the queries' exponents: log2 |g| - lse, -inf: no gradient
@@ -444,10 +446,11 @@ __global__ void __launch_bounds__(kET) corr_edge_kernel(BwdArgs a) {
   constexpr int kLT = kET;
   __shared__ float red[kLT / 64];
   __shared__ int cnt[kLT / 64], fl[kLT / 64];
+  __shared__ float2 lr[kLT / 64];
   __shared__ int bucket[kMaxGroups];
   const int e = blockIdx.x, tid = threadIdx.x, wave = tid >> 6;
   const int padded = y_tiles(a.P) * kRowsY;
-  float m = -1.f;
+  float m = -1.f, lmin = INFINITY, lmax = -INFINITY;
   int f = 0;
   for (int p = tid; p < padded; p += kLT) {
     const float l = p < a.P ? a.lse[(long)e * a.P + p] : INFINITY;
@@ -456,6 +459,7 @@ __global__ void __launch_bounds__(kET) corr_edge_kernel(BwdArgs a) {
       const float g = a.g[(long)e * a.P + p];
       m = fmaxf(fmaxf(m, 0.f), fabsf(g));
       v = log2f(fabsf(g)) - l;
+      lmin = fminf(lmin, l), lmax = fmaxf(lmax, l);
       if (g < 0.f) f |= 2;
     } else if (l < 0.f) {
       f |= 1;
@@ -465,13 +469,19 @@ __global__ void __launch_bounds__(kET) corr_edge_kernel(BwdArgs a) {
   for (int o = 32; o; o >>= 1) {
     m = fmaxf(m, __shfl_xor(m, o, 64));
     f |= __shfl_xor(f, o, 64);
+    lmin = fminf(lmin, __shfl_xor(lmin, o, 64));
+    lmax = fmaxf(lmax, __shfl_xor(lmax, o, 64));
   }
-  if ((tid & 63) == 0) red[wave] = m, fl[wave] = f;
+  if ((tid & 63) == 0) red[wave] = m, fl[wave] = f, lr[wave] = make_float2(lmin, lmax);
   __syncthreads();
   if (tid == 0) {
-    for (int w = 1; w < kLT / 64; ++w) m = fmaxf(m, red[w]), f |= fl[w];
-    a.gmax[e] = fmaxf(m, red[0]);
-    a.flags[e] = f | fl[0];
+    for (int w = 1; w < kLT / 64; ++w) {   // (this thread holds the first wave's)
+      m = fmaxf(m, red[w]), f |= fl[w];
+      lmin = fminf(lmin, lr[w].x), lmax = fmaxf(lmax, lr[w].y);
+    }
+    a.gmax[e] = m;
+    a.flags[e] = f;
+    a.range[e] = make_float2(lmin, lmax);
     a.partner[e] = -1;
   }
   // The records.  Their order within a bucket is that of the atomics; terms of one
@@ -548,10 +558,17 @@ __global__ void __launch_bounds__(kET) corr_edge_kernel(BwdArgs a) {
 __device__ __forceinline__ bool edge_in(const BwdArgs& a, int e) {
   return (unsigned)a.e1[e] < (unsigned)a.N1 && (unsigned)a.e2[e] < (unsigned)a.N2 && a.gmax[e] >= 0.f;
 }
-// Whether it is done together with its reverse.
+// The span of the row sums of two edges (empty where an edge has none that counts).
+__device__ __forceinline__ float2 edge_range(const BwdArgs& a, int e, int r) {
+  return make_float2(fminf(a.range[e].x, a.range[r].x), fmaxf(a.range[e].y, a.range[r].y));
+}
+// Whether it is done together with its reverse: the weights of both then come from
+// one exponential (bwd_edge), which holds while their lse lie within 2^kRange.
 __device__ __forceinline__ bool edge_paired(const BwdArgs& a, int e) {
   const int r = a.partner[e];
-  return r >= 0 && a.gmax[r] >= 0.f && !((a.flags[e] | a.flags[r]) & 2);
+  if (r < 0 || !(a.gmax[r] >= 0.f) || ((a.flags[e] | a.flags[r]) & 2)) return false;
+  const float2 span = edge_range(a, e, r);
+  return span.x <= span.y && span.y - span.x <= kRange;
 }
 
 // One workgroup: the units of every frame slot's items and their running sum.
@@ -663,8 +680,19 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
   const int n_y = SRC ? a.Q : a.P, K = a.K;
   const T* const frame = static_cast<const T*>(SRC ? a.f2 : a.f1) + (long)(SRC ? a.e2[es] : a.e1[ed]) * n_y * a.D;
   const float mul = ldexpf(1.f, ex), fex = (float)ex;
-  float lx[XH], gx[XH];
+  float lx[XH], gx[XH], ax[XH];
   bool live = false;   // a stationary row has a target
+  // Both directions: with m the middle of the row sums, g1 p1 + g2 p2 = u (2^b g1 + A B)
+  // where u = 2^(c s - lse_x - b), A = 2^(lse_x - m + b), B = 2^(v_y + m): one exponential
+  // a pair of rows. b = kRange / 2, and lse_x := m in a left-out row x: then u <= 1
+  // wherever x or y has a target, and is clamped to that where neither has, so that
+  // it stays finite there and the factor 0 holds. What underflows is below
+  // 2^(kRange - 126) of a probability.
+  float mid = 0.f;
+  if constexpr (SRC && DST) {
+    const float2 span = edge_range(a, es, ed);
+    mid = 0.5f * (span.x + span.y);
+  }
   if constexpr (SRC) {
     bool any = false;
 #pragma unroll
@@ -674,7 +702,13 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
       if (fabsf(lx[j]) == INFINITY) lx[j] = INFINITY;
       gx[j] = lx[j] == INFINITY ? 0.f : lx[j] == lx[j] ? a.g[(long)es * a.P + x] * mul : NAN;
       any |= lx[j] != INFINITY;
+      if constexpr (SRC && DST) {
+        if (lx[j] == INFINITY) lx[j] = mid;
+        ax[j] = __builtin_amdgcn_exp2f(lx[j] - mid + 0.5f * kRange);
+        lx[j] += 0.5f * kRange;
+      }
       if (h == 0) sh.xg[wave * XW + 32 * j + lane] = gx[j];
+      if constexpr (SRC && DST) gx[j] *= __builtin_amdgcn_exp2f(0.5f * kRange);
     }
     live = __syncthreads_or(any);
     if (!DST && !live) return;   // every row left out: nothing here, whatever the keys hold
@@ -775,14 +809,31 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
   loads_done();
   __syncthreads();
   int buf = 0;   // of tile t
+  // Half 1's second product of a tile is done in the next step, while that one's
+  // operands are on their way (nothing yet: zeros), where there are registers to
+  // keep its operands (D <= 128).
+  constexpr bool kDefer = DP <= 128;
+  constexpr int kS = KD * XH, kP = 2 * (DP / 32) * XH;   // matrix instructions of a half's logits, second product
+  vec8 ds[XH][2], ft[2][2][DP / 32];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+#pragma unroll
+    for (int j = 0; j < XH; ++j) ds[j][k] = vec8{};
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) ft[1][k][d] = vec8{};
+  }
+  auto product = [&](int half, int n) {
+    const int k = n / (kP / 2), d = n % (kP / 2) / XH, j = n % XH;
+    acc[j][d] = Op<T>::mfma(ft[half][k][d], ds[j][k], acc[j][d]);
+  };
   for (int t = t0; t < t1; ++t) {
     const int ahead = buf == 0 ? 2 : buf - 1;
     const unsigned cur = lds_addr(sh.tile[buf]), row0 = row_addr<DP>(cur, fresh(lane));
     vec8 fa[2][KD];
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll
-      for (int d = 0; d < KD; ++d) fa[k][d] = *(ptr)(uintptr_t)((row0 ^ (d << 5)) + k * 64 * DP);
+    auto read_row = [&](int n) {   // the n-th of the 2 KD operands of the logits
+      const int k = n / KD, d = n % KD;
+      fa[k][d] = *(ptr)(uintptr_t)((row0 ^ (d << 5)) + k * 64 * DP);
+    };
     // The second product's operand: rows d of the transposed tile.  As the address
     // lane 4 q + p of its 16-lane group a lane points at row 16 k + 8 u + 4 h + q,
     // values 32 d + 16 ((lane >> 4) & 1) + 4 p .. + 3; d and u move the swizzled
@@ -799,8 +850,6 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
     };
     floatx16 sc[2][XH];
     float wg[XH][16];
-    // the n-th matrix instruction of a half's logits, and of the second product
-    constexpr int kS = KD * XH, kP = 2 * (DP / 32) * XH;
     auto logit = [&](int k, int n) {
       sc[k][n % XH] = Op<T>::mfma(fa[k][n / XH], b[n % XH][n / XH], sc[k][n % XH]);
     };
@@ -810,14 +859,16 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
 #pragma unroll
         for (int i = 0; i < 16; ++i) sc[k][j][i] = 0.f;
     };
-    float ve[16];   // the exponents of the half's rows in this lane's places
+    float ve[16];   // the exponents (both directions: B) of the half's rows in this lane's places
     auto exponents = [&](int k) {
       if constexpr (DST)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          float4 v = *reinterpret_cast<const float4*>(&sh.expn[(t - t0) & 3][32 * k + 8 * q + 4 * h]);
-          if constexpr (kScaled) v.x += fex, v.y += fex, v.z += fex, v.w += fex;
-          ve[4 * q] = v.x, ve[4 * q + 1] = v.y, ve[4 * q + 2] = v.z, ve[4 * q + 3] = v.w;
+          const float4 v = *reinterpret_cast<const float4*>(&sh.expn[(t - t0) & 3][32 * k + 8 * q + 4 * h]);
+          const float vq[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            ve[4 * q + u] = SRC ? __builtin_amdgcn_exp2f(vq[u] + (mid + fex)) : kScaled ? vq[u] + fex : vq[u];
         }
     };
     // The weights of half k with N matrix instructions between them, in exactly this
@@ -831,7 +882,7 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
 #pragma unroll
         for (int e = 0; e < E; ++e) {
           const int j = (n * E + e) / 16, q = (n * E + e) % 16;
-          if constexpr (SRC) wg[j][q] = DST ? fmaf(gx[j], p1[n & 1][e], wg[j][q]) : gx[j] * p1[n & 1][e];
+          if constexpr (SRC) wg[j][q] = p1[n & 1][e] * (DST ? fmaf(ax[j], ve[q], gx[j]) : gx[j]);
         }
       };
 #pragma unroll
@@ -840,14 +891,15 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
 #pragma unroll
         for (int e = 0; e < E; ++e) {
           const int j = (n * E + e) / 16, q = (n * E + e) % 16;
-          if constexpr (DST) {
+          if constexpr (!SRC) {
             wg[j][q] = __builtin_amdgcn_exp2f(fmaf(sc[k][j][q], a.c, ve[q]));
             if constexpr (NEG)
               if (sh.yg[(t - t0) & 3][32 * k + 8 * (q >> 2) + 4 * h + (q & 3)] < 0.f) wg[j][q] = -wg[j][q];
+          } else {
+            const float u = __builtin_amdgcn_exp2f(fmaf(sc[k][j][q], a.c, -lx[j]));
+            // (the clamp takes a NaN logit, of a left-out row, to 0)
+            p1[n & 1][e] = __builtin_amdgcn_fmed3f(u, 0.f, 1.f);
           }
-          // p1 clamped to [0, 1]: a NaN logit of a left-out row counts as 0
-          if constexpr (SRC)
-            p1[n & 1][e] = __builtin_amdgcn_fmed3f(__builtin_amdgcn_exp2f(fmaf(sc[k][j][q], a.c, -lx[j])), 0.f, 1.f);
         }
         if (n) finish(n - 1);
         __builtin_amdgcn_sched_barrier(0);
@@ -856,7 +908,6 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
     };
     // the wave's records of this tile: [lo, mid) in half 0, [mid, hi) in half 1
     const int half = 2 * (t - t0), br[3] = {half ? sh.ends[wave][half - 1] : 0, sh.ends[wave][half], sh.ends[wave][half + 1]};
-    vec8 ds[XH][2];
     auto sparse_and_round = [&](int k) {
       const int lo = __builtin_amdgcn_readfirstlane(br[k]), hi = __builtin_amdgcn_readfirstlane(br[k + 1]);
       if (lo < hi) {
@@ -881,45 +932,63 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
 #pragma unroll
         for (int q = 0; q < 16; ++q) ds[j][q >> 3][q & 7] = (T)wg[j][q];
     };
-    vec8 ft[2][2][DP / 32];
-    auto read_transposed = [&](int half) {
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d) ft[half][k][d] = transposed(d, 2 * half + k);
+    auto read_transposed = [&](int half, int n) {   // the n-th of DP / 16
+      const int k = n / (DP / 32), d = n % (DP / 32);
+      ft[half][k][d] = transposed(d, 2 * half + k);
     };
-    auto product = [&](int half, int n) {
-      const int k = n / (kP / 2), d = n % (kP / 2) / XH, j = n % XH;
-      acc[j][d] = Op<T>::mfma(ft[half][k][d], ds[j][k], acc[j][d]);
-    };
-    // A step: half 0's logits, with the next loads issued between them; half 1's
-    // between half 0's weights; half 0's second product between half 1's weights;
-    // half 1's second product.
+    // A step: the last half's second product, half 0's logits; half 1's logits between
+    // half 0's weights; half 0's second product between half 1's weights.  The reads
+    // of shared memory, which take the four waves of a workgroup about 1100 clocks a step,
+    // stand between the matrix instructions too.
     zero(0);
     zero(1);
-    exponents(0);
+    if constexpr (kDefer) {
 #pragma unroll
-    for (int n = 0; n < kS; ++n) logit(0, n);
+      for (int n = 0; n < kP; ++n) {
+        product(1, n);
+#pragma unroll
+        for (int q = 2 * KD * n / kP; q < 2 * KD * (n + 1) / kP; ++q) read_row(q);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < 2 * KD; ++q) read_row(q);
+    }
     if (t + 2 < t1) {
       stage(t + 2, ahead);
       if (t + 3 < t1) stage_rows(t + 3);
     }
-    read_transposed(0);
-    __builtin_amdgcn_sched_barrier(0);
+    exponents(0);
+#pragma unroll
+    for (int n = 0; n < kS; ++n) {
+      logit(0, n);
+#pragma unroll
+      for (int q = KD * n / kS; q < KD * (n + 1) / kS; ++q) read_transposed(0, q);
+      __builtin_amdgcn_sched_barrier(0);
+    }
     weights(0, [&](int n) { logit(1, n); }, std::integral_constant<int, kS>());
     exponents(1);
     sparse_and_round(0);
-    read_transposed(1);
     __builtin_amdgcn_sched_barrier(0);
-    weights(1, [&](int n) { product(0, n); }, std::integral_constant<int, kP>());
-    sparse_and_round(1);
+    weights(1, [&](int n) {
+      product(0, n);
 #pragma unroll
-    for (int n = 0; n < kP; ++n) product(1, n);
+      for (int q = KD * n / kP; q < KD * (n + 1) / kP; ++q) read_transposed(1, q);
+    }, std::integral_constant<int, kP>());
+    sparse_and_round(1);
+    if constexpr (!kDefer) {
+#pragma unroll
+      for (int n = 0; n < kP; ++n) product(1, n);
+    }
     buf = buf == 2 ? 0 : buf + 1;
     // tile t + 1 has landed; the loads of t + 2 (and t + 3's row data) stay in flight
     if (t + 3 < t1) loads_left<kDmas<DP>, DST>(wave);
     else loads_done();
     __syncthreads();
+  }
+  if constexpr (kDefer) {
+#pragma unroll
+    for (int n = 0; n < kP; ++n) product(1, n);
   }
 }
 
@@ -1072,14 +1141,15 @@ int bwd_groups() { return device_cu_count(); }
 
 // The gradient's workspace, in bytes from its start.
 struct BwdSpace {
-  size_t gmax, partner, flags, first, expo, first_rec, rec, expn, part, bytes;
+  size_t gmax, partner, flags, range, first, expo, first_rec, rec, expn, part, bytes;
 };
 BwdSpace bwd_space(int E, int P, int Q, int V, int D, int K) {
   auto up = [](size_t n) { return (n + 15) / 16 * 16; };
   BwdSpace s{};
   s.partner = s.gmax + up((size_t)E * 4);
   s.flags = s.partner + up((size_t)E * 4);
-  s.first = s.flags + up((size_t)E * 4);
+  s.range = s.flags + up((size_t)E * 4);
+  s.first = s.range + up((size_t)E * 8);
   s.expo = s.first + up(((size_t)V + 1) * 8);
   s.first_rec = s.expo + up((size_t)V * 4);
   s.rec = s.first_rec + up((size_t)E * (ceil_div(Q, 64) + 1) * 4);
@@ -1180,6 +1250,7 @@ int droid_corr_loss_backward(int dtype, const void* fmap1, const void* fmap2, co
   a.part = reinterpret_cast<float*>(w + sp.part), a.flags = reinterpret_cast<int*>(w + sp.flags);
   a.expn = reinterpret_cast<float*>(w + sp.expn), a.first_rec = reinterpret_cast<int*>(w + sp.first_rec);
   a.rec = reinterpret_cast<uint2*>(w + sp.rec), a.groups = ceil_div(Q, 64);
+  a.range = reinterpret_cast<float2*>(w + sp.range);
   a.E = E, a.N1 = N1, a.P = P, a.N2 = N2, a.Q = Q, a.D = D, a.K = K, a.shared = shared != 0;
   a.tiles1 = ceil_div(P, bwd_rows(D)), a.tiles2 = ceil_div(Q, bwd_rows(D));
   a.n1 = n1, a.V = n1 + n2, a.G = bwd_groups();
