@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(kLT) corr_loss_row_kernel(RowArgs a) {
 // places took 1137 us, shares of the streamed axis by a cost model 867 us, with
 // uneven graphs up to twice their even share.)
 
-constexpr int kUnitBoth = 6, kUnitSrc = 4, kUnitDst = 5;   // relative cost of a step (measured 6300 : 4100 : 5400 clk)
+constexpr int kUnitBoth = 5, kUnitSrc = 4, kUnitDst = 4;   // relative cost of a step (measured 5670 : 4460 : 4380 clk)
 // Rows x of a wave, in 32s.  Two where their accumulators fit the registers of one
 // wave a SIMD: a tile read from LDS then serves twice the products.  With one (two
 // waves a SIMD) the LDS pipe bound the kernel: four clips 508 us, the same without

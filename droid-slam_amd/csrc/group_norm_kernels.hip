@@ -165,15 +165,23 @@ __global__ void __launch_bounds__(kGnT) gn_stats_kernel(const T* __restrict__ x,
       }
       f += sp.active;
       int cnt = 1;
-#pragma unroll 4
-      for (; cnt < kFlush && f < f1; ++cnt, f += sp.active) {
-        const Piece<T> p = load_piece(xb + f * V);
+      while (cnt < kFlush && f < f1) {
+        Piece<T> p[4];   // loads in flight
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-          const float d = (float)p.v[k] - k0[k];
-          a[k] += d;
-          b[k] = fmaf(d, d, b[k]);
-        }
+        for (int u = 0; u < 4; ++u)
+          if (f + u * sp.active < f1) p[u] = load_piece(xb + (f + u * sp.active) * V);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (f + u * sp.active < f1) {
+            ++cnt;
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+              const float d = (float)p[u].v[k] - k0[k];
+              a[k] += d;
+              b[k] = fmaf(d, d, b[k]);
+            }
+          }
+        f += 4 * sp.active;
       }
 #pragma unroll
       for (int k = 0; k < V; ++k) {   // about k0: sum = n k0 + a, squares = b + 2 k0 a + n k0^2
@@ -232,6 +240,7 @@ __device__ __forceinline__ void gn_finish_stats(const double2* part, int n, int 
   const int t = threadIdx.x, L = lanes_per(G), g = t / L, l = t % L;
   double a = 0.0, b = 0.0;
   if (g < G)
+#pragma unroll 4
     for (int s = l; s < S; s += L) {
       const double2 v = part[((long)n * S + s) * G + g];
       a += v.x;
@@ -291,14 +300,26 @@ __global__ void __launch_bounds__(kGnT) gn_apply_kernel(const T* x, const T* res
   constexpr int V = Elem<T>::V;
   constexpr bool RES = MODE == kResRelu || MODE == kAddRelu;
   __shared__ double2 st[kGnMaxC];
+  constexpr int U = 4;
   const int n = blockIdx.y, t = threadIdx.x;
+  const long base = (long)n * HW * C;
+  const long c0 = sp.chunks * blockIdx.x / gridDim.x, c1 = sp.chunks * (blockIdx.x + 1) / gridDim.x;
+  const long f1 = t < sp.active ? min(c1 * sp.active, sp.pieces) : 0;
+  Piece<T> p[U], rp[U];
+  auto load = [&](long f) {   // U pieces in flight a thread
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (f + u * sp.active < f1) {
+        p[u] = load_piece(x + base + (f + u * sp.active) * V);
+        if constexpr (RES) rp[u] = load_piece(res + base + (f + u * sp.active) * V);
+      }
+  };
+  long f = c0 * sp.active + t;
+  load(f);   // on their way while the statistics are added up
   gn_finish_stats(part, n, S, G, (long)HW * (C / G), eps, st, blockIdx.x == 0 ? stats_out : nullptr);
   if (t >= sp.active) return;
   ChanConst<V> cc;
   gn_consts<T>(cc, st, w, b, wdt, C, G);
-  const long base = (long)n * HW * C;
-  const long c0 = sp.chunks * blockIdx.x / gridDim.x, c1 = sp.chunks * (blockIdx.x + 1) / gridDim.x;
-  const long f1 = min(c1 * sp.active, sp.pieces);
   auto piece = [&](const Piece<T>& p, const Piece<T>& rp) {
     Piece<T> o;
 #pragma unroll
@@ -308,12 +329,12 @@ __global__ void __launch_bounds__(kGnT) gn_apply_kernel(const T* x, const T* res
     }
     return o;
   };
-#pragma unroll 4
-  for (long f = c0 * sp.active + t; f < f1; f += sp.active) {
-    const Piece<T> p = load_piece(x + base + f * V);
-    Piece<T> rp;
-    if constexpr (RES) rp = load_piece(res + base + f * V);
-    store_piece(out + base + f * V, piece(p, rp));
+  while (f < f1) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (f + u * sp.active < f1) store_piece(out + base + (f + u * sp.active) * V, piece(p[u], rp[u]));
+    f += U * sp.active;
+    load(f);
   }
   if (sp.tail && c1 == sp.chunks && sp.pieces % sp.active == t) {
     const long o = base + sp.pieces * V;
@@ -324,42 +345,69 @@ __global__ void __launch_bounds__(kGnT) gn_apply_kernel(const T* x, const T* res
   }
 }
 
-// dn and dres of one value (v: x, r: res, g: dy).  stw: the group's 64-bit
-// (mean, rstd); tolc = kTol (2 |b| + |m rw|), the channel's share of the bound
-// on n's fp32 error.
+// dn and dres of one value (r: res, g: dy, n: the normed value).  tol = kTol times
+// the largest 2 |b| + |m rw| of the thread's channels bounds n's fp32 error;
+// returns whether a ReLU's argument is within that of zero.
 template <int MODE>
-__device__ __forceinline__ void gn_slope(float v, float r, float g, float n, float tolc, const double2* stw, float w,
-                                         float b, float& dn, float& dres) {
-  dres = g;
-  if constexpr (MODE == kNone) {
-    dn = g;
-  } else if constexpr (MODE == kSilu) {
+__device__ __forceinline__ bool gn_slope(float r, float g, float n, float tol, float& dn, float& dres) {
+  dres = dn = g;
+  if constexpr (MODE == kSilu) {
     const float sg = __builtin_amdgcn_rcpf(1.f + __expf(-n));
     dn = g * sg * (1.f + n * (1.f - sg));
   } else if constexpr (MODE == kRelu) {
-    bool on = n > 0.f;
-    if (fabsf(n) <= tolc) on = ((double)v - stw->x) * (stw->y * (double)w) + (double)b > 0.0;
-    dn = on ? g : 0.f;
-  } else {
-    const float tol = fmaf(kTol, fabsf(r), tolc);
-    bool on_n = n > 0.f, on_o;
-    float pre;
-    bool near;
-    if constexpr (MODE == kResRelu) {
-      pre = r + fmaxf(n, 0.f);
-      near = fabsf(n) <= tolc || (n > 0.f && fabsf(pre) <= tol);
-    } else {
-      pre = n + r;
-      near = fabsf(pre) <= tol;
+    dn = n > 0.f ? g : 0.f;
+    return fabsf(n) <= tol;
+  } else if constexpr (MODE == kResRelu) {
+    const float pre = r + fmaxf(n, 0.f);
+    dres = pre > 0.f ? g : 0.f;
+    dn = n > 0.f ? dres : 0.f;
+    return fabsf(n) <= tol || (n > 0.f && fabsf(pre) <= fmaf(kTol, fabsf(r), tol));   // (n < 0: pre is r itself)
+  } else if constexpr (MODE == kAddRelu) {
+    const float pre = n + r;
+    dn = dres = pre > 0.f ? g : 0.f;
+    return fabsf(pre) <= fmaf(kTol, fabsf(r), tol);
+  }
+  return false;
+}
+
+// dn and dres of a piece of cnt values at x + o.  The 64-bit decisions, a branch
+// hardly ever taken, are made one value at a time with everything read again and
+// kept as two bit masks: unrolled, they took more registers than all the rest.
+template <typename T, int MODE>
+__device__ __forceinline__ void gn_slopes(const float (&nn)[Elem<T>::V], const Piece<T>& rp, const Piece<T>& gp,
+                                          float tol, const T* x, const T* res, long o, int cnt, const double2* st,
+                                          const void* w, const void* b, int wdt, int C, int cpg,
+                                          float (&dn)[Elem<T>::V], float (&dr)[Elem<T>::V]) {
+  constexpr int V = Elem<T>::V;
+  constexpr bool RES = MODE == kResRelu || MODE == kAddRelu;
+  bool near = false;
+#pragma unroll
+  for (int k = 0; k < V; ++k)
+    near |= gn_slope<MODE>(RES ? (float)rp.v[k] : 0.f, (float)gp.v[k], nn[k], tol, dn[k], dr[k]);
+  if constexpr (MODE != kNone && MODE != kSilu) {
+    if (__builtin_expect(near, 0)) {
+      int t = threadIdx.x;
+      asm volatile("" : "+v"(t));   // (or its channel arithmetic moves out of the loop)
+      int c = (t * V) % C;
+      unsigned on_n = 0, on_o = 0;
+#pragma unroll 1
+      for (int k = 0; k < cnt; ++k) {
+        const double2 sg = st[c / cpg];
+        const double n = ((double)(float)x[o + k] - sg.x) * (sg.y * (double)param(w, wdt, c, 1.f)) +
+                         (double)param(b, wdt, c, 0.f);
+        const double rv = RES ? (double)(float)res[o + k] : 0.0;
+        on_n |= (unsigned)(n > 0.0) << k;
+        on_o |= (unsigned)((MODE == kResRelu ? rv + fmax(n, 0.0) : n + rv) > 0.0) << k;
+        c = c + 1 == C ? 0 : c + 1;
+      }
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const float g = (float)gp.v[k];
+        if constexpr (RES) dr[k] = on_o >> k & 1 ? g : 0.f;
+        if constexpr (MODE == kAddRelu) dn[k] = dr[k];
+        if constexpr (MODE != kAddRelu) dn[k] = on_n >> k & 1 ? dr[k] : 0.f;
+      }
     }
-    on_o = pre > 0.f;
-    if (near) {
-      const double nd = ((double)v - stw->x) * (stw->y * (double)w) + (double)b;
-      on_n = nd > 0.0;
-      on_o = (MODE == kResRelu ? (double)r + fmax(nd, 0.0) : nd + (double)r) > 0.0;
-    }
-    dres = on_o ? g : 0.f;
-    dn = MODE == kResRelu && !on_n ? 0.f : dres;
   }
 }
 
@@ -367,7 +415,7 @@ __device__ __forceinline__ void gn_slope(float v, float r, float g, float n, flo
 // (cpart[n][s][c]) and the group sums of w dn and w dn xhat (gpart[n][s][g]);
 // writes dres.
 template <typename T, int MODE>
-__global__ void __launch_bounds__(kGnT) gn_bwd_stats_kernel(const T* __restrict__ x, const T* __restrict__ res,
+__global__ void __launch_bounds__(kGnT, 4) gn_bwd_stats_kernel(const T* __restrict__ x, const T* __restrict__ res,
                                                             const T* __restrict__ dy, T* __restrict__ dres,
                                                             const void* __restrict__ w, const void* __restrict__ b,
                                                             int wdt, const double2* __restrict__ stats, int HW, int C,
@@ -380,54 +428,68 @@ __global__ void __launch_bounds__(kGnT) gn_bwd_stats_kernel(const T* __restrict_
   const int n = blockIdx.y, s = blockIdx.x, S = gridDim.x, t = threadIdx.x;
   const int cpg = C / G;
   const double2* st = stats + (long)n * G;
-  ChanConst<V> cc;
-  gn_consts<T>(cc, st, w, b, wdt, C, G);
-  float rs[V], tolc[V], a1[V], a2[V];
-  int cg = (int)(((long)t * V) % C);
+  // channel constants: xhat = (x - m) rs, n = xhat wc + bc
+  float m[V], rs[V], wc[V], bc[V], a1[V], a2[V], tol = 0.f;
+  int cg = (t * V) % C;
 #pragma unroll
   for (int k = 0; k < V; ++k) {
-    rs[k] = (float)st[cg / cpg].y;
-    tolc[k] = kTol * (2.f * fabsf(cc.b[k]) + fabsf(cc.m[k] * cc.rw[k]));
+    const double2 v = st[cg / cpg];
+    m[k] = (float)v.x;
+    rs[k] = (float)v.y;
+    wc[k] = param(w, wdt, cg, 1.f);
+    bc[k] = param(b, wdt, cg, 0.f);
+    tol = fmaxf(tol, kTol * (2.f * fabsf(bc[k]) + fabsf(m[k] * rs[k] * wc[k])));
     a1[k] = a2[k] = 0.f;
     cg = cg + 1 == C ? 0 : cg + 1;
   }
   const long base = (long)n * HW * C;
   const long c0 = sp.chunks * s / S, c1 = sp.chunks * (s + 1) / S;
   const long f1 = min(c1 * sp.active, sp.pieces);
-  auto piece = [&](const Piece<T>& p, const Piece<T>& rp, const Piece<T>& gp, int m) {
-    Piece<T> o;
-    int c = (int)(((long)t * V) % C);
+  auto piece = [&](const Piece<T>& p, const Piece<T>& rp, const Piece<T>& gp, long at, int cnt) {
+    float xh[V], nn[V], dn[V], dr[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      const float v = (float)p.v[k], d = v - cc.m[k];
-      const float nn = fmaf(d, cc.rw[k], cc.b[k]);
-      float dn, dr;
-      gn_slope<MODE>(v, RES ? (float)rp.v[k] : 0.f, (float)gp.v[k], nn, tolc[k], st + c / cpg, param(w, wdt, c, 1.f),
-                     cc.b[k], dn, dr);
-      if (k < m) {
-        a1[k] += dn;
-        a2[k] = fmaf(dn, d * rs[k], a2[k]);
+      xh[k] = ((float)p.v[k] - m[k]) * rs[k];
+      nn[k] = fmaf(xh[k], wc[k], bc[k]);
+    }
+    gn_slopes<T, MODE>(nn, rp, gp, tol, x, res, at, cnt, st, w, b, wdt, C, cpg, dn, dr);
+    Piece<T> o;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      if (k < cnt) {
+        a1[k] += dn[k];
+        a2[k] = fmaf(dn[k], xh[k], a2[k]);
       }
-      o.v[k] = (T)dr;
-      c = c + 1 == C ? 0 : c + 1;
+      o.v[k] = (T)dr[k];
     }
     return o;
   };
   if (t < sp.active) {
-#pragma unroll 2
-    for (long f = c0 * sp.active + t; f < f1; f += sp.active) {
-      const Piece<T> p = load_piece(x + base + f * V), gp = load_piece(dy + base + f * V);
-      Piece<T> rp;
-      if constexpr (RES) rp = load_piece(res + base + f * V);
-      const Piece<T> o = piece(p, rp, gp, V);
-      if constexpr (RES) store_piece(dres + base + f * V, o);
+    // two pieces' loads in flight a thread
+    for (long f = c0 * sp.active + t; f < f1; f += 2 * sp.active) {
+      Piece<T> p[2], gp[2], rp[2];
+      const bool two = f + sp.active < f1;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if (u == 0 || two) {
+          const long o = base + (f + u * sp.active) * V;
+          p[u] = load_piece(x + o), gp[u] = load_piece(dy + o);
+          if constexpr (RES) rp[u] = load_piece(res + o);
+        }
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if (u == 0 || two) {
+          const long at = base + (f + u * sp.active) * V;
+          const Piece<T> o = piece(p[u], rp[u], gp[u], at, V);
+          if constexpr (RES) store_piece(dres + at, o);
+        }
     }
     if (sp.tail && c1 == sp.chunks && sp.pieces % sp.active == t) {
       const long o0 = base + sp.pieces * V;
       const Piece<T> p = load_tail(x + o0, sp.tail), gp = load_tail(dy + o0, sp.tail);
       Piece<T> rp;
       if constexpr (RES) rp = load_tail(res + o0, sp.tail);
-      const Piece<T> o = piece(p, rp, gp, sp.tail);
+      const Piece<T> o = piece(p, rp, gp, o0, sp.tail);
       if constexpr (RES) store_tail(dres + o0, o, sp.tail);
     }
 #pragma unroll
@@ -472,7 +534,7 @@ __global__ void __launch_bounds__(kGnT) gn_bwd_stats_kernel(const T* __restrict_
 // pass 2 of the backward: dx; the grid's last row of workgroups (blockIdx.y ==
 // N) adds up the channel sums to dw and db instead.
 template <typename T, int MODE>
-__global__ void __launch_bounds__(kGnT) gn_bwd_apply_kernel(const T* __restrict__ x, const T* __restrict__ dyr,
+__global__ void __launch_bounds__(kGnT, 4) gn_bwd_apply_kernel(const T* __restrict__ x, const T* __restrict__ dyr,
                                                             T* __restrict__ dx, const void* __restrict__ w,
                                                             const void* __restrict__ b, int wdt,
                                                             const double2* __restrict__ stats, int N, int HW, int C,
@@ -481,14 +543,15 @@ __global__ void __launch_bounds__(kGnT) gn_bwd_apply_kernel(const T* __restrict_
                                                             void* __restrict__ db) {
   constexpr int V = Elem<T>::V;
   __shared__ double2 sm[kGnT];
-  const int n = blockIdx.y, t = threadIdx.x;
-  if (n == N) {
+  const int t = threadIdx.x;
+  if (blockIdx.y == N) {
     // 16 channels a workgroup, 32 lanes over the N S partials of each
     const int l = t / 16;
     for (int c0 = blockIdx.x * 16; c0 < C; c0 += gridDim.x * 16) {
       const int c = c0 + t % 16;
       double u = 0.0, v = 0.0;
       if (c < C)
+#pragma unroll 4
         for (int i = l; i < N * S; i += kGnT / 16) {
           const double2 p = cpart[(long)i * C + c];
           u += p.x;
@@ -517,12 +580,14 @@ __global__ void __launch_bounds__(kGnT) gn_bwd_apply_kernel(const T* __restrict_
     }
     return;
   }
-  const int cpg = C / G;
+  // the images in the other order: the last ones are still in the cache
+  const int cpg = C / G, n = N - 1 - blockIdx.y;
   const double2* st = stats + (long)n * G;
   {
     const int L = lanes_per(G), g = t / L, l = t % L;
     double u = 0.0, v = 0.0;
     if (g < G)
+#pragma unroll 4
       for (int s = l; s < S; s += L) {
         const double2 p = gpart[((long)n * S + s) * G + g];
         u += p.x;
@@ -538,15 +603,15 @@ __global__ void __launch_bounds__(kGnT) gn_bwd_apply_kernel(const T* __restrict_
   // dx = rstd w dn - rstd (k1 + xhat k2): per channel rw = rstd w, q1 = rstd k1, q2 = rstd^2 k2
   ChanConst<V> cc;
   gn_consts<T>(cc, st, w, b, wdt, C, G);
-  float q1[V], q2[V], tolc[V];
-  int cg = (int)(((long)t * V) % C);
+  float q1[V], q2[V], tol = 0.f;
+  int cg = (t * V) % C;
 #pragma unroll
   for (int k = 0; k < V; ++k) {
     const double r = st[cg / cpg].y;
     const double2 kk = sm[cg / cpg];
     q1[k] = (float)(r * kk.x);
     q2[k] = (float)(r * r * kk.y);
-    tolc[k] = kTol * (2.f * fabsf(cc.b[k]) + fabsf(cc.m[k] * cc.rw[k]));
+    tol = fmaxf(tol, kTol * (2.f * fabsf(cc.b[k]) + fabsf(cc.m[k] * cc.rw[k])));
     cg = cg + 1 == C ? 0 : cg + 1;
   }
   const long base = (long)n * HW * C;
@@ -555,29 +620,39 @@ __global__ void __launch_bounds__(kGnT) gn_bwd_apply_kernel(const T* __restrict_
   // the outer ReLU's slope is in dyr (= dres) already: what is left is mode 0's
   // ReLU (mode 1's inner one), or SiLU's slope
   constexpr int LEFT = MODE == kResRelu ? (int)kRelu : MODE == kAddRelu ? (int)kNone : MODE;
-  auto piece = [&](const Piece<T>& p, const Piece<T>& gp) {
-    Piece<T> o;
-    int c = (int)(((long)t * V) % C);
+  auto piece = [&](const Piece<T>& p, const Piece<T>& gp, long at, int cnt) {
+    float d[V], nn[V], dn[V], dr[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      const float v = (float)p.v[k], d = v - cc.m[k];
-      const float nn = fmaf(d, cc.rw[k], cc.b[k]);
-      float dn, dr;
-      gn_slope<LEFT>(v, 0.f, (float)gp.v[k], nn, tolc[k], st + c / cpg, param(w, wdt, c, 1.f), cc.b[k], dn, dr);
-      o.v[k] = (T)(fmaf(dn, cc.rw[k], -fmaf(d, q2[k], q1[k])));
-      c = c + 1 == C ? 0 : c + 1;
+      d[k] = (float)p.v[k] - cc.m[k];
+      nn[k] = fmaf(d[k], cc.rw[k], cc.b[k]);
     }
+    gn_slopes<T, LEFT>(nn, gp, gp, tol, x, nullptr, at, cnt, st, w, b, wdt, C, cpg, dn, dr);
+    Piece<T> o;
+#pragma unroll
+    for (int k = 0; k < V; ++k) o.v[k] = (T)(fmaf(dn[k], cc.rw[k], -fmaf(d[k], q2[k], q1[k])));
     return o;
   };
-#pragma unroll 2
-  for (long f = c0 * sp.active + t; f < f1; f += sp.active) {
-    const Piece<T> p = load_piece(x + base + f * V), gp = load_piece(dyr + base + f * V);
-    store_piece(dx + base + f * V, piece(p, gp));
+  for (long f = c0 * sp.active + t; f < f1; f += 2 * sp.active) {
+    Piece<T> p[2], gp[2];
+    const bool two = f + sp.active < f1;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      if (u == 0 || two) {
+        const long o = base + (f + u * sp.active) * V;
+        p[u] = load_piece(x + o), gp[u] = load_piece(dyr + o);
+      }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      if (u == 0 || two) {
+        const long at = base + (f + u * sp.active) * V;
+        store_piece(dx + at, piece(p[u], gp[u], at, V));
+      }
   }
   if (sp.tail && c1 == sp.chunks && sp.pieces % sp.active == t) {
     const long o0 = base + sp.pieces * V;
     const Piece<T> p = load_tail(x + o0, sp.tail), gp = load_tail(dyr + o0, sp.tail);
-    store_tail(dx + o0, piece(p, gp), sp.tail);
+    store_tail(dx + o0, piece(p, gp, o0, sp.tail), sp.tail);
   }
 }
 

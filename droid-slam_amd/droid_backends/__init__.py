@@ -37,6 +37,32 @@ def _stream(t):
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
 
+# The calls of the operators below that take microseconds on the GPU: addresses
+# and the stream as plain ints (the signatures make them pointers), no device
+# switch where the tensors' device is the current one.
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
+class _Here:
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *exc):
+        pass
+
+
+_HERE = _Here()
+
+
+def _on(dev):
+    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _raw_stream(dev):
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
 def _check_inputs(names, tensors):
     dev = None
     for name, t in zip(names, tensors):
@@ -332,11 +358,11 @@ def corr_loss_forward(fmap1, fmap2, f1, f2, idx, logits=None, scale=1.0 / 16, te
     lse = torch.empty(rows, dtype=torch.float32, device=dev)
     if loss.numel() == 0:
         return loss, lse, prob
-    with torch.cuda.device(dev):
+    with _on(dev):
         ws = torch.empty((lib.droid_corr_loss_workspace(E, N1, P, N2, Q, D, K or 1, 0),), dtype=torch.uint8, device=dev)
-        check(lib.droid_corr_loss_forward(_LOSS_DTYPES[fmap1.dtype], _ptr(fmap1), _ptr(keys), _ptr(f1), _ptr(f2),
-                                          _ptr(idx), _ptr(logits), _ptr(loss), _ptr(lse), _ptr(prob), E, N1, P, N2, Q,
-                                          D, K or 1, scale, temperature, _ptr(ws), ws.numel(), _stream(fmap1)), fn)
+        check(lib.droid_corr_loss_forward(_LOSS_DTYPES[fmap1.dtype], _addr(fmap1), _addr(keys), _addr(f1), _addr(f2),
+                                          _addr(idx), _addr(logits), _addr(loss), _addr(lse), _addr(prob), E, N1, P, N2, Q,
+                                          D, K or 1, scale, temperature, _addr(ws), ws.numel(), _raw_stream(dev)), fn)
     return loss, lse, prob
 
 
@@ -368,13 +394,13 @@ def corr_loss_backward(gloss, fmap1, fmap2, f1, f2, idx, lse, prob=None, scale=1
     if gloss.numel() == 0:
         return d1, d2
     dev = fmap1.device
-    with torch.cuda.device(dev):
+    with _on(dev):
         ws = torch.empty((lib.droid_corr_loss_workspace(E, N1 if need1 else 0, P, N2 if need2 else 0, Q, D, K or 1,
                                                         1),), dtype=torch.uint8, device=dev)
-        check(lib.droid_corr_loss_backward(_LOSS_DTYPES[fmap1.dtype], _ptr(fmap1), _ptr(keys), _ptr(f1), _ptr(f2),
-                                           _ptr(idx), _ptr(prob), _ptr(lse), _ptr(gloss), _ptr(d1), _ptr(d2),
-                                           int(shared), E, N1, P, N2, Q, D, K or 1, scale, temperature, _ptr(ws),
-                                           ws.numel(), _stream(fmap1)), fn)
+        check(lib.droid_corr_loss_backward(_LOSS_DTYPES[fmap1.dtype], _addr(fmap1), _addr(keys), _addr(f1), _addr(f2),
+                                           _addr(idx), _addr(prob), _addr(lse), _addr(gloss), _addr(d1), _addr(d2),
+                                           int(shared), E, N1, P, N2, Q, D, K or 1, scale, temperature, _addr(ws),
+                                           ws.numel(), _raw_stream(dev)), fn)
     return d1, d2
 
 
@@ -977,10 +1003,10 @@ def group_norm_act(x, num_groups, weight=None, bias=None, mode=NORM_RELU, res=No
     N, C, H, W = x.shape
     dt, hw, dev = _NORM_DTYPES[x.dtype], H * W, x.device
     stats = torch.empty((N, num_groups, 2), dtype=torch.float64, device=dev) if return_stats else None
-    with torch.cuda.device(dev):
+    with _on(dev):
         ws = torch.empty((lib.droid_group_norm_workspace(dt, N, hw, C, num_groups, 0),), dtype=torch.uint8, device=dev)
-        check(lib.droid_group_norm_act(dt, _ptr(x), _ptr(res), _ptr(out), _ptr(weight), _ptr(bias), wdt, _ptr(stats),
-                                       N, hw, C, num_groups, mode, eps, _ptr(ws), ws.numel(), _stream(x)), fn)
+        check(lib.droid_group_norm_act(dt, _addr(x), _addr(res), _addr(out), _addr(weight), _addr(bias), wdt, _addr(stats),
+                                       N, hw, C, num_groups, mode, eps, _addr(ws), ws.numel(), _raw_stream(dev)), fn)
     return (out, stats) if return_stats else out
 
 
@@ -1008,12 +1034,12 @@ def group_norm_act_backward(dy, x, stats, num_groups, weight=None, bias=None, mo
     new = torch.empty_like if x.numel() else torch.zeros_like
     dw = new(weight) if weight is not None else None
     db = new(bias) if bias is not None else None
-    with torch.cuda.device(dev):
+    with _on(dev):
         ws = torch.empty((lib.droid_group_norm_workspace(dt, N, hw, C, num_groups, 1),), dtype=torch.uint8, device=dev)
-        check(lib.droid_group_norm_act_backward(dt, _ptr(x), _ptr(res if with_res else None), _ptr(dy), _ptr(weight),
-                                                _ptr(bias), wdt, _ptr(stats), _ptr(dx), _ptr(dres), _ptr(dw),
-                                                _ptr(db), N, hw, C, num_groups, mode, _ptr(ws), ws.numel(),
-                                                _stream(x)), fn)
+        check(lib.droid_group_norm_act_backward(dt, _addr(x), _addr(res if with_res else None), _addr(dy), _addr(weight),
+                                                _addr(bias), wdt, _addr(stats), _addr(dx), _addr(dres), _addr(dw),
+                                                _addr(db), N, hw, C, num_groups, mode, _addr(ws), ws.numel(),
+                                                _raw_stream(dev)), fn)
     return dx, dres, dw, db
 
 
