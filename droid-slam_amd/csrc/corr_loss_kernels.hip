@@ -185,7 +185,7 @@ struct FwdArgs {
 
 // Per query row the maximum and the sum of 2^(c s - max) over a share of the keys.
 template <typename T, int DP>
-__global__ void __launch_bounds__(kLT) corr_lse_kernel(FwdArgs a) {
+__global__ void __launch_bounds__(kLT, DP <= 128 ? 4 : 2) corr_lse_kernel(FwdArgs a) {
   __shared__ __attribute__((aligned(1024))) char tile[2][kRowsY * 2 * DP];
   const int item = xcd_item(blockIdx.x, a.items);
   if (item >= a.items) return;

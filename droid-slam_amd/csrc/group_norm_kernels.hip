@@ -123,8 +123,8 @@ inline Split gn_split(int N, int HW, int C, int V) {
   const int period = C / gcd_i(C, V);
   s.active = kGnT / period * period;
   s.chunks = std::max<long>(1, (s.pieces + s.active - 1) / s.active);
-  // four workgroups a CU over all images; at least one chunk each
-  s.blocks = (int)std::max<long>(1, std::min<long>(s.chunks, std::max(1, 1024 / N)));
+  // two workgroups a CU over all images, as many as run at once; at least one chunk each
+  s.blocks = (int)std::max<long>(1, std::min<long>(s.chunks, std::max(1, 512 / N)));
   return s;
 }
 
@@ -270,23 +270,21 @@ __device__ __forceinline__ float gn_act(float n, float r) {
   return n;
 }
 
-// A thread's channel constants: n = (x - m) rw + b
-template <int V>
-struct ChanConst {
-  float m[V], rw[V], b[V];
+// Channel constants: thread c < C makes channel c's (its integer divisions once, its
+// parameters read early), the threads take their V from LDS.
+struct ChanIn {
+  float w, b;
+  int g;
 };
-template <typename T>
-__device__ __forceinline__ void gn_consts(ChanConst<Elem<T>::V>& cc, const double2* st, const void* w, const void* b,
-                                          int wdt, int C, int G) {
-  constexpr int V = Elem<T>::V;
-  const int cpg = C / G;
-  int c = (int)(((long)threadIdx.x * V) % C);
+__device__ __forceinline__ ChanIn gn_channel(const void* w, const void* b, int wdt, int C, int cpg) {
+  const int c = threadIdx.x;
+  return c < C ? ChanIn{param(w, wdt, c, 1.f), param(b, wdt, c, 0.f), c / cpg} : ChanIn{0.f, 0.f, 0};
+}
+template <int V>
+__device__ __forceinline__ void gn_take(float (&v)[V], const float* lds, int c0, int C) {
 #pragma unroll
-  for (int k = 0; k < V; ++k) {
-    const double2 v = st[c / cpg];
-    cc.m[k] = (float)v.x;
-    cc.rw[k] = (float)(v.y * (double)param(w, wdt, c, 1.f));
-    cc.b[k] = param(b, wdt, c, 0.f);
+  for (int k = 0, c = c0; k < V; ++k) {
+    v[k] = lds[c];
     c = c + 1 == C ? 0 : c + 1;
   }
 }
@@ -300,6 +298,7 @@ __global__ void __launch_bounds__(kGnT) gn_apply_kernel(const T* x, const T* res
   constexpr int V = Elem<T>::V;
   constexpr bool RES = MODE == kResRelu || MODE == kAddRelu;
   __shared__ double2 st[kGnMaxC];
+  __shared__ float lds[3][kGnMaxC];
   constexpr int U = 4;
   const int n = blockIdx.y, t = threadIdx.x;
   const long base = (long)n * HW * C;
@@ -316,15 +315,26 @@ __global__ void __launch_bounds__(kGnT) gn_apply_kernel(const T* x, const T* res
   };
   long f = c0 * sp.active + t;
   load(f);   // on their way while the statistics are added up
+  const ChanIn ch = gn_channel(w, b, wdt, C, C / G);
   gn_finish_stats(part, n, S, G, (long)HW * (C / G), eps, st, blockIdx.x == 0 ? stats_out : nullptr);
+  if (t < C) {   // y = (x - m) rw + b
+    const double2 v = st[ch.g];
+    lds[0][t] = (float)v.x;
+    lds[1][t] = (float)(v.y * (double)ch.w);
+    lds[2][t] = ch.b;
+  }
+  __syncthreads();
   if (t >= sp.active) return;
-  ChanConst<V> cc;
-  gn_consts<T>(cc, st, w, b, wdt, C, G);
+  float m[V], rw[V], bc[V];
+  const int ct = (t * V) % C;
+  gn_take(m, lds[0], ct, C);
+  gn_take(rw, lds[1], ct, C);
+  gn_take(bc, lds[2], ct, C);
   auto piece = [&](const Piece<T>& p, const Piece<T>& rp) {
     Piece<T> o;
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      const float nn = fmaf((float)p.v[k] - cc.m[k], cc.rw[k], cc.b[k]);
+      const float nn = fmaf((float)p.v[k] - m[k], rw[k], bc[k]);
       o.v[k] = (T)gn_act<MODE>(nn, RES ? (float)rp.v[k] : 0.f);
     }
     return o;
@@ -430,17 +440,28 @@ __global__ void __launch_bounds__(kGnT, 4) gn_bwd_stats_kernel(const T* __restri
   const double2* st = stats + (long)n * G;
   // channel constants: xhat = (x - m) rs, n = xhat wc + bc
   float m[V], rs[V], wc[V], bc[V], a1[V], a2[V], tol = 0.f;
-  int cg = (t * V) % C;
+  {
+    float (&lds)[4][kGnMaxC] = *reinterpret_cast<float (*)[4][kGnMaxC]>(&red[0][0]);   // free again before the sums
+    const ChanIn ch = gn_channel(w, b, wdt, C, cpg);
+    if (t < C) {
+      const double2 v = st[ch.g];
+      lds[0][t] = (float)v.x;
+      lds[1][t] = (float)v.y;
+      lds[2][t] = ch.w;
+      lds[3][t] = ch.b;
+    }
+    __syncthreads();
+    const int ct = (t * V) % C;
+    gn_take(m, lds[0], ct, C);
+    gn_take(rs, lds[1], ct, C);
+    gn_take(wc, lds[2], ct, C);
+    gn_take(bc, lds[3], ct, C);
+    __syncthreads();
+  }
 #pragma unroll
   for (int k = 0; k < V; ++k) {
-    const double2 v = st[cg / cpg];
-    m[k] = (float)v.x;
-    rs[k] = (float)v.y;
-    wc[k] = param(w, wdt, cg, 1.f);
-    bc[k] = param(b, wdt, cg, 0.f);
     tol = fmaxf(tol, kTol * (2.f * fabsf(bc[k]) + fabsf(m[k] * rs[k] * wc[k])));
     a1[k] = a2[k] = 0.f;
-    cg = cg + 1 == C ? 0 : cg + 1;
   }
   const long base = (long)n * HW * C;
   const long c0 = sp.chunks * s / S, c1 = sp.chunks * (s + 1) / S;
@@ -583,6 +604,22 @@ __global__ void __launch_bounds__(kGnT, 4) gn_bwd_apply_kernel(const T* __restri
   // the images in the other order: the last ones are still in the cache
   const int cpg = C / G, n = N - 1 - blockIdx.y;
   const double2* st = stats + (long)n * G;
+  const long base = (long)n * HW * C;
+  const long c0 = sp.chunks * blockIdx.x / gridDim.x, c1 = sp.chunks * (blockIdx.x + 1) / gridDim.x;
+  const long f1 = t < sp.active ? min(c1 * sp.active, sp.pieces) : 0;
+  Piece<T> p[2], gp[2];
+  auto load = [&](long f) {   // two pieces in flight a thread
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      if (f + u * sp.active < f1) {
+        const long o = base + (f + u * sp.active) * V;
+        p[u] = load_piece(x + o), gp[u] = load_piece(dyr + o);
+      }
+  };
+  long f = c0 * sp.active + t;
+  load(f);   // on their way while the sums are added up
+  __shared__ float lds[5][kGnMaxC];
+  const ChanIn ch = gn_channel(w, b, wdt, C, cpg);
   {
     const int L = lanes_per(G), g = t / L, l = t % L;
     double u = 0.0, v = 0.0;
@@ -598,25 +635,27 @@ __global__ void __launch_bounds__(kGnT, 4) gn_bwd_apply_kernel(const T* __restri
     const double M = (double)HW * cpg;
     if (g < G && l == 0) sm[g] = make_double2(u / M, v / M);
     __syncthreads();
+    if (t < C) {
+      const double2 ms = st[ch.g], kk = sm[ch.g];
+      lds[0][t] = (float)ms.x;
+      lds[1][t] = (float)(ms.y * (double)ch.w);
+      lds[2][t] = ch.b;
+      lds[3][t] = (float)(ms.y * kk.x);
+      lds[4][t] = (float)(ms.y * ms.y * kk.y);
+    }
+    __syncthreads();
   }
   if (t >= sp.active) return;
   // dx = rstd w dn - rstd (k1 + xhat k2): per channel rw = rstd w, q1 = rstd k1, q2 = rstd^2 k2
-  ChanConst<V> cc;
-  gn_consts<T>(cc, st, w, b, wdt, C, G);
-  float q1[V], q2[V], tol = 0.f;
-  int cg = (t * V) % C;
+  float m[V], rw[V], bc[V], q1[V], q2[V], tol = 0.f;
+  const int ct = (t * V) % C;
+  gn_take(m, lds[0], ct, C);
+  gn_take(rw, lds[1], ct, C);
+  gn_take(bc, lds[2], ct, C);
+  gn_take(q1, lds[3], ct, C);
+  gn_take(q2, lds[4], ct, C);
 #pragma unroll
-  for (int k = 0; k < V; ++k) {
-    const double r = st[cg / cpg].y;
-    const double2 kk = sm[cg / cpg];
-    q1[k] = (float)(r * kk.x);
-    q2[k] = (float)(r * r * kk.y);
-    tol = fmaxf(tol, kTol * (2.f * fabsf(cc.b[k]) + fabsf(cc.m[k] * cc.rw[k])));
-    cg = cg + 1 == C ? 0 : cg + 1;
-  }
-  const long base = (long)n * HW * C;
-  const long c0 = sp.chunks * blockIdx.x / gridDim.x, c1 = sp.chunks * (blockIdx.x + 1) / gridDim.x;
-  const long f1 = min(c1 * sp.active, sp.pieces);
+  for (int k = 0; k < V; ++k) tol = fmaxf(tol, kTol * (2.f * fabsf(bc[k]) + fabsf(m[k] * rw[k])));
   // the outer ReLU's slope is in dyr (= dres) already: what is left is mode 0's
   // ReLU (mode 1's inner one), or SiLU's slope
   constexpr int LEFT = MODE == kResRelu ? (int)kRelu : MODE == kAddRelu ? (int)kNone : MODE;
@@ -624,30 +663,24 @@ __global__ void __launch_bounds__(kGnT, 4) gn_bwd_apply_kernel(const T* __restri
     float d[V], nn[V], dn[V], dr[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      d[k] = (float)p.v[k] - cc.m[k];
-      nn[k] = fmaf(d[k], cc.rw[k], cc.b[k]);
+      d[k] = (float)p.v[k] - m[k];
+      nn[k] = fmaf(d[k], rw[k], bc[k]);
     }
     gn_slopes<T, LEFT>(nn, gp, gp, tol, x, nullptr, at, cnt, st, w, b, wdt, C, cpg, dn, dr);
     Piece<T> o;
 #pragma unroll
-    for (int k = 0; k < V; ++k) o.v[k] = (T)(fmaf(dn[k], cc.rw[k], -fmaf(d[k], q2[k], q1[k])));
+    for (int k = 0; k < V; ++k) o.v[k] = (T)(fmaf(dn[k], rw[k], -fmaf(d[k], q2[k], q1[k])));
     return o;
   };
-  for (long f = c0 * sp.active + t; f < f1; f += 2 * sp.active) {
-    Piece<T> p[2], gp[2];
-    const bool two = f + sp.active < f1;
+  while (f < f1) {
 #pragma unroll
     for (int u = 0; u < 2; ++u)
-      if (u == 0 || two) {
-        const long o = base + (f + u * sp.active) * V;
-        p[u] = load_piece(x + o), gp[u] = load_piece(dyr + o);
-      }
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-      if (u == 0 || two) {
+      if (f + u * sp.active < f1) {
         const long at = base + (f + u * sp.active) * V;
         store_piece(dx + at, piece(p[u], gp[u], at, V));
       }
+    f += 2 * sp.active;
+    load(f);
   }
   if (sp.tail && c1 == sp.chunks && sp.pieces % sp.active == t) {
     const long o0 = base + sp.pieces * V;

@@ -13,6 +13,7 @@ mirror in `droid_mi355x`): `corr_pyramid_lookup`, `projective_transform`,
 `BaPlan`, and optional host copies of ii/jj for `ba` (avoids the D2H sync).
 """
 import ctypes
+import functools
 import os
 from collections import OrderedDict
 
@@ -59,6 +60,16 @@ def _on(dev):
     return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
+@functools.lru_cache(maxsize=256)
+def _group_norm_workspace(*sizes):
+    return lib.droid_group_norm_workspace(*sizes)
+
+
+@functools.lru_cache(maxsize=256)
+def _corr_loss_workspace(*sizes):
+    return lib.droid_corr_loss_workspace(*sizes)
+
+
 def _raw_stream(dev):
     return torch._C._cuda_getCurrentRawStream(dev.index)
 
@@ -70,7 +81,7 @@ def _check_inputs(names, tensors):
             raise TypeError("%s must be a torch.Tensor" % name)
         if not t.is_contiguous():
             raise RuntimeError("%s must be contiguous" % name)
-        if t.device.type != "cuda":
+        if not t.is_cuda:
             raise RuntimeError("droid_backends: %s must be a HIP device tensor (no CPU path)" % name)
         if dev is None:
             dev = t.device
@@ -359,7 +370,7 @@ def corr_loss_forward(fmap1, fmap2, f1, f2, idx, logits=None, scale=1.0 / 16, te
     if loss.numel() == 0:
         return loss, lse, prob
     with _on(dev):
-        ws = torch.empty((lib.droid_corr_loss_workspace(E, N1, P, N2, Q, D, K or 1, 0),), dtype=torch.uint8, device=dev)
+        ws = torch.empty((_corr_loss_workspace(E, N1, P, N2, Q, D, K or 1, 0),), dtype=torch.uint8, device=dev)
         check(lib.droid_corr_loss_forward(_LOSS_DTYPES[fmap1.dtype], _addr(fmap1), _addr(keys), _addr(f1), _addr(f2),
                                           _addr(idx), _addr(logits), _addr(loss), _addr(lse), _addr(prob), E, N1, P, N2, Q,
                                           D, K or 1, scale, temperature, _addr(ws), ws.numel(), _raw_stream(dev)), fn)
@@ -395,7 +406,7 @@ def corr_loss_backward(gloss, fmap1, fmap2, f1, f2, idx, lse, prob=None, scale=1
         return d1, d2
     dev = fmap1.device
     with _on(dev):
-        ws = torch.empty((lib.droid_corr_loss_workspace(E, N1 if need1 else 0, P, N2 if need2 else 0, Q, D, K or 1,
+        ws = torch.empty((_corr_loss_workspace(E, N1 if need1 else 0, P, N2 if need2 else 0, Q, D, K or 1,
                                                         1),), dtype=torch.uint8, device=dev)
         check(lib.droid_corr_loss_backward(_LOSS_DTYPES[fmap1.dtype], _addr(fmap1), _addr(keys), _addr(f1), _addr(f2),
                                            _addr(idx), _addr(prob), _addr(lse), _addr(gloss), _addr(d1), _addr(d2),
@@ -952,7 +963,7 @@ def _norm_map(fn, name, t, x=None):
     """A channels_last (N,C,H,W) map of group_norm_act, of x's shape, type and device where x is given."""
     if not isinstance(t, torch.Tensor):
         raise TypeError("%s: %s must be a torch.Tensor" % (fn, name))
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise RuntimeError("droid_backends: %s: %s must be a HIP device tensor (no CPU path)" % (fn, name))
     if t.dtype not in _NORM_DTYPES or t.dim() != 4 or not t.is_contiguous(memory_format=torch.channels_last):
         raise RuntimeError("%s: %s must be a channels_last float16, bfloat16 or float32 (N,C,H,W) tensor" % (fn, name))
@@ -1004,7 +1015,7 @@ def group_norm_act(x, num_groups, weight=None, bias=None, mode=NORM_RELU, res=No
     dt, hw, dev = _NORM_DTYPES[x.dtype], H * W, x.device
     stats = torch.empty((N, num_groups, 2), dtype=torch.float64, device=dev) if return_stats else None
     with _on(dev):
-        ws = torch.empty((lib.droid_group_norm_workspace(dt, N, hw, C, num_groups, 0),), dtype=torch.uint8, device=dev)
+        ws = torch.empty((_group_norm_workspace(dt, N, hw, C, num_groups, 0),), dtype=torch.uint8, device=dev)
         check(lib.droid_group_norm_act(dt, _addr(x), _addr(res), _addr(out), _addr(weight), _addr(bias), wdt, _addr(stats),
                                        N, hw, C, num_groups, mode, eps, _addr(ws), ws.numel(), _raw_stream(dev)), fn)
     return (out, stats) if return_stats else out
@@ -1035,7 +1046,7 @@ def group_norm_act_backward(dy, x, stats, num_groups, weight=None, bias=None, mo
     dw = new(weight) if weight is not None else None
     db = new(bias) if bias is not None else None
     with _on(dev):
-        ws = torch.empty((lib.droid_group_norm_workspace(dt, N, hw, C, num_groups, 1),), dtype=torch.uint8, device=dev)
+        ws = torch.empty((_group_norm_workspace(dt, N, hw, C, num_groups, 1),), dtype=torch.uint8, device=dev)
         check(lib.droid_group_norm_act_backward(dt, _addr(x), _addr(res if with_res else None), _addr(dy), _addr(weight),
                                                 _addr(bias), wdt, _addr(stats), _addr(dx), _addr(dres), _addr(dw),
                                                 _addr(db), N, hw, C, num_groups, mode, _addr(ws), ws.numel(),
