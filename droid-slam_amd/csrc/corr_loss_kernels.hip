@@ -129,19 +129,6 @@ __device__ __forceinline__ unsigned row_addr(unsigned tile, int lane) {
   return tile + r * 2 * DP + ((h ^ swz<DP>(r)) << 4);
 }
 
-// s[row of the tile's 32-row block][stationary row] = tile . stationary^T
-template <typename T, int DP>
-__device__ __forceinline__ floatx16 block_product(unsigned row0, int blk, const typename Op<T>::vec8 (&b)[DP / 16]) {
-  typedef const __attribute__((address_space(3))) typename Op<T>::vec8* ptr;
-  floatx16 acc;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) acc[i] = 0.f;
-#pragma unroll
-  for (int k = 0; k < DP / 16; ++k)
-    acc = Op<T>::mfma(*(ptr)(uintptr_t)((row0 ^ (k << 5)) + blk * 64 * DP), b[k], acc);
-  return acc;
-}
-
 // All of the wave's loads have landed, LDS-DMA included.  The builtin, not inline
 // asm: the compiler does not count the DMAs, and where it cannot see that its own
 // loads have landed it waits for "them" - in fact the DMAs in flight - again in
@@ -183,9 +170,19 @@ struct FwdArgs {
   float c;                     // scale / T log2(e)
 };
 
+// 32-row blocks of queries a wave: two where the registers allow three such
+// workgroups a CU, since every operand read from shared memory then feeds two matrix
+// instructions (with one, 128 B a clock of shared memory is what bounds the loop).
+template <int DP>
+constexpr int kXF = DP <= 128 ? 2 : 1;
+inline int fwd_rows(int D) { return D <= 128 ? 2 * kRowsB : kRowsB; }
+inline int fwd_groups(int D) { return D <= 128 ? 3 : 2; }   // workgroups a CU
+
 // Per query row the maximum and the sum of 2^(c s - max) over a share of the keys.
 template <typename T, int DP>
-__global__ void __launch_bounds__(kLT, DP <= 128 ? 4 : 2) corr_lse_kernel(FwdArgs a) {
+__global__ void __launch_bounds__(kLT, DP <= 128 ? 3 : 2) corr_lse_kernel(FwdArgs a) {
+  typedef const __attribute__((address_space(3))) typename Op<T>::vec8* ptr;
+  constexpr int XF = kXF<DP>;
   __shared__ __attribute__((aligned(1024))) char tile[2][kRowsY * 2 * DP];
   const int item = xcd_item(blockIdx.x, a.items);
   if (item >= a.items) return;
@@ -193,11 +190,11 @@ __global__ void __launch_bounds__(kLT, DP <= 128 ? 4 : 2) corr_lse_kernel(FwdArg
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i = a.e1[e], j = a.e2[e];
   if (i < 0 || i >= a.N1 || j < 0 || j >= a.N2) return;   // the row kernel answers NaN
-  const int p = pt * kRowsB + wave * 32 + (lane & 31);
+  const int p0 = (pt * 4 + wave) * 32 * XF;
   // rows without a target need no sum; a workgroup of them does nothing
   bool want = false;
-  if (p < a.P)
-    for (int k = 0; k < a.K; ++k) want |= a.idx[((long)e * a.P + p) * a.K + k] >= 0;
+  if (p0 + lane < a.P && lane < 32 * XF)
+    for (int k = 0; k < a.K; ++k) want |= a.idx[((long)e * a.P + p0 + lane) * a.K + k] >= 0;
   if (!__syncthreads_or(want)) return;
   const T* f1 = static_cast<const T*>(a.f1) + (long)i * a.P * a.D;
   const T* f2 = static_cast<const T*>(a.f2) + (long)j * a.Q * a.D;
@@ -205,46 +202,63 @@ __global__ void __launch_bounds__(kLT, DP <= 128 ? 4 : 2) corr_lse_kernel(FwdArg
   lane_offsets<DP>(off, a.D, wave, lane);
   const int nt = (a.Q + kRowsY - 1) / kRowsY;
   const int t0 = nt * s / a.S, t1 = nt * (s + 1) / a.S;
-  typename Op<T>::vec8 b[DP / 16];
-  load_rows<T, DP>(b, f1, p, a.P, a.D, lane >> 5);
   auto none = [](int) { return false; };
   stage_tile<T, DP>(f2, tile[0], t0 * kRowsY, a.Q, a.D, off, wave, lane, none);
+  typename Op<T>::vec8 b[XF][DP / 16];
+#pragma unroll
+  for (int x = 0; x < XF; ++x) load_rows<T, DP>(b[x], f1, p0 + 32 * x + (lane & 31), a.P, a.D, lane >> 5);
   loads_done();
   __syncthreads();
-  float m = kNegBig, l = 0.f;
+  float m[XF], l[XF];
+#pragma unroll
+  for (int x = 0; x < XF; ++x) m[x] = kNegBig, l[x] = 0.f;
   for (int t = t0; t < t1; ++t) {
     const unsigned row0 = row_addr<DP>(lds_addr(tile[(t - t0) & 1]), lane);
     if (t + 1 < t1) stage_tile<T, DP>(f2, tile[(t + 1 - t0) & 1], (t + 1) * kRowsY, a.Q, a.D, off, wave, lane, none);
-    floatx16 sc[2];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) sc[k] = block_product<T, DP>(row0, k, b);
-    if ((t + 1) * kRowsY > a.Q) {   // keys past the end
-      const int y = t * kRowsY + 4 * (lane >> 5);
+    for (int k = 0; k < 2; ++k) {
+      floatx16 sc[XF];
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
+      for (int x = 0; x < XF; ++x)
 #pragma unroll
-        for (int q = 0; q < 16; ++q)
-          if (y + 32 * k + 8 * (q >> 2) + (q & 3) >= a.Q) sc[k][q] = -INFINITY;
+        for (int q = 0; q < 16; ++q) sc[x][q] = 0.f;
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) {
+        const typename Op<T>::vec8 f = *(ptr)(uintptr_t)((row0 ^ (d << 5)) + k * 64 * DP);
+#pragma unroll
+        for (int x = 0; x < XF; ++x) sc[x] = Op<T>::mfma(f, b[x][d], sc[x]);
+      }
+      if (t * kRowsY + 32 * k + 32 > a.Q) {   // keys past the end
+        const int y = t * kRowsY + 32 * k + 4 * (lane >> 5);
+#pragma unroll
+        for (int x = 0; x < XF; ++x)
+#pragma unroll
+          for (int q = 0; q < 16; ++q)
+            if (y + 8 * (q >> 2) + (q & 3) >= a.Q) sc[x][q] = -INFINITY;
+      }
+#pragma unroll
+      for (int x = 0; x < XF; ++x) {
+        float mx = sc[x][0];
+#pragma unroll
+        for (int q = 1; q < 16; ++q) mx = fmaxf(mx, sc[x][q]);
+        const float mn = fmaxf(m[x], mx * a.c);
+        l[x] *= __builtin_amdgcn_exp2f(m[x] - mn);
+        m[x] = mn;
+#pragma unroll
+        for (int q = 0; q < 16; ++q) l[x] += __builtin_amdgcn_exp2f(fmaf(sc[x][q], a.c, -mn));
+      }
     }
-    float mx = sc[0][0];
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll
-      for (int q = 0; q < 16; ++q) mx = fmaxf(mx, sc[k][q]);
-    const float mn = fmaxf(m, mx * a.c);
-    l *= __builtin_amdgcn_exp2f(m - mn);
-    m = mn;
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll
-      for (int q = 0; q < 16; ++q) l += __builtin_amdgcn_exp2f(fmaf(sc[k][q], a.c, -m));
     loads_done();
     __syncthreads();
   }
-  const float mo = __shfl_xor(m, 32, 64), lo = __shfl_xor(l, 32, 64);
-  const float mm = fmaxf(m, mo);
-  l = l * __builtin_amdgcn_exp2f(m - mm) + lo * __builtin_amdgcn_exp2f(mo - mm);
-  if (lane < 32 && p < a.P) a.part[((long)e * a.P + p) * a.S + s] = make_float2(mm, l);
+#pragma unroll
+  for (int x = 0; x < XF; ++x) {
+    const float mo = __shfl_xor(m[x], 32, 64), lo = __shfl_xor(l[x], 32, 64);
+    const float mm = fmaxf(m[x], mo);
+    const float sum = l[x] * __builtin_amdgcn_exp2f(m[x] - mm) + lo * __builtin_amdgcn_exp2f(mo - mm);
+    const int p = p0 + 32 * x + (lane & 31);
+    if (lane < 32 && p < a.P) a.part[((long)e * a.P + p) * a.S + s] = make_float2(mm, sum);
+  }
 }
 
 struct RowArgs {
@@ -1130,10 +1144,17 @@ __global__ void __launch_bounds__(kLT) corr_loss_join_kernel(BwdArgs a) {
   }
 }
 
-// Shares of the streamed axis: enough workgroups for the 256 CUs, no more shares than tiles.
-int fwd_split(int E, int P, int Q) {
-  const long blocks = (long)E * ceil_div(P, kRowsB);
-  return (int)std::max<long>(1, std::min<long>(ceil_div(Q, kRowsY), 1024 / std::max<long>(1, blocks)));
+// Shares of the keys: the split with the least steps of a workgroup one after the
+// other, a share costing about two steps more than its tiles (its start and join).
+int fwd_split(int E, int P, int Q, int D) {
+  const long blocks = (long)E * ceil_div(P, fwd_rows(D)), tiles = ceil_div(Q, kRowsY);
+  const long at_once = (long)fwd_groups(D) * device_cu_count();
+  long best = 1, least = -1;
+  for (long s = 1; s <= std::min<long>(tiles, std::max<long>(8, at_once / std::max<long>(1, blocks))); ++s) {
+    const long steps = (blocks * s + at_once - 1) / at_once * ((tiles + s - 1) / s + 2);
+    if (least < 0 || steps < least) best = s, least = steps;
+  }
+  return (int)best;
 }
 
 // Workgroups of the gradient kernel: as many as run at once, one a CU by its registers.
@@ -1189,7 +1210,7 @@ extern "C" {
 
 size_t droid_corr_loss_workspace(int E, int N1, int P, int N2, int Q, int D, int K, int backward) {
   if (E <= 0 || N1 < 0 || P <= 0 || N2 < 0 || Q <= 0 || D <= 0 || K <= 0) return 0;
-  if (!backward) return (size_t)E * P * fwd_split(E, P, Q) * sizeof(float2);
+  if (!backward) return (size_t)E * P * fwd_split(E, P, Q, D) * sizeof(float2);
   return bwd_space(E, P, Q, N1 + N2, D, K).bytes;
 }
 
@@ -1206,8 +1227,8 @@ int droid_corr_loss_forward(int dtype, const void* fmap1, const void* fmap2, con
   if (unaligned(fmap1) || unaligned(fmap2)) return fail(kInvalidArgument, what + ": features must be 16-B aligned");
   if (!ws || ws_bytes < droid_corr_loss_workspace(E, N1, P, N2, Q, D, K, 0))
     return fail(kInvalidArgument, what + ": workspace too small");
-  FwdArgs a{fmap1, fmap2, f1, f2, idx, static_cast<float2*>(ws), E, N1, P, N2, Q, D, K, ceil_div(P, kRowsB),
-            fwd_split(E, P, Q), 0, scale / temperature * kLog2e};
+  FwdArgs a{fmap1, fmap2, f1, f2, idx, static_cast<float2*>(ws), E, N1, P, N2, Q, D, K, ceil_div(P, fwd_rows(D)),
+            fwd_split(E, P, Q, D), 0, scale / temperature * kLog2e};
   a.items = E * a.tiles * a.S;
 #define LSE(T, DP) corr_lse_kernel<T, DP><<<(a.items + 7) / 8 * 8, kLT, 0, stream>>>(a)
   CORR_TYPES(LSE)
