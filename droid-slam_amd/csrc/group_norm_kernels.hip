@@ -357,7 +357,8 @@ __global__ void __launch_bounds__(kGnT) gn_apply_kernel(const T* x, const T* res
 
 // dn and dres of one value (r: res, g: dy, n: the normed value).  tol = kTol times
 // the largest 2 |b| + |m rw| of the thread's channels bounds n's fp32 error;
-// returns whether a ReLU's argument is within that of zero.
+// returns whether a ReLU's argument is within that of zero (never where it is
+// exact: channels with weight and bias 0, an image of zeros).
 template <int MODE>
 __device__ __forceinline__ bool gn_slope(float r, float g, float n, float tol, float& dn, float& dres) {
   dres = dn = g;
@@ -366,16 +367,16 @@ __device__ __forceinline__ bool gn_slope(float r, float g, float n, float tol, f
     dn = g * sg * (1.f + n * (1.f - sg));
   } else if constexpr (MODE == kRelu) {
     dn = n > 0.f ? g : 0.f;
-    return fabsf(n) <= tol;
+    return fabsf(n) < tol;
   } else if constexpr (MODE == kResRelu) {
     const float pre = r + fmaxf(n, 0.f);
     dres = pre > 0.f ? g : 0.f;
     dn = n > 0.f ? dres : 0.f;
-    return fabsf(n) <= tol || (n > 0.f && fabsf(pre) <= fmaf(kTol, fabsf(r), tol));   // (n < 0: pre is r itself)
+    return fabsf(n) < tol || (n > 0.f && fabsf(pre) < fmaf(kTol, fabsf(r), tol));   // (n < 0: pre is r itself)
   } else if constexpr (MODE == kAddRelu) {
     const float pre = n + r;
     dn = dres = pre > 0.f ? g : 0.f;
-    return fabsf(pre) <= fmaf(kTol, fabsf(r), tol);
+    return fabsf(pre) < fmaf(kTol, fabsf(r), tol);
   }
   return false;
 }

@@ -10,7 +10,11 @@ Weights: p off by a factor of at most 1 + r + Q u + 8 u (1 + |lse|); p - pi
 and its product with g a rounding each, then one rounding to the features'
 type: h |ds| (fp16 weights are scaled to 2^13 times the edge's largest |g|
 share, so what underflows is below 2^-38 of it).  Gradients: these sums over
-the other rows, n fp32 additions of them, one rounding at the end."""
+the other rows, n fp32 additions of them, one rounding at the end.
+An edge and its reverse with upstream gradients >= 0 share one exponential:
+the weights are products of three powers of two whose exponents are below
+60 + |log2 g| + 1.5 |lse| each and are rounded once: PAIR u more, relative to p,
+and what underflows is below 2^-86 of a probability."""
 import numpy as np
 import pytest
 import torch
@@ -21,6 +25,7 @@ from oracle import corr_loss as oc
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
 U = 2.0 ** -24
+PAIR = 256
 TYPES = {"fp16": torch.float16, "bf16": torch.bfloat16}
 
 
@@ -53,7 +58,7 @@ def _run(a, b, f1, f2, idx, logits, g, shared, scale, T):
     return loss.detach(), torch.autograd.grad(loss, leaves, _t(g))
 
 
-def _check(dt, a, b, f1, f2, idx, logits, g, shared, scale, T, loss, grads):
+def _check(dt, a, b, f1, f2, idx, logits, g, shared, scale, T, loss, grads, more=0):
     A, B = host(a.double()), host(b.double())
     T = T if logits is not None else 1.0
     D, Q, h = A.shape[-1], B.shape[1], torch.finfo(dt).eps / 2
@@ -66,7 +71,7 @@ def _check(dt, a, b, f1, f2, idx, logits, g, shared, scale, T, loss, grads):
             logits is not None)                       # logf / expf of the teacher's weights: K entries, a few u each
         assert (np.abs(host(loss)[e] - want[e]) <= tol).all(), e
         ge = np.abs(g[e])[:, None] * T * scale
-        rel = (r + Q * U + 8 * U * (1 + np.abs(lse)))[:, None]
+        rel = (r + Q * U + 8 * U * (1 + np.abs(lse)) + more * U)[:, None]
         # rows with a target: also where p - pi is exactly 0 (one key: p = 1 up to its error), left-out rows are exact
         on = (q.max(1, keepdims=True) > 0)
         floor = np.abs(g).max() * T * scale * 2.0 ** -38 if dt == torch.float16 else 0.0
@@ -248,3 +253,130 @@ def test_device_refusals_and_empty_calls():
     assert loss.shape == (0, 20) and prob is None
     d1, d2 = nb.corr_loss_backward(loss, a, b, e, e, torch.empty((0, 20), dtype=torch.int32, device=DEV), lse)
     assert d1.shape == a.shape and d2.shape == b.shape and not d1.any() and not d2.any()
+
+
+GRAPHS = {   # edges of a frame graph: both directions, one, twice the same, a frame with itself
+    "pairs": ([0, 1, 1, 2, 0, 2, 3, 2], [1, 0, 2, 1, 2, 0, 2, 3]),
+    "mixed": ([0, 1, 0, 1, 2, 2, 3, 0, 1], [1, 0, 1, 2, 2, 2, 0, 0, 3]),
+    "loops": ([1, 1, 2], [1, 1, 2])}
+
+
+@pytest.mark.parametrize("K", [0, 5, 64])
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("graph", list(GRAPHS))
+@pytest.mark.parametrize("P,D,amp", [(190, 128, 1.0), (70, 40, 1.0), (129, 200, 1.0), (130, 128, 5.0), (65, 128, 0.0)])
+def test_frame_graph_with_positive_gradients(P, D, amp, graph, dtype, K):
+    """The gradient of a mean or a weighted sum: g >= 0, some of it 0 or tiny;
+    amp 5: the rows' sums lie further apart than one exponential may serve;
+    amp 0: all logits equal."""
+    dt = TYPES[dtype]
+    a, _, _, _, _, _, _ = _problem(P + D, dt, 0, 1, 4, P, 4, P, D, amp, shared=True)
+    f1, f2 = (np.array(v, np.int32) for v in GRAPHS[graph])
+    E = len(f1)
+    _, _, _, _, idx, logits, g = _problem(P, dt, K, E, 4, P, 4, P, D, shared=True)
+    g = np.abs(g)
+    g[:, ::7] = 0.0
+    g[:, 1::9] *= 1e-6
+    p = (a, a, f1, f2, idx, logits, g)
+    loss, grads = _run(*p, True, 1 / 16, 1.0)
+    _check(dt, *p, True, 1 / 16, 1.0, loss, grads, PAIR)
+
+
+def test_pairs_whose_one_side_is_dead_or_wrong():
+    """An edge without a target, an edge out of range and left-out rows that are
+    not finite, each with a live reverse."""
+    dt = torch.float16
+    a, _, _, _, idx, logits, g = _problem(21, dt, 3, 6, 4, 150, 4, 150, 64, shared=True)
+    g = np.abs(g)
+    f1, f2 = np.array([0, 1, 0, 2, 1, 3], np.int32), np.array([1, 0, 2, 0, 3, 1], np.int32)
+    idx[1] = -1                               # (1, 0) has no target
+    loss, grads = _run(a, a, f1, f2, idx, logits, g, True, 1 / 16, 1.0)
+    _check(dt, a, a, f1, f2, idx, logits, g, True, 1 / 16, 1.0, loss, grads, PAIR)
+    h1 = f1.copy()
+    h1[5] = 4                                 # (3, 1) becomes an edge of a frame that is not there
+    loss, grads = _run(a, a, h1, f2, idx, logits, g, True, 1 / 16, 1.0)
+    on = torch.from_numpy((idx[5] >= 0).any(-1)).to(DEV)   # left-out rows: loss 0 there too
+    assert torch.equal(loss[5].isnan(), on) and not loss[:5].isnan().any()
+    assert not grads[0][[0, 2]].isnan().any()
+    # frame 3's rows 5..9 have no target in their own edge, and are no key of a live edge
+    b = a.clone()
+    b[3, 5:10] = float("nan")
+    idx[5, 5:10], idx[4] = -1, -1
+    loss, grads = _run(b, b, f1, f2, idx, logits, g, True, 1 / 16, 1.0)
+    b[3, 5:10] = 0.0
+    _check(dt, b, b, f1, f2, idx, logits, g, True, 1 / 16, 1.0, loss, grads, PAIR)
+
+
+def test_one_bad_row_of_a_pair():
+    """A row whose target is out of range is NaN in both of its gradients and
+    leaves the other frames alone."""
+    dt = torch.bfloat16
+    a, _, _, _, idx, _, g = _problem(22, dt, 0, 3, 3, 70, 3, 70, 32, shared=True)
+    f1, f2 = np.array([0, 1, 2], np.int32), np.array([1, 0, 2], np.int32)
+    idx[0, :, 0] = -1
+    idx[0, 7, 0] = 70
+    idx[1, :, 0] = np.where(np.arange(70) == 3, -1, 5)
+    loss, grads = _run(a, a, f1, f2, idx, None, np.abs(g), True, 1 / 16, 1.0)
+    assert loss[0, 7].isnan() and loss.isnan().sum() == 1
+    assert grads[0][0, 7].isnan().all() and not grads[0][2].isnan().any()
+
+
+@pytest.mark.parametrize("K", [0, 3])
+@pytest.mark.parametrize("sign", [False, True])
+def test_many_edges(sign, K):
+    """More edges than one pass over the edge list holds, most of them paired."""
+    dt = torch.float16
+    p = list(_problem(23, dt, K, 700, 6, 70, 6, 70, 32, shared=True))
+    if not sign:
+        p[-1] = np.abs(p[-1])
+    loss, grads = _run(*p, True, 1 / 16, 1.0)
+    _check(dt, *p, True, 1 / 16, 1.0, loss, grads, PAIR)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_many_frames(dtype):
+    """More frames than the plan's workgroup has threads, few of them used."""
+    dt = TYPES[dtype]
+    p = list(_problem(24, dt, 0, 40, 1500, 9, 1100, 12, 16))
+    loss, grads = _run(*p, False, 1 / 16, 1.0)
+    _check(dt, *p, False, 1 / 16, 1.0, loss, grads)
+    unused = np.setdiff1d(np.arange(1500), p[2])
+    assert not grads[0][torch.from_numpy(unused).to(DEV)].any()
+
+
+@pytest.mark.parametrize("P,Q,K", [(130, 9000, 0), (9000, 130, 0), (70, 9000, 5), (9000, 70, 5)])
+def test_long_frames(P, Q, K):
+    """Frames longer than the streamed range whose sparse terms are sorted at once."""
+    dt = torch.bfloat16
+    p = list(_problem(25, dt, K, 2, 1, P, 2, Q, 8))
+    loss, grads = _run(*p, False, 1 / 16, 1.0)
+    _check(dt, *p, False, 1 / 16, 1.0, loss, grads)
+
+
+def test_long_frames_both_ways():
+    dt = torch.float16
+    a, _, _, _, _, _, _ = _problem(26, dt, 0, 1, 2, 8300, 2, 8300, 8, shared=True)
+    rng = np.random.default_rng(26)
+    idx = rng.integers(-1, 8300, (2, 8300, 1)).astype(np.int32)
+    f1, f2 = np.array([0, 1], np.int32), np.array([1, 0], np.int32)
+    g = rng.random((2, 8300)).astype(np.float32)
+    loss, grads = _run(a, a, f1, f2, idx, None, g, True, 1 / 16, 1.0)
+    _check(dt, a, a, f1, f2, idx, None, g, True, 1 / 16, 1.0, loss, grads, PAIR)
+
+
+@pytest.mark.parametrize("positive", [False, True])
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_many_targets_on_few_keys(dtype, positive):
+    """64 targets a row, all rows the same 64 keys and some keys twice: more
+    sparse terms at one place than are kept in shared memory."""
+    dt = TYPES[dtype]
+    a, _, f1, f2, idx, logits, g = _problem(27, dt, 64, 3, 2, 700, 2, 700, 64, shared=True)
+    f1[:], f2[:] = [0, 1, 0], [1, 0, 0]
+    idx[:] = np.arange(64)
+    idx[:, :, 60:] = 3
+    idx[:, ::5, 10:20] = -1
+    if positive:
+        g = np.abs(g)
+    p = (a, a, f1, f2, idx, logits, g)
+    loss, grads = _run(*p, True, 1 / 16, 1.0)
+    _check(dt, *p, True, 1 / 16, 1.0, loss, grads, PAIR)
