@@ -10,28 +10,49 @@ reference runs it (the parity bridge for the tests).
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 import droid_backends
 
 DIM = 32
 
 
+def _group_norm_act_plain(x, num_groups, weight, bias, mode, res, eps):
+    nb = droid_backends
+    f = lambda t: None if t is None else t.float()
+    n = F.group_norm(x.float(), num_groups, f(weight), f(bias), eps)
+    if mode == nb.NORM_RELU:
+        n = torch.relu(n)
+    elif mode == nb.NORM_RES_RELU:
+        n = torch.relu(res.float() + torch.relu(n))
+    elif mode == nb.NORM_ADD_RELU:
+        n = torch.relu(n + res.float())
+    elif mode == nb.NORM_SILU:
+        n = F.silu(n)
+    return n.to(x.dtype)
+
+
 class GroupNormAct(torch.autograd.Function):
     """Group norm + activation / residual add (droid_group_norm_act and its
-    backward): statistics in 64 bits, gradients of every input."""
+    backward): statistics in 64 bits, gradients of every input.  A backward pass
+    that is itself differentiated (create_graph) goes through torch's operators."""
 
     @staticmethod
     def forward(ctx, x, num_groups, weight, bias, mode, res, eps):
         y, stats = droid_backends.group_norm_act(x, num_groups, weight, bias, mode, res, eps=eps, return_stats=True)
         ctx.save_for_backward(x, weight, bias, res, stats)
-        ctx.num_groups, ctx.mode = num_groups, mode
+        ctx.num_groups, ctx.mode, ctx.eps = num_groups, mode, eps
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
         x, weight, bias, res, stats = ctx.saved_tensors
+        if torch.is_grad_enabled():
+            # (views: x and res may be one tensor)
+            ins = {i: t.view_as(t) for i, t in ((0, x), (2, weight), (3, bias), (5, res)) if t is not None}
+            y = _group_norm_act_plain(ins[0], ctx.num_groups, ins.get(2), ins.get(3), ctx.mode, ins.get(5), ctx.eps)
+            want = [i for i in ins if ctx.needs_input_grad[i]]
+            grads = dict(zip(want, torch.autograd.grad(y, [ins[i] for i in want], dy, create_graph=True)))
+            return tuple(grads.get(i) for i in range(7))
         dy = dy.contiguous(memory_format=torch.channels_last)
         dx, dres, dw, db = droid_backends.group_norm_act_backward(dy, x, stats, ctx.num_groups, weight, bias, ctx.mode,
                                                                   res)
@@ -58,6 +79,12 @@ def _norm(kind, planes):
     return nn.Sequential()
 
 
+def _norm_act(norm, x, mode, res=None):
+    """nn.GroupNorm on a convolution's output, with the activation / residual add after it."""
+    return group_norm_act(x.contiguous(memory_format=torch.channels_last), norm.num_groups, norm.weight, norm.bias,
+                          mode, res, norm.eps)
+
+
 class ResidualBlock(nn.Module):
     """extractor.py:6-55 (3x3 conv - norm - ReLU twice, 1x1 strided shortcut)."""
 
@@ -80,6 +107,16 @@ class ResidualBlock(nn.Module):
         if self.downsample is not None:
             x = self.downsample(x)
         return self.relu(x + y)
+
+    def forward_group(self, x):
+        """channels_last in and out, group norm fused with what follows it."""
+        nb = droid_backends
+        y = _norm_act(self.norm1, self.conv1(x), nb.NORM_RELU)
+        y2 = self.conv2(y)
+        if self.downsample is None:
+            return _norm_act(self.norm2, y2, nb.NORM_RES_RELU, x)          # relu(x + relu(n(y2)))
+        y = _norm_act(self.norm2, y2, nb.NORM_RELU)
+        return _norm_act(self.norm3, self.downsample[0](x), nb.NORM_ADD_RELU, y)
 
     def forward_fast(self, x):
         """channels_last fp16 in and out (instance or no norm)."""
@@ -155,11 +192,31 @@ class BasicEncoder(nn.Module):
         _, c2, h2, w2 = x.shape
         return x.view(b, n, c2, h2, w2)
 
+    def forward_group(self, x):
+        """forward_reference with norm_fn 'group' on the GPU, for training and
+        inference: channels_last throughout, every norm one operator with its
+        activation and residual add, in the convolutions' type (fp16 / bf16 under
+        autocast, else x's)."""
+        b, n, c1, h1, w1 = x.shape
+        x = x.reshape(b * n, c1, h1, w1).contiguous(memory_format=torch.channels_last)
+        x = _norm_act(self.norm1, self.conv1(x), droid_backends.NORM_RELU)
+        for layer in (self.layer1, self.layer2, self.layer3):
+            for blk in layer:
+                x = blk.forward_group(x)
+        x = self.conv2(x)
+        _, c2, h2, w2 = x.shape
+        return x.contiguous().view(b, n, c2, h2, w2)
+
     def forward(self, x):
         """(b, n, 3, H, W) -> (b, n, C, H/8, W/8) fp16: the MI355X path for the
         norms DroidNet uses (instance: fnet, none: cnet - no running statistics,
         so train and eval mode agree; the reference never applies its dropout).
-        Training (gradients through the encoder) runs the reference ops."""
+        Training (gradients through the encoder) runs the reference ops, except
+        with norm_fn 'group', whose norms are one operator each (forward_group)."""
+        if self.norm_fn == "group" and x.is_cuda:
+            dt = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
+            if dt in (torch.float16, torch.bfloat16, torch.float32) and self.norm1.weight.dtype in (torch.float32, dt):
+                return self.forward_group(x)
         if (self.norm_fn not in ("instance", "none") or not x.is_cuda
                 or (torch.is_grad_enabled() and self.conv1.weight.requires_grad)):
             return self.forward_reference(x)
