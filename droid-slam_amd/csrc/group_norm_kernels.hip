@@ -146,7 +146,7 @@ template <typename T>
 __global__ void __launch_bounds__(kGnT) gn_stats_kernel(const T* __restrict__ x, int HW, int C, int G, Split sp,
                                                         double2* __restrict__ part) {
   constexpr int V = Elem<T>::V;
-  __shared__ double red[kGnT * V];
+  __shared__ double2 red[kGnT * V];
   const int n = blockIdx.y, s = blockIdx.x, S = gridDim.x, t = threadIdx.x;
   const T* xb = x + (long)n * HW * C;
   const long c0 = sp.chunks * s / S, c1 = sp.chunks * (s + 1) / S;
@@ -204,11 +204,8 @@ __global__ void __launch_bounds__(kGnT) gn_stats_kernel(const T* __restrict__ x,
   const int cpg = C / G;
   int r = V;
   while (cpg % r) r /= 2;
-  const int runs = V / r;
-  const int per = cpg / r;                       // runs of one group in one period
-  const int copies = sp.active * V / C;          // periods over the active threads
-  const int L = lanes_per(G), g = t / L, l = t % L;
-  double out[2];
+  const int runs = V / r, span = C / r;            // run e of the active threads is run e % span of the channels
+  const int copies = sp.active * V / C;
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
     double (&v)[V] = q ? s2 : s1;
@@ -221,17 +218,35 @@ __global__ void __launch_bounds__(kGnT) gn_stats_kernel(const T* __restrict__ x,
       for (int k = 0; k < V / 4; ++k) v[k] = v[2 * k] + v[2 * k + 1];
     }
     if (r >= 8) v[0] = v[0] + v[1];
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < V; ++k)
-      if (k < runs && t < sp.active) red[t * runs + k] = v[k];
-    __syncthreads();
-    double acc = 0.0;
-    if (g < G)
-      for (int i = l; i < copies * per; i += L) acc += red[(i / per) * (C / r) + g * per + i % per];
-    out[q] = wave_sum(acc, L);
   }
-  if (g < G && l == 0) part[((long)n * S + s) * G + g] = make_double2(out[0], out[1]);
+#pragma unroll
+  for (int k = 0; k < V; ++k)
+    if (k < runs && t < sp.active) red[t * runs + k] = make_double2(s1[k], s2[k]);
+  __syncthreads();
+  // a run of the channels over lanes of its own, then the runs and lanes of a group
+  const int lanes = kGnT / span, run = t % span, ln = t / span;
+  double u = 0.0, v = 0.0;
+  if (ln < lanes)
+#pragma unroll 4
+    for (int i = ln; i < copies; i += lanes) {
+      const double2 p = red[run + i * span];
+      u += p.x;
+      v += p.y;
+    }
+  __syncthreads();
+  if (ln < lanes) red[run * lanes + ln] = make_double2(u, v);
+  __syncthreads();
+  const int L = lanes_per(G), g = t / L, l = t % L, terms = cpg / r * lanes;
+  u = v = 0.0;
+  if (g < G)
+    for (int i = l; i < terms; i += L) {
+      const double2 p = red[g * terms + i];
+      u += p.x;
+      v += p.y;
+    }
+  u = wave_sum(u, L);
+  v = wave_sum(v, L);
+  if (g < G && l == 0) part[((long)n * S + s) * G + g] = make_double2(u, v);
 }
 
 // mean and rstd of image n's groups from the S partials, in LDS (and to stats)
