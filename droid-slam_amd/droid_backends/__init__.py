@@ -1034,23 +1034,28 @@ def group_norm_act_backward(dy, x, stats, num_groups, weight=None, bias=None, mo
     if with_res:
         _norm_map(fn, "res", res, x)
     wdt = _norm_params(fn, x, num_groups, weight, bias)
-    N, C, H, W = x.shape
-    dt, hw, dev = _NORM_DTYPES[x.dtype], H * W, x.device
-    if (stats.dtype != torch.float64 or stats.shape != (N, num_groups, 2) or stats.device != dev
+    if (stats.dtype != torch.float64 or stats.shape != (x.shape[0], num_groups, 2) or stats.device != x.device
             or not stats.is_contiguous()):
         raise RuntimeError("%s: stats must be group_norm_act's contiguous (N, groups, 2) float64 tensor" % fn)
+    return _group_norm_act_backward(dy, x, stats, num_groups, weight, bias, mode, res if with_res else None, wdt)
+
+
+def _group_norm_act_backward(dy, x, stats, num_groups, weight, bias, mode, res, wdt):
+    """group_norm_act_backward on checked arguments."""
+    N, C, H, W = x.shape
+    dt, hw, dev = _NORM_DTYPES[x.dtype], H * W, x.device
     dx = torch.empty_like(x, memory_format=torch.channels_last)
-    dres = torch.empty_like(x, memory_format=torch.channels_last) if with_res else None
+    dres = torch.empty_like(x, memory_format=torch.channels_last) if res is not None else None
     # an empty map launches nothing: its parameters' gradients are sums of nothing
     new = torch.empty_like if x.numel() else torch.zeros_like
     dw = new(weight) if weight is not None else None
     db = new(bias) if bias is not None else None
     with _on(dev):
         ws = torch.empty((_group_norm_workspace(dt, N, hw, C, num_groups, 1),), dtype=torch.uint8, device=dev)
-        check(lib.droid_group_norm_act_backward(dt, _addr(x), _addr(res if with_res else None), _addr(dy), _addr(weight),
+        check(lib.droid_group_norm_act_backward(dt, _addr(x), _addr(res), _addr(dy), _addr(weight),
                                                 _addr(bias), wdt, _addr(stats), _addr(dx), _addr(dres), _addr(dw),
                                                 _addr(db), N, hw, C, num_groups, mode, _addr(ws), ws.numel(),
-                                                _raw_stream(dev)), fn)
+                                                _raw_stream(dev)), "group_norm_act_backward")
     return dx, dres, dw, db
 
 

@@ -41,6 +41,7 @@ class GroupNormAct(torch.autograd.Function):
         y, stats = droid_backends.group_norm_act(x, num_groups, weight, bias, mode, res, eps=eps, return_stats=True)
         ctx.save_for_backward(x, weight, bias, res, stats)
         ctx.num_groups, ctx.mode, ctx.eps = num_groups, mode, eps
+        ctx.wdt = droid_backends._norm_params("group_norm_act", x, num_groups, weight, bias)
         return y
 
     @staticmethod
@@ -53,9 +54,11 @@ class GroupNormAct(torch.autograd.Function):
             want = [i for i in ins if ctx.needs_input_grad[i]]
             grads = dict(zip(want, torch.autograd.grad(y, [ins[i] for i in want], dy, create_graph=True)))
             return tuple(grads.get(i) for i in range(7))
-        dy = dy.contiguous(memory_format=torch.channels_last)
-        dx, dres, dw, db = droid_backends.group_norm_act_backward(dy, x, stats, ctx.num_groups, weight, bias, ctx.mode,
-                                                                  res)
+        # the forward call checked them; saved-tensor hooks may return another layout
+        cl = torch.channels_last
+        dx, dres, dw, db = droid_backends._group_norm_act_backward(
+            dy.contiguous(memory_format=cl), x.contiguous(memory_format=cl), stats.contiguous(), ctx.num_groups,
+            weight, bias, ctx.mode, None if res is None else res.contiguous(memory_format=cl), ctx.wdt)
         return dx, None, dw, db, None, dres, None
 
 

@@ -151,3 +151,23 @@ def test_second_derivatives(mode):
         first, = torch.autograd.grad(y, [x], g.to(DEV), retain_graph=True)
         again, = torch.autograd.grad(y, [x], g.to(DEV), create_graph=True)
         assert _rel(again, first) < 1e-5
+
+
+def test_saved_tensors_kept_on_the_host():
+    """save_on_cpu hands back maps that are not channels_last."""
+    from droid_backends import NORM_ADD_RELU
+    from droid_mi355x import group_norm_act
+    torch.manual_seed(0)
+    x, r = (torch.randn(2, 24, 9, 7, device=DEV).contiguous(memory_format=torch.channels_last) for _ in range(2))
+    w, b, g = torch.rand(24, device=DEV), torch.randn(24, device=DEV), torch.randn(2, 24, 9, 7, device=DEV)
+
+    def grads():
+        leaves = [t.clone().requires_grad_() for t in (x, w, b, r)]
+        y = group_norm_act(leaves[0], 4, leaves[1], leaves[2], NORM_ADD_RELU, leaves[3])
+        return y, leaves
+
+    y, leaves = grads()
+    want = torch.autograd.grad(y, leaves, g)
+    with torch.autograd.graph.save_on_cpu():
+        y, leaves = grads()
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y, leaves, g), want))
