@@ -822,6 +822,16 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
   if (t0 + 1 < t1) stage(t0 + 1, 1);
   loads_done();
   __syncthreads();
+  // Both directions: the exponents v become B in place, a step before their tile's, by
+  // one wave for all (each lane for itself: 32 exponentials a step).
+  auto make_b = [&](int t) {
+    float& v = sh.expn[(t - t0) & 3][lane];
+    v = __builtin_amdgcn_exp2f(v + (mid + fex));
+  };
+  if constexpr (SRC && DST) {
+    if (wave == 3) make_b(t0);
+    __syncthreads();
+  }
   int buf = 0;   // of tile t
   // Half 1's second product of a tile is done in the next step, while that one's
   // operands are on their way (nothing yet: zeros), where there are registers to
@@ -882,7 +892,7 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
           const float vq[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
           for (int u = 0; u < 4; ++u)
-            ve[4 * q + u] = SRC ? __builtin_amdgcn_exp2f(vq[u] + (mid + fex)) : kScaled ? vq[u] + fex : vq[u];
+            ve[4 * q + u] = !SRC && kScaled ? vq[u] + fex : vq[u];
         }
     };
     // The weights of half k with N matrix instructions between them, in exactly this
@@ -971,6 +981,9 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
     if (t + 2 < t1) {
       stage(t + 2, ahead);
       if (t + 3 < t1) stage_rows(t + 3);
+    }
+    if constexpr (SRC && DST) {
+      if (wave == 3 && t + 1 < t1) make_b(t + 1);
     }
     exponents(0);
 #pragma unroll
