@@ -506,9 +506,14 @@ __global__ void __launch_bounds__(kET) corr_edge_kernel(BwdArgs a) {
   const int total = a.P * a.K;
   for (int q = tid; q < a.groups; q += kLT) bucket[q] = 0;
   __syncthreads();
-  for (int q = tid; q < total; q += kLT) {
-    const unsigned v = a.idx[ent + q];
-    if (v < (unsigned)a.Q) atomicAdd(&bucket[v / 64], 1);
+  constexpr int kBatch = 8;   // terms a thread reads at once
+  for (int q0 = tid; q0 < total; q0 += kLT * kBatch) {
+    unsigned v[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) v[u] = q0 + u * kLT < total ? a.idx[ent + q0 + u * kLT] : -1;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+      if (v[u] < (unsigned)a.Q) atomicAdd(&bucket[v[u] / 64], 1);
   }
   __syncthreads();
   int carry = 0;
@@ -535,13 +540,27 @@ __global__ void __launch_bounds__(kET) corr_edge_kernel(BwdArgs a) {
   }
   if (tid == 0) a.first_rec[(long)e * (a.groups + 1) + a.groups] = carry;
   __syncthreads();
-  for (int q = tid; q < total; q += kLT) {
-    const unsigned v = a.idx[ent + q];
-    if (v >= (unsigned)a.Q) continue;
-    const int p = q / a.K, at = atomicAdd(&bucket[v / 64], 1);
-    const float pi = a.prob ? a.prob[ent + q] : 1.f;
-    const bool out = fabsf(a.lse[(long)e * a.P + p]) == INFINITY;
-    a.rec[ent + at] = make_uint2((unsigned)p << 6 | (v & 63), __float_as_uint(out || pi == 0.f ? 0.f : a.g[(long)e * a.P + p] * pi));
+  for (int q0 = tid; q0 < total; q0 += kLT * kBatch) {
+    unsigned v[kBatch];
+    int p[kBatch];
+    float pi[kBatch], l[kBatch], g[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int q = q0 + u * kLT;
+      const bool in = q < total;
+      p[u] = in ? q / a.K : 0;
+      v[u] = in ? a.idx[ent + q] : -1;
+      pi[u] = in && a.prob ? a.prob[ent + q] : 1.f;
+      l[u] = a.lse[(long)e * a.P + p[u]];
+      g[u] = a.g[(long)e * a.P + p[u]];
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+      if (v[u] < (unsigned)a.Q) {
+        const int at = atomicAdd(&bucket[v[u] / 64], 1);
+        const bool out = fabsf(l[u]) == INFINITY || pi[u] == 0.f;
+        a.rec[ent + at] = make_uint2((unsigned)p[u] << 6 | (v[u] & 63), __float_as_uint(out ? 0.f : g[u] * pi[u]));
+      }
   }
   if (!a.shared) return;
   const int i = a.e1[e], j = a.e2[e];
@@ -696,6 +715,7 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
   const float mul = ldexpf(1.f, ex), fex = (float)ex;
   float lx[XH], gx[XH], ax[XH];
   bool live = false;   // a stationary row has a target
+  constexpr int kBatch = 8;   // sparse terms a lane reads at once
   // Both directions: with m the middle of the row sums, g1 p1 + g2 p2 = u (2^b g1 + A B)
   // where u = 2^(c s - lse_x - b), A = 2^(lse_x - m + b), B = 2^(v_y + m): one exponential
   // a pair of rows. b = kRange / 2, and lse_x := m in a left-out row x: then u <= 1
@@ -734,14 +754,23 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
     if constexpr (SRC) {
       const long first = (long)es * a.P + x0 + wave * XW;
       const int n = min(XW, R - x0 - wave * XW) * K;
-#pragma unroll 4
-      for (int q = v; q < n; q += 64) {
-        const int y = a.idx[first * K + q];
-        if (y >= ya && y < yb) {
-          const int r = q / K;
-          const float pi = a.prob ? a.prob[first * K + q] : 1.f;
-          if (pi != 0.f) f(y, r, sh.xg[wave * XW + r] * pi);
+      const float inv = 1.f / (float)K;   // q / K by a product: q < 2^12, its distance from a whole number 2^-7
+#pragma unroll 1
+      for (int q0 = v; q0 < n; q0 += 64 * kBatch) {
+        int y[kBatch];
+        float pi[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const int q = q0 + 64 * u;
+          y[u] = q < n ? a.idx[first * K + q] : -1;
+          pi[u] = q < n && a.prob ? a.prob[first * K + q] : 1.f;
         }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+          if (y[u] >= ya && y[u] < yb && pi[u] != 0.f) {
+            const int r = (int)(((float)(q0 + 64 * u) + 0.5f) * inv);
+            f(y[u], r, sh.xg[wave * XW + r] * pi[u]);
+          }
       }
     }
     if constexpr (DST) {
@@ -751,11 +780,16 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
         const int* p = a.first_rec + (long)ed * (a.groups + 1) + group;
         const int lo = p[0], hi = p[1];
         const uint2* rec = a.rec + (long)ed * a.P * K;
-#pragma unroll 4
-        for (int q = lo + v; q < hi; q += 64) {
-          const uint2 r = rec[q];
-          const int y = r.x >> 6, k = (int)(r.x & 63) - (x & 63);
-          if (y >= ya && y < yb && (XW == 64 || (k >= 0 && k < XW))) f(y, k, __uint_as_float(r.y) * mul);
+#pragma unroll 1
+        for (int q0 = lo + v; q0 < hi; q0 += 64 * kBatch) {
+          uint2 r[kBatch];
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u) r[u] = q0 + 64 * u < hi ? rec[q0 + 64 * u] : make_uint2(0xffffffffu, 0u);
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u) {
+            const int y = r[u].x >> 6, k = (int)(r[u].x & 63) - (x & 63);
+            if (y >= ya && y < yb && (XW == 64 || (k >= 0 && k < XW))) f(y, k, __uint_as_float(r[u].y) * mul);
+          }
         }
       }
     }
