@@ -17,7 +17,15 @@
 // the accumulator's layout is already the B operand's of the second product
 // (its k slots (h, j) carry row 8 (j / 4) + 4 h + j % 4 of 16; the other
 // operand comes by transposed LDS reads in the same order), so the weights ds
-// never pass through LDS.
+// never pass through LDS.  The weights are rounded to the features' type for that
+// product, after the sparse terms are subtracted in fp32, and fp16 ones are scaled
+// by a power of two per frame: half a step of each, as the features' own rounding.
+//
+// What bounds it: the matrix instructions, at the 1.11 (fp16) to 1.16 (bf16) PFLOP/s
+// that a large library product reaches on this card, with the exponentials' vector
+// work beside them.  Four clips (96 edges of 2560 x 2560 rows, D = 128, bf16): row
+// sums 171 us (161 GFLOP, 0.94 PFLOP/s), losses 36 us, gradient 438 us (349 GFLOP,
+// 0.80 PFLOP/s) and 33 us beside it; one clip in fp16 53 + 12 + 142 + 28 us.
 #include "lds_dma.hpp"
 
 #include <algorithm>
@@ -172,7 +180,8 @@ struct FwdArgs {
 
 // 32-row blocks of queries a wave: two where the registers allow three such
 // workgroups a CU, since every operand read from shared memory then feeds two matrix
-// instructions (with one, 128 B a clock of shared memory is what bounds the loop).
+// instructions (with one, 128 B a clock of shared memory are as busy as they: four
+// clips 178 us, with two 171; accumulators in AGPRs, copied out, 183).
 template <int DP>
 constexpr int kXF = DP <= 128 ? 2 : 1;
 inline int fwd_rows(int D) { return D <= 128 ? 2 * kRowsB : kRowsB; }
@@ -274,11 +283,14 @@ struct RowArgs {
 
 // One query row on 16 lanes: joins the shares of its sum, takes the K target
 // logits as fp32 dot products (a row of D values is 16 lanes x 16 B) and forms
-// the loss.  Rows without a target (all negative, or logits of -inf): loss 0 and lse = +inf, or -inf
-// where the row's features are not all finite (the backward pass must not touch
-// those).  A target >= Q, an edge outside the
-// frames: NaN.
-template <typename T>
+// the loss.  Rows without a target (all negative, or logits of -inf): loss 0 and
+// lse = +inf, or -inf where the row's features are not all finite (the backward
+// pass must not touch those).  A target >= Q, an edge outside the frames: NaN.
+// SLOTS: targets a lane holds (K <= 16 SLOTS); kBatch: target rows read at once.
+// Bound by the rows it gathers, 256 B each, mostly from L2: 246 thousand queries
+// with one target 36 us (as <4, 4>: 57), with 16 100 us (10 TB/s; as <4, 4> 131,
+// one row at a time 155).
+template <typename T, int SLOTS, int kBatch>
 __global__ void __launch_bounds__(kLT) corr_loss_row_kernel(RowArgs a) {
   const long row = (long)blockIdx.x * (kLT / 16) + threadIdx.x / 16;
   const int l = threadIdx.x & 15;
@@ -299,15 +311,17 @@ __global__ void __launch_bounds__(kLT) corr_loss_row_kernel(RowArgs a) {
     return v;
   };
   // the targets' weights: lane l has entries l, l + 16, ...
-  float pi[kMaxK / 16];
+  float pi[SLOTS];
+  int own[SLOTS];
   float top = -INFINITY;
   bool used = false, bad = !edge;
 #pragma unroll
-  for (int n = 0; n < kMaxK / 16; ++n) {
+  for (int n = 0; n < SLOTS; ++n) {
     pi[n] = -INFINITY;
+    own[n] = -1;
     const int k = l + 16 * n;
     if (k < a.K) {
-      const int t = idx[k];
+      const int t = own[n] = idx[k];
       if (t >= 0) pi[n] = a.logits ? a.logits[row * a.K + k] * a.invT : 0.f;
       used |= pi[n] != -INFINITY;          // a logit of -inf: no target either
       bad |= t >= a.Q || pi[n] != pi[n];
@@ -337,7 +351,7 @@ __global__ void __launch_bounds__(kLT) corr_loss_row_kernel(RowArgs a) {
   top = max16(top);
   float tot = 0.f;
 #pragma unroll
-  for (int n = 0; n < kMaxK / 16; ++n) {
+  for (int n = 0; n < SLOTS; ++n) {
     pi[n] = __expf(pi[n] - top);
     if (l + 16 * n >= a.K) pi[n] = 0.f;
     tot += pi[n];
@@ -345,10 +359,9 @@ __global__ void __launch_bounds__(kLT) corr_loss_row_kernel(RowArgs a) {
   tot = sum16(tot);
   float ent = 0.f;
 #pragma unroll
-  for (int n = 0; n < kMaxK / 16; ++n) {
+  for (int n = 0; n < SLOTS; ++n) {
     pi[n] /= tot;
     if (pi[n] > 0.f) ent += pi[n] * logf(pi[n]);
-    if (a.prob && l + 16 * n < a.K) a.prob[row * a.K + l + 16 * n] = pi[n];
   }
   // the row's sum over all keys
   float m = kNegBig;
@@ -363,22 +376,56 @@ __global__ void __launch_bounds__(kLT) corr_loss_row_kernel(RowArgs a) {
   const float lse2 = sum > 0.f ? m + log2f(sum) : NAN;
   // sum_k pi_k s_k, as one dot product with the pi-weighted sum of the target rows
   const T* f2 = static_cast<const T*>(a.f2) + (long)j * a.Q * a.D;
-  float dot = 0.f;
-  for (int k = 0; k < a.K; ++k) {
-    const int t = idx[k];
-    float w = 0.f;
+  // The weights kept for the gradient: a key that a row names more than once has all
+  // of its weight at the first place, so that no place of ds has more than one term
+  // of an edge (and their sum no order).
+  float dot = 0.f, kept[SLOTS] = {};
+  bool again[SLOTS] = {};
+  typedef typename Op<T>::vec8 vec8;
+  vec8 x[2] = {};             // the row's values 8 l .. + 7, and 128 further
 #pragma unroll
-    for (int n = 0; n < kMaxK / 16; ++n)
-      if (k / 16 == n) w = __shfl(pi[n], k & 15, 16);
-    if (t < 0 || w == 0.f) continue;
-    float v = 0.f;
-    for (int d = 8 * l; d < a.D; d += 128) {
-      const auto x = *reinterpret_cast<const typename Op<T>::vec8*>(f1 + d);
-      const auto y = *reinterpret_cast<const typename Op<T>::vec8*>(f2 + (long)t * a.D + d);
+  for (int h = 0; h < 2; ++h)
+    if (8 * l + 128 * h < a.D) x[h] = *reinterpret_cast<const vec8*>(f1 + 8 * l + 128 * h);
+  for (int k0 = 0; k0 < a.K; k0 += kBatch) {
+    int t[kBatch];
+    float w[kBatch];
+    vec8 y[kBatch][2];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) v = fmaf((float)x[q], (float)y[q], v);
+    for (int u = 0; u < kBatch; ++u) {
+      t[u] = -1, w[u] = 0.f;
+#pragma unroll
+      for (int n = 0; n < SLOTS; ++n)   // (a lane past K holds -1 and 0)
+        if (k0 / 16 == n) t[u] = __shfl(own[n], (k0 + u) & 15, 16), w[u] = __shfl(pi[n], (k0 + u) & 15, 16);
+      if (w[u] == 0.f) t[u] = -1;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (t[u] >= 0 && 8 * l + 128 * h < a.D)
+          y[u][h] = *reinterpret_cast<const vec8*>(f2 + (long)t[u] * a.D + 8 * l + 128 * h);
     }
-    dot = fmaf(w, v, dot);
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      if (t[u] < 0) continue;
+      if (a.prob) {
+#pragma unroll
+        for (int n = 0; n < SLOTS; ++n)
+          if (16 * n < a.K) {
+            again[n] |= own[n] == t[u] && k0 + u < l + 16 * n;
+            kept[n] += own[n] == t[u] ? w[u] : 0.f;
+          }
+      }
+      float v = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (8 * l + 128 * h < a.D)
+#pragma unroll
+          for (int q = 0; q < 8; ++q) v = fmaf((float)x[h][q], (float)y[u][h][q], v);
+      dot = fmaf(w[u], v, dot);
+    }
+  }
+  if (a.prob) {
+#pragma unroll
+    for (int n = 0; n < SLOTS; ++n)
+      if (l + 16 * n < a.K) a.prob[row * a.K + l + 16 * n] = again[n] ? 0.f : kept[n];
   }
   dot = sum16(dot);
   ent = sum16(ent);
@@ -405,6 +452,16 @@ __global__ void __launch_bounds__(kLT) corr_loss_row_kernel(RowArgs a) {
 // workgroup each left half the chip idle in the last round: 560 items on 512
 // places took 1137 us, shares of the streamed axis by a cost model 867 us, with
 // uneven graphs up to twice their even share.)
+//
+// One workgroup a CU, one wave a SIMD with all 512 registers, so the order of a
+// step's instructions is written out: matrix instructions between the exponentials,
+// shared memory read between matrix instructions, the last second product of a tile
+// in the next step.  A step of a pair takes 5050 clocks for 2048 of matrix
+// instructions; the rest is the exponentials (32 a lane and half, 8 clocks each),
+// the conversion to 16 bits, accumulators copied out of AGPRs, two waits at the barrier
+// (480) and the tile's loads.  On the way, four clips: 32 rows a wave 531 us, 64
+// rows 522, the sparse terms sorted beforehand 479, one exponential for both
+// directions and this order 455, the streamed factor made once a workgroup 438.
 
 constexpr int kUnitBoth = 5, kUnitSrc = 4, kUnitDst = 4;   // relative cost of a step (measured 5670 : 4460 : 4380 clk)
 // Rows x of a wave, in 32s.  Two where their accumulators fit the registers of one
@@ -453,6 +510,8 @@ __device__ __forceinline__ int g_exponent(float gmax) {
   return max(-100, min(100, 14 - ex));
 }
 
+// (96 edges of 2560 rows: 13 us with one target a row, 35 with 16 - one term read at
+// a time 59 -, sorted anew by every workgroup of the gradient kernel 500 in all.)
 // One workgroup an edge: what the gradient kernel wants of its rows, its sparse
 // terms by 64 keys (a counting sort), and the reverse edge it may be paired with
 // (the k-th copy of (i, j) with the k-th of (j, i)).
@@ -498,8 +557,9 @@ __global__ void __launch_bounds__(kET) corr_edge_kernel(BwdArgs a) {
     a.range[e] = make_float2(lmin, lmax);
     a.partner[e] = -1;
   }
-  // The records.  Their order within a bucket is that of the atomics; terms of one
-  // place (y, x) are added in LDS in any order anyway.  More keys than buckets: a
+  // The records.  Their order within a bucket is that of the atomics: a place (y, x)
+  // has at most one of an edge (corr_loss_row_kernel), one more of its reverse, and
+  // their sum has no order.  More keys than buckets: a
   // bucket holds several groups, told apart by the reader (rec holds the key's low
   // bits only), so such sizes are refused on the host.
   const long ent = (long)e * a.P * a.K;
@@ -1284,8 +1344,17 @@ int droid_corr_loss_forward(int dtype, const void* fmap1, const void* fmap2, con
   RowArgs r{fmap1, fmap2, f1, f2, idx, logits, a.part, loss, lse, logits ? prob : nullptr, N1, P, N2, Q, D, K, a.S,
             (long)E * P, scale, 1.f / temperature, temperature * temperature};
   const int grid = (int)((r.rows + kLT / 16 - 1) / (kLT / 16));
-  if (dtype == 0) corr_loss_row_kernel<_Float16><<<grid, kLT, 0, stream>>>(r);
-  else corr_loss_row_kernel<__bf16><<<grid, kLT, 0, stream>>>(r);
+#define ROW(SLOTS, BATCH)                                                                       \
+  if (dtype == 0) corr_loss_row_kernel<_Float16, SLOTS, BATCH><<<grid, kLT, 0, stream>>>(r);    \
+  else corr_loss_row_kernel<__bf16, SLOTS, BATCH><<<grid, kLT, 0, stream>>>(r)
+  if (K == 1) {
+    ROW(1, 1);
+  } else if (K <= 16) {
+    ROW(1, 4);
+  } else {
+    ROW(4, 4);
+  }
+#undef ROW
   DROID_LAUNCH_CHECK();
   return kOk;
 }

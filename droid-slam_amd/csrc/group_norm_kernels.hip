@@ -14,6 +14,10 @@
 // Every pass is a stream over maps, bound by HBM (or, for one frame, by the two
 // launches): forward reads x twice and writes y; backward's first pass reads x,
 // dy (and res) and writes dres, its second reads x and dy (dres) and writes dx.
+// 28 maps of 32 x 160 x 256 in bf16, relu(res + relu(n)): 15.5 + 37 us forward,
+// 48 + 40 us backward, 5.7 TB/s over what the passes move (a large copy: 5.1; the
+// second passes find part of it in the last-level cache); what the operator cannot
+// do without is 114 us of that copy.  One frame of 128 x 40 x 64: 5.4 + 5.8 us.
 //
 // Layout of the work.  An image is a flat run of HW C values, cut into pieces
 // of V = 16 B.  Piece f starts at channel (V f) mod C, so with A threads, A a
@@ -123,7 +127,8 @@ inline Split gn_split(int N, int HW, int C, int V) {
   const int period = C / gcd_i(C, V);
   s.active = kGnT / period * period;
   s.chunks = std::max<long>(1, (s.pieces + s.active - 1) / s.active);
-  // two workgroups a CU over all images, as many as run at once; at least one chunk each
+  // two workgroups a CU over all images, as many as run at once (four: a stereo frame
+  // at half resolution 10.2 + 13.7 us instead of 7.4 + 8.9); at least one chunk each
   s.blocks = (int)std::max<long>(1, std::min<long>(s.chunks, std::max(1, 512 / N)));
   return s;
 }
@@ -286,7 +291,8 @@ __device__ __forceinline__ float gn_act(float n, float r) {
 }
 
 // Channel constants: thread c < C makes channel c's (its integer divisions once, its
-// parameters read early), the threads take their V from LDS.
+// parameters read early), the threads take their V from LDS (each thread for its own
+// channels: one frame's second pass 8.2 us instead of 5.8).
 struct ChanIn {
   float w, b;
   int g;

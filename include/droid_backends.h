@@ -147,8 +147,9 @@ int droid_corr_alt_ce0_ordered(const void* const* pyr, const int* Hl, const int*
  *   loss[e][p] = T^2 KL(pi || softmax_q(s_pq))          (f32).
  * A row without a target: loss 0, no gradient, its query features unread by the
  * sums.  A target >= Q, an edge outside the frames: loss NaN.
- * Outputs for the backward pass: lse (E,P) f32 (log2 units; +inf: no target), prob
- * (E,P,K) f32 (with logits only).
+ * Outputs for the backward pass: lse (E,P) f32 (log2 units; no target: +inf, or -inf
+ * where the row's features are not finite), prob (E,P,K) f32 (with logits only; a key
+ * that a row names twice has its whole weight at the first place).
  * ws: droid_corr_loss_workspace bytes (backward: N1 / N2 = 0 for a gradient that is not
  * wanted, N2 = 0 with shared), used until the kernels end. */
 size_t droid_corr_loss_workspace(int E, int N1, int P, int N2, int Q, int D, int K, int backward);

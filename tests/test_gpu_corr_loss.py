@@ -380,3 +380,23 @@ def test_many_targets_on_few_keys(dtype, positive):
     p = (a, a, f1, f2, idx, logits, g)
     loss, grads = _run(*p, True, 1 / 16, 1.0)
     _check(dt, *p, True, 1 / 16, 1.0, loss, grads, PAIR)
+
+
+def test_a_key_named_often_is_added_in_one_order():
+    """Every row names three keys twenty times each with weights far apart:
+    equal bits in every run."""
+    import droid_backends as nb
+    a, _, f1, f2, idx, logits, g = _problem(28, torch.float16, 60, 4, 2, 130, 2, 130, 64, shared=True)
+    f1[:], f2[:] = [0, 1, 0, 1], [1, 0, 0, 1]
+    idx[:] = (np.arange(60) % 3) * 40 + np.arange(130)[:, None] % 7
+    k = (a, None, _t(f1), _t(f2), _t(idx))
+    first = None
+    for _ in range(4):
+        loss, lse, prob = nb.corr_loss_forward(*k, _t(logits))
+        d, _ = nb.corr_loss_backward(_t(np.abs(g)), *k, lse, prob)
+        if first is None:
+            first = (loss, prob, d)
+        assert all(torch.equal(p, q) for p, q in zip(first, (loss, prob, d)))
+    assert (prob[..., :3] > 0).any() and not prob[..., 3:].any()
+    p = (a, a, f1, f2, idx, logits, np.abs(g))
+    _check(torch.float16, *p, True, 1 / 16, 1.0, loss, [d], PAIR)
