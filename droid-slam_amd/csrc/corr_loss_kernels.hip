@@ -816,21 +816,23 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
       const int n = min(XW, R - x0 - wave * XW) * K;
       const float inv = 1.f / (float)K;   // q / K by a product: q < 2^12, its distance from a whole number 2^-7
 #pragma unroll 1
-      for (int q0 = v; q0 < n; q0 += 64 * kBatch) {
+      for (int q0 = 0; q0 < n; q0 += 64 * kBatch) {
         int y[kBatch];
         float pi[kBatch];
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
-          const int q = q0 + 64 * u;
+          const int q = q0 + 64 * u + v;
           y[u] = q < n ? a.idx[first * K + q] : -1;
           pi[u] = q < n && a.prob ? a.prob[first * K + q] : 1.f;
         }
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u)
+        for (int u = 0; u < kBatch; ++u) {
+          if (q0 + 64 * u >= n) break;
           if (y[u] >= ya && y[u] < yb && pi[u] != 0.f) {
-            const int r = (int)(((float)(q0 + 64 * u) + 0.5f) * inv);
+            const int r = (int)(((float)(q0 + 64 * u + v) + 0.5f) * inv);
             f(y[u], r, sh.xg[wave * XW + r] * pi[u]);
           }
+        }
       }
     }
     if constexpr (DST) {
@@ -838,15 +840,17 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
       const int x = x0 + wave * XW, group = x / 64;
       if (x < R) {
         const int* p = a.first_rec + (long)ed * (a.groups + 1) + group;
-        const int lo = p[0], hi = p[1];
+        const int lo = __builtin_amdgcn_readfirstlane(p[0]), hi = __builtin_amdgcn_readfirstlane(p[1]);
         const uint2* rec = a.rec + (long)ed * a.P * K;
 #pragma unroll 1
-        for (int q0 = lo + v; q0 < hi; q0 += 64 * kBatch) {
+        for (int q0 = lo; q0 < hi; q0 += 64 * kBatch) {
           uint2 r[kBatch];
 #pragma unroll
-          for (int u = 0; u < kBatch; ++u) r[u] = q0 + 64 * u < hi ? rec[q0 + 64 * u] : make_uint2(0xffffffffu, 0u);
+          for (int u = 0; u < kBatch; ++u)
+            r[u] = q0 + 64 * u + v < hi ? rec[q0 + 64 * u + v] : make_uint2(0xffffffffu, 0u);
 #pragma unroll
           for (int u = 0; u < kBatch; ++u) {
+            if (q0 + 64 * u >= hi) break;
             const int y = r[u].x >> 6, k = (int)(r[u].x & 63) - (x & 63);
             if (y >= ya && y < yb && (XW == 64 || (k >= 0 && k < XW))) f(y, k, __uint_as_float(r[u].y) * mul);
           }
