@@ -1261,7 +1261,8 @@ int fwd_split(int E, int P, int Q, int D) {
   const long blocks = (long)E * ceil_div(P, fwd_rows(D)), tiles = ceil_div(Q, kRowsY);
   const long at_once = (long)fwd_groups(D) * device_cu_count();
   long best = 1, least = -1;
-  for (long s = 1; s <= std::min<long>(tiles, std::max<long>(8, at_once / std::max<long>(1, blocks))); ++s) {
+  const long most = std::min<long>(tiles, std::max<long>(8, at_once / std::max<long>(1, blocks)));
+  for (long s = 1; s <= most; s += 1 + s / 64) {
     const long steps = (blocks * s + at_once - 1) / at_once * ((tiles + s - 1) / s + 2);
     if (least < 0 || steps < least) best = s, least = steps;
   }

@@ -339,6 +339,8 @@ def _corr_loss_check(fn, fmap1, fmap2, f1, f2, idx, K):
     P, Q = fmap1.shape[1:-1].numel(), keys.shape[1:-1].numel()
     if f1.dim() != 1 or f2.shape != f1.shape:
         raise RuntimeError("%s: f1 and f2 must have one entry per edge" % fn)
+    if max(N1, P, N2, Q, E) > 0x7fffffff:   # the C ABI's int
+        raise RuntimeError("%s: %d frames of %d rows, %d of %d, %d edges: too large" % (fn, N1, P, N2, Q, E))
     rows = (E,) + tuple(fmap1.shape[1:-1])
     if tuple(idx.shape) != rows + (() if K is None else (K,)):
         raise RuntimeError("%s: indices %s do not match the edges' query rows %s" % (fn, tuple(idx.shape), rows))
@@ -977,6 +979,8 @@ def _norm_params(fn, x, num_groups, weight, bias):
     if C == 0 or C > 512 or num_groups <= 0 or C % num_groups:
         raise RuntimeError("%s: %d channels in %d groups (0 < C <= 512, C a multiple of the groups)"
                            % (fn, C, num_groups))
+    if max(N, H * W) > 0x7fffffff:   # the C ABI's int
+        raise RuntimeError("%s: a map of %d x %d x %d is too large" % (fn, N, H, W))
     wdt = None
     for name, t in (("weight", weight), ("bias", bias)):
         if t is None:

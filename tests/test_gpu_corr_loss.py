@@ -400,3 +400,28 @@ def test_a_key_named_often_is_added_in_one_order():
     assert (prob[..., :3] > 0).any() and not prob[..., 3:].any()
     p = (a, a, f1, f2, idx, logits, np.abs(g))
     _check(torch.float16, *p, True, 1 / 16, 1.0, loss, [d], PAIR)
+
+
+def test_offsets_past_32_bits():
+    """2.6e9 feature values: the last two frames' edges as with these frames alone."""
+    from droid_mi355x import corr_cross_entropy
+    P, D, N = 65536, 128, 310
+    g = torch.Generator(device=DEV).manual_seed(0)
+    two = torch.randn((2, P, D), generator=g, device=DEV).bfloat16()
+    t = torch.randint(0, P, (2, P), generator=g, device=DEV, dtype=torch.int32)
+    t[:, ::3] = -1
+    up = torch.rand((2, P), generator=g, device=DEV)
+    many = torch.zeros((N, P, D), dtype=torch.bfloat16, device=DEV)
+    many[-2:] = two
+    out = []
+    for x in (two, many):
+        x = x.requires_grad_()
+        k = x.shape[0] - 2
+        f1, f2 = _t(np.array([k, k + 1], np.int32)), _t(np.array([k + 1, k], np.int32))
+        loss = corr_cross_entropy(x, None, f1, f2, t)
+        out.append((loss.detach(), torch.autograd.grad(loss, [x], up)[0]))
+    assert torch.equal(out[0][0], out[1][0])
+    d, e = out[0][1].float(), out[1][1][-2:].float()
+    # the same sums in shares that may be cut elsewhere: a rounding to bf16 each
+    assert ((d - e).abs() <= 2.0 ** -7 * d.abs() + 1e-6 * d.abs().max()).all()
+    assert not out[1][1][:-2].any()

@@ -208,3 +208,30 @@ def test_refusals_on_the_device():
         assert y.shape == e.shape
         dx, _, dw, db = nb.group_norm_act_backward(y, e, st, 2, w, b)
         assert dx.shape == e.shape and not dw.any() and not db.any()
+
+
+def test_offsets_past_32_bits_and_maps_past_the_abi():
+    """2.4e9 values: the last image as alone (another split of its sums: one
+    rounding of the output apart); more than 2^31 - 1 pixels are refused."""
+    import droid_backends as nb
+    one = torch.randn(1, 256, 1024, 1024, device=DEV).half().contiguous(memory_format=torch.channels_last)
+    dy1 = torch.randn(1, 256, 1024, 1024, device=DEV).half().contiguous(memory_format=torch.channels_last)
+    w, b = torch.rand(256, device=DEV) + 0.5, torch.randn(256, device=DEV)
+
+    def both(x, dy):
+        y, st = nb.group_norm_act(x, 8, w, b, nb.NORM_SILU, return_stats=True)
+        return y[-1], nb.group_norm_act_backward(dy, x, st, 8, w, b, nb.NORM_SILU)[0][-1]
+
+    def many(t):
+        m = torch.empty((9, 256, 1024, 1024), dtype=t.dtype, device=DEV, memory_format=torch.channels_last)
+        m[:8] = 0
+        m[8:] = t
+        return m
+
+    for got, want in zip(both(many(one), many(dy1)), both(one, dy1)):
+        for c in range(0, 256, 64):   # (in parts: bounds the memory of the comparison)
+            g, e = got[c:c + 64].float(), want[c:c + 64].float()
+            assert ((g - e).abs() <= 2.0 ** -10 * e.abs() + 2.0 ** -20).all()
+    big = torch.empty((1, 1, 65536, 32768), dtype=torch.float16, device=DEV)
+    with pytest.raises(RuntimeError, match="too large"):
+        nb.group_norm_act(big.contiguous(memory_format=torch.channels_last), 1)
