@@ -17,7 +17,7 @@
 // 28 maps of 32 x 160 x 256 in bf16, relu(res + relu(n)): 15.5 + 37 us forward,
 // 48 + 40 us backward, 5.7 TB/s over what the passes move (a large copy: 5.1; the
 // second passes find part of it in the last-level cache); what the operator cannot
-// do without is 114 us of that copy.  One frame of 128 x 40 x 64: 5.4 + 5.8 us.
+// do without is 114 us of that copy.
 //
 // Layout of the work.  An image is a flat run of HW C values, cut into pieces
 // of V = 16 B.  Piece f starts at channel (V f) mod C, so with A threads, A a
@@ -376,6 +376,90 @@ __global__ void __launch_bounds__(kGnT) gn_apply_kernel(const T* x, const T* res
   }
 }
 
+// The forward in one launch for small maps: one workgroup an image's group, whose
+// pieces (cpg a multiple of V) stay in registers between the sums and the output.
+// Bound by one trip to memory and the join of the sums.  Maps of 128 x 40 x 64 in
+// fp16, 16 groups, us for 1, 4, 8, 12 of them: 7.1, 9.9, 13.4, 17.3; as two launches
+// 10.3, 13.3, 14.2, 14.3.
+constexpr int kSmallT = 1024, kSmallU = 4;
+constexpr long kSmallBytes = 4 << 20;
+template <typename T, int MODE>
+__global__ void __launch_bounds__(kSmallT) gn_small_kernel(const T* x, const T* res, T* out,
+                                                           const void* __restrict__ w, const void* __restrict__ b,
+                                                           int wdt, int HW, int C, int G, float eps,
+                                                           double2* __restrict__ stats_out) {
+  constexpr int V = Elem<T>::V, U = kSmallU;
+  constexpr bool RES = MODE == kResRelu || MODE == kAddRelu;
+  __shared__ double2 red[kSmallT / 64];
+  __shared__ __attribute__((aligned(16))) float rw[kGnMaxC], bc[kGnMaxC];
+  const int n = blockIdx.y, g = blockIdx.x, t = threadIdx.x, cpg = C / G, per = cpg / V, total = HW * per;
+  const long base = (long)n * HW * C + (long)g * cpg;
+  Piece<T> p[U], rp[U];
+  int at[U], part[U];   // a piece's place in the image, its first channel in the group
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int q = t + u * kSmallT;
+    if (q < total) {
+      const int pixel = q / per;
+      part[u] = (q - pixel * per) * V;
+      at[u] = pixel * C + part[u];
+      p[u] = load_piece(x + base + at[u]);
+      if constexpr (RES) rp[u] = load_piece(res + base + at[u]);
+    }
+  }
+  const float wc = t < cpg ? param(w, wdt, g * cpg + t, 1.f) : 0.f;
+  if (t < cpg) bc[t] = param(b, wdt, g * cpg + t, 0.f);
+  double s1 = 0.0, s2 = 0.0;
+  if (t < total) {   // about the thread's first value, as gn_stats_kernel
+    const float k0 = (float)p[0].v[0];
+    float a = 0.f, q2 = 0.f;
+    int cnt = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (t + u * kSmallT < total) {
+        cnt += V;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          const float d = (float)p[u].v[k] - k0;
+          a += d;
+          q2 = fmaf(d, d, q2);
+        }
+      }
+    const double q = k0, da = a;
+    s1 = cnt * q + da;
+    s2 = (double)q2 + q * (2.0 * da + cnt * q);
+  }
+  s1 = wave_sum(s1, 64);
+  s2 = wave_sum(s2, 64);
+  if ((t & 63) == 0) red[t / 64] = make_double2(s1, s2);
+  __syncthreads();
+  s1 = s2 = 0.0;
+#pragma unroll
+  for (int i = 0; i < kSmallT / 64; ++i) {
+    s1 += red[i].x;
+    s2 += red[i].y;
+  }
+  const double M = (double)HW * cpg, mean = s1 / M;
+  double var = s2 / M - mean * mean;
+  if (var < 0.0) var = 0.0;   // (a NaN stays one)
+  const double rstd = 1.0 / sqrt(var + (double)eps);
+  if (t == 0 && stats_out) stats_out[(long)n * G + g] = make_double2(mean, rstd);
+  if (t < cpg) rw[t] = (float)(rstd * (double)wc);
+  __syncthreads();
+  const float m = (float)mean;
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (t + u * kSmallT < total) {
+      Piece<T> o;
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const float nn = fmaf((float)p[u].v[k] - m, rw[part[u] + k], bc[part[u] + k]);
+        o.v[k] = (T)gn_act<MODE>(nn, RES ? (float)rp[u].v[k] : 0.f);
+      }
+      store_piece(out + base + at[u], o);
+    }
+}
+
 // dn and dres of one value (r: res, g: dy, n: the normed value).  tol = kTol times
 // the largest 2 |b| + |m rw| of the thread's channels bounds n's fp32 error;
 // returns whether a ReLU's argument is within that of zero (never where it is
@@ -713,6 +797,15 @@ __global__ void __launch_bounds__(kGnT, 4) gn_bwd_apply_kernel(const T* __restri
 
 inline int gn_vec(int dtype) { return dtype == 1 ? 4 : 8; }
 
+// Whether the forward is one launch: the group's values fit the registers of a
+// workgroup, and the maps are small (the 16-B pieces of neighbouring groups share
+// lines that each workgroup fetches again).
+inline bool gn_is_small(int dtype, int N, int HW, int C, int G) {
+  const int V = gn_vec(dtype), cpg = C / G;
+  return cpg % V == 0 && (long)HW * (cpg / V) <= kSmallT * kSmallU &&
+         (long)N * HW * C * (16 / V) <= kSmallBytes;
+}
+
 int gn_check(const char* what, int dtype, int wdtype, int N, int HW, int C, int G, int mode) {
   if (dtype != 0 && dtype != 1 && dtype != 3)
     return fail(kInvalidArgument, std::string(what) + ": dtype must be float16, float32 or bfloat16");
@@ -751,6 +844,7 @@ extern "C" {
 
 size_t droid_group_norm_workspace(int dtype, int N, int HW, int C, int G, int backward) {
   if (gn_check("group_norm_workspace", dtype, 1, N, HW, C, G, 0) != kOk || N == 0 || HW == 0) return 0;
+  if (!backward && gn_is_small(dtype, N, HW, C, G)) return 0;
   const Split sp = gn_split(N, HW, C, gn_vec(dtype));
   return (size_t)N * sp.blocks * (G + (backward ? C : 0)) * sizeof(double2);
 }
@@ -762,6 +856,15 @@ int droid_group_norm_act(int dtype, const void* x, const void* res, void* out, c
   if (N == 0 || HW == 0) return kOk;
   const bool need_res = mode == kResRelu || mode == kAddRelu;
   if (!x || !out || (need_res && !res)) return fail(kInvalidArgument, "group_norm_act: null map");
+  if (gn_is_small(dtype, N, HW, C, G)) {
+#define GN_SMALL(T, M, ...)                                                                                          \
+  gn_small_kernel<T, M><<<dim3(G, N), kSmallT, 0, stream>>>((const T*)x, (const T*)res, (T*)out, weight, bias, wdtype, \
+                                                            HW, C, G, eps, (double2*)stats)
+    GN_TYPES(GN_SMALL, 0)
+#undef GN_SMALL
+    DROID_LAUNCH_CHECK();
+    return kOk;
+  }
   if (!ws || ws_bytes < droid_group_norm_workspace(dtype, N, HW, C, G, 0))
     return fail(kInvalidArgument, "group_norm_act: workspace too small");
   const Split sp = gn_split(N, HW, C, gn_vec(dtype));

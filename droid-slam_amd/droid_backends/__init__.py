@@ -1019,9 +1019,10 @@ def group_norm_act(x, num_groups, weight=None, bias=None, mode=NORM_RELU, res=No
     dt, hw, dev = _NORM_DTYPES[x.dtype], H * W, x.device
     stats = torch.empty((N, num_groups, 2), dtype=torch.float64, device=dev) if return_stats else None
     with _on(dev):
-        ws = torch.empty((_group_norm_workspace(dt, N, hw, C, num_groups, 0),), dtype=torch.uint8, device=dev)
+        n = _group_norm_workspace(dt, N, hw, C, num_groups, 0)   # none: small maps take one launch
+        ws = torch.empty((n,), dtype=torch.uint8, device=dev) if n else None
         check(lib.droid_group_norm_act(dt, _addr(x), _addr(res), _addr(out), _addr(weight), _addr(bias), wdt, _addr(stats),
-                                       N, hw, C, num_groups, mode, eps, _addr(ws), ws.numel(), _raw_stream(dev)), fn)
+                                       N, hw, C, num_groups, mode, eps, _addr(ws), n, _raw_stream(dev)), fn)
     return (out, stats) if return_stats else out
 
 

@@ -356,8 +356,8 @@ int droid_instance_norm_act_f16(const void* x, const void* res, void* out, int N
  * type wdtype (DROID_F32 or dtype), either may be NULL.  Statistics and
  * arithmetic in >= 32 bits, one rounding at the end.  out may be x or res.
  * stats: NULL, or (N, G, 2) doubles that receive mean and 1/std for the
- * backward pass.  ws: droid_group_norm_workspace bytes (backward 0 / 1), used
- * by this call only until its kernels end. */
+ * backward pass.  ws: droid_group_norm_workspace bytes (backward 0 / 1; 0 bytes,
+ * ws NULL, for small maps), used by this call only until its kernels end. */
 size_t droid_group_norm_workspace(int dtype, int N, int HW, int C, int G, int backward);
 int droid_group_norm_act(int dtype, const void* x, const void* res, void* out, const void* weight, const void* bias,
                          int wdtype, void* stats, int N, int HW, int C, int G, int mode, float eps, void* ws,

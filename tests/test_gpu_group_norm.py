@@ -235,3 +235,22 @@ def test_offsets_past_32_bits_and_maps_past_the_abi():
     big = torch.empty((1, 1, 65536, 32768), dtype=torch.float16, device=DEV)
     with pytest.raises(RuntimeError, match="too large"):
         nb.group_norm_act(big.contiguous(memory_format=torch.channels_last), 1)
+
+
+@pytest.mark.parametrize("mode", range(5))
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("N,C,H,W,G", [(1, 16, 64, 64, 2), (1, 16, 64, 65, 2), (1, 16, 32, 64, 2), (3, 32, 50, 101, 4),
+                                       (2, 64, 97, 43, 16), (9, 8, 1, 1, 1), (40, 64, 41, 25, 8)])
+def test_forward_and_backward_around_one_launch(N, C, H, W, G, dtype, mode):
+    """Groups that just fit one workgroup's registers, just do not, and maps too
+    large for one launch; the output in x's and in res's place."""
+    import droid_backends as nb
+    dt = TYPES[dtype]
+    x, res, dy, w, b = _inputs(dt, N, C, H, W, seed=C + H + mode)
+    y, stats = nb.group_norm_act(x, G, w, b, mode, res, return_stats=True)
+    dx, dres, dw, db = nb.group_norm_act_backward(dy, x, stats, G, w, b, mode, res)
+    _check(dt, x, res, dy, w, b, G, mode, y, dx, dres, dw, db)
+    for place in ("x", "res"):
+        xi, ri = x.clone(memory_format=torch.channels_last), res.clone(memory_format=torch.channels_last)
+        out = xi if place == "x" else ri
+        assert torch.equal(nb.group_norm_act(xi, G, w, b, mode, ri, out=out), y)
