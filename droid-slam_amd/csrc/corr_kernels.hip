@@ -879,7 +879,7 @@ static_assert(kCeLds <= 160 * 1024, "corr_ce0 LDS budget");
 __device__ __forceinline__ void ce_dma4(rsrc_t rs, unsigned lds, unsigned voff) {
   const rsrc_t r = {__builtin_amdgcn_readfirstlane(rs.x), __builtin_amdgcn_readfirstlane(rs.y),
                     __builtin_amdgcn_readfirstlane(rs.z), __builtin_amdgcn_readfirstlane(rs.w)};
-  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dword %1, %2, 0 offen lds"
                :
                : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(r)
                : "memory", "m0");
