@@ -177,7 +177,7 @@ __device__ __forceinline__ void alt_box_dma(const AltArgs& a, int l, int f2, int
     const int piece = (lane & 15) ^ (tap & 15);
     const int ry = (int)(((float)tap + 0.5f) * inv), rx = tap - ry * gbw;
     const unsigned off = tap < tn ? (unsigned)((((gy0 + ry) * Wl + gx0 + rx) * 128 + piece * 8) * 2) : kOob;
-    dma16(rs, box + ins * 1024, off);
+    dma16_late(rs, box + ins * 1024, off);
   }
 }
 

@@ -875,7 +875,8 @@ static_assert(kCeLds <= 160 * 1024, "corr_ce0 LDS budget");
 #pragma clang diagnostic ignored "-Winline-asm"
 // LDS-DMA of 4 B per lane (buffer_load_dword ... lds): lane l's dword lands at
 // LDS byte `lds` + 4 l.  Preceded by lgkmcnt(0) so that the issuing wave's
-// earlier ds_reads of the destination have returned (write-after-read).
+// earlier ds_reads of the destination have returned (write-after-read).  The
+// descriptor may come from a vector instruction just before: dma16_late's waits.
 __device__ __forceinline__ void ce_dma4(rsrc_t rs, unsigned lds, unsigned voff) {
   const rsrc_t r = {__builtin_amdgcn_readfirstlane(rs.x), __builtin_amdgcn_readfirstlane(rs.y),
                     __builtin_amdgcn_readfirstlane(rs.z), __builtin_amdgcn_readfirstlane(rs.w)};

@@ -65,7 +65,7 @@ struct Op<__bf16> {
   }
 };
 
-// lds_dma.hpp's dma16 with 4 B a lane.
+// lds_dma.hpp's dma16_late with 4 B a lane.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void dma4(rsrc_t rs, unsigned lds, unsigned voff) {
@@ -112,7 +112,7 @@ __device__ __forceinline__ void stage_tile(const T* frame, char* lds, int y0, in
 #pragma unroll
   for (int q = 0; q < kDmas<DP>; ++q) {
     const int o = (wave * kDmas<DP> + q) * 1024;
-    dma16(rs, lds_addr(lds) + o, skip((o + lane * 16) / (2 * DP)) ? kOob : off[q]);
+    dma16_late(rs, lds_addr(lds) + o, skip((o + lane * 16) / (2 * DP)) ? kOob : off[q]);
   }
 }
 
