@@ -362,6 +362,7 @@ __global__ void __launch_bounds__(kLT) corr_loss_row_kernel(RowArgs a) {
   for (int n = 0; n < SLOTS; ++n) {
     pi[n] /= tot;
     if (pi[n] > 0.f) ent += pi[n] * logf(pi[n]);
+    if (pi[n] == 0.f) own[n] = -1;   // no target: a later place of its key may have weight
   }
   // the row's sum over all keys
   float m = kNegBig;
@@ -377,8 +378,8 @@ __global__ void __launch_bounds__(kLT) corr_loss_row_kernel(RowArgs a) {
   // sum_k pi_k s_k, as one dot product with the pi-weighted sum of the target rows
   const T* f2 = static_cast<const T*>(a.f2) + (long)j * a.Q * a.D;
   // The weights kept for the gradient: a key that a row names more than once has all
-  // of its weight at the first place, so that no place of ds has more than one term
-  // of an edge (and their sum no order).
+  // of its weight at the first place that has any, so that no place of ds has more than
+  // one term of an edge (and their sum no order).
   float dot = 0.f, kept[SLOTS] = {};
   bool again[SLOTS] = {};
   typedef typename Op<T>::vec8 vec8;
@@ -396,7 +397,6 @@ __global__ void __launch_bounds__(kLT) corr_loss_row_kernel(RowArgs a) {
 #pragma unroll
       for (int n = 0; n < SLOTS; ++n)   // (a lane past K holds -1 and 0)
         if (k0 / 16 == n) t[u] = __shfl(own[n], (k0 + u) & 15, 16), w[u] = __shfl(pi[n], (k0 + u) & 15, 16);
-      if (w[u] == 0.f) t[u] = -1;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         if (t[u] >= 0 && 8 * l + 128 * h < a.D)

@@ -149,7 +149,7 @@ int droid_corr_alt_ce0_ordered(const void* const* pyr, const int* Hl, const int*
  * sums.  A target >= Q, an edge outside the frames: loss NaN.
  * Outputs for the backward pass: lse (E,P) f32 (log2 units; no target: +inf, or -inf
  * where the row's features are not finite), prob (E,P,K) f32 (with logits only; a key
- * that a row names twice has its whole weight at the first place).
+ * that a row names twice has its whole weight at the first place that has any).
  * ws: droid_corr_loss_workspace bytes (backward: N1 / N2 = 0 for a gradient that is not
  * wanted, N2 = 0 with shared), used until the kernels end. */
 size_t droid_corr_loss_workspace(int E, int N1, int P, int N2, int Q, int D, int K, int backward);
