@@ -146,12 +146,10 @@ __device__ __forceinline__ void loads_done() {
   asm volatile("" ::: "memory");
 }
 
-// The same, but for the wave's last N LDS-DMAs (and one more of the first two
-// waves, where AUX).
-template <int N, bool AUX>
-__device__ __forceinline__ void loads_left(int wave) {
-  if (AUX && wave < 2) __builtin_amdgcn_s_waitcnt(0x0f70 | (N + 1));
-  else __builtin_amdgcn_s_waitcnt(0x0f70 | N);
+// The same, but for the wave's last N LDS-DMAs.
+template <int N>
+__device__ __forceinline__ void loads_left() {
+  __builtin_amdgcn_s_waitcnt(0x0f70 | N);
   asm volatile("" ::: "memory");
 }
 
@@ -1077,8 +1075,8 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
       for (int q = 0; q < 2 * KD; ++q) read_row(q);
     }
     if (t + 2 < t1) {
+      if (t + 3 < t1) stage_rows(t + 3);   // before the tile: landed when this step ends
       stage(t + 2, ahead);
-      if (t + 3 < t1) stage_rows(t + 3);
     }
     if constexpr (SRC && DST) {
       if (wave == 3 && t + 1 < t1) make_b(t + 1);
@@ -1106,8 +1104,9 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
       for (int n = 0; n < kP; ++n) product(1, n);
     }
     buf = buf == 2 ? 0 : buf + 1;
-    // tile t + 1 has landed; the loads of t + 2 (and t + 3's row data) stay in flight
-    if (t + 3 < t1) loads_left<kDmas<DP>, DST>(wave);
+    // tile t + 1 and t + 3's row data, which the next step's stage reads, have landed;
+    // the loads of tile t + 2 stay in flight
+    if (t + 3 < t1) loads_left<kDmas<DP>>();
     else loads_done();
     __syncthreads();
   }
