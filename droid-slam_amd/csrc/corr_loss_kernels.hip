@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(kLT) corr_loss_row_kernel(RowArgs a) {
     const int k = l + 16 * n;
     if (k < a.K) {
       const int t = own[n] = idx[k];
-      if (t >= 0) pi[n] = a.logits ? a.logits[row * a.K + k] * a.invT : 0.f;
+      if (t >= 0) pi[n] = a.logits ? a.logits[row * a.K + k] : 0.f;
       used |= pi[n] != -INFINITY;          // a logit of -inf: no target either
       bad |= t >= a.Q || pi[n] != pi[n];
       top = fmaxf(top, pi[n]);
@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(kLT) corr_loss_row_kernel(RowArgs a) {
   float tot = 0.f;
 #pragma unroll
   for (int n = 0; n < SLOTS; ++n) {
-    pi[n] = __expf(pi[n] - top);
+    pi[n] = __expf((pi[n] - top) * a.invT);   // (over T last: a lowest value over T < 1 is -inf)
     if (l + 16 * n >= a.K) pi[n] = 0.f;
     tot += pi[n];
   }

@@ -67,3 +67,19 @@ def test_teacher_logits_that_are_no_numbers_are_not_dropped(value):
     bad[1, 7] = True
     assert torch.equal(loss.isnan().cpu(), bad)
     assert grads[0][f1[1], 7].isnan().all()
+
+
+@pytest.mark.parametrize("T", [0.5, 1.0, 2.0])
+def test_logits_masked_with_the_lowest_value(T):
+    """The type's lowest value is a logit like any other: a row of nothing else is
+    uniform, beside an ordinary one it has no weight - at T < 1 too, where it
+    overflows when divided."""
+    dt = torch.bfloat16
+    a, b, f1, f2, idx, logits, g = _problem(52, dt, 5, 2, 2, 70, 2, 90, 64)
+    idx[:] = np.random.default_rng(52).random((2, 70, 90)).argsort(-1)[..., :5]
+    logits[:, ::2, :4] = np.finfo(np.float32).min
+    logits[:, ::3] = np.finfo(np.float32).min
+    p = (a, b, f1, f2, idx, logits, g)
+    loss, grads = _run(*p, False, 1 / 16, T)
+    assert (loss[:, ::3] != 0).all()
+    _check(dt, *p, False, 1 / 16, T, loss, grads)
