@@ -29,7 +29,8 @@
 // Statistics: a thread sums its values in fp32 relative to the first one it
 // met (no cancellation where the mean is far from zero) over at most kFlush
 // pieces, then adds them to 64-bit sums; everything after that is 64-bit and
-// added in a fixed order, so results do not depend on the schedule.  mean and
+// added in a fixed order, so results do not depend on the schedule.  The
+// backward pass's sums of dn and dn xhat likewise.  mean and
 // rstd are kept in 64 bits for the backward pass: where a ReLU's argument is
 // within rounding of zero its sign is decided in 64 bits, because one wrong
 // sign moves a whole gradient, not its last bit.
@@ -539,7 +540,7 @@ __global__ void __launch_bounds__(kGnT, 4) gn_bwd_stats_kernel(const T* __restri
                                                             double2* __restrict__ gpart) {
   constexpr int V = Elem<T>::V;
   constexpr bool RES = MODE == kResRelu || MODE == kAddRelu;
-  __shared__ float red[2][kGnT * V];
+  __shared__ double red[2][V][kGnT + 8];   // value k of thread t at [k][t]; + 8: the channels read across the k below
   __shared__ double2 sum[kGnT];
   const int n = blockIdx.y, s = blockIdx.x, S = gridDim.x, t = threadIdx.x;
   const int cpg = C / G;
@@ -547,7 +548,7 @@ __global__ void __launch_bounds__(kGnT, 4) gn_bwd_stats_kernel(const T* __restri
   // channel constants: xhat = (x - m) rs, n = xhat wc + bc
   float m[V], rs[V], wc[V], bc[V], a1[V], a2[V], tol = 0.f;
   {
-    float (&lds)[4][kGnMaxC] = *reinterpret_cast<float (*)[4][kGnMaxC]>(&red[0][0]);   // free again before the sums
+    float (&lds)[4][kGnMaxC] = *reinterpret_cast<float (*)[4][kGnMaxC]>(&red[0][0][0]);   // free again before the sums
     const ChanIn ch = gn_channel(w, b, wdt, C, cpg);
     if (t < C) {
       const double2 v = st[ch.g];
@@ -568,7 +569,17 @@ __global__ void __launch_bounds__(kGnT, 4) gn_bwd_stats_kernel(const T* __restri
   for (int k = 0; k < V; ++k) {
     tol = fmaxf(tol, kTol * (2.f * fabsf(bc[k]) + fabsf(m[k] * rs[k] * wc[k])));
     a1[k] = a2[k] = 0.f;
+    red[0][k][t] = red[1][k][t] = 0.0;
   }
+  // from fp32 to 64 bits, in LDS: in registers the kernel would spill
+  auto flush = [&]() {
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      red[0][k][t] += (double)a1[k];
+      red[1][k][t] += (double)a2[k];
+      a1[k] = a2[k] = 0.f;
+    }
+  };
   const long base = (long)n * HW * C;
   const long c0 = sp.chunks * s / S, c1 = sp.chunks * (s + 1) / S;
   const long f1 = min(c1 * sp.active, sp.pieces);
@@ -593,7 +604,10 @@ __global__ void __launch_bounds__(kGnT, 4) gn_bwd_stats_kernel(const T* __restri
   };
   if (t < sp.active) {
     // two pieces' loads in flight a thread
+    int cnt = 0;
     for (long f = c0 * sp.active + t; f < f1; f += 2 * sp.active) {
+      if (cnt == kFlush) flush(), cnt = 0;
+      cnt += 2;
       Piece<T> p[2], gp[2], rp[2];
       const bool two = f + sp.active < f1;
 #pragma unroll
@@ -619,11 +633,7 @@ __global__ void __launch_bounds__(kGnT, 4) gn_bwd_stats_kernel(const T* __restri
       const Piece<T> o = piece(p, rp, gp, o0, sp.tail);
       if constexpr (RES) store_tail(dres + o0, o, sp.tail);
     }
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      red[0][t * V + k] = a1[k];
-      red[1][t * V + k] = a2[k];
-    }
+    flush();
   }
   __syncthreads();
   // channel c: the flat values c, c + C, ... of the active threads, over lanes of
@@ -633,8 +643,9 @@ __global__ void __launch_bounds__(kGnT, 4) gn_bwd_stats_kernel(const T* __restri
   double u = 0.0, v = 0.0;
   if (l < L)
     for (int i = l; i < copies; i += L) {
-      u += (double)red[0][c + i * C];
-      v += (double)red[1][c + i * C];
+      const int f = c + i * C;
+      u += red[0][f % V][f / V];
+      v += red[1][f % V][f / V];
     }
   sum[t] = make_double2(u, v);
   __syncthreads();

@@ -1028,8 +1028,8 @@ def group_norm_act(x, num_groups, weight=None, bias=None, mode=NORM_RELU, res=No
 
 def group_norm_act_backward(dy, x, stats, num_groups, weight=None, bias=None, mode=NORM_RELU, res=None):
     """Gradients of group_norm_act: (dx, dres, dweight, dbias); dres is None
-    without a residual, dweight / dbias (summed in 64 bits, in a fixed order)
-    are None where the parameter is.  stats: group_norm_act's."""
+    without a residual, dweight / dbias (summed in a fixed order, in fp32 over at
+    most 32 values, in 64 bits beyond) are None where the parameter is.  stats: group_norm_act's."""
     fn = "group_norm_act_backward"
     _norm_map(fn, "x", x)
     _norm_map(fn, "dy", dy, x)

@@ -363,8 +363,8 @@ int droid_group_norm_act(int dtype, const void* x, const void* res, void* out, c
                          int wdtype, void* stats, int N, int HW, int C, int G, int mode, float eps, void* ws,
                          size_t ws_bytes, hipStream_t stream);
 /* its gradients from dy, the forward call's inputs and its stats: dx, dres
- * (modes 1, 2), dweight and dbias (wdtype, (C), either may be NULL; summed in 64
- * bits in a fixed order).  Maps must not overlap.  A ReLU argument within fp32
+ * (modes 1, 2), dweight and dbias (wdtype, (C), either may be NULL; summed in a
+ * fixed order, in fp32 over at most 32 values, in 64 bits beyond).  Maps must not overlap.  A ReLU argument within fp32
  * rounding of zero has its sign decided in 64 bits. */
 int droid_group_norm_act_backward(int dtype, const void* x, const void* res, const void* dy, const void* weight,
                                   const void* bias, int wdtype, const void* stats, void* dx, void* dres, void* dweight,
