@@ -83,32 +83,45 @@ def corr_distillation(fmap1, fmap2, f1, f2, idx, logits, scale=1.0 / 16, tempera
     return _corr_loss(fmap1, fmap2, f1, f2, idx, logits, scale, temperature)
 
 
-def nearest_targets(coords, ht, wd, valid=None):
-    """The key row of each reprojected coordinate (DepthVideo.reproject: (..., 2)
-    as (x, y)) in an (ht, wd) map: int32 (...), -1 outside the map or where valid
-    is zero - corr_cross_entropy's target."""
-    x, y = coords[..., 0].round(), coords[..., 1].round()
-    ok = (x >= 0) & (x < wd) & (y >= 0) & (y < ht)
+def _inside(x, y, ht, wd, ok):
+    """Where (x, y) is a pixel of the map, and its row there (-1 elsewhere).  The row
+    is made in integers: half types hold whole numbers up to 2048 or 256 only."""
+    ok = ok & (x >= 0) & (x < wd) & (y >= 0) & (y < ht)
+    x, y = (torch.where(ok, v, torch.zeros_like(v)).long() for v in (x, y))
+    return ok, torch.where(ok, y * wd + x, torch.full_like(x, -1)).to(torch.int32)
+
+
+def _valid_coords(fn, coords, valid):
+    """coords in fp32 at least, and where they count."""
+    if not coords.dtype.is_floating_point or coords.dtype.itemsize < 4:
+        coords = coords.float()
+    ok = torch.isfinite(coords).all(-1)
     if valid is not None:
         ok = ok & (valid > 0)
-    return torch.where(ok, y * wd + x, torch.full_like(x, -1)).to(torch.int32)
+    return coords, ok
+
+
+def nearest_targets(coords, ht, wd, valid=None):
+    """The key row of each reprojected coordinate (DepthVideo.reproject: (..., 2)
+    as (x, y), any float type) in an (ht, wd) map: int32 (...), -1 outside the map
+    or where valid is zero - corr_cross_entropy's target."""
+    coords, ok = _valid_coords("nearest_targets", coords, valid)
+    return _inside(coords[..., 0].round(), coords[..., 1].round(), ht, wd, ok)[1]
 
 
 def bilinear_targets(coords, ht, wd, valid=None):
     """The four pixels around each reprojected coordinate and the logarithms of
     their bilinear weights, (..., 4) int32 and float32 - corr_distillation's idx
-    and logits (temperature 1).  Neighbours outside the map: -1."""
+    and logits (temperature 1).  Neighbours outside the map: -1.  coords and valid
+    as nearest_targets."""
+    coords, ok = _valid_coords("bilinear_targets", coords, valid)
     x0, y0 = coords[..., 0].floor(), coords[..., 1].floor()
     fx, fy = coords[..., 0] - x0, coords[..., 1] - y0
-    ok = torch.isfinite(coords).all(-1)
-    if valid is not None:
-        ok = ok & (valid > 0)
     idx, w = [], []
     for dy, wy in ((0, 1 - fy), (1, fy)):
         for dx, wx in ((0, 1 - fx), (1, fx)):
-            x, y = x0 + dx, y0 + dy
-            inside = ok & (x >= 0) & (x < wd) & (y >= 0) & (y < ht)
-            idx.append(torch.where(inside, y * wd + x, torch.full_like(x, -1)).to(torch.int32))
+            inside, row = _inside(x0 + dx, y0 + dy, ht, wd, ok)
+            idx.append(row)
             w.append(torch.where(inside, wx * wy, torch.zeros_like(wx)))
     return torch.stack(idx, -1), torch.stack(w, -1).float().log()
 
