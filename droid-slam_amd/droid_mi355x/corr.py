@@ -97,14 +97,19 @@ def _valid_coords(fn, coords, valid):
         coords = coords.float()
     ok = torch.isfinite(coords).all(-1)
     if valid is not None:
-        ok = ok & (valid > 0)
+        if valid.shape == ok.shape + (1,):    # as DepthVideo.reproject returns it
+            valid = valid[..., 0]
+        shape, ok = ok.shape, ok & (valid > 0)
+        if ok.shape != shape:
+            raise RuntimeError("%s: valid %s does not match coordinates %s"
+                               % (fn, tuple(valid.shape), tuple(coords.shape)))
     return coords, ok
 
 
 def nearest_targets(coords, ht, wd, valid=None):
     """The key row of each reprojected coordinate (DepthVideo.reproject: (..., 2)
     as (x, y), any float type) in an (ht, wd) map: int32 (...), -1 outside the map
-    or where valid is zero - corr_cross_entropy's target."""
+    or where valid ((...) or (..., 1)) is zero - corr_cross_entropy's target."""
     coords, ok = _valid_coords("nearest_targets", coords, valid)
     return _inside(coords[..., 0].round(), coords[..., 1].round(), ht, wd, ok)[1]
 

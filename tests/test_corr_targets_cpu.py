@@ -40,3 +40,16 @@ def test_maps_wider_than_a_half_type_counts():
     c = torch.tensor([[2048.0, 0.0], [2050.0, 0.0], [float("inf"), 0.0], [0.0, float("nan")]]).half()
     assert nearest_targets(c, 1, 2049).tolist() == [2048, -1, -1, -1]
     assert bilinear_targets(c, 1, 2049)[0][:, 0].tolist() == [2048, -1, -1, -1]
+
+
+def test_valid_as_reproject_returns_it():
+    c = _grid(4, 6).float().expand(3, 4, 6, 2)
+    valid = (torch.rand(3, 4, 6, 1, generator=torch.Generator().manual_seed(0)) > 0.5).float()
+    for fn in (lambda v: nearest_targets(c, 4, 6, v), lambda v: bilinear_targets(c, 4, 6, v)[0]):
+        assert torch.equal(fn(valid), fn(valid[..., 0]))
+        assert (fn(valid) < 0).any() and (fn(valid) >= 0).any()
+        assert torch.equal(fn(torch.ones(4, 6)), fn(None))
+        with pytest.raises(RuntimeError):
+            fn(torch.ones(5, 3, 4, 6))
+        with pytest.raises(RuntimeError):
+            fn(torch.ones(3, 3, 4, 6, 1))
