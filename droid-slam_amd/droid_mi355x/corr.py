@@ -17,6 +17,8 @@ from torch.autograd.function import once_differentiable
 
 import droid_backends
 
+from . import tracing
+
 
 class CorrSampler(torch.autograd.Function):
     """corr.py:6-20."""
@@ -48,13 +50,15 @@ class CorrLoss(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
+        tracing.refuse_upstream("CorrLoss.backward", g)
         fmap1, fmap2, f1, f2, idx, lse, prob = ctx.saved_tensors
         d1, d2 = droid_backends.corr_loss_backward(g.contiguous(), fmap1, fmap2, f1, f2, idx, lse, prob, ctx.scale,
                                                    ctx.temperature, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
         return d1, d2, None, None, None, None, None, None
 
 
-def _corr_loss(fmap1, fmap2, f1, f2, idx, logits, scale, temperature):
+def _corr_loss(fn, fmap1, fmap2, f1, f2, idx, logits, scale, temperature):
+    tracing.refuse(fn, fmap1, fmap2, logits)
     if torch.is_grad_enabled() and (fmap1.requires_grad or (fmap2 is not None and fmap2.requires_grad)):
         return CorrLoss.apply(fmap1, fmap2, f1, f2, idx, logits, scale, temperature)
     return droid_backends.corr_loss_forward(fmap1, fmap2, f1, f2, idx, logits, scale, temperature)[0]
@@ -69,8 +73,9 @@ def corr_cross_entropy(fmap1, fmap2, f1, f2, target, scale=1.0 / 16):
     features, as in a frame graph), fp16 or bf16, D a multiple of 8 up to 256;
     f1/f2 (E) int32 frame rows; target (E, query rows...) int32 key row, negative:
     the row is left out (loss 0).  -> loss (E, query rows...) float32, unreduced,
-    differentiable in the features."""
-    return _corr_loss(fmap1, fmap2, f1, f2, target, None, scale, 1.0)
+    differentiable in the features, once and in reverse mode (forward-mode tangents,
+    function transforms and tracers are refused)."""
+    return _corr_loss("corr_cross_entropy", fmap1, fmap2, f1, f2, target, None, scale, 1.0)
 
 
 def corr_distillation(fmap1, fmap2, f1, f2, idx, logits, scale=1.0 / 16, temperature=1.0):
@@ -80,7 +85,7 @@ def corr_distillation(fmap1, fmap2, f1, f2, idx, logits, scale=1.0 / 16, tempera
     float32 (-inf: weight 0).  Features, edges and result as corr_cross_entropy;
     no gradient reaches the teacher's logits.  With logits = log(weight) the rows
     of bilinear_targets give sub-pixel correspondences."""
-    return _corr_loss(fmap1, fmap2, f1, f2, idx, logits, scale, temperature)
+    return _corr_loss("corr_distillation", fmap1, fmap2, f1, f2, idx, logits, scale, temperature)
 
 
 def _inside(x, y, ht, wd, ok):

@@ -10,8 +10,11 @@ reference runs it (the parity bridge for the tests).
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 import droid_backends
+
+from . import tracing
 
 DIM = 32
 
@@ -34,7 +37,8 @@ def _group_norm_act_plain(x, num_groups, weight, bias, mode, res, eps):
 class GroupNormAct(torch.autograd.Function):
     """Group norm + activation / residual add (droid_group_norm_act and its
     backward): statistics in 64 bits, gradients of every input.  A backward pass
-    that is itself differentiated (create_graph) goes through torch's operators."""
+    that is itself differentiated (create_graph) or batched (is_grads_batched) goes
+    through torch's operators."""
 
     @staticmethod
     def forward(ctx, x, num_groups, weight, bias, mode, res, eps):
@@ -47,12 +51,16 @@ class GroupNormAct(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         x, weight, bias, res, stats = ctx.saved_tensors
-        if torch.is_grad_enabled():
-            # (views: x and res may be one tensor)
-            ins = {i: t.view_as(t) for i, t in ((0, x), (2, weight), (3, bias), (5, res)) if t is not None}
-            y = _group_norm_act_plain(ins[0], ctx.num_groups, ins.get(2), ins.get(3), ctx.mode, ins.get(5), ctx.eps)
-            want = [i for i in ins if ctx.needs_input_grad[i]]
-            grads = dict(zip(want, torch.autograd.grad(y, [ins[i] for i in want], dy, create_graph=True)))
+        again = torch.is_grad_enabled()
+        if again or tracing.followed(dy) or tracing.batched(dy):   # differentiated again, or a batch of dy
+            with torch.enable_grad():
+                # (views: x and res may be one tensor)
+                ins = {i: t.view_as(t) for i, t in ((0, x), (2, weight), (3, bias), (5, res)) if t is not None}
+                want = [i for i in ins if ctx.needs_input_grad[i]]
+                if not again:
+                    ins = {i: t.detach().requires_grad_(i in want) for i, t in ins.items()}
+                y = _group_norm_act_plain(ins[0], ctx.num_groups, ins.get(2), ins.get(3), ctx.mode, ins.get(5), ctx.eps)
+                grads = dict(zip(want, torch.autograd.grad(y, [ins[i] for i in want], dy, create_graph=again)))
             return tuple(grads.get(i) for i in range(7))
         # the forward call checked them; saved-tensor hooks may return another layout
         cl = torch.channels_last
@@ -64,9 +72,12 @@ class GroupNormAct(torch.autograd.Function):
 
 def group_norm_act(x, num_groups, weight=None, bias=None, mode=droid_backends.NORM_RELU, res=None, eps=1e-5):
     """droid_backends.group_norm_act under autograd: x (and res) channels_last
-    (N,C,H,W) fp16 / bf16 / fp32 on the GPU; gradients reach x, weight, bias and res."""
+    (N,C,H,W) fp16 / bf16 / fp32 on the GPU; gradients reach x, weight, bias and res.
+    Under forward mode, function transforms and tracers: torch's operators in fp32."""
     if mode not in (droid_backends.NORM_RES_RELU, droid_backends.NORM_ADD_RELU):
         res = None
+    if tracing.followed(x, weight, bias, res):
+        return _group_norm_act_plain(x, num_groups, weight, bias, mode, res, eps)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, res)):
         return GroupNormAct.apply(x, num_groups, weight, bias, mode, res, eps)
     return droid_backends.group_norm_act(x, num_groups, weight, bias, mode, res, eps=eps)
@@ -86,6 +97,19 @@ def _norm_act(norm, x, mode, res=None):
     """nn.GroupNorm on a convolution's output, with the activation / residual add after it."""
     return group_norm_act(x.contiguous(memory_format=torch.channels_last), norm.num_groups, norm.weight, norm.bias,
                           mode, res, norm.eps)
+
+
+def _plain(m, kind):
+    """Whether a module does what its type says and nobody listens to its calls."""
+    return (type(m) is kind and not m._forward_hooks and not m._forward_pre_hooks and not m._backward_hooks
+            and not m._backward_pre_hooks and "forward" not in m.__dict__)
+
+
+def _plain_norm(m, dt):
+    if not _plain(m, nn.GroupNorm) or m.num_channels > 512:
+        return False
+    kinds = {t.dtype for t in (m.weight, m.bias) if t is not None}
+    return len(kinds) <= 1 and kinds <= {torch.float32, dt}
 
 
 class ResidualBlock(nn.Module):
@@ -210,16 +234,31 @@ class BasicEncoder(nn.Module):
         _, c2, h2, w2 = x.shape
         return x.contiguous().view(b, n, c2, h2, w2)
 
+    def _fuses_group(self, x):
+        """Whether forward_group stands for forward_reference here: nothing but autograd's
+        tape follows the tensors, and every module that it does not call is the plain one,
+        without hooks, in a type and size of the operator."""
+        if (tracing.followed(x) or forward_ad._current_level >= 0 or torch.nn.modules.module._has_any_global_hook()
+                or x.dim() != 5 or x.shape[0] * x.shape[1] > 65534):
+            return False
+        dt = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
+        if dt not in (torch.float16, torch.bfloat16, torch.float32):
+            return False
+        blocks = [blk for layer in (self.layer1, self.layer2, self.layer3) for blk in layer]
+        return (_plain_norm(self.norm1, dt) and _plain(self.relu1, nn.ReLU)
+                and all(_plain_norm(b.norm1, dt) and _plain_norm(b.norm2, dt) and _plain(b.relu, nn.ReLU)
+                        and (b.downsample is None
+                             or _plain(b.downsample, nn.Sequential) and len(b.downsample) == 2
+                             and b.downsample[1] is b.norm3 and _plain_norm(b.norm3, dt)) for b in blocks))
+
     def forward(self, x):
         """(b, n, 3, H, W) -> (b, n, C, H/8, W/8) fp16: the MI355X path for the
         norms DroidNet uses (instance: fnet, none: cnet - no running statistics,
         so train and eval mode agree; the reference never applies its dropout).
         Training (gradients through the encoder) runs the reference ops, except
         with norm_fn 'group', whose norms are one operator each (forward_group)."""
-        if self.norm_fn == "group" and x.is_cuda:
-            dt = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
-            if dt in (torch.float16, torch.bfloat16, torch.float32) and self.norm1.weight.dtype in (torch.float32, dt):
-                return self.forward_group(x)
+        if self.norm_fn == "group" and x.is_cuda and self._fuses_group(x):
+            return self.forward_group(x)
         if (self.norm_fn not in ("instance", "none") or not x.is_cuda
                 or (torch.is_grad_enabled() and self.conv1.weight.requires_grad)):
             return self.forward_reference(x)
