@@ -94,9 +94,10 @@ def _norm(kind, planes):
 
 
 def _norm_act(norm, x, mode, res=None):
-    """nn.GroupNorm on a convolution's output, with the activation / residual add after it."""
-    return group_norm_act(x.contiguous(memory_format=torch.channels_last), norm.num_groups, norm.weight, norm.bias,
-                          mode, res, norm.eps)
+    """nn.GroupNorm on a convolution's output, with the activation / residual add after
+    it; under autocast in fp32, as torch's autocast runs group norm and what follows."""
+    x = x.to(torch.float32 if torch.is_autocast_enabled("cuda") else x.dtype, memory_format=torch.channels_last)
+    return group_norm_act(x, norm.num_groups, norm.weight, norm.bias, mode, res, norm.eps)
 
 
 def _plain(m, kind):
@@ -222,8 +223,8 @@ class BasicEncoder(nn.Module):
     def forward_group(self, x):
         """forward_reference with norm_fn 'group' on the GPU, for training and
         inference: channels_last throughout, every norm one operator with its
-        activation and residual add, in the convolutions' type (fp16 / bf16 under
-        autocast, else x's)."""
+        activation and residual add.  Maps between the convolutions have x's type,
+        under autocast fp32 (a module and input in half precision keep them in it)."""
         b, n, c1, h1, w1 = x.shape
         x = x.reshape(b * n, c1, h1, w1).contiguous(memory_format=torch.channels_last)
         x = _norm_act(self.norm1, self.conv1(x), droid_backends.NORM_RELU)
@@ -241,9 +242,9 @@ class BasicEncoder(nn.Module):
         if (tracing.followed(x) or forward_ad._current_level >= 0 or torch.nn.modules.module._has_any_global_hook()
                 or x.dim() != 5 or x.shape[0] * x.shape[1] > 65534):
             return False
-        dt = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
-        if dt not in (torch.float16, torch.bfloat16, torch.float32):
+        if x.dtype not in (torch.float16, torch.bfloat16, torch.float32):
             return False
+        dt = torch.float32 if torch.is_autocast_enabled("cuda") else x.dtype
         blocks = [blk for layer in (self.layer1, self.layer2, self.layer3) for blk in layer]
         return (_plain_norm(self.norm1, dt) and _plain(self.relu1, nn.ReLU)
                 and all(_plain_norm(b.norm1, dt) and _plain_norm(b.norm2, dt) and _plain(b.relu, nn.ReLU)
