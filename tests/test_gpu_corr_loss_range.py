@@ -72,4 +72,4 @@ def test_upstream_gradients_times_a_power_of_two(shared, positive):
         past |= over.any()
         assert (np.abs(got - s)[fits] <= bound[fits]).all()
         assert (got[over] == np.sign(s[over]) * np.inf).all()
-    assert past
+    assert past or not shared    # (separate frames: no gradient reaches a quarter)
