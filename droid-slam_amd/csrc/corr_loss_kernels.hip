@@ -29,6 +29,7 @@
 #include "lds_dma.hpp"
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <type_traits>
 
@@ -1298,6 +1299,10 @@ int corr_loss_check(const std::string& w, int dtype, int E, int N1, int P, int N
     return fail(kInvalidArgument, w + ": bad arguments (Q > 0, 0 < D <= 256, D % 8 == 0, 1 <= K <= 64)");
   if (!(scale > 0.f) || !std::isfinite(scale) || !(T > 0.f) || !std::isfinite(T))
     return fail(kInvalidArgument, w + ": scale and temperature must be positive and finite");
+  // (a product of 0 times a key past the end's -inf, or an infinite one, would be NaN)
+  for (const float f : {scale / T, scale / T * kLog2e, scale * T, T * T})
+    if (!(f >= FLT_MIN && f <= FLT_MAX))
+      return fail(kInvalidArgument, w + ": scale / temperature, their product and temperature^2 must be normal numbers");
   if (std::max(P, Q) > 64 * kMaxGroups || (long)std::max(P, Q) * D * 2 > 0x7fffffffL || (long)P * K > 0x1fffffffL || (long)E * std::max(1, ceil_div(P, kRowsB)) > 0x3fffffL ||
       (long)(N1 + (long)N2) * ceil_div(std::max(P, Q), kRowsB) > 0x3fffffL)
     return fail(kUnsupported, w + ": maps too large");
