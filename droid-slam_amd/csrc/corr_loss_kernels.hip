@@ -474,6 +474,7 @@ constexpr int kJoin = 8;                     // workgroups that join one item
 constexpr int kET = 1024;                    // threads of the edge kernel
 constexpr float kRange = 40.f;                // see edge_paired
 constexpr int kMaxGroups = 8192;             // of 64 keys: frames of up to 524288 rows
+constexpr int kMaxEdges = 65536;             // between as many frames of one row 93 ms, growing with the square
 constexpr int kMinUnits = 32;                // smallest share worth a workgroup
 
 struct BwdArgs {
@@ -1375,6 +1376,8 @@ int droid_corr_loss_backward(int dtype, const void* fmap1, const void* fmap2, co
   const std::string what = "corr_loss_backward";
   if (const int st = corr_loss_check(what, dtype, E, N1, P, N2, Q, D, K, scale, temperature)) return st;
   if (E == 0 || P == 0) return fail(kInvalidArgument, what + ": no edges or no queries");
+  // the reverse of an edge is looked for, and a frame's edges gathered, in the whole list
+  if (E > kMaxEdges) return fail(kUnsupported, what + ": more than 65536 edges");
   if (!fmap1 || !fmap2 || !f1 || !f2 || !idx || !lse || !gloss || (!dfmap1 && !dfmap2))
     return fail(kInvalidArgument, what + ": null tensor");
   if (!prob && K != 1) return fail(kInvalidArgument, what + ": one target a row without weights");

@@ -159,7 +159,7 @@ int droid_corr_loss_forward(int dtype, const void* fmap1, const void* fmap2, con
                             size_t ws_bytes, hipStream_t stream);
 /* gloss (E,P) f32 -> dfmap1 (N1,P,D), dfmap2 (N2,Q,D) of the features' type, each
  * element written once (either may be NULL); shared != 0: fmap1 == fmap2 and dfmap1
- * receives the sum of both roles (dfmap2 NULL).  No atomics on global memory: the
+ * receives the sum of both roles (dfmap2 NULL).  At most 65536 edges.  No atomics on global memory: the
  * result does not depend on the schedule. */
 int droid_corr_loss_backward(int dtype, const void* fmap1, const void* fmap2, const int* f1, const int* f2,
                              const int* idx, const float* prob, const float* lse, const float* gloss, void* dfmap1,
