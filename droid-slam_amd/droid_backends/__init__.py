@@ -321,6 +321,12 @@ def corr_alt_ce0(pyramid, f1, f2, coords, w, bias, out=None, order=None):
 _LOSS_DTYPES = {torch.float16: 0, torch.bfloat16: 3}
 
 
+def _last(fn, idx):
+    if not isinstance(idx, torch.Tensor) or idx.dim() == 0:
+        raise RuntimeError("%s: idx must be an int32 tensor (edges, query rows..., K)" % fn)
+    return idx.shape[-1]
+
+
 def _corr_loss_check(fn, fmap1, fmap2, f1, f2, idx, K):
     """Shapes and types shared by the two directions -> (keys' tensor, N1, P, N2, Q, D, E)."""
     shared = fmap2 is None
@@ -339,6 +345,10 @@ def _corr_loss_check(fn, fmap1, fmap2, f1, f2, idx, K):
     P, Q = fmap1.shape[1:-1].numel(), keys.shape[1:-1].numel()
     if f1.dim() != 1 or f2.shape != f1.shape:
         raise RuntimeError("%s: f1 and f2 must have one entry per edge" % fn)
+    if E and (N1 == 0 or N2 == 0):
+        raise RuntimeError("%s: edges between no frames" % fn)
+    if K is not None and not 1 <= K <= 64:
+        raise RuntimeError("%s: %d targets a row (1 to 64)" % (fn, K))
     if max(N1, P, N2, Q, E) > 0x7fffffff:   # the C ABI's int
         raise RuntimeError("%s: %d frames of %d rows, %d of %d, %d edges: too large" % (fn, N1, P, N2, Q, E))
     rows = (E,) + tuple(fmap1.shape[1:-1])
@@ -356,14 +366,14 @@ def corr_loss_forward(fmap1, fmap2, f1, f2, idx, logits=None, scale=1.0 / 16, te
     negative = none.  -> loss (E, query rows...) float32, lse, prob: the saved
     tensors of corr_loss_backward."""
     fn = "corr_loss_forward"
-    K = None if logits is None else idx.shape[-1]
+    K = None if logits is None else _last(fn, idx)
     keys, N1, P, N2, Q, D, E = _corr_loss_check(fn, fmap1, fmap2, f1, f2, idx, K)
     prob = None
     if logits is not None:
         _check_inputs(("fmap1", "logits"), (fmap1, logits))
         _need(logits, torch.float32, "logits")
-        if logits.shape != idx.shape or not 1 <= K <= 64:
-            raise RuntimeError("%s: logits must match idx, 1 <= K <= 64" % fn)
+        if logits.shape != idx.shape:
+            raise RuntimeError("%s: logits must match idx" % fn)
         prob = torch.empty_like(logits)
     dev = fmap1.device
     rows = idx.shape if logits is None else idx.shape[:-1]
@@ -385,7 +395,7 @@ def corr_loss_backward(gloss, fmap1, fmap2, f1, f2, idx, lse, prob=None, scale=1
     features are both queries and keys and dfmap1 has the sum of both roles.
     need1 / need2: compute only the gradients that are used (None otherwise)."""
     fn = "corr_loss_backward"
-    K = None if prob is None else idx.shape[-1]
+    K = None if prob is None else _last(fn, idx)
     keys, N1, P, N2, Q, D, E = _corr_loss_check(fn, fmap1, fmap2, f1, f2, idx, K)
     shared = fmap2 is None
     rows = idx.shape if prob is None else idx.shape[:-1]
