@@ -1055,16 +1055,16 @@ def group_norm_act_backward(dy, x, stats, num_groups, weight=None, bias=None, mo
     return _group_norm_act_backward(dy, x, stats, num_groups, weight, bias, mode, res if with_res else None, wdt)
 
 
-def _group_norm_act_backward(dy, x, stats, num_groups, weight, bias, mode, res, wdt):
-    """group_norm_act_backward on checked arguments."""
+def _group_norm_act_backward(dy, x, stats, num_groups, weight, bias, mode, res, wdt, need_w=True, need_b=True):
+    """group_norm_act_backward on checked arguments; without need_w / need_b that gradient is None."""
     N, C, H, W = x.shape
     dt, hw, dev = _NORM_DTYPES[x.dtype], H * W, x.device
     dx = torch.empty_like(x, memory_format=torch.channels_last)
     dres = torch.empty_like(x, memory_format=torch.channels_last) if res is not None else None
     # an empty map launches nothing: its parameters' gradients are sums of nothing
     new = torch.empty_like if x.numel() else torch.zeros_like
-    dw = new(weight) if weight is not None else None
-    db = new(bias) if bias is not None else None
+    dw = new(weight) if need_w and weight is not None else None
+    db = new(bias) if need_b and bias is not None else None
     with _on(dev):
         ws = torch.empty((_group_norm_workspace(dt, N, hw, C, num_groups, 1),), dtype=torch.uint8, device=dev)
         check(lib.droid_group_norm_act_backward(dt, _addr(x), _addr(res), _addr(dy), _addr(weight),

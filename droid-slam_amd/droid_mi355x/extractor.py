@@ -66,7 +66,8 @@ class GroupNormAct(torch.autograd.Function):
         cl = torch.channels_last
         dx, dres, dw, db = droid_backends._group_norm_act_backward(
             dy.contiguous(memory_format=cl), x.contiguous(memory_format=cl), stats.contiguous(), ctx.num_groups,
-            weight, bias, ctx.mode, None if res is None else res.contiguous(memory_format=cl), ctx.wdt)
+            weight, bias, ctx.mode, None if res is None else res.contiguous(memory_format=cl), ctx.wdt,
+            *ctx.needs_input_grad[2:4])
         return dx, None, dw, db, None, dres, None
 
 
