@@ -1018,8 +1018,8 @@ __device__ __forceinline__ void band_epilogue(const ConvArgs& a, floatx4 (&acc)[
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
         if constexpr (kPre) {
-          // the staged pre-activation: bias added two values at a time (v_pk_add_f32)
-          // and rounded two at a time (v_cvt_pk_f16_f32); the halves go to their rows
+          // the staged pre-activation: bias added to two values and both rounded at once
+          // (v_cvt_pk_f16_f32); the halves go to their rows
           typedef float f2_t __attribute__((ext_vector_type(2)));
           typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
           const f2_t b2 = {bv, bv};
@@ -1162,8 +1162,8 @@ __device__ __forceinline__ void band_epilogue_core(const ConvArgs& a, _Float16* 
       // sigmoid / tanh go through f32 (torch evaluates them in f32 and rounds).
       if constexpr (kPre) {
         const half8 x = v + ppre[q];   // the gate argument: per-edge conv + per-frame term
-        // sigmoid / tanh two at a time: the exp argument scaling and the "+ 1" on
-        // packed f32 (v_pk_mul_f32 / v_pk_add_f32), exp and rcp per value
+        // sigmoid / tanh written two at a time (the build has no packed fp32
+        // instructions: each is two of the plain ones)
         typedef float f2_t __attribute__((ext_vector_type(2)));
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
@@ -2203,11 +2203,11 @@ constexpr int glo_lds(int ring) { return ring * 2 * kGloTP * 128; }
 // split: blockIdx.y of gridDim.y pixel ranges of the edge (whole 64-pixel tiles);
 // range y writes its share of the mean to glo + y * E * 128 (the caller adds
 // the ranges in order; one range = the plain mean)
-// PK (the product, kGloPkProd): sigmoid(y + b) * h on packed fp32 (v_pk_fma_f32
-// / v_pk_add_f32, two values per instruction; the exp argument as one fma of y
-// with the scaled bias) - the kernel is VALU-bound on this (2 transcendentals
-// per value); 0.3835 vs 0.4249 ms at C3 for the scalar form, which the A/B
-// build keeps (droid_glo_set_pk; profiles/r05/r05pk_glo_pk_ab.txt)
+// PK (the product, kGloPkProd): sigmoid(y + b) * h two values at a time, the exp
+// argument as one fma of y with the scaled bias (the build has no packed fp32
+// instructions: plain ones) - the kernel is VALU-bound on this (2 transcendentals
+// per value); 0.371 vs 0.399 ms at C3 for the form of one value at a time, which the
+// A/B build keeps (droid_glo_set_pk; profiles/glo_pair_ab.txt)
 template <int kGloRing, bool PK>
 __global__ void __launch_bounds__(256) gru_glo_kernel(const __half* __restrict__ h, const __half* __restrict__ w,
                                                       const float* __restrict__ bias, float* __restrict__ glo,

@@ -351,7 +351,9 @@ __global__ void __launch_bounds__(kLT) corr_loss_row_kernel(RowArgs a) {
   float tot = 0.f;
 #pragma unroll
   for (int n = 0; n < SLOTS; ++n) {
-    pi[n] = __expf((pi[n] - top) * a.invT);   // (over T last: a lowest value over T < 1 is -inf)
+    // over T last: a lowest value over T < 1 is -inf.  The hardware's exponential: off by
+    // t 2^-24 and two units of fp32 for an exponent -t, whose weight is e^-t of the largest
+    pi[n] = __expf((pi[n] - top) * a.invT);
     if (l + 16 * n >= a.K) pi[n] = 0.f;
     tot += pi[n];
   }
@@ -780,8 +782,9 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
   // where u = 2^(c s - lse_x - b), A = 2^(lse_x - m + b), B = 2^(v_y + m): one exponential
   // a pair of rows. b = kRange / 2, and lse_x := m in a left-out row x: then u <= 1
   // wherever x or y has a target, and is clamped to that where neither has, so that
-  // it stays finite there and the factor 0 holds. What underflows is below
-  // 2^(kRange - 126) of a probability.
+  // it stays finite there and the factor 0 holds. u underflows where
+  // c s < lse_x + b - 126: there p2 = 2^(c s - lse_y), with lse_x - lse_y up to kRange,
+  // is below 2^(1.5 kRange - 126) = 2^-66.
   float mid = 0.f;
   if constexpr (SRC && DST) {
     const float2 span = edge_range(a, es, ed);

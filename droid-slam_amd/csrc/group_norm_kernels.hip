@@ -282,6 +282,9 @@ __device__ __forceinline__ void gn_finish_stats(const double2* part, int n, int 
 
 __device__ __forceinline__ float relu(float v) { return v < 0.f ? 0.f : v; }   // passes a NaN on, as torch's
 
+// SiLU's exponential and reciprocal are the hardware's: exp(-n) is off by |n| 2^-24
+// (its argument's product with log2 e) and two units of fp32, the reciprocal by one,
+// relative to silu(n) - which is exp(-|n|) |n| where |n| is large and negative.
 template <int MODE>
 __device__ __forceinline__ float gn_act(float n, float r) {
   if constexpr (MODE == kRelu) return relu(n);
