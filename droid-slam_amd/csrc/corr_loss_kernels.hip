@@ -19,7 +19,11 @@
 // operand comes by transposed LDS reads in the same order), so the weights ds
 // never pass through LDS.  The weights are rounded to the features' type for that
 // product, after the sparse terms are subtracted in fp32, and fp16 ones are scaled
-// by a power of two per frame: half a step of each, as the features' own rounding.
+// by a power of two per frame.  Half tiles with a target take what the rounding left
+// in a second product: a target's weight is most of its row's, and its half a step
+// alone made the gradient's error 1.2 to 1.45 times that of rounding the result
+// (four clips 603 -> 632 us, 501 points 273 -> 302); elsewhere the weights are
+// probabilities, and half a step of them is nothing beside that.
 //
 // What bounds it: the matrix instructions, at the 1.11 (fp16) to 1.16 (bf16) PFLOP/s
 // that a large library product reaches on this card, with the exponentials' vector
@@ -1056,6 +1060,18 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
       for (int j = 0; j < XH; ++j)
 #pragma unroll
         for (int q = 0; q < 16; ++q) ds[j][q >> 3][q & 7] = (T)wg[j][q];
+      if (lo < hi) {   // what the rounding left
+        vec8 low[XH][2];
+#pragma unroll
+        for (int j = 0; j < XH; ++j)
+#pragma unroll
+          for (int q = 0; q < 16; ++q) low[j][q >> 3][q & 7] = (T)(wg[j][q] - (float)ds[j][q >> 3][q & 7]);
+#pragma unroll
+        for (int n = 0; n < kP; ++n) {
+          const int u = n / (kP / 2), d = n % (kP / 2) / XH, j = n % XH;
+          acc[j][d] = Op<T>::mfma(ft[k][u][d], low[j][u], acc[j][d]);
+        }
+      }
     };
     auto read_transposed = [&](int half, int n) {   // the n-th of DP / 16
       const int k = n / (DP / 32), d = n % (DP / 32);
