@@ -281,7 +281,7 @@ struct RowArgs {
   float *loss, *lse, *prob;    // (E, P), (E, P) log2 units, (E, P, K)
   int N1, P, N2, Q, D, K, S;
   long rows;
-  float scale, invT, T2;
+  float invT, T2, c;           // c: scale / T log2(e)
 };
 
 // One query row on 16 lanes: joins the shares of its sum, takes the K target
@@ -379,13 +379,14 @@ __global__ void __launch_bounds__(kLT) corr_loss_row_kernel(RowArgs a) {
     sum += v.y * __builtin_amdgcn_exp2f(v.x - m);
   }
   sum = sum16(sum);
-  const float lse2 = sum > 0.f ? m + log2f(sum) : NAN;
+  const float over = sum > 0.f ? log2f(sum) : NAN, lse2 = m + over;
   // sum_k pi_k s_k, as one dot product with the pi-weighted sum of the target rows
   const T* f2 = static_cast<const T*>(a.f2) + (long)j * a.Q * a.D;
   // The weights kept for the gradient: a key that a row names more than once has all
   // of its weight at the first place that has any, so that no place of ds has more than
   // one term of an edge (and their sum no order).
-  float dot = 0.f, kept[SLOTS] = {};
+  double dot = 0.0;
+  float kept[SLOTS] = {};
   bool again[SLOTS] = {};
   typedef typename Op<T>::vec8 vec8;
   vec8 x[2] = {};             // the row's values 8 l .. + 7, and 128 further
@@ -418,13 +419,18 @@ __global__ void __launch_bounds__(kLT) corr_loss_row_kernel(RowArgs a) {
             kept[n] += own[n] == t[u] ? w[u] : 0.f;
           }
       }
+      // (products of two features are exact in fp32; added as a tree: fewer roundings)
       float v = 0.f;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        if (8 * l + 128 * h < a.D)
+        if (8 * l + 128 * h < a.D) {
+          float p[4];
 #pragma unroll
-          for (int q = 0; q < 8; ++q) v = fmaf((float)x[h][q], (float)y[u][h][q], v);
-      dot = fmaf(w[u], v, dot);
+          for (int q = 0; q < 4; ++q)
+            p[q] = fmaf((float)x[h][q], (float)y[u][h][q], (float)x[h][q + 4] * (float)y[u][h][q + 4]);
+          v += (p[0] + p[2]) + (p[1] + p[3]);
+        }
+      dot = fma((double)w[u], (double)v, dot);
     }
   }
   if (a.prob) {
@@ -432,10 +438,13 @@ __global__ void __launch_bounds__(kLT) corr_loss_row_kernel(RowArgs a) {
     for (int n = 0; n < SLOTS; ++n)
       if (l + 16 * n < a.K) a.prob[row * a.K + l + 16 * n] = again[n] ? 0.f : kept[n];
   }
-  dot = sum16(dot);
+#pragma unroll
+  for (int o = 8; o; o >>= 1) dot += __shfl_xor(dot, o, 16);
   ent = sum16(ent);
   if (l == 0) {
-    a.loss[row] = a.T2 * (ent + fmaf(lse2, kLn2, -dot * (a.scale * a.invT)));
+    // lse - sum_k pi_k s_k relative to the largest logit m: where a target is near it
+    // the loss is a small difference, whose rounding would be m's
+    a.loss[row] = a.T2 * fmaf(over + (float)((double)m - dot * (double)a.c), kLn2, ent);
     a.lse[row] = lse2;
   }
 }
@@ -1371,7 +1380,7 @@ int droid_corr_loss_forward(int dtype, const void* fmap1, const void* fmap2, con
 #undef LSE
   DROID_LAUNCH_CHECK();
   RowArgs r{fmap1, fmap2, f1, f2, idx, logits, a.part, loss, lse, logits ? prob : nullptr, N1, P, N2, Q, D, K, a.S,
-            (long)E * P, scale, 1.f / temperature, temperature * temperature};
+            (long)E * P, 1.f / temperature, temperature * temperature, a.c};
   const int grid = (int)((r.rows + kLT / 16 - 1) / (kLT / 16));
 #define ROW(SLOTS, BATCH)                                                                       \
   if (dtype == 0) corr_loss_row_kernel<_Float16, SLOTS, BATCH><<<grid, kLT, 0, stream>>>(r);    \

@@ -44,3 +44,28 @@ def test_error_is_that_of_the_result(K, P, Q, D, shared, sign, dtype):
         off = host(got.double()) - want
         bound = 1.02 * np.sqrt((own ** 2).sum() + 4 * s)
         assert np.sqrt((off ** 2).sum()) <= bound, np.sqrt((off ** 2).sum() / (own ** 2).sum())
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("K,T", [(0, 1.0), (1, 1.0), (2, 2.0)])
+def test_small_losses_of_large_logits(K, T, dtype):
+    """Each row's target is its own copy among the keys, the features small whole
+    numbers: all products and their sums are exact in fp32, the logits about 1000 and
+    the losses next to nothing.  What is left: at most Q + 8 roundings of a sum that is
+    2^(half a step of the largest logit), and as many units for the hardware's
+    exponential and logarithm: T^2 (Q + 16) 2^-24; roundings of the logits or of lse
+    themselves would be 6e-5 each."""
+    dt = TYPES[dtype]
+    rng = np.random.default_rng(K)
+    a = torch.from_numpy(rng.integers(-3, 4, (2, 150, 128))).to(dt).to("cuda:0")
+    f = np.array([0, 1], np.int32)
+    idx = np.zeros((2, 150, max(1, K)), np.int32)
+    idx[..., 0] = np.arange(150)
+    logits = np.zeros(idx.shape, np.float32) if K else None
+    if K == 2:
+        idx[..., 1], logits[..., 1] = 7, -np.inf
+    g = np.ones((2, 150), np.float32)
+    loss, _ = _run(a, a.clone(), f, f, idx, logits, g, False, 2.0, T)
+    want = oc.corr_loss(host(a.double()), host(a.double()), f, f, idx, logits, 2.0, T)
+    off = np.abs(host(loss.double()) - want)
+    assert off.max() <= T * T * (150 + 16) * 2.0 ** -24, off.max()
