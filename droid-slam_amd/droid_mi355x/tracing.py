@@ -38,8 +38,9 @@ def batched(g):
 
 def refuse(fn, *tensors):
     """For operators without such a form.  Dispatch modes that only watch (counters,
-    selective checkpointing) are let through, tracers are not."""
-    if (_compiling() or _tracing() or _transform() is not None or _carries(tensors)
+    selective checkpointing) are let through, tracers are not; torch.compile runs the
+    operator between two graphs and needs no refusal."""
+    if (_tracing() or _transform() is not None or _carries(tensors)
             or _modes() > 0 and any(torch._C._get_dispatch_mode(k) is not None for k in _MODES)):
         _refused(fn)
 

@@ -59,3 +59,23 @@ def test_the_largest_edge_list():
     more = torch.cat([a, a[:1]]), torch.cat([b, b[:1]]), torch.cat([t, t[:1]])
     with pytest.raises(RuntimeError, match="65536 edges"):
         torch.autograd.grad(corr_cross_entropy(f, None, *more).sum(), f)
+
+
+@pytest.mark.parametrize("K", [0, 3])
+def test_compiled_between_two_graphs(K):
+    """torch.compile leaves the operator to the eager mode: the same loss and gradient."""
+    from droid_mi355x import corr_cross_entropy, corr_distillation
+    f, e, idx, logits = _call()
+
+    def step(x):
+        x = x * 2
+        loss = (corr_distillation(x, None, e, e.flip(0), idx, logits) if K
+                else corr_cross_entropy(x, None, e, e.flip(0), idx[..., 0].contiguous()))
+        return loss.sum() * 3
+
+    out = []
+    for fn in (step, torch.compile(step, backend="eager")):
+        x = f.clone().requires_grad_()
+        y = fn(x)
+        out.append((y.detach(), torch.autograd.grad(y, x)[0]))
+    assert torch.equal(out[0][0], out[1][0]) and torch.equal(out[0][1], out[1][1]) and out[0][1].any()

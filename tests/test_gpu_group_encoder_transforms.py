@@ -118,3 +118,11 @@ def test_the_losses_refuse_a_batch_of_upstream_gradients():
     with pytest.raises(RuntimeError, match="do not reach"):
         torch.autograd.grad(loss, f, torch.ones((3, 2, 30), device=DEV), is_grads_batched=True, retain_graph=True)
     assert torch.autograd.grad(loss, f, torch.ones((2, 30), device=DEV))[0].any()
+
+
+def test_compiled():
+    """torch.compile traces the modules one by one."""
+    enc, x = _encoder(8, 16).to(DEV), _frames().to(DEV)
+    want = copy.deepcopy(enc).double().cpu().forward_reference(x.double().cpu())
+    got = torch.compile(enc, backend="eager")(x)
+    assert _rel(got.detach(), want.detach()) < 2e-3
