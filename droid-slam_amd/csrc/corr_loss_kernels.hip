@@ -22,7 +22,7 @@
 // by a power of two per frame.  Half tiles with a target take what the rounding left
 // in a second product: a target's weight is most of its row's, and its half a step
 // alone made the gradient's error 1.2 to 1.45 times that of rounding the result
-// (four clips 603 -> 632 us, 501 points 273 -> 302); elsewhere the weights are
+// (it costs four clips 603 -> 613 us, 501 points 273 -> 300); elsewhere the weights are
 // probabilities, and half a step of them is nothing beside that.
 //
 // What bounds it: the matrix instructions, at the 1.11 (fp16) to 1.16 (bf16) PFLOP/s
@@ -1070,16 +1070,17 @@ __device__ __forceinline__ void bwd_edge(const BwdArgs& a, BwdShared<DP>& sh, in
 #pragma unroll
         for (int q = 0; q < 16; ++q) ds[j][q >> 3][q & 7] = (T)wg[j][q];
       if (lo < hi) {   // what the rounding left
-        vec8 low[XH][2];
 #pragma unroll
         for (int j = 0; j < XH; ++j)
 #pragma unroll
-          for (int q = 0; q < 16; ++q) low[j][q >> 3][q & 7] = (T)(wg[j][q] - (float)ds[j][q >> 3][q & 7]);
+          for (int u = 0; u < 2; ++u) {
+            vec8 high = ds[j][u], low;
+            asm("" : "+v"(high));   // (or every step converts one value at a time, for these)
 #pragma unroll
-        for (int n = 0; n < kP; ++n) {
-          const int u = n / (kP / 2), d = n % (kP / 2) / XH, j = n % XH;
-          acc[j][d] = Op<T>::mfma(ft[k][u][d], low[j][u], acc[j][d]);
-        }
+            for (int q = 0; q < 8; ++q) low[q] = (T)(wg[j][8 * u + q] - (float)high[q]);
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d) acc[j][d] = Op<T>::mfma(ft[k][u][d], low, acc[j][d]);
+          }
       }
     };
     auto read_transposed = [&](int half, int n) {   // the n-th of DP / 16
