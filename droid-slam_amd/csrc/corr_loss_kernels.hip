@@ -28,8 +28,11 @@
 // What bounds it: the matrix instructions, at the 1.11 (fp16) to 1.16 (bf16) PFLOP/s
 // that a large library product reaches on this card, with the exponentials' vector
 // work beside them.  Four clips (96 edges of 2560 x 2560 rows, D = 128, bf16): row
-// sums 171 us (161 GFLOP, 0.94 PFLOP/s), losses 36 us, gradient 438 us (349 GFLOP,
-// 0.80 PFLOP/s) and 33 us beside it; one clip in fp16 53 + 12 + 142 + 28 us.
+// sums 162 us (161 GFLOP, 0.99 PFLOP/s), losses 33 us, gradient 385 us (349 GFLOP,
+// 0.91 PFLOP/s) and 34 us beside it, 614 in all; one clip in fp16 50 + 11 + 134 + 28.
+// (100 calls after another.  The comparisons in the comments below are of 15 calls,
+// whose clock is lower: the gradient of 383 us before the second product of the
+// remainder took 438 there.)
 #include "lds_dma.hpp"
 
 #include <algorithm>
@@ -292,7 +295,7 @@ struct RowArgs {
 // SLOTS: targets a lane holds (K <= 16 SLOTS); kBatch: target rows read at once.
 // Bound by the rows it gathers, 256 B each, mostly from L2: 246 thousand queries
 // with one target 36 us (as <4, 4>: 57), with 16 100 us (10 TB/s; as <4, 4> 131,
-// one row at a time 155).
+// one row at a time 155); 33 and 92 in a long run.
 template <typename T, int SLOTS, int kBatch>
 __global__ void __launch_bounds__(kLT) corr_loss_row_kernel(RowArgs a) {
   const long row = (long)blockIdx.x * (kLT / 16) + threadIdx.x / 16;
@@ -470,8 +473,8 @@ __global__ void __launch_bounds__(kLT) corr_loss_row_kernel(RowArgs a) {
 // One workgroup a CU, one wave a SIMD with all 512 registers, so the order of a
 // step's instructions is written out: matrix instructions between the exponentials,
 // shared memory read between matrix instructions, the last second product of a tile
-// in the next step.  A step of a pair takes 5050 clocks for 2048 of matrix
-// instructions; the rest is the exponentials (32 a lane and half, 8 clocks each),
+// in the next step.  A step of a pair takes 5200 clocks for 2048 of matrix
+// instructions (512 more in a half tile with targets); the rest is the exponentials (32 a lane and half, 8 clocks each),
 // the conversion to 16 bits, accumulators copied out of AGPRs, two waits at the barrier
 // (480) and the tile's loads.  On the way, four clips: 32 rows a wave 531 us, 64
 // rows 522, the sparse terms sorted beforehand 479, one exponential for both

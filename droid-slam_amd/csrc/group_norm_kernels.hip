@@ -14,10 +14,10 @@
 // Every pass is a stream over maps, bound by HBM (or, for one frame, by the two
 // launches): forward reads x twice and writes y; backward's first pass reads x,
 // dy (and res) and writes dres, its second reads x and dy (dres) and writes dx.
-// 28 maps of 32 x 160 x 256 in bf16, relu(res + relu(n)): 15.5 + 37 us forward,
-// 48 + 40 us backward, 5.7 TB/s over what the passes move (a large copy: 5.1; the
+// 28 maps of 32 x 160 x 256 in bf16, relu(res + relu(n)): 16 + 37 us forward,
+// 50 + 40 us backward, 5.6 TB/s over what the passes move (a large copy: 5.1; the
 // second passes find part of it in the last-level cache); what the operator cannot
-// do without is 114 us of that copy.
+// do without is 115 us of that copy.
 //
 // Layout of the work.  An image is a flat run of HW C values, cut into pieces
 // of V = 16 B.  Piece f starts at channel (V f) mod C, so with A threads, A a
