@@ -1,8 +1,8 @@
-"""A/B of gru_glo_kernel's sigmoid sum on packed fp32 (A/B build:
+"""A/B of gru_glo_kernel's sigmoid sum one value or two at a time (A/B build:
 droid_glo_set_pk) at the C3 shape (2048 edges of 48x64 x 128 channels), ring 3,
-one pixel range per edge: scalar (the product until this A/B) vs packed (the
-product after it), interleaved rounds in one process; the two differ by fp32
-rounding only (the exp argument as one fma).  Result: profiles/r05/r05pk_glo_pk_ab.txt.
+one pixel range per edge, interleaved rounds in one process; the two differ by
+fp32 rounding only (the exp argument as one fma).  Result: profiles/glo_pair_ab.txt
+(with packed fp32 instructions in the build: profiles/r05/r05pk_glo_pk_ab.txt).
 Run with DROID_HIP_LIB=droid-slam_amd/lib/ab/libdroid_hip.so."""
 import ctypes
 import os
